@@ -355,6 +355,59 @@ int32_t cf_paged_write(const CfTensor* x_new, const CfTensor* slot_mapping,
 int32_t cf_paged_gather(const CfTensor* cache, const CfTensor* block_tables,
                         const CfTensor* scale, CfTensor* out, void* stream);
 
+/* ---- Eviction by accumulated attention weight -----------------------------
+ * No counterpart in the reference.  A sequence's account holds, per KV head
+ * (or once for all heads), the attention weight that each cached token has
+ * drawn so far: cf_paged_decode_weights and cf_chunk_weights write it,
+ * cf_evict_select chooses by it which tokens stay, cf_evict_move closes the
+ * holes.  Row b of every tensor below belongs to row b of the block tables.
+ * Attention does not depend on the order of a sequence's tokens in its
+ * slots, so eviction moves only tokens that lie past the new end.
+ *
+ * positions [B, Hw, S] i32 is where each slot's token stands in the text; it
+ * is needed once tokens have been moved.  Slots from kept[b] on hold the
+ * tokens appended since the last eviction: slot i's position is then seen[b]
+ * - len + i, seen[b] being all the tokens the sequence has had.  So after an
+ * eviction the caller sets kept to new_lens and leaves positions alone until
+ * the next one.  Without positions (kept and seen NULL too) a slot's index is
+ * its position. */
+
+/* keep[b, h, j] = the slot whose token belongs in slot j after sequence b is
+ * cut to n = min(len, budget) tokens, len = seq_lens[b] within [0, S]; -1 for
+ * j >= n.  Kept are the tokens at positions below `sink` and the last
+ * `recent` positions, then those of the greatest weight, equal weights by the
+ * lower slot; NaN counts as greater than every number.  A kept token in a
+ * slot below n stays there; the k-th kept one of the others, by slot, goes to
+ * the k-th slot below n that is free.
+ *   weights    [B, H, S]        f32, S stride 1
+ *   positions  [B, H, S]        i32, S stride 1, or NULL
+ *   seq_lens, kept, seen  [B]   i32
+ *   keep       [B, H, budget]   i32, last stride 1 (output)
+ *   new_lens   [B]              i32: n (output)
+ * budget >= 1, sink, recent >= 0, sink + recent <= budget. */
+int32_t cf_evict_select(const CfTensor* weights, const CfTensor* seq_lens, const CfTensor* positions,
+                        const CfTensor* kept, const CfTensor* seen, int32_t sink, int32_t recent, CfTensor* keep,
+                        CfTensor* new_lens, void* stream);
+
+/* Moves the K and V rows of every slot j with keep[b, h, j] != j from slot
+ * keep[b, h, j], in place (the codes of e4m3fn caches as they are), and its
+ * weight and position with them; slots below n that were appended since the
+ * last eviction get their position.  Slots that are nobody's destination are
+ * left as they were.  Where either block id of a move lies outside [0, NB)
+ * the rows stay.
+ *   keep          [B, Hw, budget]   i32, last stride 1: cf_evict_select's, Hw = Hkv,
+ *                                   or 1 (all heads move together)
+ *   seq_lens      [B]               i32, as given to cf_evict_select
+ *   block_tables  [B, Mb]           i32
+ *   k_cache, v_cache  [NB, bs, Hkv, D]  of one dtype, any strides
+ *   weights       [B, Hw, S]        f32, S stride 1, or NULL
+ *   positions     [B, Hw, S]        i32, S stride 1, or NULL (then kept and seen too)
+ * The destinations must not be shared with another sequence: make shared
+ * blocks the sequence's own first (cf_bp_prepare_writes, cf_copy_blocks). */
+int32_t cf_evict_move(const CfTensor* keep, const CfTensor* seq_lens, const CfTensor* block_tables, CfTensor* k_cache,
+                      CfTensor* v_cache, CfTensor* weights, CfTensor* positions, const CfTensor* kept,
+                      const CfTensor* seen, void* stream);
+
 /* Uploads `bytes` (a multiple of 16; both pointers 16-byte aligned) from
  * pinned, mapped host memory (hipHostMalloc, torch pin_memory) to device
  * memory with a kernel on `stream`, so the upload is ordered with the

@@ -172,6 +172,8 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "cf_kv_write_fp8": (ctypes.c_int32, [_P, _P, _P, _P, _P, _P, _P, ctypes.c_void_p]),
     "cf_paged_write": (ctypes.c_int32, [_P, _P, _P, _P, ctypes.c_void_p]),
     "cf_paged_gather": (ctypes.c_int32, [_P, _P, _P, _P, ctypes.c_void_p]),
+    "cf_evict_select": (ctypes.c_int32, [_P, _P, _P, _P, _P, ctypes.c_int32, ctypes.c_int32, _P, _P, ctypes.c_void_p]),
+    "cf_evict_move": (ctypes.c_int32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_void_p]),
     "cf_bp_create": (ctypes.c_int32, [ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_void_p)]),
     "cf_bp_destroy": (ctypes.c_int32, [ctypes.c_void_p]),
     "cf_bp_num_free": (ctypes.c_int32, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64)]),

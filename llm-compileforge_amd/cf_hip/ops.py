@@ -593,6 +593,87 @@ def paged_gather(
     return out
 
 
+def _int32(name: str, value: int) -> int:
+    if not -(1 << 31) <= value < 1 << 31:
+        raise ValueError(f"{name} ({value}) does not fit 32 bits")
+    return value
+
+
+def evict_select(
+    weights: torch.Tensor,
+    seq_lens: torch.Tensor,
+    budget: int,
+    sink: int = 0,
+    recent: int = 0,
+    positions: torch.Tensor | None = None,
+    kept: torch.Tensor | None = None,
+    seen: torch.Tensor | None = None,
+    keep: torch.Tensor | None = None,
+    new_lens: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Which of a sequence's cached tokens each head keeps when it is cut to
+    `budget` tokens: (keep [B, H, budget], new_lens [B]), both int32.
+
+    weights [B, H, S] f32; seq_lens int32 [B]; positions int32 [B, H, S] with
+    kept and seen int32 [B], or none of the three (cf_hip.h gives their
+    meaning).  keep[b, h, j] is the slot whose token belongs in slot j, -1 past
+    new_lens[b] = min(seq_lens[b], budget): the first `sink` and last `recent`
+    positions, then the greatest weights, equal ones by the lower slot.
+    """
+    budget, sink, recent = _int32("budget", int(budget)), _int32("sink", int(sink)), _int32("recent", int(recent))
+    given = [("weights", weights), ("seq_lens", seq_lens)]
+    given += [(n, t) for n, t in (("positions", positions), ("kept", kept), ("seen", seen), ("keep", keep),
+                                  ("new_lens", new_lens)) if t is not None]
+    for name, t in given:
+        _require_device(name, t)
+    dev = _same_device(*(t for _, t in given))
+    if weights.dim() != 3:
+        raise ValueError(f"weights must be [sequences, heads, slots], got {tuple(weights.shape)}")
+    if budget < 1:
+        raise ValueError(f"budget ({budget}) must be positive")
+    if keep is None:
+        keep = torch.empty(weights.shape[0], weights.shape[1], budget, dtype=torch.int32, device=dev)
+    elif keep.dim() != 3 or keep.shape[2] != budget:
+        raise ValueError(f"keep must be [sequences, heads, {budget}], got {tuple(keep.shape)}")
+    if new_lens is None:
+        new_lens = torch.empty(weights.shape[0], dtype=torch.int32, device=dev)
+    d = [descriptor(t) if t is not None else None for t in (weights, seq_lens, positions, kept, seen)]
+    dk, dn = descriptor(keep), descriptor(new_lens)
+    with _on(dev):
+        rc = lib().cf_evict_select(*(ref(x) for x in d), sink, recent, ref(dk), ref(dn), stream_handle(dev))
+    check(rc, "cf_evict_select")
+    return keep, new_lens
+
+
+def evict_move(
+    keep: torch.Tensor,
+    seq_lens: torch.Tensor,
+    block_tables: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    weights: torch.Tensor | None = None,
+    positions: torch.Tensor | None = None,
+    kept: torch.Tensor | None = None,
+    seen: torch.Tensor | None = None,
+) -> None:
+    """Moves the rows that evict_select's `keep` sends to another slot, in
+    place: K and V (any layout; e4m3fn codes as they are) and, where given, the
+    weights and positions of their slots.  The destinations must be the
+    sequence's own blocks."""
+    given = [("keep", keep), ("seq_lens", seq_lens), ("block_tables", block_tables), ("k_cache", k_cache),
+             ("v_cache", v_cache)]
+    given += [(n, t) for n, t in (("weights", weights), ("positions", positions), ("kept", kept), ("seen", seen))
+              if t is not None]
+    for name, t in given:
+        _require_device(name, t)
+    dev = _same_device(*(t for _, t in given))
+    d = [descriptor(t) if t is not None else None
+         for t in (keep, seq_lens, block_tables, k_cache, v_cache, weights, positions, kept, seen)]
+    with _on(dev):
+        rc = lib().cf_evict_move(*(ref(x) for x in d), stream_handle(dev))
+    check(rc, "cf_evict_move")
+
+
 def stage_from_host(host_ptr: int, dev_ptr: int, nbytes: int, device: torch.device) -> bool:
     """Uploads nbytes (a multiple of 16) from mapped pinned host memory to
     device memory with the library's upload kernel on the current stream;
@@ -758,6 +839,8 @@ __all__ = [
     "block_tables_apply",
     "copy_blocks",
     "decode_workspace_bytes",
+    "evict_move",
+    "evict_select",
     "prefill_chunk",
     "prefill_workspace_bytes",
     "new_workspace",

@@ -12,6 +12,7 @@
 
 #include "cf_host.hpp"
 #include "decode_params.hpp"
+#include "kv_evict.hpp"
 #include "kv_fp8.hpp"
 #include "paged_io.hpp"
 #include "prefill_params.hpp"
@@ -178,6 +179,47 @@ Rank4 rank4_of(const View& v) {
     r.stride[lead + i] = v.stride[i];
   }
   return r;
+}
+
+// [B] i32.
+int32_t row_view(const CfTensor* t, const char* name, int64_t B, const int32_t** ptr, int64_t* stride) {
+  View v;
+  int32_t rc = view_of(t, name, 1, &v);
+  if (rc) return rc;
+  CF_CHECK(v.dtype == CF_I32, "%s: expected i32, got %s", name, dtype_name(v.dtype));
+  CF_CHECK(v.size[0] == B, "%s has %lld entries, batch is %lld", name, (long long)v.size[0], (long long)B);
+  *ptr = (const int32_t*)v.base;
+  *stride = v.stride[0];
+  return CF_OK;
+}
+
+// An account or its positions: [B, H, S] with unit S stride, rows apart.
+int32_t account_view(const CfTensor* t, const char* name, int dtype, View* v) {
+  int32_t rc = view_of(t, name, 3, v);
+  if (rc) return rc;
+  CF_CHECK(v->dtype == dtype, "%s: expected %s, got %s", name, dtype_name(dtype), dtype_name(v->dtype));
+  CF_CHECK(v->stride[2] == 1 || v->size[2] <= 1, "%s: the last stride must be 1", name);
+  for (int i = 0; i < 2; ++i)
+    CF_CHECK(v->size[i] <= 1 || v->stride[i] >= v->size[2], "%s: rows overlap (stride %lld on dim %d)", name,
+             (long long)v->stride[i], i);
+  CF_CHECK(v->size[0] <= 1 || v->size[1] <= 1 || v->stride[0] != v->stride[1], "%s: rows overlap", name);
+  CF_CHECK(v->size[2] < (int64_t)INT32_MAX - (1 << 20), "%s: too many slots", name);
+  return CF_OK;
+}
+
+// positions, kept and seen of an eviction: all of them, or none.
+int32_t position_views(const CfTensor* positions, const CfTensor* kept, const CfTensor* seen, const View& like,
+                       View* v, const int32_t** kp, int64_t* ks, const int32_t** sp, int64_t* ss) {
+  CF_CHECK((positions == nullptr) == (kept == nullptr) && (kept == nullptr) == (seen == nullptr),
+           "positions, kept and seen go together");
+  if (positions == nullptr) return CF_OK;
+  int32_t rc;
+  if ((rc = account_view(positions, "positions", CF_I32, v))) return rc;
+  for (int i = 0; i < 2; ++i)
+    CF_CHECK(v->size[i] == like.size[i], "positions: size %lld on dim %d, expected %lld", (long long)v->size[i], i,
+             (long long)like.size[i]);
+  if ((rc = row_view(kept, "kept", like.size[0], kp, ks))) return rc;
+  return row_view(seen, "seen", like.size[0], sp, ss);
 }
 
 int32_t view_of_34(const CfTensor* t, const char* name, View* v) {
@@ -882,6 +924,113 @@ int32_t cf_paged_gather(const CfTensor* cache, const CfTensor* block_tables, con
   p.D = (int)vc.size[3];
   p.bs = (int)vc.size[1];
   return launch_paged_gather(p, vc.dtype, vo.dtype, as_stream(stream));
+}
+
+int32_t cf_evict_select(const CfTensor* weights, const CfTensor* seq_lens, const CfTensor* positions,
+                        const CfTensor* kept, const CfTensor* seen, int32_t sink, int32_t recent, CfTensor* keep,
+                        CfTensor* new_lens, void* stream) {
+  View vw, vp{}, vk, vn;
+  EvictSelectParams p{};
+  int32_t rc;
+  if ((rc = account_view(weights, "weights", CF_F32, &vw))) return rc;
+  if ((rc = account_view(keep, "keep", CF_I32, &vk))) return rc;
+  const int64_t B = vw.size[0], H = vw.size[1], S = vw.size[2], budget = vk.size[2];
+  CF_CHECK(vk.size[0] == B && vk.size[1] == H, "keep must be [%lld, %lld, budget]", (long long)B, (long long)H);
+  CF_CHECK(budget >= 1, "budget must be positive");
+  CF_CHECK(sink >= 0 && recent >= 0 && (int64_t)sink + recent <= budget,
+           "sink (%d) and recent (%d) must not be negative and fit the budget (%lld) together", sink, recent,
+           (long long)budget);
+  if ((rc = row_view(seq_lens, "seq_lens", B, &p.lens, &p.l_s))) return rc;
+  if ((rc = position_views(positions, kept, seen, vw, &vp, &p.kept, &p.kept_s, &p.seen, &p.seen_s))) return rc;
+  CF_CHECK(positions == nullptr || vp.size[2] == S, "positions has %lld slots, weights %lld", (long long)vp.size[2],
+           (long long)S);
+  if ((rc = view_of(new_lens, "new_lens", 1, &vn))) return rc;
+  CF_CHECK(vn.dtype == CF_I32 && vn.size[0] == B, "new_lens must be i32 [%lld]", (long long)B);
+  CF_CHECK(B * H < (int64_t)INT32_MAX, "too many rows");
+  if (B * H == 0) return CF_OK;
+  p.weights = (const float*)vw.base;
+  p.w_sb = vw.stride[0];
+  p.w_sh = vw.stride[1];
+  p.positions = positions == nullptr ? nullptr : (const int32_t*)vp.base;
+  p.p_sb = vp.stride[0];
+  p.p_sh = vp.stride[1];
+  p.keep = (int32_t*)vk.base;
+  p.k_sb = vk.stride[0];
+  p.k_sh = vk.stride[1];
+  p.new_lens = (int32_t*)vn.base;
+  p.n_s = vn.stride[0];
+  p.B = (int)B;
+  p.H = (int)H;
+  p.S = (int)S;
+  p.budget = (int)budget;
+  p.sink = sink;
+  p.recent = recent;
+  return launch_evict_select(p, as_stream(stream));
+}
+
+int32_t cf_evict_move(const CfTensor* keep, const CfTensor* seq_lens, const CfTensor* block_tables, CfTensor* k_cache,
+                      CfTensor* v_cache, CfTensor* weights, CfTensor* positions, const CfTensor* kept,
+                      const CfTensor* seen, void* stream) {
+  View vk, vt, vc[2], vw{}, vp{};
+  EvictMoveParams p{};
+  int32_t rc;
+  if ((rc = account_view(keep, "keep", CF_I32, &vk))) return rc;
+  if ((rc = view_of(block_tables, "block_tables", 2, &vt))) return rc;
+  if ((rc = view_of(k_cache, "k_cache", 4, &vc[0]))) return rc;
+  if ((rc = view_of(v_cache, "v_cache", 4, &vc[1]))) return rc;
+  const int64_t B = vk.size[0], Hw = vk.size[1], budget = vk.size[2];
+  CF_CHECK(vt.dtype == CF_I32, "block_tables: expected i32, got %s", dtype_name(vt.dtype));
+  CF_CHECK(vt.size[0] == B, "block_tables has %lld rows, batch is %lld", (long long)vt.size[0], (long long)B);
+  CF_CHECK(is_float_dtype(vc[0].dtype) || vc[0].dtype == CF_F8E4M3FN,
+           "k_cache: dtype must be f32, f16, bf16 or f8e4m3fn, got %s", dtype_name(vc[0].dtype));
+  CF_CHECK(vc[1].dtype == vc[0].dtype, "v_cache dtype %s differs from k_cache dtype %s", dtype_name(vc[1].dtype),
+           dtype_name(vc[0].dtype));
+  for (int i = 0; i < 4; ++i)
+    CF_CHECK(vc[1].size[i] == vc[0].size[i], "v_cache shape differs from k_cache shape on dim %d", i);
+  const int64_t NB = vc[0].size[0], bs = vc[0].size[1], Hkv = vc[0].size[2], D = vc[0].size[3];
+  CF_CHECK(bs > 0, "cache block size must be positive");
+  CF_CHECK(Hw == Hkv || Hw == 1, "keep has %lld heads, the cache %lld (one account a KV head, or one for all)",
+           (long long)Hw, (long long)Hkv);
+  CF_CHECK(bs < 65536 && Hkv < 65536 && D < 65536 && Hkv * D < (int64_t)INT32_MAX / 256, "cache dims too large");
+  CF_CHECK(NB * bs < (int64_t)INT32_MAX && vt.size[1] * bs < (int64_t)INT32_MAX, "too many cache slots");
+  if ((rc = row_view(seq_lens, "seq_lens", B, &p.lens, &p.l_s))) return rc;
+  int64_t S = vt.size[1] * bs;
+  if (weights != nullptr) {
+    if ((rc = account_view(weights, "weights", CF_F32, &vw))) return rc;
+    CF_CHECK(vw.size[0] == B && vw.size[1] == Hw, "weights must be [%lld, %lld, S]", (long long)B, (long long)Hw);
+    S = std::min(S, vw.size[2]);
+  }
+  if ((rc = position_views(positions, kept, seen, vk, &vp, &p.kept, &p.kept_s, &p.seen, &p.seen_s))) return rc;
+  if (positions != nullptr) S = std::min(S, vp.size[2]);
+  const int64_t groups = ceil_div(budget, 64) * B * Hw;
+  CF_CHECK(groups < (int64_t)INT32_MAX, "too many slots");
+  if (groups == 0 || NB == 0 || Hkv * D == 0) return CF_OK;
+  p.keep = (const int32_t*)vk.base;
+  p.k_sb = vk.stride[0];
+  p.k_sh = vk.stride[1];
+  p.tables = (const int32_t*)vt.base;
+  p.t_sb = vt.stride[0];
+  p.t_sm = vt.stride[1];
+  for (int c = 0; c < 2; ++c) {
+    p.cache[c] = vc[c].base;
+    for (int i = 0; i < 4; ++i) p.c_s[c][i] = vc[c].stride[i];
+  }
+  p.weights = weights == nullptr ? nullptr : (float*)vw.base;
+  p.w_sb = vw.stride[0];
+  p.w_sh = vw.stride[1];
+  p.positions = positions == nullptr ? nullptr : (int32_t*)vp.base;
+  p.p_sb = vp.stride[0];
+  p.p_sh = vp.stride[1];
+  p.NB = NB;
+  p.B = (int)B;
+  p.Hw = (int)Hw;
+  p.Hkv = (int)Hkv;
+  p.D = (int)D;
+  p.bs = (int)bs;
+  p.Mb = (int)vt.size[1];
+  p.S = (int)S;
+  p.budget = (int)budget;
+  return launch_evict_move(p, vc[0].elem, as_stream(stream));
 }
 
 int32_t cf_stage_from_host(const void* host_src, void* dev_dst, uint64_t bytes, void* stream) {

@@ -1,0 +1,118 @@
+"""Eviction without a GPU: what its entry points refuse, and the plain
+statement itself."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from cf_hip import _abi
+from kernels.kv_eviction import evict_move, evict_select
+from oracle import kv_eviction as oracle
+
+
+def test_cpu_tensors_are_refused():
+    w, n = torch.zeros(1, 2, 32), torch.ones(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="ROCm"):
+        evict_select(w, n, 8)
+    k = torch.zeros(4, 16, 2, 64)
+    with pytest.raises(ValueError, match="ROCm"):
+        evict_move(torch.zeros(1, 2, 8, dtype=torch.int32), n, torch.zeros(1, 2, dtype=torch.int32), k, k)
+
+
+def _i32(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+def _select(**change):
+    a = dict(weights=torch.zeros(2, 4, 64), seq_lens=_i32(2), positions=_i32(2, 4, 64), kept=_i32(2), seen=_i32(2),
+             keep=_i32(2, 4, 16), new_lens=_i32(2), sink=1, recent=2)
+    a.update(change)
+    d = {n: None if a[n] is None else _abi.descriptor(a[n])
+         for n in ("weights", "seq_lens", "positions", "kept", "seen", "keep", "new_lens")}
+    for x in d.values():
+        if x is not None:
+            x.t.device = _abi.SFA_ROCM  # reach the checks; every call here is refused before a launch
+    r = {n: _abi.ref(x) for n, x in d.items()}
+    return _abi.lib().cf_evict_select(r["weights"], r["seq_lens"], r["positions"], r["kept"], r["seen"], a["sink"],
+                                      a["recent"], r["keep"], r["new_lens"], None)
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(weights=torch.zeros(2, 4, 64, dtype=torch.float16)), "weights: expected f32"),
+    (dict(weights=torch.zeros(2, 4)), "weights: expected rank 3"),
+    (dict(weights=torch.zeros(2, 4, 128)[:, :, ::2]), "the last stride must be 1"),
+    (dict(weights=torch.zeros(2, 1, 64).expand(2, 4, 64)), "rows overlap"),
+    (dict(seq_lens=_i32(3)), "seq_lens has 3 entries"),
+    (dict(seq_lens=torch.zeros(2, dtype=torch.int64)), "seq_lens: expected i32"),
+    (dict(positions=None), "go together"),
+    (dict(seen=None), "go together"),
+    (dict(positions=_i32(2, 4, 63)), "positions has 63 slots"),
+    (dict(positions=_i32(2, 3, 64)), "positions: size 3"),
+    (dict(kept=_i32(1)), "kept has 1 entries"),
+    (dict(keep=_i32(2, 3, 16)), "keep must be"),
+    (dict(keep=_i32(2, 4, 0)), "budget must be positive"),
+    (dict(keep=_i32(2, 1, 16).expand(2, 4, 16)), "keep: rows overlap"),
+    (dict(new_lens=_i32(1)), "new_lens"),
+    (dict(sink=-1), "sink"),
+    (dict(sink=10, recent=7), "fit the budget"),
+    (dict(sink=2**31 - 1, recent=2**31 - 1), "fit the budget"),
+])
+def test_select_refuses(change, message):
+    assert _select(**change) == _abi.CF_ERR_INVALID
+    assert message in _abi.last_error()
+
+
+def _move(**change):
+    a = dict(keep=_i32(2, 4, 16), seq_lens=_i32(2), tables=_i32(2, 3), k=torch.zeros(9, 16, 4, 64),
+             v=torch.zeros(9, 16, 4, 64), weights=torch.zeros(2, 4, 48), positions=_i32(2, 4, 48), kept=_i32(2),
+             seen=_i32(2))
+    a.update(change)
+    d = [None if t is None else _abi.descriptor(t) for t in a.values()]
+    for x in d:
+        if x is not None:
+            x.t.device = _abi.SFA_ROCM
+    return _abi.lib().cf_evict_move(*(_abi.ref(x) for x in d), None)
+
+
+@pytest.mark.parametrize("change, message", [
+    (dict(keep=_i32(2, 3, 16)), "one account a KV head, or one for all"),
+    (dict(keep=torch.zeros(2, 4, 16)), "keep: expected i32"),
+    (dict(tables=_i32(3, 3)), "block_tables has 3 rows"),
+    (dict(tables=torch.zeros(2, 3, dtype=torch.int64)), "block_tables: expected i32"),
+    (dict(k=torch.zeros(9, 16, 4, 64, dtype=torch.int32)), "k_cache: dtype"),
+    (dict(v=torch.zeros(9, 16, 4, 64, dtype=torch.float16)), "v_cache dtype"),
+    (dict(v=torch.zeros(9, 16, 4, 32)), "v_cache shape"),
+    (dict(weights=torch.zeros(2, 1, 48)), "weights must be"),
+    (dict(positions=None), "go together"),
+    (dict(positions=_i32(1, 4, 48)), "positions: size 1"),
+    (dict(seq_lens=_i32(1)), "seq_lens has 1"),
+])
+def test_move_refuses(change, message):
+    assert _move(**change) == _abi.CF_ERR_INVALID
+    assert message in _abi.last_error()
+
+
+def test_moves_into_two_thousand_million_slots_are_refused():
+    d = torch.zeros(9, 16, 4, 64)
+    big = _abi.descriptor(d)
+    a = [_abi.descriptor(t) for t in (_i32(2, 4, 16), _i32(2), _i32(2, 3))]
+    for x in (big, *a):
+        x.t.device = _abi.SFA_ROCM
+    big.t.r4.sizes[0] = 1 << 28
+    assert _abi.lib().cf_evict_move(*(_abi.ref(x) for x in a), _abi.ref(big), _abi.ref(big), None, None, None, None,
+                                    None) == _abi.CF_ERR_INVALID
+    assert "too many cache slots" in _abi.last_error()
+
+
+def test_the_plain_statement():
+    w = np.array([5.0, 1.0, 9.0, 1.0, 7.0, 0.0, 9.0, 2.0])
+    keep, n = oracle.select(w, 8, 4)
+    assert n == 4 and keep.tolist() == [0, 4, 2, 6]
+    assert oracle.select(w, 8, 4, sink=2, recent=1)[0].tolist() == [0, 1, 2, 7]
+    assert oracle.select(w, 3, 4)[0].tolist() == [0, 1, 2, -1]
+    assert oracle.select(np.ones(6), 6, 3)[0].tolist() == [0, 1, 2]
+    assert oracle.select(np.array([1.0, np.nan, np.inf]), 3, 1)[0].tolist() == [1]
+    # slot 0 holds the newest position: kept as recent
+    assert oracle.select(np.zeros(4), 4, 2, recent=1, positions=np.array([9, 3, 4]), kept=3, seen=11)[0].tolist() == [0, 3]
