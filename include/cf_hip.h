@@ -355,6 +355,50 @@ int32_t cf_paged_write(const CfTensor* x_new, const CfTensor* slot_mapping,
 int32_t cf_paged_gather(const CfTensor* cache, const CfTensor* block_tables,
                         const CfTensor* scale, CfTensor* out, void* stream);
 
+/* ---- Rotary positions ------------------------------------------------------
+ * No kernel in the reference rotates (its models are traced with their own
+ * rotary arithmetic, ahead of its cache intercept).  Channel pair j of a row
+ * turns by the angle pos[a][t] * inv_freq[j], a being the pair's axis:
+ *   (x1, x2) -> rotary_scale * (x1 cos - x2 sin, x2 cos + x1 sin).
+ * The pair is channels (j, j + pairs), or (2j, 2j + 1) with
+ * CF_ROTARY_ADJACENT; channels from 2 * pairs on pass unchanged.  With several
+ * axes (time, height, width of images and video) the first sections[0] pairs
+ * follow axis 0, the next sections[1] axis 1 and so on, or with
+ * CF_ROTARY_CYCLED pair j follows axis a = j % axes while j < axes *
+ * sections[a], and axis 0 after that; the sections sum to the pairs.  Angles
+ * are exact to about 1e-7 of a turn for any position; results are computed in
+ * float32 and rounded once. */
+#define CF_ROTARY_MAX_AXES 4
+enum {
+    CF_ROTARY_CYCLED = 1,
+    CF_ROTARY_ADJACENT = 2,
+};
+
+/* out[t, h] = x[t, h] rotated.  out may be x itself.
+ *   x, out     [T, H, D]            f32 | f16 | bf16, one dtype, any strides
+ *   positions  [T] or [axes, T]     i32 | i64
+ *   inv_freq   [pairs]              f32, 2 * pairs <= D
+ *   sections   axes host values, or NULL with one axis; axes 1..4
+ *   flags      CF_ROTARY_* */
+int32_t cf_rotary(const CfTensor* x, const CfTensor* positions, const CfTensor* inv_freq, const int32_t* sections,
+                  int32_t axes, int32_t flags, float rotary_scale, CfTensor* out, void* stream);
+
+/* A step's new rows: q_out = q rotated, k_new rotated and v_new as it is into
+ * the paged caches (cf_paged_write's placement: slots outside the cache are
+ * skipped, slots must be distinct, and the blocks the sequence's own), in one
+ * launch.  Codes of e4m3fn caches are e4m3fn(rotated float32 value / scale[h]).
+ *   q, q_out      [T, Hq, D]        f32 | f16 | bf16, one dtype; q_out may be q
+ *   k_new, v_new  [T, Hkv, D]       q's dtype
+ *   slot_mapping  [T]               i32 | i64: block * bs + offset
+ *   k_cache, v_cache  [NB, bs, Hkv, D]  f32 | f16 | bf16 | e4m3fn, one dtype, any strides
+ *   k_scale, v_scale  [Hkv] or [1] f32 for e4m3fn caches, NULL otherwise
+ * The rest as cf_rotary. */
+int32_t cf_rotary_cache_write(const CfTensor* q, const CfTensor* k_new, const CfTensor* v_new,
+                              const CfTensor* positions, const CfTensor* inv_freq, const int32_t* sections,
+                              int32_t axes, int32_t flags, float rotary_scale, const CfTensor* slot_mapping,
+                              CfTensor* k_cache, CfTensor* v_cache, const CfTensor* k_scale, const CfTensor* v_scale,
+                              CfTensor* q_out, void* stream);
+
 /* ---- Eviction by accumulated attention weight -----------------------------
  * No counterpart in the reference.  A sequence's account holds, per KV head
  * (or once for all heads), the attention weight that each cached token has

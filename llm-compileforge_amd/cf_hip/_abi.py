@@ -110,8 +110,12 @@ def descriptor(t: torch.Tensor) -> CfTensor:
         raise ValueError(f"cf_hip descriptors have rank 1..4, got a rank-{rank} tensor")
     esize = t.element_size()
     off = t.storage_offset()
-    # The storage base plus the element offset, like a memref descriptor.
-    base = t.data_ptr() - off * esize
+    # The storage base plus the element offset, like a memref descriptor (an
+    # empty view has no address, whatever its offset).
+    ptr = t.data_ptr()
+    if ptr == 0:
+        off = 0
+    base = ptr - off * esize
     return CfTensor.from_buffer_copy(_PACK[rank].pack(
         SFA_ROCM if t.is_cuda else SFA_CPU, rank, esize, base, base, off, *t.shape, *t.stride(),
         dtype_code(t.dtype), 0))
@@ -172,6 +176,15 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "cf_kv_write_fp8": (ctypes.c_int32, [_P, _P, _P, _P, _P, _P, _P, ctypes.c_void_p]),
     "cf_paged_write": (ctypes.c_int32, [_P, _P, _P, _P, ctypes.c_void_p]),
     "cf_paged_gather": (ctypes.c_int32, [_P, _P, _P, _P, ctypes.c_void_p]),
+    "cf_rotary": (
+        ctypes.c_int32,
+        [_P, _P, _P, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_float, _P, ctypes.c_void_p],
+    ),
+    "cf_rotary_cache_write": (
+        ctypes.c_int32,
+        [_P, _P, _P, _P, _P, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_float, _P, _P, _P, _P, _P, _P,
+         ctypes.c_void_p],
+    ),
     "cf_evict_select": (ctypes.c_int32, [_P, _P, _P, _P, _P, ctypes.c_int32, ctypes.c_int32, _P, _P, ctypes.c_void_p]),
     "cf_evict_move": (ctypes.c_int32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_void_p]),
     "cf_bp_create": (ctypes.c_int32, [ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_void_p)]),

@@ -599,6 +599,92 @@ def _int32(name: str, value: int) -> int:
     return value
 
 
+ROTARY_MAX_AXES = 4  # CF_ROTARY_MAX_AXES
+_AXIS_ORDERS = {"blocks": 0, "cycled": 1}  # CF_ROTARY_CYCLED
+
+
+def _rotary_axes(positions: torch.Tensor, sections, axis_order: str, interleaved: bool) -> tuple:
+    """(axes, sections array or None, flags) of a rotary call."""
+    if axis_order not in _AXIS_ORDERS:
+        raise ValueError(f"axis_order must be 'blocks' or 'cycled', got {axis_order!r}")
+    axes = positions.shape[0] if positions.dim() == 2 else 1
+    flags = _AXIS_ORDERS[axis_order] | (2 if interleaved else 0)  # CF_ROTARY_ADJACENT
+    if sections is None:
+        return axes, None, flags
+    if len(sections) != axes:
+        raise ValueError(f"{len(sections)} sections for {axes} rows of positions")
+    if axes > ROTARY_MAX_AXES:
+        raise ValueError(f"{axes} axes, at most {ROTARY_MAX_AXES} are supported")
+    return axes, (ctypes.c_int32 * axes)(*(_int32("section", int(n)) for n in sections)), flags
+
+
+def rotary(
+    x: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    sections=None,
+    axis_order: str = "blocks",
+    interleaved: bool = False,
+    rotary_scale: float = 1.0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """x [T, H, D] with its channel pairs turned by positions [T] or [axes, T]
+    (int32 or int64) times inv_freq [pairs] (float32); see cf_hip.h."""
+    given = [("x", x), ("positions", positions), ("inv_freq", inv_freq)] + ([("out", out)] if out is not None else [])
+    for name, t in given:
+        _require_device(name, t)
+    dev = _same_device(*(t for _, t in given))
+    axes, arr, flags = _rotary_axes(positions, sections, axis_order, interleaved)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dx, dp, df, do = descriptor(x), descriptor(positions), descriptor(inv_freq), descriptor(out)
+    with _on(dev):
+        rc = lib().cf_rotary(ref(dx), ref(dp), ref(df), arr, axes, flags, float(rotary_scale), ref(do),
+                             stream_handle(dev))
+    check(rc, "cf_rotary")
+    return out
+
+
+def rotary_cache_write(
+    q: torch.Tensor,
+    k_new: torch.Tensor,
+    v_new: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    sections=None,
+    axis_order: str = "blocks",
+    interleaved: bool = False,
+    rotary_scale: float = 1.0,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Rotates q [T, Hq, D] (returned) and k_new [T, Hkv, D], and writes the
+    rotated keys and v_new to the paged caches at slot_mapping [T], in one
+    launch.  Slots outside the cache are skipped; slots must be distinct."""
+    given = [("q", q), ("k_new", k_new), ("v_new", v_new), ("positions", positions), ("inv_freq", inv_freq),
+             ("slot_mapping", slot_mapping), ("k_cache", k_cache), ("v_cache", v_cache)]
+    given += [(n, t) for n, t in (("k_scale", k_scale), ("v_scale", v_scale), ("out", out)) if t is not None]
+    for name, t in given:
+        _require_device(name, t)
+    dev = _same_device(*(t for _, t in given))
+    axes, arr, flags = _rotary_axes(positions, sections, axis_order, interleaved)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    d = [descriptor(t) for t in (q, k_new, v_new, positions, inv_freq)]
+    ds, dk, dv, do = descriptor(slot_mapping), descriptor(k_cache), descriptor(v_cache), descriptor(out)
+    dks = descriptor(k_scale.reshape(-1)) if k_scale is not None else None
+    dvs = descriptor(v_scale.reshape(-1)) if v_scale is not None else None
+    with _on(dev):
+        rc = lib().cf_rotary_cache_write(*(ref(x) for x in d), arr, axes, flags, float(rotary_scale), ref(ds), ref(dk),
+                                         ref(dv), ref(dks), ref(dvs), ref(do), stream_handle(dev))
+    check(rc, "cf_rotary_cache_write")
+    return out
+
+
 def evict_select(
     weights: torch.Tensor,
     seq_lens: torch.Tensor,
@@ -833,6 +919,7 @@ class KernelTimer:
 __all__ = [
     "DEFAULT_PARTITION_TOKENS",
     "NOALLOC_SCRATCH_BYTES",
+    "ROTARY_MAX_AXES",
     "DecodePlan",
     "KernelTimer",
     "block_span_view",
@@ -856,6 +943,8 @@ __all__ = [
     "paged_decode_noalloc",
     "paged_gather",
     "paged_write",
+    "rotary",
+    "rotary_cache_write",
     "shared_prefix_lens",
     "stage_from_host",
     "stage_tables",

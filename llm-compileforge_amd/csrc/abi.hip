@@ -16,6 +16,7 @@
 #include "kv_fp8.hpp"
 #include "paged_io.hpp"
 #include "prefill_params.hpp"
+#include "rotary.hpp"
 
 namespace cf {
 
@@ -220,6 +221,58 @@ int32_t position_views(const CfTensor* positions, const CfTensor* kept, const Cf
              (long long)like.size[i]);
   if ((rc = row_view(kept, "kept", like.size[0], kp, ks))) return rc;
   return row_view(seen, "seen", like.size[0], sp, ss);
+}
+
+// Positions, frequencies and axes of a rotary call over rows [T, H, D].
+int32_t rotary_views(const CfTensor* positions, const CfTensor* inv_freq, const int32_t* sections, int32_t axes,
+                     int32_t flags, float rotary_scale, RotaryParams* p) {
+  View vp, vf;
+  int32_t rc;
+  CF_CHECK(positions != nullptr, "positions: descriptor is NULL");
+  CF_CHECK(positions->t.rank == 1 || positions->t.rank == 2, "positions: expected rank 1 or 2, got %d",
+           positions->t.rank);
+  if ((rc = view_of(positions, "positions", positions->t.rank, &vp))) return rc;
+  if ((rc = view_of(inv_freq, "inv_freq", 1, &vf))) return rc;
+  CF_CHECK(vp.dtype == CF_I32 || vp.dtype == CF_I64, "positions: expected i32 or i64, got %s", dtype_name(vp.dtype));
+  CF_CHECK(vf.dtype == CF_F32, "inv_freq: expected f32, got %s", dtype_name(vf.dtype));
+  CF_CHECK(axes >= 1 && axes <= kMaxRotaryAxes, "axes (%d) must be 1..%d", axes, kMaxRotaryAxes);
+  CF_CHECK((flags & ~(CF_ROTARY_CYCLED | CF_ROTARY_ADJACENT)) == 0, "unknown flags %d", flags);
+  CF_CHECK(std::isfinite(rotary_scale), "rotary_scale must be finite");
+  CF_CHECK(vp.rank == 2 ? vp.size[0] == axes : axes == 1, "positions: expected [%d, T]", axes);
+  CF_CHECK(vp.size[vp.rank - 1] == p->T, "positions: %lld rows, expected %lld", (long long)vp.size[vp.rank - 1],
+           (long long)p->T);
+  CF_CHECK(2 * vf.size[0] <= p->D, "inv_freq: %lld pairs do not fit head_dim %d", (long long)vf.size[0], p->D);
+  p->pairs = (int)vf.size[0];
+  CF_CHECK(sections != nullptr || axes == 1, "sections are needed with several axes");
+  int64_t sum = 0;
+  for (int a = 0; a < axes; ++a) {
+    p->section[a] = sections != nullptr ? sections[a] : p->pairs;
+    CF_CHECK(p->section[a] >= 0, "sections must not be negative");
+    sum += p->section[a];
+  }
+  CF_CHECK(sum == p->pairs, "sections sum to %lld, inv_freq has %d pairs", (long long)sum, p->pairs);
+  p->cycled = (flags & CF_ROTARY_CYCLED) != 0;
+  if (p->cycled)
+    for (int a = 1; a < axes; ++a)
+      CF_CHECK(p->section[a] == 0 || a + axes * (p->section[a] - 1) < p->pairs,
+               "sections: axis %d has more pairs than its turns in the cycle", a);
+  p->adjacent = (flags & CF_ROTARY_ADJACENT) != 0;
+  p->axes = axes;
+  p->positions = vp.base;
+  p->pos64 = vp.dtype == CF_I64;
+  p->p_sa = vp.rank == 2 ? vp.stride[0] : 0;
+  p->p_st = vp.stride[vp.rank - 1];
+  p->inv_freq = (const float*)vf.base;
+  p->f_s = vf.stride[0];
+  p->rotary_scale = rotary_scale;
+  return CF_OK;
+}
+
+// Rows a kernel writes: no two of its elements may be the same.
+int32_t check_apart(const View& v, const char* name) {
+  for (int i = 0; i < v.rank; ++i)
+    CF_CHECK(v.size[i] <= 1 || v.stride[i] != 0, "%s: rows overlap (stride 0 on dim %d)", name, i);
+  return CF_OK;
 }
 
 int32_t view_of_34(const CfTensor* t, const char* name, View* v) {
@@ -924,6 +977,106 @@ int32_t cf_paged_gather(const CfTensor* cache, const CfTensor* block_tables, con
   p.D = (int)vc.size[3];
   p.bs = (int)vc.size[1];
   return launch_paged_gather(p, vc.dtype, vo.dtype, as_stream(stream));
+}
+
+int32_t cf_rotary(const CfTensor* x, const CfTensor* positions, const CfTensor* inv_freq, const int32_t* sections,
+                  int32_t axes, int32_t flags, float rotary_scale, CfTensor* out, void* stream) {
+  View vx, vo;
+  int32_t rc;
+  if ((rc = view_of(x, "x", 3, &vx))) return rc;
+  if ((rc = view_of(out, "out", 3, &vo))) return rc;
+  CF_CHECK(is_float_dtype(vx.dtype), "x: dtype must be f32, f16 or bf16, got %s", dtype_name(vx.dtype));
+  CF_CHECK(vo.dtype == vx.dtype, "out dtype %s differs from x dtype %s", dtype_name(vo.dtype), dtype_name(vx.dtype));
+  for (int i = 0; i < 3; ++i) CF_CHECK(vo.size[i] == vx.size[i], "out shape differs from x on dim %d", i);
+  if ((rc = check_apart(vo, "out"))) return rc;
+  CF_CHECK(vx.size[1] < 65536 && vx.size[2] <= 4096, "x: heads or head_dim too large");
+  RotaryParams p{};
+  p.T = vx.size[0];
+  p.Hq = (int)vx.size[1];
+  p.D = (int)vx.size[2];
+  if ((rc = rotary_views(positions, inv_freq, sections, axes, flags, rotary_scale, &p))) return rc;
+  if (p.Hq == 0) return CF_OK;
+  p.x[0] = vx.base;
+  p.out = vo.base;
+  for (int i = 0; i < 3; ++i) {
+    p.x_s[0][i] = vx.stride[i];
+    p.o_s[i] = vo.stride[i];
+  }
+  return launch_rotary(p, vx.dtype, vx.dtype, as_stream(stream));
+}
+
+int32_t cf_rotary_cache_write(const CfTensor* q, const CfTensor* k_new, const CfTensor* v_new,
+                              const CfTensor* positions, const CfTensor* inv_freq, const int32_t* sections,
+                              int32_t axes, int32_t flags, float rotary_scale, const CfTensor* slot_mapping,
+                              CfTensor* k_cache, CfTensor* v_cache, const CfTensor* k_scale, const CfTensor* v_scale,
+                              CfTensor* q_out, void* stream) {
+  View vx[3], vo, vsl, vc[2];
+  int32_t rc;
+  const CfTensor* in[3] = {q, k_new, v_new};
+  const char* names[3] = {"q", "k_new", "v_new"};
+  for (int i = 0; i < 3; ++i) {
+    if ((rc = view_of(in[i], names[i], 3, &vx[i]))) return rc;
+    CF_CHECK(is_float_dtype(vx[i].dtype), "%s: dtype must be f32, f16 or bf16, got %s", names[i],
+             dtype_name(vx[i].dtype));
+    CF_CHECK(vx[i].dtype == vx[0].dtype, "%s dtype %s differs from q dtype %s", names[i], dtype_name(vx[i].dtype),
+             dtype_name(vx[0].dtype));
+    CF_CHECK(vx[i].size[0] == vx[0].size[0] && vx[i].size[2] == vx[0].size[2],
+             "%s must be [%lld, heads, %lld]", names[i], (long long)vx[0].size[0], (long long)vx[0].size[2]);
+  }
+  if ((rc = view_of(q_out, "q_out", 3, &vo))) return rc;
+  if ((rc = view_of(slot_mapping, "slot_mapping", 1, &vsl))) return rc;
+  if ((rc = view_of(k_cache, "k_cache", 4, &vc[0]))) return rc;
+  if ((rc = view_of(v_cache, "v_cache", 4, &vc[1]))) return rc;
+  CF_CHECK(vo.dtype == vx[0].dtype, "q_out dtype %s differs from q dtype %s", dtype_name(vo.dtype),
+           dtype_name(vx[0].dtype));
+  for (int i = 0; i < 3; ++i) CF_CHECK(vo.size[i] == vx[0].size[i], "q_out shape differs from q on dim %d", i);
+  if ((rc = check_apart(vo, "q_out"))) return rc;
+  const int64_t T = vx[0].size[0], Hkv = vx[1].size[1], D = vx[0].size[2];
+  CF_CHECK(vx[2].size[1] == Hkv, "v_new has %lld heads, k_new %lld", (long long)vx[2].size[1], (long long)Hkv);
+  CF_CHECK(vsl.dtype == CF_I32 || vsl.dtype == CF_I64, "slot_mapping: expected i32 or i64, got %s",
+           dtype_name(vsl.dtype));
+  CF_CHECK(vsl.size[0] == T, "slot_mapping has %lld entries, %lld rows given", (long long)vsl.size[0], (long long)T);
+  CF_CHECK(is_float_dtype(vc[0].dtype) || vc[0].dtype == CF_F8E4M3FN,
+           "k_cache: dtype must be f32, f16, bf16 or f8e4m3fn, got %s", dtype_name(vc[0].dtype));
+  CF_CHECK(vc[1].dtype == vc[0].dtype, "v_cache dtype %s differs from k_cache dtype %s", dtype_name(vc[1].dtype),
+           dtype_name(vc[0].dtype));
+  for (int i = 0; i < 4; ++i)
+    CF_CHECK(vc[1].size[i] == vc[0].size[i], "v_cache shape differs from k_cache shape on dim %d", i);
+  CF_CHECK(vc[0].size[2] == Hkv && vc[0].size[3] == D, "cache [NB, bs, %lld, %lld] does not match rows [T, %lld, %lld]",
+           (long long)vc[0].size[2], (long long)vc[0].size[3], (long long)Hkv, (long long)D);
+  CF_CHECK(vc[0].size[1] > 0, "cache block size must be positive");
+  CF_CHECK(vx[0].size[1] < 65536 && Hkv < 65536 && D <= 4096 && vc[0].size[1] < 65536, "dims too large");
+  RotaryParams p{};
+  p.T = T;
+  p.Hq = (int)vx[0].size[1];
+  p.Hkv = (int)Hkv;
+  p.D = (int)D;
+  if ((rc = rotary_views(positions, inv_freq, sections, axes, flags, rotary_scale, &p))) return rc;
+  const CfTensor* sc[2] = {k_scale, v_scale};
+  const char* sc_names[2] = {"k_scale", "v_scale"};
+  for (int i = 0; i < 2; ++i) {
+    if (vc[0].dtype == CF_F8E4M3FN) {
+      CF_CHECK(sc[i] != nullptr, "f8e4m3fn caches need %s", sc_names[i]);
+      if ((rc = scale_view(sc[i], sc_names[i], Hkv, &p.scale[i], &p.sc_s[i]))) return rc;
+    } else {
+      CF_CHECK(sc[i] == nullptr, "%s applies to f8e4m3fn caches only", sc_names[i]);
+    }
+    p.cache[i] = vc[i].base;
+    for (int d = 0; d < 4; ++d) p.c_s[i][d] = vc[i].stride[d];
+  }
+  for (int i = 0; i < 3; ++i) {
+    p.x[i] = vx[i].base;
+    for (int d = 0; d < 3; ++d) p.x_s[i][d] = vx[i].stride[d];
+    p.o_s[i] = vo.stride[i];
+  }
+  p.out = vo.base;
+  p.slots = vsl.base;
+  p.slot64 = vsl.dtype == CF_I64;
+  p.slot_s = vsl.stride[0];
+  p.NB = vc[0].size[0];
+  p.bs = (int)vc[0].size[1];
+  if (p.Hq == 0 && p.Hkv == 0) return CF_OK;
+  return launch_rotary(p, vx[0].dtype, vc[0].dtype, as_stream(stream));
 }
 
 int32_t cf_evict_select(const CfTensor* weights, const CfTensor* seq_lens, const CfTensor* positions,
