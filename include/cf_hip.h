@@ -186,6 +186,30 @@ int32_t cf_paged_decode_shared_noalloc(const CfTensor* q, const CfTensor* k_cach
                                        int32_t partition_tokens, CfTensor* out,
                                        void* stream);
 
+/* Workspace of cf_paged_decode_weights: cf_paged_decode's, and a float32 score
+ * for each query head and token that the block tables can hold (64 sequences
+ * of 32 heads and 8,192 tokens: 67 MB). */
+int32_t cf_paged_decode_weights_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+                                                int64_t head_dim, int64_t max_blocks_per_seq, int32_t block_size,
+                                                uint64_t* bytes_out);
+
+/* cf_paged_decode_shared (same arguments and outputs; shared_prefix_lens may
+ * be NULL) that also keeps each sequence's account of attention weight:
+ *   weights[b, hw, t] = (t newest ? 0 : decay * weights[b, hw, t])
+ *                       + sum over the query heads of hw of softmax weight t
+ * for the tokens t that sequence b attends to; other entries are left as they
+ * were.  The newest token, at seq_lens[b] - 1, has no history: what its entry
+ * held is not read, nor is any entry's with decay 0.
+ *   weights  [B, Hw, S]  f32, S stride 1, S >= Mb * bs; Hw = Hkv (an account a
+ *                        KV head), or 1 (one for all query heads)
+ * Tokens in blocks outside [0, NB) draw nothing.
+ * workspace: cf_paged_decode_weights_workspace_bytes() bytes, 256-byte aligned. */
+int32_t cf_paged_decode_weights(const CfTensor* q, const CfTensor* k_cache, const CfTensor* v_cache,
+                                const CfTensor* block_tables, const CfTensor* seq_lens,
+                                const CfTensor* shared_prefix_lens, const CfTensor* k_scale, const CfTensor* v_scale,
+                                float scale, int32_t block_size, CfTensor* weights, float decay, CfTensor* out,
+                                void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* Workspace with which cf_prefill_chunk_fp8 runs num_q_tokens query rows in
  * num_chunks chunks best (on the current device): small records that grow with
  * the chunks and the query blocks, not with the cached context, and, for calls

@@ -250,6 +250,64 @@ def paged_decode_noalloc(
     return out
 
 
+def decode_weights_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                                   max_blocks_per_seq: int, block_size: int) -> int:
+    out = ctypes.c_uint64(0)
+    rc = lib().cf_paged_decode_weights_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, max_blocks_per_seq,
+                                                       block_size, ctypes.byref(out))
+    check(rc, "cf_paged_decode_weights_workspace_bytes")
+    return int(out.value)
+
+
+def paged_decode_weights(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    weights: torch.Tensor,
+    scale: float,
+    block_size: int,
+    decay: float = 1.0,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    shared_prefix_lens: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """paged_decode that also adds each token's attention weight to weights
+    [B, Hkv or 1, S] (float32, S >= the tables' tokens), in place: decay times
+    what the entry held (nothing for the newest token) plus the weights of its
+    query heads.  workspace: decode_weights_workspace_bytes() bytes, by default
+    a cached one per (device, stream)."""
+    given = [("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables),
+             ("seq_lens", seq_lens), ("weights", weights)]
+    given += [(n, t) for n, t in (("k_scale", k_scale), ("v_scale", v_scale), ("out", out), ("workspace", workspace),
+                                  ("shared_prefix_lens", shared_prefix_lens)) if t is not None]
+    for name, t in given:
+        _require_device(name, t)
+    dev = _same_device(*(t for _, t in given))
+    if q.dim() != 3 or k_cache.dim() != 4 or block_tables.dim() != 2:
+        raise ValueError(f"q must be [B, Hq, D], caches [NB, bs, Hkv, D], block_tables [B, Mb]; got {tuple(q.shape)}, "
+                         f"{tuple(k_cache.shape)}, {tuple(block_tables.shape)}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    need = decode_weights_workspace_bytes(q.shape[0], q.shape[1], k_cache.shape[2], q.shape[2], block_tables.shape[1],
+                                          block_size)
+    if workspace is None:
+        workspace = _cached_workspace(need, dev)
+    elif workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"workspace of {need} bytes needed, {workspace.numel() * workspace.element_size()} given")
+    d = [descriptor(t) if t is not None else None
+         for t in (q, k_cache, v_cache, block_tables, seq_lens, shared_prefix_lens, k_scale, v_scale)]
+    dw, do = descriptor(weights), descriptor(out)
+    with _on(dev):
+        rc = lib().cf_paged_decode_weights(*(ref(x) for x in d), float(scale), int(block_size), ref(dw), float(decay),
+                                           ref(do), workspace.data_ptr(), need, stream_handle(dev))
+    check(rc, "cf_paged_decode_weights")
+    return out
+
+
 def prefill_workspace_bytes(num_q_tokens: int, num_chunks: int, num_q_heads: int, num_kv_heads: int,
                             head_dim: int, block_size: int = 16) -> int:
     out = ctypes.c_uint64(0)
@@ -925,6 +983,7 @@ __all__ = [
     "block_span_view",
     "block_tables_apply",
     "copy_blocks",
+    "decode_weights_workspace_bytes",
     "decode_workspace_bytes",
     "evict_move",
     "evict_select",
@@ -941,6 +1000,7 @@ __all__ = [
     "kv_write_fp8",
     "paged_decode",
     "paged_decode_noalloc",
+    "paged_decode_weights",
     "paged_gather",
     "paged_write",
     "rotary",

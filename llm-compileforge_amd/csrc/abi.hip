@@ -430,12 +430,17 @@ int32_t cf_paged_decode(const CfTensor* q, const CfTensor* k_cache, const CfTens
                                 block_size, partition_tokens, out, workspace, workspace_bytes, stream);
 }
 
-int32_t cf_paged_decode_shared(const CfTensor* q, const CfTensor* k_cache, const CfTensor* v_cache,
-                               const CfTensor* block_tables, const CfTensor* seq_lens,
-                               const CfTensor* shared_prefix_lens, const CfTensor* k_scale,
-                               const CfTensor* v_scale, float scale, int32_t block_size,
-                               int32_t partition_tokens, CfTensor* out, void* workspace,
-                               uint64_t workspace_bytes, void* stream) {
+// The score rows and final (m, l) of a decode call with accounts, behind its
+// plain workspace: [plain, padded] [(m, l) per row, padded] [scores].
+static int64_t score_row(int64_t max_blocks, int64_t bs) { return (max_blocks * bs + 31) & ~(int64_t)31; }
+static uint64_t pad256(uint64_t x) { return (x + 255) & ~(uint64_t)255; }
+
+// A decode call; with `weights`, one whose sequences' accounts are kept.
+static int32_t decode_call(const CfTensor* q, const CfTensor* k_cache, const CfTensor* v_cache,
+                           const CfTensor* block_tables, const CfTensor* seq_lens,
+                           const CfTensor* shared_prefix_lens, const CfTensor* k_scale, const CfTensor* v_scale,
+                           float scale, int32_t block_size, int32_t partition_tokens, CfTensor* weights, float decay,
+                           CfTensor* out, void* workspace, uint64_t workspace_bytes, void* stream) {
   View vq, vk, vv, vt, vs, vo;
   int32_t rc;
   if ((rc = view_of(q, "q", 3, &vq))) return rc;
@@ -479,7 +484,7 @@ int32_t cf_paged_decode_shared(const CfTensor* q, const CfTensor* k_cache, const
   CF_CHECK(vt.size[1] * (int64_t)bs < (int64_t)INT32_MAX, "block table capacity overflows int32");
   CF_CHECK(std::isfinite(scale), "scale must be finite");
 
-  DecodeParams p{};
+  DecodeWeightsParams p{};
   p.q = vq.base;
   p.q_sb = vq.stride[0];
   p.q_sh = vq.stride[1];
@@ -525,8 +530,36 @@ int32_t cf_paged_decode_shared(const CfTensor* q, const CfTensor* k_cache, const
   } else {
     CF_CHECK(k_scale == nullptr && v_scale == nullptr, "k_scale/v_scale apply to f8e4m3fn caches only");
   }
+  if (weights != nullptr) {
+    View vw;
+    if ((rc = account_view(weights, "weights", CF_F32, &vw))) return rc;
+    CF_CHECK(vw.size[0] == B && (vw.size[1] == Hkv || vw.size[1] == 1),
+             "weights must be [%lld, %lld or 1, S] (one account a KV head, or one for all)", (long long)B,
+             (long long)Hkv);
+    CF_CHECK(vw.size[2] >= vt.size[1] * (int64_t)bs, "weights has %lld slots, the block tables hold %lld tokens",
+             (long long)vw.size[2], (long long)(vt.size[1] * (int64_t)bs));
+    CF_CHECK(std::isfinite(decay), "decay must be finite");
+    p.weights = (float*)vw.base;
+    p.w_sb = vw.stride[0];
+    p.w_sh = vw.stride[1];
+    p.Hw = (int)vw.size[1];
+    p.decay = decay;
+    uint64_t total = 0;
+    if ((rc = cf_paged_decode_weights_workspace_bytes(B, Hq, Hkv, D, vt.size[1], block_size, &total))) return rc;
+    if (workspace == nullptr || workspace_bytes < total) {
+      set_error("workspace of %llu bytes needed, %llu given", (unsigned long long)total,
+                (unsigned long long)workspace_bytes);
+      return CF_ERR_WORKSPACE;
+    }
+    CF_CHECK(((uintptr_t)workspace & 255) == 0, "workspace must be 256-byte aligned");
+    p.s_cap = score_row(vt.size[1], bs);
+    p.ws_s = (float*)((char*)workspace + (total - (uint64_t)B * Hq * p.s_cap * 4));
+    p.ws_fin = (float*)((char*)p.ws_s - pad256((uint64_t)B * Hq * 8));
+    workspace_bytes = (uint64_t)((char*)p.ws_fin - (char*)workspace);
+  }
   if (B == 0) return CF_OK;
 
+  const DecodeParams& plain = p;
   bool mfma = decode_mfma_supported(p, vq.dtype, vk.dtype);
   // fp32 caches also run on the generic kernel.  It takes the calls that it is
   // faster for, those that ask for a partition length of their own (the MFMA
@@ -557,11 +590,60 @@ int32_t cf_paged_decode_shared(const CfTensor* q, const CfTensor* k_cache, const
   }
 
   hipStream_t st = as_stream(stream);
-  if (mfma) return launch_decode_mfma(p, vq.dtype, vk.dtype, st);
-  rc = launch_decode_generic(p, vq.dtype, vk.dtype, st);
+  if (weights == nullptr) {
+    if (mfma) return launch_decode_mfma(plain, vq.dtype, vk.dtype, st);
+    rc = launch_decode_generic(plain, vq.dtype, vk.dtype, st);
+    if (rc) return rc;
+    if (p.max_parts > 1) rc = launch_decode_reduce(plain, vq.dtype, st);
+    return rc;
+  }
+  if (mfma) {
+    if ((rc = launch_decode_mfma(p, vq.dtype, vk.dtype, st))) return rc;
+  } else {
+    if ((rc = launch_decode_generic(p, vq.dtype, vk.dtype, st))) return rc;
+    if (p.max_parts > 1 && (rc = launch_decode_reduce(p, vq.dtype, st))) return rc;
+  }
+  return launch_decode_weights(p, mfma, st);
+}
+
+int32_t cf_paged_decode_shared(const CfTensor* q, const CfTensor* k_cache, const CfTensor* v_cache,
+                               const CfTensor* block_tables, const CfTensor* seq_lens,
+                               const CfTensor* shared_prefix_lens, const CfTensor* k_scale,
+                               const CfTensor* v_scale, float scale, int32_t block_size,
+                               int32_t partition_tokens, CfTensor* out, void* workspace,
+                               uint64_t workspace_bytes, void* stream) {
+  return decode_call(q, k_cache, v_cache, block_tables, seq_lens, shared_prefix_lens, k_scale, v_scale, scale,
+                     block_size, partition_tokens, nullptr, 1.0f, out, workspace, workspace_bytes, stream);
+}
+
+// The default partition length, as a whole number of blocks.
+static int32_t default_partition(int32_t bs) {
+  return bs >= CF_DEFAULT_PARTITION_TOKENS ? bs : CF_DEFAULT_PARTITION_TOKENS / bs * bs;
+}
+
+int32_t cf_paged_decode_weights_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+                                                int64_t head_dim, int64_t max_blocks_per_seq, int32_t block_size,
+                                                uint64_t* bytes_out) {
+  CF_CHECK(block_size > 0, "block_size must be positive");
+  uint64_t plain = 0;
+  const int32_t rc = cf_paged_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, max_blocks_per_seq,
+                                                     block_size, default_partition(block_size), &plain);
   if (rc) return rc;
-  if (p.max_parts > 1) rc = launch_decode_reduce(p, vq.dtype, st);
-  return rc;
+  *bytes_out = pad256(plain) + pad256((uint64_t)batch * num_q_heads * 8) +
+               (uint64_t)batch * num_q_heads * score_row(max_blocks_per_seq, block_size) * 4;
+  return CF_OK;
+}
+
+int32_t cf_paged_decode_weights(const CfTensor* q, const CfTensor* k_cache, const CfTensor* v_cache,
+                                const CfTensor* block_tables, const CfTensor* seq_lens,
+                                const CfTensor* shared_prefix_lens, const CfTensor* k_scale, const CfTensor* v_scale,
+                                float scale, int32_t block_size, CfTensor* weights, float decay, CfTensor* out,
+                                void* workspace, uint64_t workspace_bytes, void* stream) {
+  CF_CHECK(weights != nullptr, "weights: descriptor is NULL");
+  CF_CHECK(block_size > 0, "block_size must be positive");
+  return decode_call(q, k_cache, v_cache, block_tables, seq_lens, shared_prefix_lens, k_scale, v_scale, scale,
+                     block_size, default_partition(block_size), weights, decay, out, workspace, workspace_bytes,
+                     stream);
 }
 
 int32_t cf_paged_decode_shared_noalloc(const CfTensor* q, const CfTensor* k_cache, const CfTensor* v_cache,

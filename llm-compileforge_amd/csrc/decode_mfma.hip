@@ -82,6 +82,10 @@ constexpr int kMinShareTiles = 2;  // shortest shared prefix (32-token tiles) gi
 constexpr int kSlotCols = 16;      // columns of one partial slot (the MFMA width)
 constexpr int kOwn = 0, kPrefix = 1;
 
+// P: DecodeParams, or DecodeWeightsParams for a call that also keeps its scores.
+template <class P>
+constexpr bool kKeeps = std::is_same<P, DecodeWeightsParams>::value;
+
 // Read-only inputs the tile walk indexes with wave-uniform addresses.  Passed
 // as separate __restrict__ kernel arguments so the compiler may read them
 // through the scalar cache (s_load, counted by lgkmcnt) instead of vector
@@ -465,8 +469,8 @@ __device__ __forceinline__ float o_elem(const f32x4_t* o, int t, int e) {
 // Writes out a finished run (normalized output, record or wave-slot
 // partial) and, from the wave holding the run's first tile, the merge
 // descriptors of the sequences it covers.
-template <int QT, bool PL, int D, bool QUAD = false>
-__device__ __forceinline__ void flush_run(const DecodeParams& p, const Index& ix, const Plan* pl, const Coord& c,
+template <int QT, bool PL, int D, bool QUAD = false, class P>
+__device__ __forceinline__ void flush_run(const P& p, const Index& ix, const Plan* pl, const Coord& c,
                                           const f32x4_t* o, float m, float l, int run_j0, bool first_run,
                                           int64_t chunk, int w, int lane) {
   constexpr int pad = PL ? kRunPad : 0;
@@ -507,6 +511,13 @@ __device__ __forceinline__ void flush_run(const DecodeParams& p, const Index& ix
     }
   }
   if (li >= c.ncols) return;
+  if constexpr (kKeeps<P>) {
+    if (direct && lq == 0) {
+      float* fin = p.ws_fin + ((int64_t)c.b * p.Hq + c.h * G + li) * 2;
+      fin[0] = m;
+      fin[1] = lt;
+    }
+  }
   if (direct && QT == kF32) {
     // one rounding per output: divide, rather than multiply by 1 / l
     const int64_t orow = (int64_t)c.b * p.o_sb + (int64_t)(c.h * G + li) * p.o_sh;
@@ -567,6 +578,15 @@ __device__ __forceinline__ int stream_wave(int w, int Wtot, int Hkv) {
   return (lw % Hkv) * (Wtot / Hkv) + k;
 }
 
+// Keeps four scores of column li, tokens `at` .. + 3 of the sequence that the
+// column belongs to.
+template <class P>
+__device__ __forceinline__ void keep_scores(const P& p, const Coord& c, int li, int at, float4 s) {
+  if (li >= c.ncols) return;
+  const int m = li / p.G, g = li - m * p.G;
+  *(float4*)(p.ws_s + ((int64_t)(c.b + m) * p.Hq + c.h * p.G + g) * p.s_cap + at) = s;
+}
+
 // A wave's tiles of an fp32 cache under fp32 queries: as the loop of
 // decode_stream_kernel, on v_mfma_f32_16x16x4_f32.  A tile is 2 x 16 KiB at
 // head_dim 128 (128 VGPRs), so it is not double-buffered: the next tile's K
@@ -576,8 +596,8 @@ __device__ __forceinline__ int stream_wave(int w, int Wtot, int Hkv) {
 // 6 TB/s over 1024 waves: bound by HBM.  16 sequences of 256-2,048 tokens
 // (147 MB, 32 query / 8 KV heads of 128): 102 us on the generic kernel (VALU,
 // 4 bytes a load), 39 us here.
-template <int D, bool PL, bool VTOK>
-__device__ __forceinline__ void stream_f32(const DecodeParams& p, const Index& ix, const Seqs<PL>& seqs,
+template <int D, bool PL, bool VTOK, class P>
+__device__ __forceinline__ void stream_f32(const P& p, const Index& ix, const Seqs<PL>& seqs,
                                            const Plan* pl, const KvCacheView& kv, Coord c0, Coord c1, bool has1,
                                            int64_t v_end, int64_t chunk, int w, int lane) {
   constexpr int NC = D / 16, NV = D / 16;
@@ -677,6 +697,12 @@ __device__ __forceinline__ void stream_f32(const DecodeParams& p, const Index& i
         }
       }
     }
+    if constexpr (kKeeps<P>) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        keep_scores(p, c0, li, 32 * c0.j + 16 * x + 4 * lq,
+                    make_float4(sc[4 * x], sc[4 * x + 1], sc[4 * x + 2], sc[4 * x + 3]));
+    }
     float mt = sc[0];
 #pragma unroll
     for (int v = 1; v < 8; ++v) mt = fmaxf(mt, sc[v]);
@@ -751,8 +777,8 @@ __device__ __forceinline__ void stream_f32(const DecodeParams& p, const Index& i
   }
 }
 
-template <int QT, int KT, int D, bool PL, bool VTOK>
-__global__ __launch_bounds__(256) void decode_stream_kernel(DecodeParams p, const int32_t* __restrict__ tables,
+template <int QT, int KT, int D, bool PL, bool VTOK, class P>
+__global__ __launch_bounds__(256) void decode_stream_kernel(P p, const int32_t* __restrict__ tables,
                                                             const int32_t* __restrict__ lens,
                                                             const float* __restrict__ kscale,
                                                             const float* __restrict__ vscale,
@@ -943,6 +969,12 @@ __global__ __launch_bounds__(256) void decode_stream_kernel(DecodeParams p, cons
 #pragma unroll
       for (int t = 0; t < NV; ++t) vraw[t] = mask_tokens(vraw[t], nvalid);
     }
+    if constexpr (kKeeps<P>) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        keep_scores(p, c0, li, 32 * c0.j + 8 * lq + 4 * x,
+                    make_float4(sc[4 * x], sc[4 * x + 1], sc[4 * x + 2], sc[4 * x + 3]));
+    }
     float mt = sc[0];
 #pragma unroll
     for (int v = 1; v < 8; ++v) mt = fmaxf(mt, sc[v]);
@@ -1081,8 +1113,8 @@ __device__ __forceinline__ float merge_weight(float m, float M) {
 // grids); one wave of the first does the work when the partials fit its
 // registers, all four waves of each otherwise.  Partial rows hold the G
 // heads of h in consecutive rows.
-template <int QT, int D, int G, int NSL>
-__global__ __launch_bounds__(256) void decode_merge_kernel(DecodeParams p) {
+template <int QT, int D, int G, int NSL, class P>
+__global__ __launch_bounds__(256) void decode_merge_kernel(P p) {
   constexpr int E = G * D / 64;  // output elements per lane
   constexpr int kWaves = 4;
   const int h = blockIdx.x, b = blockIdx.y;
@@ -1130,6 +1162,16 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(DecodeParams p) {
           const float w = merge_weight(mk[k][g], Mg[g]);
           mk[k][g] = w;  // now the weight
           Lg[g] += w * lk[k][g];
+        }
+      }
+    }
+    if constexpr (kKeeps<P>) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        if (lane == g) {
+          float* fin = p.ws_fin + ((int64_t)b * p.Hq + h * G + g) * 2;
+          fin[0] = Mg[g];
+          fin[1] = Lg[g];
         }
       }
     }
@@ -1262,6 +1304,13 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(DecodeParams p) {
     }
     __syncthreads();  // the next chunk restages sm, sl, srow
   }
+  if constexpr (kKeeps<P>) {
+    if (blockIdx.z == 0 && tid < G) {
+      float* fin = p.ws_fin + ((int64_t)b * p.Hq + h * G + tid) * 2;
+      fin[0] = run_m[tid];
+      fin[1] = run_l[tid];
+    }
+  }
   if constexpr (NP > 1) {
     if (ph > 0) red[ph - 1][fs[0] % NF4] = acc[0];
     __syncthreads();
@@ -1313,12 +1362,12 @@ constexpr size_t stream_lds_bytes() {
   return (PL ? kPlanLdsBytes : 0) + (VTOK && KT != kF32 ? 4 * (size_t)vtok_stage_bytes<D, KvTraits<KT>::kBytes>() : 0);
 }
 
-template <int QT, int KT, int D, bool PL, bool VTOK>
+template <int QT, int KT, int D, bool PL, bool VTOK, class P>
 int blocks_per_cu() {
   static int cached = 0;
   if (cached == 0) {
     int n = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_stream_kernel<QT, KT, D, PL, VTOK>, 256,
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_stream_kernel<QT, KT, D, PL, VTOK, P>, 256,
                                                      stream_lds_bytes<KT, D, PL, VTOK>()) != hipSuccess ||
         n < 1)
       n = 1;
@@ -1327,11 +1376,11 @@ int blocks_per_cu() {
   return cached;
 }
 
-template <int QT, int KT, int D, bool PL, bool VTOK>
-int32_t launch_stream_t(const DecodeParams& p, hipStream_t stream) {
-  const int blocks = cu_count() * blocks_per_cu<QT, KT, D, PL, VTOK>();
+template <int QT, int KT, int D, bool PL, bool VTOK, class P>
+int32_t launch_stream_t(const P& p, hipStream_t stream) {
+  const int blocks = cu_count() * blocks_per_cu<QT, KT, D, PL, VTOK, P>();
   ProfileScope prof("cf_decode_mfma", stream);
-  CF_LAUNCH((decode_stream_kernel<QT, KT, D, PL, VTOK>), dim3(blocks), dim3(256), (stream_lds_bytes<KT, D, PL, VTOK>()),
+  CF_LAUNCH((decode_stream_kernel<QT, KT, D, PL, VTOK, P>), dim3(blocks), dim3(256), (stream_lds_bytes<KT, D, PL, VTOK>()),
             stream, p, p.tables, p.seq_lens, p.k_scale, p.v_scale, PL ? p.shared : nullptr);
   CF_HIP_CHECK(hipGetLastError());
   return CF_OK;
@@ -1341,14 +1390,14 @@ int32_t launch_stream_t(const DecodeParams& p, hipStream_t stream) {
 // channel stride) rather than the native channel-major tile.
 bool v_token_major(const DecodeParams& p) { return p.v_s[3] == 1 && p.v_s[1] != 1; }
 
-template <int QT, int KT, int D, bool VTOK>
-int32_t launch_pl(const DecodeParams& p, hipStream_t stream) {
+template <int QT, int KT, int D, bool VTOK, class P>
+int32_t launch_pl(const P& p, hipStream_t stream) {
   return p.B <= kPlanMaxB ? launch_stream_t<QT, KT, D, true, VTOK>(p, stream)
                           : launch_stream_t<QT, KT, D, false, VTOK>(p, stream);
 }
 
-template <int QT, int KT, int D>
-int32_t launch_t(const DecodeParams& p, hipStream_t stream) {
+template <int QT, int KT, int D, class P>
+int32_t launch_t(const P& p, hipStream_t stream) {
   int32_t rc;
   rc = v_token_major(p) ? launch_pl<QT, KT, D, true>(p, stream) : launch_pl<QT, KT, D, false>(p, stream);
   if (rc) return rc;
@@ -1358,8 +1407,8 @@ int32_t launch_t(const DecodeParams& p, hipStream_t stream) {
   const dim3 grid(p.Hkv, p.B, split ? 4 : 1);
   ProfileScope prof("cf_decode_merge", stream);
 #define CF_MERGE(G)                                                                         \
-  if (split) CF_LAUNCH((decode_merge_kernel<QT, D, G, 4>), grid, dim3(256), 0, stream, p); \
-  else CF_LAUNCH((decode_merge_kernel<QT, D, G, 1>), grid, dim3(256), 0, stream, p);
+  if (split) CF_LAUNCH((decode_merge_kernel<QT, D, G, 4, P>), grid, dim3(256), 0, stream, p); \
+  else CF_LAUNCH((decode_merge_kernel<QT, D, G, 1, P>), grid, dim3(256), 0, stream, p);
   switch (p.G) {
     case 1: CF_MERGE(1) break;
     case 2: CF_MERGE(2) break;
@@ -1446,19 +1495,32 @@ bool decode_mfma_supported(const DecodeParams& p, int q_dt, int kv_dt) {
   return true;
 }
 
-template <int QT, int KT>
-int32_t launch_d(const DecodeParams& p, hipStream_t stream) {
+template <int QT, int KT, class P>
+int32_t launch_d(const P& p, hipStream_t stream) {
   if (p.D == 128) return launch_t<QT, KT, 128>(p, stream);
   if (p.D == 64) return launch_t<QT, KT, 64>(p, stream);
   set_error("MFMA decode: unsupported head_dim %d", p.D);
   return CF_ERR_UNSUPPORTED;
 }
 
-int32_t launch_decode_mfma(const DecodeParams& p, int q_dt, int kv_dt, hipStream_t stream) {
+namespace {
+
+template <class P>
+int32_t launch_any(const P& p, int q_dt, int kv_dt, hipStream_t stream) {
   if (q_dt == kF16) return kv_dt == kE4M3 ? launch_d<kF16, kE4M3>(p, stream) : launch_d<kF16, kF16>(p, stream);
   if (q_dt == kF32 && kv_dt == kF32) return launch_d<kF32, kF32>(p, stream);
   if (q_dt == kF32) return kv_dt == kE4M3 ? launch_d<kF32, kE4M3>(p, stream) : launch_d<kF32, kBF16>(p, stream);
   return kv_dt == kE4M3 ? launch_d<kBF16, kE4M3>(p, stream) : launch_d<kBF16, kBF16>(p, stream);
+}
+
+}  // namespace
+
+int32_t launch_decode_mfma(const DecodeParams& p, int q_dt, int kv_dt, hipStream_t stream) {
+  return launch_any(p, q_dt, kv_dt, stream);
+}
+
+int32_t launch_decode_mfma(const DecodeWeightsParams& p, int q_dt, int kv_dt, hipStream_t stream) {
+  return launch_any(p, q_dt, kv_dt, stream);
 }
 
 }  // namespace cf

@@ -37,15 +37,33 @@ struct DecodeParams {
   int NB;  // cache blocks; a block id outside [0, NB) contributes no tokens
 };
 
+// A decode call that also accounts for the weights: the kernels leave every
+// score and the rows' final (m, l), from which decode_weights_kernel forms them.
+struct DecodeWeightsParams : DecodeParams {
+  float* ws_s;    // scores [B, Hq, s_cap]: log2 units (MFMA path) or natural ones, -inf where masked
+  float* ws_fin;  // [B, Hq, 2] final reference and sum of a row
+  int64_t s_cap;  // tokens of a score row, a multiple of 32
+  float* weights;  // [B, Hw, >= Mb * bs] f32, last stride 1
+  int64_t w_sb, w_sh;
+  int Hw;  // Hkv, or 1
+  float decay;
+};
+
 // Launchers (return a CF_* status; kernels are enqueued on `stream`).
 int32_t launch_decode_generic(const DecodeParams& p, int q_dt, int kv_dt, hipStream_t stream);
 int32_t launch_decode_mfma(const DecodeParams& p, int q_dt, int kv_dt, hipStream_t stream);
+// The same with scores and final (m, l) written (the call is one that the
+// plain launcher takes), and the accounts formed from them.
+int32_t launch_decode_generic(const DecodeWeightsParams& p, int q_dt, int kv_dt, hipStream_t stream);
+int32_t launch_decode_mfma(const DecodeWeightsParams& p, int q_dt, int kv_dt, hipStream_t stream);
+int32_t launch_decode_weights(const DecodeWeightsParams& p, bool log2_units, hipStream_t stream);
 bool decode_mfma_supported(const DecodeParams& p, int q_dt, int kv_dt);
 // Workspace of the MFMA path: two (m, l, o) partial slots per launched wave.
 uint64_t decode_mfma_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim);
 void decode_mfma_bind_workspace(DecodeParams& p, void* workspace);
 
 int32_t launch_decode_reduce(const DecodeParams& p, int q_dt, hipStream_t stream);
+int32_t launch_decode_reduce(const DecodeWeightsParams& p, int q_dt, hipStream_t stream);
 // LDS bytes of one generic-kernel workgroup (G query heads, partition PT).
 size_t generic_lds_bytes(int64_t G, int64_t D, int64_t PT, int64_t bs);
 

@@ -18,6 +18,8 @@
 // P.V: the G * D outputs are spread over the 256 threads and, when there are
 // fewer outputs than threads, the partition's tokens are split between
 // thread groups whose sums meet in LDS.
+#include <type_traits>
+
 #include "cf_device.hpp"
 #include "cf_host.hpp"
 #include "decode_params.hpp"
@@ -35,8 +37,12 @@ __device__ __forceinline__ int effective_len(const DecodeParams& p, int b) {
   return ctx > 0 ? ctx : 0;
 }
 
-template <int QT, int KT, bool DIRECT>
-__global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(DecodeParams p) {
+// P: DecodeParams, or DecodeWeightsParams for a call that also keeps its scores.
+template <class P>
+constexpr bool kKeeps = std::is_same<P, DecodeWeightsParams>::value;
+
+template <int QT, int KT, bool DIRECT, class P>
+__global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(P p) {
   extern __shared__ float smem[];
   const int part = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x;
@@ -129,6 +135,13 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(DecodeP
       for (int g = 0; g < G; ++g) sc[g * PT + i] = blk_ok ? sc[g * PT + i] * qk_scale : -INFINITY;
   }
   __syncthreads();
+  if constexpr (kKeeps<P>) {
+    for (int u = tid; u < G * count; u += kGenericThreads) {
+      const int g = u / count, i = u - g * count;
+      p.ws_s[((int64_t)b * p.Hq + h * G + g) * p.s_cap + start + i] = sc[g * PT + i];
+    }
+    __syncthreads();
+  }
 
   // softmax statistics per query head: one wave per head
   const int wave = tid / 64, lane = tid % 64;
@@ -148,6 +161,11 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(DecodeP
     if (lane == 0) {
       sml[2 * g] = m;
       sml[2 * g + 1] = l;
+      if constexpr (kKeeps<P> && DIRECT) {
+        float* fin = p.ws_fin + ((int64_t)b * p.Hq + h * G + g) * 2;
+        fin[0] = m;
+        fin[1] = l;
+      }
     }
   }
   __syncthreads();
@@ -234,8 +252,8 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(DecodeP
 // 256 threads: (m, l) are read lane-parallel and reduced across the block;
 // the weighted sum takes the partitions in 256 / D interleaved groups (all
 // their loads independent), whose sums meet in LDS.
-template <int OT>
-__global__ __launch_bounds__(256) void decode_reduce_kernel(DecodeParams p) {
+template <int OT, class P>
+__global__ __launch_bounds__(256) void decode_reduce_kernel(P p) {
   __shared__ float red[8];
   __shared__ float part_acc[256];
   const int hq = blockIdx.x, b = blockIdx.y;
@@ -266,6 +284,13 @@ __global__ __launch_bounds__(256) void decode_reduce_kernel(DecodeParams p) {
   if (lane == 0) red[4 + wave] = lloc;
   __syncthreads();
   const float L = (red[4] + red[5]) + (red[6] + red[7]);
+  if constexpr (kKeeps<P>) {
+    if (tid == 0) {
+      float* fin = p.ws_fin + ((int64_t)b * p.Hq + hq) * 2;
+      fin[0] = M;
+      fin[1] = L;
+    }
+  }
   const float inv = L > 0.0f ? 1.0f / L : 0.0f;
   if (p.D > 128) {
     for (int d = tid; d < p.D; d += 256) {
@@ -295,8 +320,8 @@ __global__ __launch_bounds__(256) void decode_reduce_kernel(DecodeParams p) {
   }
 }
 
-template <int QT, int KT>
-int32_t launch_generic_t(const DecodeParams& p, hipStream_t stream) {
+template <int QT, int KT, class P>
+int32_t launch_generic_t(const P& p, hipStream_t stream) {
   const dim3 grid(p.max_parts, p.Hkv, p.B);
   const size_t lds = generic_lds_bytes(p.G, p.D, p.PT, p.bs);
   if (lds > 64 * 1024) {
@@ -306,17 +331,17 @@ int32_t launch_generic_t(const DecodeParams& p, hipStream_t stream) {
   }
   if (p.max_parts == 1) {
     ProfileScope prof("cf_decode_generic", stream);
-    CF_LAUNCH((decode_generic_kernel<QT, KT, true>), grid, dim3(kGenericThreads), lds, stream, p);
+    CF_LAUNCH((decode_generic_kernel<QT, KT, true, P>), grid, dim3(kGenericThreads), lds, stream, p);
   } else {
     ProfileScope prof("cf_decode_generic", stream);
-    CF_LAUNCH((decode_generic_kernel<QT, KT, false>), grid, dim3(kGenericThreads), lds, stream, p);
+    CF_LAUNCH((decode_generic_kernel<QT, KT, false, P>), grid, dim3(kGenericThreads), lds, stream, p);
   }
   CF_HIP_CHECK(hipGetLastError());
   return CF_OK;
 }
 
-template <int QT>
-int32_t launch_generic_q(const DecodeParams& p, int kv_dt, hipStream_t stream) {
+template <int QT, class P>
+int32_t launch_generic_q(const P& p, int kv_dt, hipStream_t stream) {
   switch (kv_dt) {
     case kF32: return launch_generic_t<QT, kF32>(p, stream);
     case kF16: return launch_generic_t<QT, kF16>(p, stream);
@@ -329,7 +354,10 @@ int32_t launch_generic_q(const DecodeParams& p, int kv_dt, hipStream_t stream) {
 
 }  // namespace
 
-int32_t launch_decode_generic(const DecodeParams& p, int q_dt, int kv_dt, hipStream_t stream) {
+namespace {
+
+template <class P>
+int32_t launch_generic_any(const P& p, int q_dt, int kv_dt, hipStream_t stream) {
   switch (q_dt) {
     case kF32: return launch_generic_q<kF32>(p, kv_dt, stream);
     case kF16: return launch_generic_q<kF16>(p, kv_dt, stream);
@@ -339,23 +367,42 @@ int32_t launch_decode_generic(const DecodeParams& p, int q_dt, int kv_dt, hipStr
   return CF_ERR_UNSUPPORTED;
 }
 
-size_t generic_lds_bytes(int64_t G, int64_t D, int64_t PT, int64_t bs) {
-  // q [G][D], scores [G][PT], block ids [PT / bs] (even), (m, l) [G][2], P.V sums [256]
-  return (size_t)(G * D + G * PT + ((PT / bs + 1) & ~1) + 2 * G + kGenericThreads) * 4;
-}
-
-int32_t launch_decode_reduce(const DecodeParams& p, int q_dt, hipStream_t stream) {
+template <class P>
+int32_t launch_reduce_any(const P& p, int q_dt, hipStream_t stream) {
   const dim3 grid(p.Hq, p.B);
   const int threads = 256;
   ProfileScope prof("cf_decode_reduce", stream);
   switch (q_dt) {
-    case kF32: CF_LAUNCH((decode_reduce_kernel<kF32>), grid, dim3(threads), 0, stream, p); break;
-    case kF16: CF_LAUNCH((decode_reduce_kernel<kF16>), grid, dim3(threads), 0, stream, p); break;
-    case kBF16: CF_LAUNCH((decode_reduce_kernel<kBF16>), grid, dim3(threads), 0, stream, p); break;
+    case kF32: CF_LAUNCH((decode_reduce_kernel<kF32, P>), grid, dim3(threads), 0, stream, p); break;
+    case kF16: CF_LAUNCH((decode_reduce_kernel<kF16, P>), grid, dim3(threads), 0, stream, p); break;
+    case kBF16: CF_LAUNCH((decode_reduce_kernel<kBF16, P>), grid, dim3(threads), 0, stream, p); break;
     default: set_error("unsupported output dtype %d", q_dt); return CF_ERR_UNSUPPORTED;
   }
   CF_HIP_CHECK(hipGetLastError());
   return CF_OK;
+}
+
+}  // namespace
+
+int32_t launch_decode_generic(const DecodeParams& p, int q_dt, int kv_dt, hipStream_t stream) {
+  return launch_generic_any(p, q_dt, kv_dt, stream);
+}
+
+int32_t launch_decode_generic(const DecodeWeightsParams& p, int q_dt, int kv_dt, hipStream_t stream) {
+  return launch_generic_any(p, q_dt, kv_dt, stream);
+}
+
+int32_t launch_decode_reduce(const DecodeParams& p, int q_dt, hipStream_t stream) {
+  return launch_reduce_any(p, q_dt, stream);
+}
+
+int32_t launch_decode_reduce(const DecodeWeightsParams& p, int q_dt, hipStream_t stream) {
+  return launch_reduce_any(p, q_dt, stream);
+}
+
+size_t generic_lds_bytes(int64_t G, int64_t D, int64_t PT, int64_t bs) {
+  // q [G][D], scores [G][PT], block ids [PT / bs] (even), (m, l) [G][2], P.V sums [256]
+  return (size_t)(G * D + G * PT + ((PT / bs + 1) & ~1) + 2 * G + kGenericThreads) * 4;
 }
 
 }  // namespace cf

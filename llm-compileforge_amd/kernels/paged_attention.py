@@ -257,6 +257,52 @@ def paged_attention(
     return dict(zip(rids, out.unbind(0)))
 
 
+def paged_attention_weights(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    weights: torch.Tensor,
+    block_size: int = 16,
+    scale: float | None = None,
+    *,
+    decay: float = 1.0,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    shared_prefix_lens: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """`paged_attention_tensors` that also keeps each sequence's account of
+    attention weight, from which kernels.kv_eviction chooses what stays.
+
+    Args:
+        weights: float32 [B, Hkv, S], or [B, 1, S] for one account over all
+            heads; S at least the tables' tokens, last stride 1.  Updated in
+            place for the tokens attended to: decay * weights (nothing for the
+            newest token, which has no history) + the softmax weights of the
+            account's query heads.
+        decay: what the account keeps of earlier steps; 0 leaves this step's
+            weights alone, whatever was there.
+        workspace: cf_hip.ops.decode_weights_workspace_bytes() bytes, by
+            default a cached one per (device, stream).
+
+    The other arguments and the result are those of `paged_attention_tensors`.
+    """
+    _require_rocm(q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if block_tables.dtype != torch.int32:
+        block_tables = block_tables.to(torch.int32)
+    if seq_lens.dtype != torch.int32:
+        seq_lens = seq_lens.to(torch.int32)
+    return _ops.paged_decode_weights(
+        q, k_cache, v_cache, block_tables, seq_lens, weights, float(scale), int(block_size), float(decay),
+        k_scale=k_scale, v_scale=v_scale, out=out, workspace=workspace, shared_prefix_lens=shared_prefix_lens,
+    )
+
+
 def chunked_prefill_attention(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -306,4 +352,5 @@ def chunked_prefill_attention(
     )
 
 
-__all__ = ["DEFAULT_PARTITION_TOKENS", "chunked_prefill_attention", "paged_attention", "paged_attention_tensors"]
+__all__ = ["DEFAULT_PARTITION_TOKENS", "chunked_prefill_attention", "paged_attention", "paged_attention_tensors",
+           "paged_attention_weights"]
