@@ -261,6 +261,33 @@ int32_t cf_prefill_chunk_fp8(const CfTensor* q, const CfTensor* k_cache,
                              float scale, int32_t block_size, CfTensor* out,
                              void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* Workspace of cf_chunk_weights for tables of max_blocks_per_seq blocks: 8
+ * bytes a query row, head and piece of at least 1,024 tokens (256 in small
+ * calls; at most 16 pieces), and sums of 4 bytes a token and head for each
+ * 256 to 1,024 query rows x heads. */
+int32_t cf_chunk_weights_workspace_bytes(int64_t num_q_tokens, int64_t num_chunks, int64_t num_q_heads,
+                                         int64_t num_kv_heads, int64_t head_dim, int64_t max_blocks_per_seq,
+                                         int32_t block_size, uint64_t* bytes_out);
+
+/* The accounts of cf_paged_decode_weights for the rows of prompts and chunks
+ * (q, k_cache, block_tables, seq_lens, q_start and k_scale as
+ * cf_prefill_chunk_fp8, whose attention this does not repeat):
+ *   weights[n, hw, t] = (t of the chunk ? 0 : decay * weights[n, hw, t])
+ *       + sum over the chunk's rows and the query heads of hw of softmax weight t
+ * for the first min(seq_lens[n], Mb * 16) tokens of every chunk that has rows;
+ * other entries are left as they were.  Tokens that came with the chunk, the
+ * last q_start[n + 1] - q_start[n] of seq_lens[n], have no history.
+ *   observe  only the last `observe` rows of each chunk count; 0: all of them
+ *   weights  [N, Hw, S]  f32, S stride 1, S >= Mb * 16; Hw = Hkv or 1
+ * Takes q bf16 over bf16 or e4m3fn, q f16 over f16 or e4m3fn; head_dim 64 or
+ * 128; at most 64 query heads a KV head; K rows of unit channel stride, 16-byte
+ * aligned (every layout of cf_hip.layout).  Others return CF_ERR_UNSUPPORTED.
+ * workspace: cf_chunk_weights_workspace_bytes() bytes, 256-byte aligned. */
+int32_t cf_chunk_weights(const CfTensor* q, const CfTensor* k_cache, const CfTensor* block_tables,
+                         const CfTensor* seq_lens, const CfTensor* q_start, const CfTensor* k_scale, float scale,
+                         int32_t block_size, int32_t observe, CfTensor* weights, float decay, void* workspace,
+                         uint64_t workspace_bytes, void* stream);
+
 /* Per-head FP8 scale: scales[h] = amax/448 over x[:, h, :], clamped below
  * at 1e-12, and 1.0 where amax == 0.  This is
  * FP8KVCacheQuantizer.quantize_block's scale rule (reference

@@ -175,6 +175,16 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [_P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_float, ctypes.c_int32, _P, ctypes.c_void_p, ctypes.c_uint64,
          ctypes.c_void_p],
     ),
+    "cf_chunk_weights_workspace_bytes": (
+        ctypes.c_int32,
+        [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+         ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)],
+    ),
+    "cf_chunk_weights": (
+        ctypes.c_int32,
+        [_P, _P, _P, _P, _P, _P, ctypes.c_float, ctypes.c_int32, ctypes.c_int32, _P, ctypes.c_float, ctypes.c_void_p,
+         ctypes.c_uint64, ctypes.c_void_p],
+    ),
     "cf_fp8_amax_scale": (ctypes.c_int32, [_P, _P, ctypes.c_void_p]),
     "cf_kv_amax_scale": (ctypes.c_int32, [_P, _P, ctypes.c_void_p]),
     "cf_fp8_quantize": (ctypes.c_int32, [_P, _P, _P, ctypes.c_void_p]),

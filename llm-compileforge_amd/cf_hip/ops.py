@@ -376,6 +376,58 @@ def prefill_chunk(
     return out
 
 
+def chunk_weights_workspace_bytes(num_q_tokens: int, num_chunks: int, num_q_heads: int, num_kv_heads: int,
+                                  head_dim: int, max_blocks_per_seq: int, block_size: int = 16) -> int:
+    out = ctypes.c_uint64(0)
+    rc = lib().cf_chunk_weights_workspace_bytes(num_q_tokens, num_chunks, num_q_heads, num_kv_heads, head_dim,
+                                                max_blocks_per_seq, block_size, ctypes.byref(out))
+    check(rc, "cf_chunk_weights_workspace_bytes")
+    return int(out.value)
+
+
+def chunk_weights(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    q_start: torch.Tensor,
+    weights: torch.Tensor,
+    scale: float,
+    block_size: int = 16,
+    decay: float = 1.0,
+    observe: int = 0,
+    k_scale: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Adds the attention weights of prompt chunks' rows (prefill_chunk's q,
+    tables, lengths and q_start) to weights [N, Hkv or 1, S], in place; with
+    observe > 0 only each chunk's last `observe` rows count.  workspace:
+    chunk_weights_workspace_bytes() bytes, by default a cached one per
+    (device, stream)."""
+    given = [("q", q), ("k_cache", k_cache), ("block_tables", block_tables), ("seq_lens", seq_lens),
+             ("q_start", q_start), ("weights", weights)]
+    given += [(n, t) for n, t in (("k_scale", k_scale), ("workspace", workspace)) if t is not None]
+    for name, t in given:
+        _require_device(name, t)
+    dev = _same_device(*(t for _, t in given))
+    if q.dim() != 3 or k_cache.dim() != 4 or block_tables.dim() != 2:
+        raise ValueError(f"q must be [Tq, Hq, D], k_cache [NB, 16, Hkv, D], block_tables [N, Mb]; got "
+                         f"{tuple(q.shape)}, {tuple(k_cache.shape)}, {tuple(block_tables.shape)}")
+    need = chunk_weights_workspace_bytes(q.shape[0], block_tables.shape[0], q.shape[1], k_cache.shape[2], q.shape[2],
+                                         block_tables.shape[1], block_size)
+    if workspace is None:
+        workspace = _cached_workspace(need, dev)
+    elif workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"workspace of {need} bytes needed, {workspace.numel() * workspace.element_size()} given")
+    d = [descriptor(t) if t is not None else None for t in (q, k_cache, block_tables, seq_lens, q_start, k_scale)]
+    dw = descriptor(weights)
+    with _on(dev):
+        rc = lib().cf_chunk_weights(*(ref(x) for x in d), float(scale), int(block_size), _int32("observe", int(observe)),
+                                    ref(dw), float(decay), workspace.data_ptr(), need, stream_handle(dev))
+    check(rc, "cf_chunk_weights")
+    return weights
+
+
 class DecodePlan:
     """A paged decode call with its descriptors built once.
 
@@ -982,6 +1034,8 @@ __all__ = [
     "KernelTimer",
     "block_span_view",
     "block_tables_apply",
+    "chunk_weights",
+    "chunk_weights_workspace_bytes",
     "copy_blocks",
     "decode_weights_workspace_bytes",
     "decode_workspace_bytes",

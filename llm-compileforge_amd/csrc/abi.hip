@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "cf_host.hpp"
+#include "chunk_weights.hpp"
 #include "decode_params.hpp"
 #include "kv_evict.hpp"
 #include "kv_fp8.hpp"
@@ -784,6 +785,113 @@ int32_t cf_prefill_chunk_fp8(const CfTensor* q, const CfTensor* k_cache, const C
   }
   CF_CHECK(((uintptr_t)workspace & 255) == 0, "workspace must be 256-byte aligned");
   return launch_prefill(p, vq.dtype, vk.dtype, as_stream(stream));
+}
+
+int32_t cf_chunk_weights_workspace_bytes(int64_t num_q_tokens, int64_t num_chunks, int64_t num_q_heads,
+                                         int64_t num_kv_heads, int64_t head_dim, int64_t max_blocks_per_seq,
+                                         int32_t block_size, uint64_t* bytes_out) {
+  CF_CHECK(bytes_out != nullptr, "bytes_out is NULL");
+  CF_CHECK(num_q_tokens >= 0 && num_chunks >= 0 && num_q_heads > 0 && num_kv_heads > 0 && head_dim > 0 &&
+               max_blocks_per_seq >= 0,
+           "invalid sizes");
+  CF_CHECK(num_q_heads % num_kv_heads == 0, "num_heads %lld is not a multiple of num_kv_heads %lld",
+           (long long)num_q_heads, (long long)num_kv_heads);
+  CF_CHECK(block_size == 16, "block_size must be 16, got %d", block_size);
+  CF_CHECK(num_q_heads / num_kv_heads <= 64, "at most 64 query heads a KV head, got %lld",
+           (long long)(num_q_heads / num_kv_heads));
+  *bytes_out = chunk_weights_workspace_bytes(num_q_tokens, num_chunks, num_q_heads, num_kv_heads, max_blocks_per_seq);
+  return CF_OK;
+}
+
+int32_t cf_chunk_weights(const CfTensor* q, const CfTensor* k_cache, const CfTensor* block_tables,
+                         const CfTensor* seq_lens, const CfTensor* q_start, const CfTensor* k_scale, float scale,
+                         int32_t block_size, int32_t observe, CfTensor* weights, float decay, void* workspace,
+                         uint64_t workspace_bytes, void* stream) {
+  View vq, vk, vt, vqs, vw;
+  int32_t rc;
+  if ((rc = view_of(q, "q", 3, &vq))) return rc;
+  if ((rc = view_of(k_cache, "k_cache", 4, &vk))) return rc;
+  if ((rc = view_of(block_tables, "block_tables", 2, &vt))) return rc;
+  if ((rc = view_of(q_start, "q_start", 1, &vqs))) return rc;
+  if ((rc = account_view(weights, "weights", CF_F32, &vw))) return rc;
+  CF_CHECK(vq.dtype == CF_BF16 || vq.dtype == CF_F16, "q: dtype must be bf16 or f16, got %s", dtype_name(vq.dtype));
+  CF_CHECK(vk.dtype == CF_BF16 || vk.dtype == CF_F16 || vk.dtype == CF_F8E4M3FN,
+           "k_cache: dtype must be bf16, f16 or f8e4m3fn, got %s", dtype_name(vk.dtype));
+  CF_CHECK(vt.dtype == CF_I32, "block_tables: expected i32, got %s", dtype_name(vt.dtype));
+  CF_CHECK(vqs.dtype == CF_I32, "q_start: expected i32, got %s", dtype_name(vqs.dtype));
+  const int64_t Tq = vq.size[0], Hq = vq.size[1], D = vq.size[2];
+  const int64_t NB = vk.size[0], bs = vk.size[1], Hkv = vk.size[2], N = vt.size[0], cap = vt.size[1] * 16;
+  CF_CHECK(vk.size[3] == D, "k_cache head_dim %lld differs from q head_dim %lld", (long long)vk.size[3],
+           (long long)D);
+  CF_CHECK(block_size == 16, "block_size must be 16, got %d", block_size);
+  CF_CHECK(bs == block_size, "k_cache block dim %lld differs from block_size %d", (long long)bs, block_size);
+  CF_CHECK(Hq > 0, "q has no heads");
+  CF_CHECK(Hkv > 0 && Hq % Hkv == 0, "num_heads %lld is not a multiple of num_kv_heads %lld", (long long)Hq,
+           (long long)Hkv);
+  CF_CHECK(vqs.size[0] == N + 1, "q_start must have %lld entries, got %lld", (long long)(N + 1),
+           (long long)vqs.size[0]);
+  CF_CHECK(vw.size[0] == N && (vw.size[1] == Hkv || vw.size[1] == 1),
+           "weights must be [%lld, %lld or 1, S] (one account a KV head, or one for all)", (long long)N,
+           (long long)Hkv);
+  CF_CHECK(vw.size[2] >= cap, "weights has %lld slots, the block tables hold %lld tokens", (long long)vw.size[2],
+           (long long)cap);
+  CF_CHECK(vq.stride[2] == 1, "q: head_dim stride must be 1");
+  CF_CHECK(NB < (int64_t)INT32_MAX && cap < (int64_t)1 << 30, "too many cache blocks");
+  CF_CHECK(Tq < (int64_t)INT32_MAX / 2 && N < (int64_t)INT32_MAX / 2, "too many query rows or chunks");
+  CF_CHECK(Hkv < 65536, "too many KV heads");
+  CF_CHECK(std::isfinite(scale) && std::isfinite(decay), "scale and decay must be finite");
+  CF_CHECK(observe >= 0, "observe (%d) must not be negative", observe);
+  ChunkWeightsParams p{};
+  if ((rc = row_view(seq_lens, "seq_lens", N, &p.seq_lens, &p.sl_s))) return rc;
+  if (vk.dtype == CF_F8E4M3FN) {
+    CF_CHECK(k_scale != nullptr, "f8e4m3fn caches need k_scale");
+    if ((rc = scale_view(k_scale, "k_scale", Hkv, &p.k_scale, &p.ks_s))) return rc;
+  } else {
+    CF_CHECK(k_scale == nullptr, "k_scale applies to f8e4m3fn caches only");
+  }
+  p.q = vq.base;
+  p.q_sr = vq.stride[0];
+  p.q_sh = vq.stride[1];
+  p.k = vk.base;
+  for (int i = 0; i < 4; ++i) p.k_s[i] = vk.stride[i];
+  p.tables = (const int32_t*)vt.base;
+  p.t_sb = vt.stride[0];
+  p.t_sm = vt.stride[1];
+  p.q_start = (const int32_t*)vqs.base;
+  p.qs_s = vqs.stride[0];
+  p.weights = (float*)vw.base;
+  p.w_sb = vw.stride[0];
+  p.w_sh = vw.stride[1];
+  p.scale = scale;
+  p.decay = decay;
+  p.observe = observe;
+  p.N = (int)N;
+  p.Tq = (int)Tq;
+  p.Hq = (int)Hq;
+  p.Hkv = (int)Hkv;
+  p.Hw = (int)vw.size[1];
+  p.G = (int)(Hq / Hkv);
+  p.D = (int)D;
+  p.Mb = (int)vt.size[1];
+  p.NB = (int)NB;
+  if (!chunk_weights_supported(p, vq.dtype, vk.dtype)) {
+    set_error("chunk weights: needs bf16 q over bf16/e4m3 caches or f16 q over f16/e4m3 caches, head_dim 64/128, at "
+              "most 64 query heads a KV head, K rows with unit channel stride and 16-byte aligned blocks, heads and "
+              "token rows, and 16-byte aligned q rows");
+    return CF_ERR_UNSUPPORTED;
+  }
+  if (Tq == 0 || N == 0 || cap == 0) return CF_OK;
+  CF_CHECK((Tq / 4 + 2 * N) * Hkv < (int64_t)INT32_MAX && ceil_div(cap, 256) * N * Hkv < (int64_t)INT32_MAX,
+           "too many rows");
+  const uint64_t need = chunk_weights_workspace_bytes(Tq, N, Hq, Hkv, vt.size[1]);
+  if (workspace == nullptr || workspace_bytes < need) {
+    set_error("workspace of %llu bytes needed, %llu given", (unsigned long long)need,
+              (unsigned long long)workspace_bytes);
+    return CF_ERR_WORKSPACE;
+  }
+  CF_CHECK(((uintptr_t)workspace & 255) == 0, "workspace must be 256-byte aligned");
+  chunk_weights_bind_workspace(p, workspace);
+  return launch_chunk_weights(p, vq.dtype, vk.dtype, as_stream(stream));
 }
 
 int32_t cf_fp8_amax_scale(const CfTensor* x, CfTensor* scales, void* stream) {

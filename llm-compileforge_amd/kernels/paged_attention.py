@@ -352,5 +352,45 @@ def chunked_prefill_attention(
     )
 
 
-__all__ = ["DEFAULT_PARTITION_TOKENS", "chunked_prefill_attention", "paged_attention", "paged_attention_tensors",
+def chunk_attention_weights(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    q_start: torch.Tensor,
+    weights: torch.Tensor,
+    block_size: int = 16,
+    scale: float | None = None,
+    *,
+    decay: float = 1.0,
+    observe: int = 0,
+    k_scale: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The accounts of `paged_attention_weights` for the rows of prompts and
+    chunks, next to `chunked_prefill_attention` over the same arguments.
+
+    Args:
+        weights: float32 [N, Hkv, S], or [N, 1, S] for one account over all
+            heads; S at least the tables' tokens, last stride 1.  Updated in
+            place for every token of a sequence that has rows: decay * weights
+            (nothing for the chunk's own tokens) + the softmax weights of the
+            rows and query heads that see it.
+        decay: what the account keeps of earlier chunks.
+        observe: only the last `observe` rows of each chunk count (a window of
+            observers, at a fraction of the cost); 0 counts all.
+
+    The other arguments are those of `chunked_prefill_attention`.  Returns
+    weights.
+    """
+    _require_rocm(q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    block_tables, seq_lens, q_start = (t if t.dtype == torch.int32 else t.to(torch.int32)
+                                       for t in (block_tables, seq_lens, q_start))
+    return _ops.chunk_weights(q, k_cache, block_tables, seq_lens, q_start, weights, float(scale), int(block_size),
+                              float(decay), int(observe), k_scale=k_scale, workspace=workspace)
+
+
+__all__ = ["DEFAULT_PARTITION_TOKENS", "chunk_attention_weights", "chunked_prefill_attention", "paged_attention", "paged_attention_tensors",
            "paged_attention_weights"]
