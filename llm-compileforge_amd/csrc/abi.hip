@@ -1345,9 +1345,9 @@ int32_t cf_evict_move(const CfTensor* keep, const CfTensor* seq_lens, const CfTe
   }
   if ((rc = position_views(positions, kept, seen, vk, &vp, &p.kept, &p.kept_s, &p.seen, &p.seen_s))) return rc;
   if (positions != nullptr) S = std::min(S, vp.size[2]);
-  const int64_t groups = ceil_div(budget, 64) * B * Hw;
+  const int64_t groups = ceil_div(budget, 16) * B * Hkv;
   CF_CHECK(groups < (int64_t)INT32_MAX, "too many slots");
-  if (groups == 0 || NB == 0 || Hkv * D == 0) return CF_OK;
+  if (groups == 0 || NB == 0 || Hkv * D == 0 || S == 0) return CF_OK;
   p.keep = (const int32_t*)vk.base;
   p.k_sb = vk.stride[0];
   p.k_sh = vk.stride[1];

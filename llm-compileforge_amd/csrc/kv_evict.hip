@@ -18,6 +18,7 @@
 #include "cf_device.hpp"
 #include "cf_host.hpp"
 #include "kv_evict.hpp"
+#include "mfma_tile.hpp"
 
 namespace cf {
 
@@ -28,11 +29,15 @@ namespace {
 // One workgroup a (sequence, head).  A weight becomes a 32-bit key in the
 // order above (protected tokens the greatest key, indices past the sequence
 // 0), held in registers: wave v's item e of lane l is index
-// (v * E + e) * 64 + l, so loads are whole runs and ranks follow the index.
-// The budget-th greatest key is found from the top bit downwards, a count of
-// the keys at or above a candidate for each bit; a count is one comparison a
-// key and scalar popcounts, where a histogram's LDS atomics would meet in few
-// bins (accounts differ by little in their leading bits).
+// (v * items + e) * 64 + l, so loads are whole runs and ranks follow the index.
+// The budget-th greatest key is found in two steps: a histogram of the ten
+// bits below the first in which keys differ (so that accounts, which share
+// their leading bits, spread over its bins), and, among the keys of the bin
+// that it lies in, a search two bits at a time by counts of the keys at or
+// above the three candidates.  The bin's keys are gathered in LDS, a key a
+// lane of one wave; if they are too many, a histogram of the bin's next ten
+// bits comes first.  A workgroup is bound by its instructions a key (some 80)
+// and the latency of its barriers and LDS steps.
 
 __device__ __forceinline__ uint32_t key_of(float w) {
   if (w != w) return 0xFFFFFFFEu;
@@ -45,13 +50,17 @@ constexpr uint32_t kSafe = 0xFFFFFFFFu;  // a protected token's key
 struct SelectRow {
   const float* w;
   const int32_t* pos;  // null: a slot's index is its position
+  int last;             // of the buffer's slots
   int len, kept, first, sink;
   int64_t recent_from;  // positions at or above it are protected
-  __device__ __forceinline__ uint32_t key(int i) const {
-    if (i >= len) return 0u;
-    const uint32_t k = key_of(w[i]);
-    const int64_t at = pos == nullptr ? i : (i < kept ? (int64_t)pos[i] : (int64_t)first + i);
-    return at < sink || at >= recent_from ? kSafe : k;
+  // (loads of indices past the end take the last one: they need no branch, so
+  // all of a lane's are in flight together)
+  __device__ __forceinline__ float weight(int i) const { return w[(uint32_t)min(i, last)]; }
+  __device__ __forceinline__ int position(int i) const { return pos[(uint32_t)min(i, last)]; }
+  __device__ __forceinline__ uint32_t key(int i, float wi, int stored) const {
+    const int64_t at = pos != nullptr && i < kept ? (int64_t)stored : (int64_t)first + i;
+    const uint32_t k = at < sink || at >= recent_from ? kSafe : key_of(wi);
+    return i < len ? k : 0u;
   }
 };
 
@@ -60,199 +69,518 @@ __device__ __forceinline__ int rank_in(uint64_t mask) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
 }
 
-// Sum of v over the waves before this one, and over all (v wave-uniform).
-// `slot`: LDS of one int a wave that no wave still reads.
-template <int WAVES>
-__device__ __forceinline__ int2 before_and_all(int* slot, int v, int wave) {
-  if ((threadIdx.x & 63) == 0) slot[wave] = v;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) {
-    const int x = slot[i];
-    all += x;
-    before += i < wave ? x : 0;
-  }
-  return make_int2(before, all);
+// Sum over N consecutive lanes, N a power of two up to 16, of values that
+// repeat every N lanes (rotations within a row of 16).
+template <int N>
+__device__ __forceinline__ int ring_sum(int v) {
+  if constexpr (N > 8) v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false);
+  if constexpr (N > 4) v += __builtin_amdgcn_update_dpp(0, v, 0x124, 0xF, 0xF, false);
+  if constexpr (N > 2) v += __builtin_amdgcn_update_dpp(0, v, 0x122, 0xF, 0xF, false);
+  if constexpr (N > 1) v += __builtin_amdgcn_update_dpp(0, v, 0x121, 0xF, 0xF, false);
+  return __builtin_amdgcn_readfirstlane(v);
 }
 
+// The waves' values meet in LDS: each wave writes its own and reads all, a
+// wave's a lane (one read, where a broadcast read of each would be 16).
+// `slot`: LDS of a value a wave that no wave still reads.
+
+// Sum of v over the waves before this one, and over all (v wave-uniform).
+template <int WAVES>
+__device__ __forceinline__ int2 before_and_all(int* slot, int v, int wave) {
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) slot[wave] = v;
+  __syncthreads();
+  const int x = slot[lane & (WAVES - 1)];
+  return make_int2(ring_sum<WAVES>((lane & (WAVES - 1)) < wave ? x : 0), ring_sum<WAVES>(x));
+}
+
+// a + b, at most 2^32 - 1 (a key that no unprotected token has).
+__device__ __forceinline__ uint32_t plus(uint32_t a, uint32_t b) { return a > 0xFFFFFFFFu - b ? 0xFFFFFFFFu : a + b; }
+
 constexpr int kListCap = 4096;  // movers handed to their holes at a time
+constexpr int kBinBits = 10;    // of the histogram
+constexpr int kLaneBins = (1 << kBinBits) / 64;
+constexpr int kGather = 512;    // keys of one bin that are searched apart
 
 // E > 0: up to E * THREADS keys in registers; E == 0: any number, read again
 // for every use.
 template <int THREADS, int E>
 __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictSelectParams p) {
   constexpr int WAVES = THREADS / 64;
-  __shared__ int counts[4][WAVES];
-  __shared__ int list[kListCap];
+  __shared__ int counts[3][WAVES];
+  __shared__ int4 votes[2][WAVES];
+  __shared__ __align__(16) int hist[1 << kBinBits];
+  __shared__ int found[3], gathered;
+  __shared__ uint32_t few[kGather];
   const int b = blockIdx.x / p.H, h = blockIdx.x - b * p.H;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int raw = p.lens[(int64_t)b * p.l_s];
-  const int len = raw < 0 ? 0 : (raw < p.S ? raw : p.S);
   const int budget = p.budget;
   int32_t* keep = p.keep + (int64_t)b * p.k_sb + (int64_t)h * p.k_sh;
+  SelectRow row;
+  row.w = p.weights + (int64_t)b * p.w_sb + (int64_t)h * p.w_sh;
+  row.pos = p.positions == nullptr ? nullptr : p.positions + (int64_t)b * p.p_sb + (int64_t)h * p.p_sh;
+  row.last = p.S - 1;
+  const int items = (p.S + THREADS - 1) / THREADS;  // of a lane
+  const int base = wave * items * 64 + lane;
+  // all loads go out before the length is known (the buffer is S long)
+  uint32_t reg[E > 0 ? E : 1];
+  if constexpr (E > 0) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) reg[e] = p.S > 0 ? f2u(row.weight(base + e * 64)) : 0u;
+  }
+  const int raw = p.lens[(int64_t)b * p.l_s];
+  const int seen = p.positions == nullptr ? 0 : p.seen[(int64_t)b * p.seen_s];
+  row.kept = p.positions == nullptr ? 0 : p.kept[(int64_t)b * p.kept_s];
+  const int len = raw < 0 ? 0 : (raw < p.S ? raw : p.S);
   if (h == 0 && threadIdx.x == 0) p.new_lens[(int64_t)b * p.n_s] = len < budget ? len : budget;
   if (len <= budget) {
     for (int j = threadIdx.x; j < budget; j += THREADS) keep[j] = j < len ? j : -1;
     return;
   }
-  SelectRow row;
-  row.w = p.weights + (int64_t)b * p.w_sb + (int64_t)h * p.w_sh;
-  row.pos = p.positions == nullptr ? nullptr : p.positions + (int64_t)b * p.p_sb + (int64_t)h * p.p_sh;
   row.len = len;
   row.sink = p.sink;
-  const int seen = p.positions == nullptr ? len : p.seen[(int64_t)b * p.seen_s];
-  row.kept = p.positions == nullptr ? 0 : p.kept[(int64_t)b * p.kept_s];
-  row.first = seen - len;
-  row.recent_from = (int64_t)seen - p.recent;
-
-  const int items = E > 0 ? E : (len + THREADS - 1) / THREADS;  // of a lane
-  const int base = wave * items * 64 + lane;
-  uint32_t reg[E > 0 ? E : 1];
+  row.first = p.positions == nullptr ? 0 : seen - len;
+  row.recent_from = (int64_t)row.first + len - p.recent;
   if constexpr (E > 0) {
+    constexpr int kBatch = 8 < E ? 8 : E;  // positions in flight at a time
 #pragma unroll
-    for (int e = 0; e < E; ++e) reg[e] = row.key(base + e * 64);
+    for (int e0 = 0; e0 < E; e0 += kBatch) {
+      int at[kBatch];
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) at[e] = row.pos != nullptr ? row.position(base + (e0 + e) * 64) : 0;
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) reg[e0 + e] = row.key(base + (e0 + e) * 64, u2f(reg[e0 + e]), at[e]);
+    }
   }
   auto each = [&](auto f) {
     if constexpr (E > 0) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) f(base + e * 64, reg[e]);
+      for (int e = 0; e < E; ++e) {
+        if (e < items) f(base + e * 64, reg[e]);
+      }
     } else {
-      for (int e = 0; e < items; ++e) f(base + e * 64, row.key(base + e * 64));
+      for (int e = 0; e < items; ++e) {
+        const int i = base + e * 64;
+        f(i, row.key(i, row.weight(i), row.pos != nullptr ? row.position(i) : 0));
+      }
     }
   };
 
-  // the greatest key that at least `budget` keys reach
-  uint32_t top = 0u;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t cand = top | (1u << bit);
-    int n = 0;
-    each([&](int, uint32_t k) { n += __popcll(__ballot(k >= cand)); });
-    if (before_and_all<WAVES>(counts[bit & 1], n, wave).y >= budget) top = cand;
+  // the range of the unprotected keys, and how many are protected
+  // (0 and kSafe step aside: one below 0 and one above kSafe wrap round)
+  uint32_t lo = 0xFFFFFFFFu, hi = 0u;
+  int safe = 0;
+  each([&](int, uint32_t k) {
+    lo = min(lo, k - 1u);
+    hi = max(hi, k + 1u);
+    safe += k == kSafe ? 1 : 0;
+  });
+  lo += 1u;
+  hi -= 1u;
+  safe = wave_last(wave_incl_scan(safe, lane));
+  lo = ~wave_umax(~lo);
+  hi = wave_umax(hi);
+  if (lane == 0) votes[0][wave] = make_int4((int)lo, (int)hi, safe, 0);
+  __syncthreads();
+  {
+    const int4 v = votes[0][lane & (WAVES - 1)];
+    lo = ~wave_umax(~(uint32_t)v.x);
+    hi = wave_umax((uint32_t)v.y);
+    safe = ring_sum<WAVES>(v.z);
+  }
+  // the greatest key that at least `budget` keys reach, how many keys are
+  // above it and how many equal it
+  uint32_t top = kSafe;
+  int above = 0, equal = safe;
+  if (safe < budget) {
+    int first = lo == hi ? 0 : 32 - __builtin_clz(lo ^ hi);  // bits in which the keys left differ
+    top = first == 32 ? 0u : hi >> first << first;           // the lowest that they can be
+    above = safe;
+    int members, shift;
+    do {
+      shift = first > kBinBits ? first - kBinBits : 0;
+      for (int i = threadIdx.x; i < 1 << kBinBits; i += THREADS) hist[i] = 0;
+      if (threadIdx.x == 0) gathered = 0;
+      __syncthreads();
+      each([&](int, uint32_t k) {
+        const uint32_t at = (k - top) >> shift;
+        if (at < 1u << (first - shift) && k - 1u < kSafe - 1u) atomicAdd(&hist[at], 1);  // (neither 0 nor protected)
+      });
+      __syncthreads();
+      if (wave == 0) {  // lane l: kLaneBins bins, lane 0 the highest
+        const int low = (63 - lane) * kLaneBins;
+        int own[kLaneBins], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kLaneBins; i += 4) {
+          const int4 v = *(const int4*)&hist[low + i];
+          own[i] = v.x, own[i + 1] = v.y, own[i + 2] = v.z, own[i + 3] = v.w;
+          sum += (v.x + v.y) + (v.z + v.w);
+        }
+        int run = above + wave_incl_scan(sum, lane) - sum;
+        if (run < budget && run + sum >= budget) {
+#pragma unroll
+          for (int i = kLaneBins - 1; i >= 0; --i) {
+            if (run < budget && run + own[i] >= budget) {
+              found[0] = low + i;
+              found[1] = run;
+              found[2] = own[i];
+            }
+            run += own[i];
+          }
+        }
+      }
+      __syncthreads();
+      top += (uint32_t)found[0] << shift;
+      above = found[1];
+      members = found[2];
+      first = shift;
+    } while (shift > 0 && members > kGather);
+    const int need = budget - above;  // 1 <= need <= members
+    if (shift == 0) {
+      equal = members;
+    } else {
+      // a lane's keys of the bin go to consecutive places
+      auto in = [&](uint32_t k) { return k - top < 1u << shift && k - 1u < kSafe - 1u; };
+      int mine = 0;
+      each([&](int, uint32_t k) { mine += in(k) ? 1 : 0; });
+      const int upto = wave_incl_scan(mine, lane);
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&gathered, wave_last(upto));
+      at = __builtin_amdgcn_readfirstlane(at) + upto - mine;
+      each([&](int, uint32_t k) {
+        if (in(k)) few[at++] = k;
+      });
+      __syncthreads();
+      if (wave == 0) {  // one wave: no barriers between its counts
+        constexpr int kOwn = kGather / 64;
+        uint32_t own[kOwn];
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) own[i] = i * 64 + lane < members ? few[i * 64 + lane] : 0u;
+        // (few keys by popcounts of masks; many by a count a lane, as each
+        // popcount waits for the scalar unit)
+        auto tally = [&](auto f) {
+          if (members <= 128) return __popcll(__ballot(f(own[0]))) + __popcll(__ballot(f(own[1])));
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < kOwn; ++i)
+            if (i * 64 < members) n += f(own[i]) ? 1 : 0;
+          return wave_last(wave_incl_scan(n, lane));
+        };
+        for (int bit = (shift + 1) & ~1; bit > 0;) {
+          bit -= 2;
+          const uint32_t c1 = plus(top, 1u << bit), c2 = plus(top, 2u << bit), c3 = plus(top, 3u << bit);
+          if (tally([&](uint32_t k) { return k >= c2; }) >= need)
+            top = tally([&](uint32_t k) { return k >= c3; }) >= need ? c3 : c2;
+          else if (tally([&](uint32_t k) { return k >= c1; }) >= need)
+            top = c1;
+        }
+        const int same = tally([&](uint32_t k) { return k == top; });
+        const int more = tally([&](uint32_t k) { return k > top; });
+        if (lane == 0) {
+          found[0] = (int)top;
+          found[1] = above + more;
+          found[2] = same;
+        }
+      }
+      __syncthreads();
+      top = (uint32_t)found[0];
+      above = found[1];
+      equal = found[2];
+    }
   }
   // of the keys equal to it, the lowest indices are kept
-  int above = 0, equal = 0;
-  each([&](int, uint32_t k) {
-    above += __popcll(__ballot(k > top));
-    equal += __popcll(__ballot(k == top));
-  });
-  const int all_above = before_and_all<WAVES>(counts[2], above, wave).y;
-  const int eq0 = before_and_all<WAVES>(counts[3], equal, wave).x;
-  const int want = budget - all_above;
-  // holes and movers of the waves before this one
-  int eq = eq0, holes = 0, movers = 0;
-  each([&](int i, uint32_t k) {
+  const int want = budget - above;
+  const bool ties = want < equal;
+  int eq = 0;
+  if (ties) {
+    int mine = 0;
+    each([&](int, uint32_t k) { mine += __popcll(__ballot(k == top)); });
+    eq = before_and_all<WAVES>(counts[1], mine, wave).x;
+  }
+  auto kept_of = [&](uint32_t k) {
+    if (!ties) return k >= top;
     const uint64_t em = __ballot(k == top);
     const bool kept = k > top || (k == top && eq + rank_in(em) < want);
     eq += __popcll(em);
-    holes += __popcll(__ballot(i < budget && !kept));
-    movers += __popcll(__ballot(i >= budget && kept));
-  });
-  const int hole0 = before_and_all<WAVES>(counts[0], holes, wave).x;
-  const int2 mv = before_and_all<WAVES>(counts[1], movers, wave);
-  // movers and holes meet in LDS, kListCap at a time
-  for (int at = 0; at == 0 || at < mv.y; at += kListCap) {
-    int r = mv.x;
-    eq = eq0;
-    each([&](int i, uint32_t k) {
-      const uint64_t em = __ballot(k == top);
-      const bool kept = k > top || (k == top && eq + rank_in(em) < want);
-      eq += __popcll(em);
-      const uint64_t mm = __ballot(i >= budget && kept);
-      const int mine = r + rank_in(mm) - at;
-      if (i >= budget && kept && mine >= 0 && mine < kListCap) list[mine] = i;
-      r += __popcll(mm);
-    });
-    __syncthreads();
-    r = hole0;
-    eq = eq0;
-    each([&](int i, uint32_t k) {
-      const uint64_t em = __ballot(k == top);
-      const bool kept = k > top || (k == top && eq + rank_in(em) < want);
-      eq += __popcll(em);
-      const uint64_t hm = __ballot(i < budget && !kept);
-      const int mine = r + rank_in(hm) - at;
-      if (i < budget) {
-        if (kept) {
-          if (at == 0) keep[i] = i;
-        } else if (mine >= 0 && mine < kListCap) {
-          keep[i] = list[mine];
-        }
+    return kept;
+  };
+
+  if constexpr (E > 0) {
+    // One bit an index, and the kept ones before each word of 64: a hole's rank
+    // is its index less the kept ones before it.
+    constexpr int kWords = THREADS * E / 64;
+    __shared__ uint64_t mask[kWords];
+    __shared__ int before[kWords];
+    __shared__ uint16_t list[THREADS * E / 2];  // at most half of the indices are movers
+    static_assert(THREADS * E <= 65536 && kWords <= THREADS, "indices of 16 bits, a word a thread");
+    uint32_t word_lo = 0u, word_hi = 0u;  // lane e: the wave's word e
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (e < items) {
+        const uint64_t m = __ballot(kept_of(reg[e]));
+        word_lo = lane == e ? (uint32_t)m : word_lo;
+        word_hi = lane == e ? (uint32_t)(m >> 32) : word_hi;
       }
-      r += __popcll(hm);
-    });
+    }
+    if (lane < items) mask[wave * items + lane] = (uint64_t)word_hi << 32 | word_lo;
     __syncthreads();
+    const int filled = WAVES * items;
+    const int mine = (int)threadIdx.x < filled ? __popcll(mask[threadIdx.x]) : 0;
+    const int upto = wave_incl_scan(mine, lane);
+    const int base0 = before_and_all<WAVES>(counts[2], wave_last(upto), wave).x;
+    if ((int)threadIdx.x < filled) before[threadIdx.x] = base0 + upto - mine;
+    __syncthreads();
+    const int words = (len + 63) >> 6, edge = budget >> 6;
+    const uint64_t low = (1ull << (budget & 63)) - 1;  // of word `edge`, the slots below budget
+    const int below = before[edge] + __popcll(mask[edge] & low);  // kept where they are
+    constexpr int kAhead = 4;  // words read ahead of the writes
+    for (int w0 = edge + wave; w0 < words; w0 += WAVES * kAhead) {
+      uint64_t m[kAhead];
+      int at[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int w = min(w0 + i * WAVES, words - 1);
+        m[i] = w0 + i * WAVES < words ? mask[w] : 0;
+        at[i] = before[w] - below;
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int idx = (w0 + i * WAVES) * 64 + lane;
+        if (((m[i] >> lane) & 1) != 0 && idx >= budget) list[at[i] + rank_in(m[i])] = (uint16_t)idx;
+      }
+    }
+    __syncthreads();
+    for (int w = wave; w * 64 < budget; w += WAVES) {
+      const uint64_t m = mask[w];
+      const int i = w * 64 + lane;
+      if (i < budget) keep[i] = ((m >> lane) & 1) != 0 ? i : (int)list[i - before[w] - rank_in(m)];
+    }
+  } else {
+    // holes and movers of the waves before this one
+    __shared__ int list[kListCap];
+    const int eq0 = eq;
+    auto each_kept = [&](auto f) {
+      eq = eq0;
+      each([&](int i, uint32_t k) { f(i, kept_of(k)); });
+    };
+    int holes = 0, movers = 0;
+    each_kept([&](int i, bool kept) {
+      holes += __popcll(__ballot(i < budget && !kept));
+      movers += __popcll(__ballot(i >= budget && kept));
+    });
+    const int hole0 = before_and_all<WAVES>(counts[2], holes, wave).x;
+    const int2 mv = before_and_all<WAVES>(counts[0], movers, wave);
+    // they meet in LDS, kListCap at a time
+    for (int at = 0; at == 0 || at < mv.y; at += kListCap) {
+      int r = mv.x - at;
+      each_kept([&](int i, bool kept) {
+        const bool mover = i >= budget && kept;
+        const uint64_t mm = __ballot(mover);
+        const int mine = r + rank_in(mm);
+        if (mover && mine >= 0 && mine < kListCap) list[mine] = i;
+        r += __popcll(mm);
+      });
+      __syncthreads();
+      r = hole0 - at;
+      each_kept([&](int i, bool kept) {
+        const bool hole = i < budget && !kept;
+        const uint64_t hm = __ballot(hole);
+        const int mine = r + rank_in(hm);
+        if (hole && mine >= 0 && mine < kListCap) keep[i] = list[mine];
+        if (i < budget && kept && at == 0) keep[i] = i;
+        r += __popcll(hm);
+      });
+      __syncthreads();
+    }
   }
 }
 
 // ---- move --------------------------------------------------------------------
 //
-// A workgroup takes kMoveSlots slots of one (sequence, account head): it
-// lists those whose token comes from elsewhere, moves their weights and
-// positions, and copies the listed rows of every KV head of the account
-// (one, or all of them).
+// Weights and positions move with a lane a slot.  K and V rows: where channels
+// are contiguous a row moves as 16-byte pieces.  Where a channel's tokens are
+// contiguous (channel-major V) it is D single elements; when most slots of a
+// 16-token run change, as when a prompt is cut, a lane takes a channel instead,
+// reads its 16 tokens from where each belongs, and writes the run whole
+// (unmoved tokens with their own value).  Two kernels: a wave a run of 16
+// slots, everything it moves in flight at once, for calls that may move much;
+// and 256 slots scanned a workgroup for those that move few (a decode batch
+// evicting its latest block), whose time is the scan.
 
-constexpr int kMoveSlots = 256;
+enum MoveMode : int { kRows = 0, kTile = 1, kElements = 2 };
 
+// Element offset of a slot in a cache, without head and channel.
+__device__ __forceinline__ int64_t slot_at(const int64_t* s, int blk, int off) {
+  return (int64_t)blk * s[0] + (int64_t)off * s[1];
+}
+
+// Slot j of sequence b, account head h: its source, and where both lie.
+struct MoveSlot {
+  int src_blk, src_off, dst_blk, dst_off;
+  bool moved;
+};
+
+// Looks slot j up and, with `account`, moves its weight and position.
+__device__ __forceinline__ MoveSlot move_slot(const EvictMoveParams& p, int b, int h, int j, bool account) {
+  MoveSlot m{0, 0, 0, 0, false};
+  // (a source outside the tables cannot come from a selection)
+  const int cap = min(p.Mb * p.bs, p.S);
+  if (j >= min(p.budget, cap)) return m;
+  const int src = p.keep[(int64_t)b * p.k_sb + (int64_t)h * p.k_sh + j];
+  if (src < 0 || src >= cap) return m;
+  if (account && p.positions != nullptr) {
+    const int kept = p.kept[(int64_t)b * p.kept_s];
+    if (src != j || j >= kept) {
+      const int raw = p.lens[(int64_t)b * p.l_s], len = raw < 0 ? 0 : (raw < p.S ? raw : p.S);
+      int32_t* pos = p.positions + (int64_t)b * p.p_sb + (int64_t)h * p.p_sh;
+      pos[j] = src < kept ? pos[src] : p.seen[(int64_t)b * p.seen_s] - len + src;
+    }
+  }
+  if (src == j) return m;
+  if (account && p.weights != nullptr) {
+    float* a = p.weights + (int64_t)b * p.w_sb + (int64_t)h * p.w_sh;
+    a[j] = a[src];
+  }
+  const int32_t* t = p.tables + (int64_t)b * p.t_sb;
+  const int jb = (int)((uint32_t)j / (uint32_t)p.bs), sb = (int)((uint32_t)src / (uint32_t)p.bs);
+  m.dst_blk = t[(int64_t)jb * p.t_sm];
+  m.src_blk = t[(int64_t)sb * p.t_sm];
+  m.dst_off = j - jb * p.bs;
+  m.src_off = src - sb * p.bs;
+  m.moved = m.dst_blk >= 0 && m.dst_blk < p.NB && m.src_blk >= 0 && m.src_blk < p.NB;
+  return m;
+}
+
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// A wave's 16 slots (lanes 0..15): rows as pieces.  Loads first, kRowsInFlight
+// pieces a lane, then stores.
 template <class T>
-__device__ __forceinline__ void copy_rows(const EvictMoveParams& p, int which, int h0, int nh, const int2* from_to,
-                                          int n) {
-  T* base = (T*)p.cache[which];
+__device__ __forceinline__ void move_rows(const EvictMoveParams& p, int which, int h, const MoveSlot& m, uint32_t bits,
+                                          int lane) {
+  constexpr int kInFlight = 4, kElems = 16 / (int)sizeof(T);
   const int64_t* s = p.c_s[which];
-  const int per = nh * p.D;
-  for (int u = threadIdx.x; u < n * per; u += 256) {
-    const int k = u / per, r = u - k * per;
-    const int h = h0 + r / p.D, d = r % p.D;
-    const int2 m = from_to[k];
-    const int64_t src = (int64_t)(m.x / p.bs) * s[0] + (int64_t)(m.x % p.bs) * s[1];
-    const int64_t dst = (int64_t)(m.y / p.bs) * s[0] + (int64_t)(m.y % p.bs) * s[1];
-    const int64_t at = (int64_t)h * s[2] + (int64_t)d * s[3];
-    base[dst + at] = base[src + at];
+  T* base = (T*)p.cache[which] + (int64_t)h * s[2];
+  const int per = p.D / kElems, n = 16 * per;
+  for (int u0 = 0; u0 < n; u0 += 64 * kInFlight) {
+    uint4 v[kInFlight];
+    T* to[kInFlight];
+    bool live[kInFlight];
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) {
+      const int u = u0 + i * 64 + lane, l = min(u, n - 1) / per, c = u - l * per;
+      live[i] = u < n && ((bits >> l) & 1u) != 0;
+      const int sb = __shfl(m.src_blk, l, 64), so = __shfl(m.src_off, l, 64);
+      const int db = __shfl(m.dst_blk, l, 64), dof = __shfl(m.dst_off, l, 64);
+      to[i] = base + slot_at(s, db, dof) + c * kElems;
+      if (live[i]) v[i] = *(const uint4*)(base + slot_at(s, sb, so) + c * kElems);
+    }
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i)
+      if (live[i]) *(uint4*)to[i] = v[i];
   }
 }
 
+// The same for 16 tokens of a block in channel-major storage.
 template <class T>
-__global__ __launch_bounds__(256) void evict_move_kernel(EvictMoveParams p) {
-  __shared__ int2 list[kMoveSlots];  // (source, destination) as block * bs + offset
-  __shared__ int count;
-  const int chunks = (p.budget + kMoveSlots - 1) / kMoveSlots;
-  const int bh = blockIdx.x / chunks, b = bh / p.Hw, h = bh - b * p.Hw;
-  const int j = (blockIdx.x - bh * chunks) * kMoveSlots + threadIdx.x;
-  if (threadIdx.x == 0) count = 0;
-  __syncthreads();
-  const int raw = p.lens[(int64_t)b * p.l_s];
-  const int src = j < p.budget ? p.keep[(int64_t)b * p.k_sb + (int64_t)h * p.k_sh + j] : -1;
-  // (a source outside the tables cannot come from a selection)
-  const int cap = p.Mb * p.bs;
-  if (src >= 0 && src < cap && src < p.S && j < cap && j < p.S) {
-    if (p.positions != nullptr) {
-      const int kept = p.kept[(int64_t)b * p.kept_s];
-      if (src != j || j >= kept) {
-        const int len = raw < 0 ? 0 : (raw < p.S ? raw : p.S);
-        int32_t* pos = p.positions + (int64_t)b * p.p_sb + (int64_t)h * p.p_sh;
-        pos[j] = src < kept ? pos[src] : p.seen[(int64_t)b * p.seen_s] - len + src;
-      }
+__device__ __forceinline__ void move_tile(const EvictMoveParams& p, int which, int h, const MoveSlot& m, uint32_t bits,
+                                          int lane) {
+  const int64_t* s = p.c_s[which];
+  T* base = (T*)p.cache[which] + (int64_t)h * s[2];
+  const int l0 = __builtin_ctz(bits);
+  const int64_t run = slot_at(s, lane_value(m.dst_blk, l0), lane_value(m.dst_off, l0) - l0);
+  for (int d = lane; d < p.D; d += 64) {
+    T* dst = base + run + (int64_t)d * s[3];
+    union {
+      uint4 q[sizeof(T)];
+      T e[16];
+    } r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) r.q[i] = ((const uint4*)dst)[i];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if ((bits >> i) & 1u)
+        r.e[i] = base[slot_at(s, lane_value(m.src_blk, i), lane_value(m.src_off, i)) + (int64_t)d * s[3]];
     }
-    if (src != j) {
-      if (p.weights != nullptr) {
-        float* w = p.weights + (int64_t)b * p.w_sb + (int64_t)h * p.w_sh;
-        w[j] = w[src];
-      }
-      const int32_t* t = p.tables + (int64_t)b * p.t_sb;
-      const int from = t[(int64_t)(src / p.bs) * p.t_sm], to = t[(int64_t)(j / p.bs) * p.t_sm];
-      if (from >= 0 && from < p.NB && to >= 0 && to < p.NB) {
-        const int at = atomicAdd(&count, 1);  // (the order of independent copies)
-        list[at] = make_int2(from * p.bs + src % p.bs, to * p.bs + j % p.bs);
-      }
-    }
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) ((uint4*)dst)[i] = r.q[i];
   }
+}
+
+// A wave a run of 16 slots of one sequence and KV head (K in rows, V in rows or
+// tiles, blocks of a multiple of 16 tokens).
+template <class T>
+__global__ __launch_bounds__(256) void evict_move_run_kernel(EvictMoveParams p, int64_t waves) {
+  const int lane = threadIdx.x & 63;
+  const int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (w >= waves) return;
+  const int per = (p.budget + 15) >> 4;
+  const int bh = (int)(w / per), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const int j = ((int)(w - (int64_t)bh * per) << 4) + lane;
+  MoveSlot m{0, 0, 0, 0, false};
+  if (lane < 16) m = move_slot(p, b, p.Hw == 1 ? 0 : hk, j, p.Hw > 1 || hk == 0);
+  const uint32_t bits = (uint32_t)__ballot(m.moved);
+  if (bits == 0u) return;
+  move_rows<T>(p, 0, hk, m, bits, lane);
+  if (p.mode[1] == kRows) move_rows<T>(p, 1, hk, m, bits, lane);
+  else move_tile<T>(p, 1, hk, m, bits, lane);
+}
+
+// The listed rows of heads [h0, h0 + nh), by pieces (E = uint4) or elements.
+template <class E, class T>
+__device__ __forceinline__ void copy_listed(const EvictMoveParams& p, int which, int h0, int nh, const int4* list,
+                                            int n) {
+  constexpr int kInFlight = 8, kElems = (int)(sizeof(E) / sizeof(T));
+  const int64_t* s = p.c_s[which];
+  T* base = (T*)p.cache[which];
+  const int per = p.D / kElems, row = nh * per, total = n * row;
+  for (int base0 = 0; base0 < total; base0 += 256 * kInFlight) {
+    E v[kInFlight];
+    T* to[kInFlight];
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) {
+      if (base0 + i * 256 < total) {
+      const uint32_t u = (uint32_t)min(base0 + i * 256 + (int)threadIdx.x, total - 1), k = u / (uint32_t)row, r = u - k * (uint32_t)row;
+      const uint32_t hh = r / (uint32_t)per, c = r - hh * (uint32_t)per;
+      const int4 m = list[k];
+      const int64_t at = (int64_t)(h0 + (int)hh) * s[2] + (int64_t)(c * kElems) * s[3];
+      v[i] = *(const E*)(base + slot_at(s, m.x, m.y) + at);
+      to[i] = base + slot_at(s, m.z, m.w) + at;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i)
+      if (base0 + i * 256 + (int)threadIdx.x < total) *(E*)to[i] = v[i];
+  }
+}
+
+// 256 slots a workgroup; any strides.
+template <class T>
+__global__ __launch_bounds__(256) void evict_move_list_kernel(EvictMoveParams p) {
+  __shared__ int4 list[256];  // source block and offset, destination block and offset
+  __shared__ int count[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per = (p.budget + 255) >> 8;
+  const int bh = blockIdx.x / per, b = bh / p.Hw, h = bh - b * p.Hw;
+  const MoveSlot m = move_slot(p, b, h, (int)(blockIdx.x - bh * per) * 256 + (int)threadIdx.x, true);
+  const uint64_t bits = __ballot(m.moved);
+  if (lane == 0) count[wave] = __popcll(bits);
   __syncthreads();
-  const int n = count;
+  int at = 0, n = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    at += i < wave ? count[i] : 0;
+    n += count[i];
+  }
   if (n == 0) return;
+  if (m.moved) list[at + rank_in(bits)] = make_int4(m.src_blk, m.src_off, m.dst_blk, m.dst_off);
+  __syncthreads();
   const int nh = p.Hw == 1 ? p.Hkv : 1, h0 = p.Hw == 1 ? 0 : h;
-  copy_rows<T>(p, 0, h0, nh, list, n);
-  copy_rows<T>(p, 1, h0, nh, list, n);
+  for (int c = 0; c < 2; ++c) {
+    if (p.mode[c] == kRows) copy_listed<uint4, T>(p, c, h0, nh, list, n);
+    else copy_listed<T, T>(p, c, h0, nh, list, n);
+  }
 }
 
 template <int THREADS, int E>
@@ -273,13 +601,35 @@ int32_t launch_evict_select(const EvictSelectParams& p, hipStream_t stream) {
   return launch_select_t<1024, 0>(p, stream);
 }
 
-int32_t launch_evict_move(const EvictMoveParams& p, int elem_bytes, hipStream_t stream) {
-  const dim3 grid((unsigned)(ceil_div(p.budget, kMoveSlots) * p.Hw * p.B));
+int32_t launch_evict_move(const EvictMoveParams& q, int elem_bytes, hipStream_t stream) {
+  EvictMoveParams p = q;
+  for (int c = 0; c < 2; ++c) {
+    const int64_t* s = p.c_s[c];
+    auto whole = [&](int64_t stride) { return (stride * elem_bytes) % 16 == 0; };
+    const bool base = ((uintptr_t)p.cache[c] & 15) == 0 && whole(s[0]) && whole(s[2]);
+    if (base && s[3] == 1 && whole(s[1]) && whole(p.D)) p.mode[c] = kRows;
+    else if (base && s[1] == 1 && whole(s[3]) && p.bs % 16 == 0) p.mode[c] = kTile;
+    else p.mode[c] = kElements;
+  }
+  // Runs of 16 where many slots of a sequence may move: up to S - budget of
+  // them, the tokens past the new end.
+  const bool runs = p.mode[0] == kRows && p.mode[1] != kElements && p.bs % 16 == 0 && (int64_t)(p.S - p.budget) * 4 > p.budget;
   ProfileScope prof("cf_evict_move", stream);
-  switch (elem_bytes) {
-    case 1: CF_LAUNCH((evict_move_kernel<uint8_t>), grid, dim3(256), 0, stream, p); break;
-    case 2: CF_LAUNCH((evict_move_kernel<uint16_t>), grid, dim3(256), 0, stream, p); break;
-    default: CF_LAUNCH((evict_move_kernel<uint32_t>), grid, dim3(256), 0, stream, p); break;
+  if (runs) {
+    const int64_t waves = ceil_div(p.budget, 16) * p.Hkv * p.B;
+    const dim3 grid((unsigned)ceil_div(waves, 4));
+    switch (elem_bytes) {
+      case 1: CF_LAUNCH((evict_move_run_kernel<uint8_t>), grid, dim3(256), 0, stream, p, waves); break;
+      case 2: CF_LAUNCH((evict_move_run_kernel<uint16_t>), grid, dim3(256), 0, stream, p, waves); break;
+      default: CF_LAUNCH((evict_move_run_kernel<uint32_t>), grid, dim3(256), 0, stream, p, waves); break;
+    }
+  } else {
+    const dim3 grid((unsigned)(ceil_div(p.budget, 256) * p.Hw * p.B));
+    switch (elem_bytes) {
+      case 1: CF_LAUNCH((evict_move_list_kernel<uint8_t>), grid, dim3(256), 0, stream, p); break;
+      case 2: CF_LAUNCH((evict_move_list_kernel<uint16_t>), grid, dim3(256), 0, stream, p); break;
+      default: CF_LAUNCH((evict_move_list_kernel<uint32_t>), grid, dim3(256), 0, stream, p); break;
+    }
   }
   CF_HIP_CHECK(hipGetLastError());
   return CF_OK;

@@ -43,6 +43,7 @@ struct EvictMoveParams {
   int64_t kept_s, seen_s;
   int64_t NB;
   int B, Hw, Hkv, D, bs, Mb, S, budget;
+  int mode[2];  // how K and V rows move; set by the launcher
 };
 
 int32_t launch_evict_select(const EvictSelectParams& p, hipStream_t stream);

@@ -179,3 +179,23 @@ def test_nothing_to_do(gpu):
     assert keep.shape == (0, 2, 8) and new.shape == (0,)
     evict_move(keep, lens, torch.zeros(0, 4, dtype=torch.int32, device=gpu), k, v)
     assert torch.equal(_raw(k), _raw(before[0])) and torch.equal(_raw(v), _raw(before[1]))
+
+
+def test_keys_that_differ_below_their_sign_up_to_nan(gpu):
+    """The search's candidates past the greatest key: no negative weight, and NaN as the threshold."""
+    w = _weights(gpu, 1, 3, 3000, 31, "plain")
+    w[0, 0, ::3] = float("nan")
+    w[0, 1, ::3] = float("inf")
+    w[0, 2, ::2] = 0.0
+    _check_select(w, [3000], 700, 4, 64)
+    _check_select(w, [3000], 1200, 4, 64)
+
+
+@pytest.mark.parametrize("budget", [300, 1500, 2500, 3900])
+def test_weights_a_few_last_bits_apart(gpu, budget):
+    """More keys of one bin than are searched apart, next to keys a few units above them."""
+    g = torch.Generator(device=gpu).manual_seed(6)
+    steps = torch.tensor([0, 1, 2, 3, 8, 9, 11, 5000], device=gpu)
+    w = 1.0 + steps[torch.randint(0, 8, (1, 2, 4000), generator=g, device=gpu)] * 2.0**-23
+    w[0, 1, ::2] = 5.0
+    _check_select(w.float(), [4000], budget, 2, 30)
