@@ -259,7 +259,7 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictSelectParams
         for (int i = 0; i < kOwn; ++i) own[i] = i * 64 + lane < members ? few[i * 64 + lane] : 0u;
         // (few keys by popcounts of masks; many by a count a lane, as each
         // popcount waits for the scalar unit)
-        auto tally = [&](auto f) {
+        auto tally = [&](auto f) -> int {
           if (members <= 128) return __popcll(__ballot(f(own[0]))) + __popcll(__ballot(f(own[1])));
           int n = 0;
 #pragma unroll
