@@ -36,6 +36,14 @@ struct Lib {
   decltype(&cf_fp8_scale_quantize) scale_quantize = nullptr;
   decltype(&cf_fp8_dequantize_kv) dequantize_kv = nullptr;
   decltype(&cf_stage_from_host) stage = nullptr;
+  decltype(&cf_paged_decode_weights_workspace_bytes) decode_weights_ws = nullptr;
+  decltype(&cf_paged_decode_weights) decode_weights = nullptr;
+  decltype(&cf_chunk_weights_workspace_bytes) chunk_weights_ws = nullptr;
+  decltype(&cf_chunk_weights) chunk_weights = nullptr;
+  decltype(&cf_rotary) rotary = nullptr;
+  decltype(&cf_rotary_cache_write) rotary_write = nullptr;
+  decltype(&cf_evict_select) evict_select = nullptr;
+  decltype(&cf_evict_move) evict_move = nullptr;
 };
 Lib g_lib;
 PyObject* g_raw_stream = nullptr;        // device index -> hipStream_t of the current stream
@@ -461,6 +469,196 @@ PyObject* stage_tables(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// An output: the caller's tensor, or a new one of `sizes`.
+struct Output {
+  at::Tensor fresh;
+  PyObject* given;
+  CfTensor d;
+
+  Output(PyObject* o, const Call& call, at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) : given(o) {
+    if (o != Py_None) {
+      d = call.in(o);
+      return;
+    }
+    fresh = new_tensor(sizes, dtype, like);
+    d = describe(fresh);
+  }
+  PyObject* result() const {
+    if (given == Py_None) return THPVariable_Wrap(fresh);
+    Py_INCREF(given);
+    return given;
+  }
+};
+
+// (q, k_cache, v_cache, block_tables, seq_lens, weights, scale, block_size,
+// decay, k_scale, v_scale, out, workspace, shared_prefix_lens) -> out
+PyObject* paged_decode_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(args, n, 14, [](PyObject* const* a) -> PyObject* {
+    const at::Tensor& q = tensor_of(a[0]);
+    const at::Tensor& k = tensor_of(a[1]);
+    const at::Tensor& bt = tensor_of(a[3]);
+    if (q.dim() != 3 || k.dim() != 4 || bt.dim() != 2) throw Slow{};
+    const Call call(q);
+    const CfTensor dq = call.in(a[0]), dk = call.in(a[1]), dv = call.in(a[2]), dt = call.in(a[3]), dl = call.in(a[4]);
+    CfTensor dw = call.in(a[5]), dks{}, dvs{}, dsh{};
+    const double scale = as_float(a[6]), decay = as_float(a[8]);
+    const int64_t bs = as_int(a[7]);
+    if (bs != (int32_t)bs) throw Slow{};
+    if (a[9] != Py_None) dks = call.in(a[9]);
+    if (a[10] != Py_None) dvs = call.in(a[10]);
+    if (a[13] != Py_None) dsh = call.in(a[13]);
+    uint64_t need = 0;
+    if (g_lib.decode_weights_ws(q.size(0), q.size(1), k.size(2), q.size(2), bt.size(1), (int32_t)bs, &need) != CF_OK)
+      throw Slow{};
+    if (a[12] != Py_None && tensor_of(a[12]).get_device() != call.device) throw Slow{};
+    const Workspace ws(a[12], need, call, a[0]);
+    Output out(a[11], call, q.sizes(), q.scalar_type(), q);
+    const int32_t rc = without_gil([&] {
+      return g_lib.decode_weights(&dq, &dk, &dv, &dt, &dl, opt(a[13], dsh), opt(a[9], dks), opt(a[10], dvs),
+                                  (float)scale, (int32_t)bs, &dw, (float)decay, &out.d, ws.ptr, need, call.stream);
+    });
+    return rc != CF_OK ? PyLong_FromLong(rc) : out.result();
+  });
+}
+
+// (q, k_cache, block_tables, seq_lens, q_start, weights, scale, block_size,
+// decay, observe, k_scale, workspace) -> weights
+PyObject* chunk_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(args, n, 12, [](PyObject* const* a) -> PyObject* {
+    const at::Tensor& q = tensor_of(a[0]);
+    const at::Tensor& k = tensor_of(a[1]);
+    const at::Tensor& bt = tensor_of(a[2]);
+    if (q.dim() != 3 || k.dim() != 4 || bt.dim() != 2) throw Slow{};
+    const Call call(q);
+    const CfTensor dq = call.in(a[0]), dk = call.in(a[1]), dt = call.in(a[2]), dl = call.in(a[3]), ds = call.in(a[4]);
+    CfTensor dw = call.in(a[5]), dks{};
+    const double scale = as_float(a[6]), decay = as_float(a[8]);
+    const int64_t bs = as_int(a[7]), observe = as_int(a[9]);
+    if (bs != (int32_t)bs || observe != (int32_t)observe) throw Slow{};
+    if (a[10] != Py_None) dks = call.in(a[10]);
+    uint64_t need = 0;
+    if (g_lib.chunk_weights_ws(q.size(0), bt.size(0), q.size(1), k.size(2), q.size(2), bt.size(1), (int32_t)bs,
+                               &need) != CF_OK)
+      throw Slow{};
+    if (a[11] != Py_None && tensor_of(a[11]).get_device() != call.device) throw Slow{};
+    const Workspace ws(a[11], need, call, a[0]);
+    const int32_t rc = without_gil([&] {
+      return g_lib.chunk_weights(&dq, &dk, &dt, &dl, &ds, opt(a[10], dks), (float)scale, (int32_t)bs, (int32_t)observe,
+                                 &dw, (float)decay, ws.ptr, need, call.stream);
+    });
+    if (rc != CF_OK) return PyLong_FromLong(rc);
+    Py_INCREF(a[5]);
+    return a[5];
+  });
+}
+
+// The axes of a rotary call: a tuple or list of the sections, or None.
+struct Sections {
+  int32_t n[CF_ROTARY_MAX_AXES] = {};
+  const int32_t* ptr = nullptr;
+  int32_t axes = 1;
+
+  Sections(PyObject* o, const at::Tensor& positions) {
+    const int64_t rows = positions.dim() == 2 ? positions.size(0) : 1;
+    if (rows < 1 || rows > CF_ROTARY_MAX_AXES) throw Slow{};
+    axes = (int32_t)rows;
+    if (o == Py_None) return;
+    const bool tuple = PyTuple_CheckExact(o);
+    if (!tuple && !PyList_CheckExact(o)) throw Slow{};
+    if ((tuple ? PyTuple_GET_SIZE(o) : PyList_GET_SIZE(o)) != axes) throw Slow{};
+    for (int32_t i = 0; i < axes; ++i) {
+      const int64_t v = as_int(tuple ? PyTuple_GET_ITEM(o, i) : PyList_GET_ITEM(o, i));
+      if (v != (int32_t)v) throw Slow{};
+      n[i] = (int32_t)v;
+    }
+    ptr = n;
+  }
+};
+
+// (x, positions, inv_freq, sections, flags, rotary_scale, out) -> out
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(args, n, 7, [](PyObject* const* a) -> PyObject* {
+    const at::Tensor& x = tensor_of(a[0]);
+    const Call call(x);
+    const CfTensor dx = call.in(a[0]), dp = call.in(a[1]), df = call.in(a[2]);
+    const Sections sec(a[3], tensor_of(a[1]));
+    const int32_t flags = (int32_t)as_int(a[4]);
+    const double scale = as_float(a[5]);
+    Output out(a[6], call, x.sizes(), x.scalar_type(), x);
+    const int32_t rc = without_gil([&] {
+      return g_lib.rotary(&dx, &dp, &df, sec.ptr, sec.axes, flags, (float)scale, &out.d, call.stream);
+    });
+    return rc != CF_OK ? PyLong_FromLong(rc) : out.result();
+  });
+}
+
+// (q, k_new, v_new, positions, inv_freq, slot_mapping, k_cache, v_cache,
+// sections, flags, rotary_scale, k_scale, v_scale, out) -> out
+PyObject* rotary_cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(args, n, 14, [](PyObject* const* a) -> PyObject* {
+    const at::Tensor& q = tensor_of(a[0]);
+    const Call call(q);
+    const CfTensor dq = call.in(a[0]), dk = call.in(a[1]), dv = call.in(a[2]), dp = call.in(a[3]), df = call.in(a[4]),
+                   ds = call.in(a[5]);
+    CfTensor dkc = call.in(a[6]), dvc = call.in(a[7]), dks{}, dvs{};
+    const Sections sec(a[8], tensor_of(a[3]));
+    const int32_t flags = (int32_t)as_int(a[9]);
+    const double scale = as_float(a[10]);
+    if (a[11] != Py_None) dks = call.flat(a[11]);
+    if (a[12] != Py_None) dvs = call.flat(a[12]);
+    Output out(a[13], call, q.sizes(), q.scalar_type(), q);
+    const int32_t rc = without_gil([&] {
+      return g_lib.rotary_write(&dq, &dk, &dv, &dp, &df, sec.ptr, sec.axes, flags, (float)scale, &ds, &dkc, &dvc,
+                                opt(a[11], dks), opt(a[12], dvs), &out.d, call.stream);
+    });
+    return rc != CF_OK ? PyLong_FromLong(rc) : out.result();
+  });
+}
+
+// (weights, seq_lens, budget, sink, recent, positions, kept, seen, keep,
+// new_lens) -> (keep, new_lens)
+PyObject* evict_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(args, n, 10, [](PyObject* const* a) -> PyObject* {
+    const at::Tensor& w = tensor_of(a[0]);
+    if (w.dim() != 3) throw Slow{};
+    const Call call(w);
+    const CfTensor dw = call.in(a[0]), dl = call.in(a[1]);
+    const int64_t budget = as_int(a[2]), sink = as_int(a[3]), recent = as_int(a[4]);
+    if (budget < 1 || budget != (int32_t)budget || sink != (int32_t)sink || recent != (int32_t)recent) throw Slow{};
+    CfTensor dp{}, dk{}, ds{};
+    if (a[5] != Py_None) dp = call.in(a[5]);
+    if (a[6] != Py_None) dk = call.in(a[6]);
+    if (a[7] != Py_None) ds = call.in(a[7]);
+    if (a[8] != Py_None && (tensor_of(a[8]).dim() != 3 || tensor_of(a[8]).size(2) != budget)) throw Slow{};
+    Output keep(a[8], call, {w.size(0), w.size(1), budget}, at::kInt, w);
+    Output lens(a[9], call, {w.size(0)}, at::kInt, w);
+    const int32_t rc = without_gil([&] {
+      return g_lib.evict_select(&dw, &dl, opt(a[5], dp), opt(a[6], dk), opt(a[7], ds), (int32_t)sink, (int32_t)recent,
+                                &keep.d, &lens.d, call.stream);
+    });
+    if (rc != CF_OK) return PyLong_FromLong(rc);
+    return Py_BuildValue("(NN)", keep.result(), lens.result());
+  });
+}
+
+// (keep, seq_lens, block_tables, k_cache, v_cache, weights, positions, kept,
+// seen) -> 0
+PyObject* evict_move(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(args, n, 9, [](PyObject* const* a) -> PyObject* {
+    const Call call(tensor_of(a[0]));
+    const CfTensor dk = call.in(a[0]), dl = call.in(a[1]), dt = call.in(a[2]);
+    CfTensor dkc = call.in(a[3]), dvc = call.in(a[4]), dw{}, dp{}, dkept{}, dseen{};
+    if (a[5] != Py_None) dw = call.in(a[5]);
+    if (a[6] != Py_None) dp = call.in(a[6]);
+    if (a[7] != Py_None) dkept = call.in(a[7]);
+    if (a[8] != Py_None) dseen = call.in(a[8]);
+    return PyLong_FromLong(without_gil([&] {
+      return g_lib.evict_move(&dk, &dl, &dt, &dkc, &dvc, a[5] == Py_None ? nullptr : &dw,
+                              a[6] == Py_None ? nullptr : &dp, opt(a[7], dkept), opt(a[8], dseen), call.stream);
+    }));
+  });
+}
+
 template <class T>
 bool take_address(PyObject* addrs, const char* name, T* fn) {
   PyObject* v = PyDict_GetItemString(addrs, name);
@@ -486,7 +684,15 @@ PyObject* bind(PyObject*, PyObject* args) {
       !take_address(addrs, "cf_kv_write_fp8", &l.kv_write) ||
       !take_address(addrs, "cf_fp8_scale_quantize", &l.scale_quantize) ||
       !take_address(addrs, "cf_fp8_dequantize_kv", &l.dequantize_kv) ||
-      !take_address(addrs, "cf_stage_from_host", &l.stage))
+      !take_address(addrs, "cf_stage_from_host", &l.stage) ||
+      !take_address(addrs, "cf_paged_decode_weights_workspace_bytes", &l.decode_weights_ws) ||
+      !take_address(addrs, "cf_paged_decode_weights", &l.decode_weights) ||
+      !take_address(addrs, "cf_chunk_weights_workspace_bytes", &l.chunk_weights_ws) ||
+      !take_address(addrs, "cf_chunk_weights", &l.chunk_weights) ||
+      !take_address(addrs, "cf_rotary", &l.rotary) ||
+      !take_address(addrs, "cf_rotary_cache_write", &l.rotary_write) ||
+      !take_address(addrs, "cf_evict_select", &l.evict_select) ||
+      !take_address(addrs, "cf_evict_move", &l.evict_move))
     return nullptr;
   g_lib = l;
   for (auto [slot, obj] : {std::pair{&g_raw_stream, raw}, std::pair{&g_current_device, cur},
@@ -509,6 +715,12 @@ PyMethodDef kMethods[] = {
     CF_FAST(scale_quantize),
     CF_FAST(dequantize_kv),
     CF_FAST(stage_tables),
+    CF_FAST(paged_decode_weights),
+    CF_FAST(chunk_weights),
+    CF_FAST(rotary),
+    CF_FAST(rotary_cache_write),
+    CF_FAST(evict_select),
+    CF_FAST(evict_move),
     {nullptr, nullptr, 0, nullptr},
 };
 #undef CF_FAST

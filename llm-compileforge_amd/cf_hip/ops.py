@@ -280,6 +280,12 @@ def paged_decode_weights(
     what the entry held (nothing for the newest token) plus the weights of its
     query heads.  workspace: decode_weights_workspace_bytes() bytes, by default
     a cached one per (device, stream)."""
+    if _on_gpu(q):
+        r = _fast().paged_decode_weights(q, k_cache, v_cache, block_tables, seq_lens, weights, float(scale),
+                                         int(block_size), float(decay), k_scale, v_scale, out, workspace,
+                                         shared_prefix_lens)
+        if r is not None:
+            return _result(r, "cf_paged_decode_weights")
     given = [("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables),
              ("seq_lens", seq_lens), ("weights", weights)]
     given += [(n, t) for n, t in (("k_scale", k_scale), ("v_scale", v_scale), ("out", out), ("workspace", workspace),
@@ -404,6 +410,11 @@ def chunk_weights(
     observe > 0 only each chunk's last `observe` rows count.  workspace:
     chunk_weights_workspace_bytes() bytes, by default a cached one per
     (device, stream)."""
+    if _on_gpu(q):
+        r = _fast().chunk_weights(q, k_cache, block_tables, seq_lens, q_start, weights, float(scale), int(block_size),
+                                  float(decay), int(observe), k_scale, workspace)
+        if r is not None:
+            return _result(r, "cf_chunk_weights")
     given = [("q", q), ("k_cache", k_cache), ("block_tables", block_tables), ("seq_lens", seq_lens),
              ("q_start", q_start), ("weights", weights)]
     given += [(n, t) for n, t in (("k_scale", k_scale), ("workspace", workspace)) if t is not None]
@@ -740,6 +751,11 @@ def rotary(
 ) -> torch.Tensor:
     """x [T, H, D] with its channel pairs turned by positions [T] or [axes, T]
     (int32 or int64) times inv_freq [pairs] (float32); see cf_hip.h."""
+    if _on_gpu(x) and axis_order in _AXIS_ORDERS:
+        r = _fast().rotary(x, positions, inv_freq, sections, _AXIS_ORDERS[axis_order] | (2 if interleaved else 0),
+                           float(rotary_scale), out)
+        if r is not None:
+            return _result(r, "cf_rotary")
     given = [("x", x), ("positions", positions), ("inv_freq", inv_freq)] + ([("out", out)] if out is not None else [])
     for name, t in given:
         _require_device(name, t)
@@ -775,6 +791,12 @@ def rotary_cache_write(
     """Rotates q [T, Hq, D] (returned) and k_new [T, Hkv, D], and writes the
     rotated keys and v_new to the paged caches at slot_mapping [T], in one
     launch.  Slots outside the cache are skipped; slots must be distinct."""
+    if _on_gpu(q) and axis_order in _AXIS_ORDERS:
+        r = _fast().rotary_cache_write(q, k_new, v_new, positions, inv_freq, slot_mapping, k_cache, v_cache, sections,
+                                       _AXIS_ORDERS[axis_order] | (2 if interleaved else 0), float(rotary_scale),
+                                       k_scale, v_scale, out)
+        if r is not None:
+            return _result(r, "cf_rotary_cache_write")
     given = [("q", q), ("k_new", k_new), ("v_new", v_new), ("positions", positions), ("inv_freq", inv_freq),
              ("slot_mapping", slot_mapping), ("k_cache", k_cache), ("v_cache", v_cache)]
     given += [(n, t) for n, t in (("k_scale", k_scale), ("v_scale", v_scale), ("out", out)) if t is not None]
@@ -816,6 +838,11 @@ def evict_select(
     new_lens[b] = min(seq_lens[b], budget): the first `sink` and last `recent`
     positions, then the greatest weights, equal ones by the lower slot.
     """
+    if _on_gpu(weights):
+        r = _fast().evict_select(weights, seq_lens, int(budget), int(sink), int(recent), positions, kept, seen, keep,
+                                 new_lens)
+        if r is not None:
+            return _result(r, "cf_evict_select")
     budget, sink, recent = _int32("budget", int(budget)), _int32("sink", int(sink)), _int32("recent", int(recent))
     given = [("weights", weights), ("seq_lens", seq_lens)]
     given += [(n, t) for n, t in (("positions", positions), ("kept", kept), ("seen", seen), ("keep", keep),
@@ -856,6 +883,11 @@ def evict_move(
     place: K and V (any layout; e4m3fn codes as they are) and, where given, the
     weights and positions of their slots.  The destinations must be the
     sequence's own blocks."""
+    if _on_gpu(keep):
+        r = _fast().evict_move(keep, seq_lens, block_tables, k_cache, v_cache, weights, positions, kept, seen)
+        if r is not None:
+            _result(r, "cf_evict_move")
+            return
     given = [("keep", keep), ("seq_lens", seq_lens), ("block_tables", block_tables), ("k_cache", k_cache),
              ("v_cache", v_cache)]
     given += [(n, t) for n, t in (("weights", weights), ("positions", positions), ("kept", kept), ("seen", seen))

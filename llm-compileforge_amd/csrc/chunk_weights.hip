@@ -21,6 +21,7 @@
 // an addition next to 2 * D operations of the matrix pipe: the exponentials
 // bound them at head_dim 64, both about equally at 128.
 #include <algorithm>
+#include <type_traits>
 
 #include "cf_device.hpp"
 #include "cf_host.hpp"
@@ -243,44 +244,53 @@ __global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkWeightsParams p, i
         bool whole = t0 + kStage - 1 <= w_lo && t0 + kStage <= t_end;
 #pragma unroll
         for (int tt = 0; tt < kStage / 16; ++tt) whole = whole && uniform(ids[buf][tt]) >= 0;
+        // (two bodies: the masks' selects would double the vector work of a tile
+        // that needs none)
+        auto tiles = [&](auto masked) {
+          constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll
-        for (int ct = 0; ct < 4; ++ct) {
-          f32x4_t s[4];
-#pragma unroll
-          for (int tt = 0; tt < 4; ++tt) {
-            s[tt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int x = 0; x < NC; ++x)
-              s[tt] = mfma16(as_qop<QT>(*(const uint4*)(stage[buf] + (tt * 16 + li) * RB + x * 64 + lq * 16)), q[ct][x],
-                             s[tt]);
-          }
-          if (!whole) {
+          for (int ct = 0; ct < 4; ++ct) {
+            f32x4_t s[4];
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) {
-              const int last = ids[buf][tt] < 0 ? -1 : min(pos[ct], t_end - 1);
+              s[tt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-              for (int v = 0; v < 4; ++v)
-                if (t0 + tt * 16 + 4 * lq + v > last) s[tt][v] = -INFINITY;
+              for (int x = 0; x < NC; ++x)
+                s[tt] = mfma16(as_qop<QT>(*(const uint4*)(stage[buf] + (tt * 16 + li) * RB + x * 64 + lq * 16)),
+                               q[ct][x], s[tt]);
             }
-          }
-          float mx = s[0][0];
+            if constexpr (kMasked) {
 #pragma unroll
-          for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
-          mx = mx == -INFINITY ? mx : mx * f.qk;
-          // the reference moves only when a score exceeds it by more than 8
-          // (log2 units): sums of e <= 256 are as exact in float32
-          if (mx > m[ct] + 8.0f) {
-            l[ct] *= __builtin_amdgcn_exp2f(m[ct] - mx);
-            m[ct] = mx;
-          }
-          const float ref = m[ct] == -INFINITY ? 0.0f : m[ct];
+              for (int tt = 0; tt < 4; ++tt) {
+                const int last = ids[buf][tt] < 0 ? -1 : min(pos[ct], t_end - 1);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float sv = s[i >> 2][i & 3];
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sv, f.qk, -ref));
-            l[ct] += whole || sv != -INFINITY ? e : 0.0f;
+                for (int v = 0; v < 4; ++v)
+                  if (t0 + tt * 16 + 4 * lq + v > last) s[tt][v] = -INFINITY;
+              }
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
+            mx = kMasked && mx == -INFINITY ? mx : mx * f.qk;
+            // the reference moves only when a score exceeds it by more than 8
+            // (log2 units): sums of e <= 256 are as exact in float32
+            if (mx > m[ct] + 8.0f) {
+              l[ct] *= __builtin_amdgcn_exp2f(m[ct] - mx);
+              m[ct] = mx;
+            }
+            const float ref = m[ct] == -INFINITY ? 0.0f : m[ct];
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float sv = s[i >> 2][i & 3];
+              const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sv, f.qk, -ref));
+              sum[i & 3] += !kMasked || sv != -INFINITY ? e : 0.0f;
+            }
+            l[ct] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           }
-        }
+        };
+        if (whole) tiles(std::false_type{});
+        else tiles(std::true_type{});
       }
       if (more) store(t0 + kStage, buf ^ 1);
       __syncthreads();
@@ -392,32 +402,38 @@ __global__ __launch_bounds__(256) void chunk_tokens_kernel(ChunkWeightsParams p,
       // the last of these columns sees the wave's first token, and the first its last
       if (tw < vis && c.c0 + r0 + min(j0 + kStage - 1, ncol - 1) / p.G >= tw) {
         const bool whole = all_live && c.c0 + r0 + j0 / p.G >= tw + 63;
+        auto tiles = [&](auto masked) {
+          constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll
-        for (int ct = 0; ct < 4; ++ct) {
-          const float2 col = fin[j0 + ct * 16 + li];
-          QOp<QT> q[NC];
+          for (int ct = 0; ct < 4; ++ct) {
+            const float2 col = fin[j0 + ct * 16 + li];
+            QOp<QT> q[NC];
 #pragma unroll
-          for (int x = 0; x < NC; ++x)
-            q[x] = as_qop<QT>(*(const uint4*)(stage[buf] + (ct * 16 + li) * RB + x * 64 + lq * 16));
-          const int last = whole ? 0 : c.c0 + r0 + (j0 + ct * 16 + li) / p.G;
+            for (int x = 0; x < NC; ++x)
+              q[x] = as_qop<QT>(*(const uint4*)(stage[buf] + (ct * 16 + li) * RB + x * 64 + lq * 16));
+            const int j = j0 + ct * 16 + li, last = !kMasked ? 0 : (j < ncol ? c.c0 + r0 + j / p.G : -1);
 #pragma unroll
-          for (int tt = 0; tt < 4; ++tt) {
-            f32x4_t s = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int tt = 0; tt < 4; ++tt) {
+              f32x4_t s = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int x = 0; x < NC; ++x) s = mfma16(k[tt][x], q[x], s);
+              for (int x = 0; x < NC; ++x) s = mfma16(k[tt][x], q[x], s);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], f.qk, col.x));
-              const float sum = __builtin_fmaf(e, col.y, acc[tt][v]);
-              if (whole) {
-                acc[tt][v] = sum;
-              } else {
-                const bool sees = 4 * lq + v < live[tt] && tw + tt * 16 + 4 * lq + v <= last && j0 + ct * 16 + li < ncol;
-                acc[tt][v] = sees ? sum : acc[tt][v];
+              for (int v = 0; v < 4; ++v) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], f.qk, col.x));
+                const float sum = __builtin_fmaf(e, col.y, acc[tt][v]);
+                if constexpr (kMasked) {
+                  // the block's tokens that exist, up to the column's own position
+                  const int end = min(live[tt], last + 1 - (tw + tt * 16));
+                  acc[tt][v] = 4 * lq + v < end ? sum : acc[tt][v];
+                } else {
+                  acc[tt][v] = sum;
+                }
               }
             }
           }
-        }
+        };
+        if (whole) tiles(std::false_type{});
+        else tiles(std::true_type{});
       }
       if (more) store(buf ^ 1);
       __syncthreads();

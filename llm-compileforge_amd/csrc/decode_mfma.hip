@@ -578,14 +578,30 @@ __device__ __forceinline__ int stream_wave(int w, int Wtot, int Hkv) {
   return (lw % Hkv) * (Wtot / Hkv) + k;
 }
 
-// Keeps four scores of column li, tokens `at` .. + 3 of the sequence that the
-// column belongs to.
-template <class P>
-__device__ __forceinline__ void keep_scores(const P& p, const Coord& c, int li, int at, float4 s) {
-  if (li >= c.ncols) return;
-  const int m = li / p.G, g = li - m * p.G;
-  *(float4*)(p.ws_s + ((int64_t)(c.b + m) * p.Hq + c.h * p.G + g) * p.s_cap + at) = s;
-}
+// Where a lane keeps the scores of its column.  Lanes of unused columns store
+// too, all to one place in the wave's slot 1 (which nothing reads before the
+// wave's last flush fills it): a branch around the stores would leave their
+// number open, and every wait for a tile's loads would wait for the stores that
+// followed them (64 sequences of 1,024 to 8,192 tokens: 140 us with the branch).
+struct ScoreLane {
+  int64_t off = 0;  // of the column's row past its group leader's first row
+  float* spare = nullptr;
+
+  template <class P>
+  __device__ __forceinline__ ScoreLane(const P& p, int li, int w) {
+    if constexpr (kKeeps<P>) {
+      const int m = li / p.G;
+      off = ((int64_t)m * p.Hq + (li - m * p.G)) * p.s_cap;
+      spare = p.ws_o + ((int64_t)w * 2 + 1) * kSlotCols * p.D;
+    }
+  }
+  // four scores, tokens `at` .. + 3 of the sequence that the column belongs to
+  template <class P>
+  __device__ __forceinline__ void keep(const P& p, const Coord& c, int li, int at, float4 s) const {
+    float* to = p.ws_s + ((int64_t)c.b * p.Hq + c.h * p.G) * p.s_cap + off + at;
+    *(float4*)(li < c.ncols ? to : spare) = s;
+  }
+};
 
 // A wave's tiles of an fp32 cache under fp32 queries: as the loop of
 // decode_stream_kernel, on v_mfma_f32_16x16x4_f32.  A tile is 2 x 16 KiB at
@@ -602,6 +618,8 @@ __device__ __forceinline__ void stream_f32(const P& p, const Index& ix, const Se
                                            int64_t v_end, int64_t chunk, int w, int lane) {
   constexpr int NC = D / 16, NV = D / 16;
   const int li = lane & 15, lq = lane >> 4;
+  const ScoreLane scores(p, li, w);
+  (void)scores;
   TileF32<D> r;
   load_k_f32<D, VTOK>(r, kv, c0.blkA, c0.blkB, li, lq, c0.h);
   load_v_f32<D, VTOK>(r, kv, c0.blkA, c0.blkB, li, lq, c0.h);
@@ -700,7 +718,7 @@ __device__ __forceinline__ void stream_f32(const P& p, const Index& ix, const Se
     if constexpr (kKeeps<P>) {
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        keep_scores(p, c0, li, 32 * c0.j + 16 * x + 4 * lq,
+        scores.keep(p, c0, li, 32 * c0.j + 16 * x + 4 * lq,
                     make_float4(sc[4 * x], sc[4 * x + 1], sc[4 * x + 2], sc[4 * x + 3]));
     }
     float mt = sc[0];
@@ -874,6 +892,8 @@ __global__ __launch_bounds__(256) void decode_stream_kernel(P p, const int32_t* 
   // token-major V: this wave's LDS staging rows, after the plan
   uint8_t* vstage = (uint8_t*)dyn_lds + (PL ? kPlanLdsBytes : 0) + wave * vtok_stage_bytes<D, KvTraits<KT>::kBytes>();
   (void)vstage;
+  const ScoreLane scores(p, li, w);
+  (void)scores;
   TileRegs<KT, D, VTOK> r0, r1;
   load_tile<KT, D, VTOK>(r0, kv, c0.blkA, c0.blkB, li, lq, c0.h, lane);
 
@@ -972,7 +992,7 @@ __global__ __launch_bounds__(256) void decode_stream_kernel(P p, const int32_t* 
     if constexpr (kKeeps<P>) {
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        keep_scores(p, c0, li, 32 * c0.j + 8 * lq + 4 * x,
+        scores.keep(p, c0, li, 32 * c0.j + 8 * lq + 4 * x,
                     make_float4(sc[4 * x], sc[4 * x + 1], sc[4 * x + 2], sc[4 * x + 3]));
     }
     float mt = sc[0];
