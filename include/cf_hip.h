@@ -262,12 +262,12 @@ int32_t cf_prefill_chunk_fp8(const CfTensor* q, const CfTensor* k_cache,
                              void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Workspace of cf_chunk_weights for tables of max_blocks_per_seq blocks: 8
- * bytes a query row, head and piece of at least 1,024 tokens (256 in small
- * calls; at most 16 pieces), and sums of 4 bytes a token and head for each
- * 256 to 1,024 query rows x heads. */
+ * bytes a counted row, query head and piece of 1,024 tokens (down to 128 in
+ * small calls; at most 64 pieces up to a million tokens), and 4 bytes a KV head
+ * and token for each 1,024 (down to 256) counted rows x heads of the group. */
 int32_t cf_chunk_weights_workspace_bytes(int64_t num_q_tokens, int64_t num_chunks, int64_t num_q_heads,
                                          int64_t num_kv_heads, int64_t head_dim, int64_t max_blocks_per_seq,
-                                         int32_t block_size, uint64_t* bytes_out);
+                                         int32_t block_size, int32_t observe, uint64_t* bytes_out);
 
 /* The accounts of cf_paged_decode_weights for the rows of prompts and chunks
  * (q, k_cache, block_tables, seq_lens, q_start and k_scale as

@@ -178,7 +178,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "cf_chunk_weights_workspace_bytes": (
         ctypes.c_int32,
         [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
-         ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)],
+         ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)],
     ),
     "cf_chunk_weights": (
         ctypes.c_int32,

@@ -538,7 +538,7 @@ PyObject* chunk_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (a[10] != Py_None) dks = call.in(a[10]);
     uint64_t need = 0;
     if (g_lib.chunk_weights_ws(q.size(0), bt.size(0), q.size(1), k.size(2), q.size(2), bt.size(1), (int32_t)bs,
-                               &need) != CF_OK)
+                               (int32_t)observe, &need) != CF_OK)
       throw Slow{};
     if (a[11] != Py_None && tensor_of(a[11]).get_device() != call.device) throw Slow{};
     const Workspace ws(a[11], need, call, a[0]);

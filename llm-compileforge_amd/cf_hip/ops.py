@@ -383,10 +383,11 @@ def prefill_chunk(
 
 
 def chunk_weights_workspace_bytes(num_q_tokens: int, num_chunks: int, num_q_heads: int, num_kv_heads: int,
-                                  head_dim: int, max_blocks_per_seq: int, block_size: int = 16) -> int:
+                                  head_dim: int, max_blocks_per_seq: int, block_size: int = 16,
+                                  observe: int = 0) -> int:
     out = ctypes.c_uint64(0)
     rc = lib().cf_chunk_weights_workspace_bytes(num_q_tokens, num_chunks, num_q_heads, num_kv_heads, head_dim,
-                                                max_blocks_per_seq, block_size, ctypes.byref(out))
+                                                max_blocks_per_seq, block_size, observe, ctypes.byref(out))
     check(rc, "cf_chunk_weights_workspace_bytes")
     return int(out.value)
 
@@ -424,8 +425,9 @@ def chunk_weights(
     if q.dim() != 3 or k_cache.dim() != 4 or block_tables.dim() != 2:
         raise ValueError(f"q must be [Tq, Hq, D], k_cache [NB, 16, Hkv, D], block_tables [N, Mb]; got "
                          f"{tuple(q.shape)}, {tuple(k_cache.shape)}, {tuple(block_tables.shape)}")
+    observe = _int32("observe", int(observe))
     need = chunk_weights_workspace_bytes(q.shape[0], block_tables.shape[0], q.shape[1], k_cache.shape[2], q.shape[2],
-                                         block_tables.shape[1], block_size)
+                                         block_tables.shape[1], block_size, observe)
     if workspace is None:
         workspace = _cached_workspace(need, dev)
     elif workspace.numel() * workspace.element_size() < need:
@@ -433,8 +435,8 @@ def chunk_weights(
     d = [descriptor(t) if t is not None else None for t in (q, k_cache, block_tables, seq_lens, q_start, k_scale)]
     dw = descriptor(weights)
     with _on(dev):
-        rc = lib().cf_chunk_weights(*(ref(x) for x in d), float(scale), int(block_size), _int32("observe", int(observe)),
-                                    ref(dw), float(decay), workspace.data_ptr(), need, stream_handle(dev))
+        rc = lib().cf_chunk_weights(*(ref(x) for x in d), float(scale), int(block_size), observe, ref(dw),
+                                    float(decay), workspace.data_ptr(), need, stream_handle(dev))
     check(rc, "cf_chunk_weights")
     return weights
 

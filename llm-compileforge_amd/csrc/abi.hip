@@ -789,8 +789,9 @@ int32_t cf_prefill_chunk_fp8(const CfTensor* q, const CfTensor* k_cache, const C
 
 int32_t cf_chunk_weights_workspace_bytes(int64_t num_q_tokens, int64_t num_chunks, int64_t num_q_heads,
                                          int64_t num_kv_heads, int64_t head_dim, int64_t max_blocks_per_seq,
-                                         int32_t block_size, uint64_t* bytes_out) {
+                                         int32_t block_size, int32_t observe, uint64_t* bytes_out) {
   CF_CHECK(bytes_out != nullptr, "bytes_out is NULL");
+  CF_CHECK(observe >= 0, "observe (%d) must not be negative", observe);
   CF_CHECK(num_q_tokens >= 0 && num_chunks >= 0 && num_q_heads > 0 && num_kv_heads > 0 && head_dim > 0 &&
                max_blocks_per_seq >= 0,
            "invalid sizes");
@@ -799,7 +800,8 @@ int32_t cf_chunk_weights_workspace_bytes(int64_t num_q_tokens, int64_t num_chunk
   CF_CHECK(block_size == 16, "block_size must be 16, got %d", block_size);
   CF_CHECK(num_q_heads / num_kv_heads <= 64, "at most 64 query heads a KV head, got %lld",
            (long long)(num_q_heads / num_kv_heads));
-  *bytes_out = chunk_weights_workspace_bytes(num_q_tokens, num_chunks, num_q_heads, num_kv_heads, max_blocks_per_seq);
+  *bytes_out = chunk_weights_workspace_bytes(num_q_tokens, num_chunks, num_q_heads, num_kv_heads, head_dim,
+                                             max_blocks_per_seq, observe);
   return CF_OK;
 }
 
@@ -877,13 +879,14 @@ int32_t cf_chunk_weights(const CfTensor* q, const CfTensor* k_cache, const CfTen
   if (!chunk_weights_supported(p, vq.dtype, vk.dtype)) {
     set_error("chunk weights: needs bf16 q over bf16/e4m3 caches or f16 q over f16/e4m3 caches, head_dim 64/128, at "
               "most 64 query heads a KV head, K rows with unit channel stride and 16-byte aligned blocks, heads and "
-              "token rows, and 16-byte aligned q rows");
+              "token rows, and 16-byte aligned q rows less than 2^20 elements apart");
     return CF_ERR_UNSUPPORTED;
   }
   if (Tq == 0 || N == 0 || cap == 0) return CF_OK;
-  CF_CHECK((Tq / 4 + 2 * N) * Hkv < (int64_t)INT32_MAX && ceil_div(cap, 256) * N * Hkv < (int64_t)INT32_MAX,
+  CF_CHECK((Tq / (256 / p.G) + N) * ceil_div(cap, 128) < (int64_t)INT32_MAX &&
+               (Tq / 4 + 2 * N) * Hkv < (int64_t)INT32_MAX && ceil_div(cap, 64) * N * Hkv < (int64_t)INT32_MAX,
            "too many rows");
-  const uint64_t need = chunk_weights_workspace_bytes(Tq, N, Hq, Hkv, vt.size[1]);
+  const uint64_t need = chunk_weights_workspace_bytes(Tq, N, Hq, Hkv, D, vt.size[1], observe);
   if (workspace == nullptr || workspace_bytes < need) {
     set_error("workspace of %llu bytes needed, %llu given", (unsigned long long)need,
               (unsigned long long)workspace_bytes);

@@ -15,8 +15,9 @@
 // of one column), so m, l, and 1 / l are lane-local and the tokens' sums meet
 // across the 16 lanes of a column group once a unit.  Work is cut into units
 // of 256 columns x TP tokens (rows kernel) and CB columns x 256 tokens (tokens
-// kernel); a unit leaves (m, l) or sums of its piece in the workspace, joined
-// in a fixed order, so there are no atomics.  Per visible pair the kernels
+// kernel), dealt out evenly to the resident workgroups; a unit leaves (m, l) or
+// sums of its piece in the workspace, joined in a fixed order, so there are no
+// atomics.  Per visible pair the kernels
 // issue a fused multiply-add, an exponential (four times the time of one) and
 // an addition next to 2 * D operations of the matrix pipe: the exponentials
 // bound them at head_dim 64, both about equally at 128.
@@ -35,6 +36,7 @@ namespace {
 constexpr int kCols = 256;   // columns of a rows-kernel unit, tokens of a tokens-kernel unit
 constexpr int kStage = 64;   // tokens or columns staged at a time
 constexpr int kMaxCB = 1024;
+constexpr int kMaxTP = 16384;
 
 // A chunk, as the kernels see it.  All wave-uniform.
 struct Chunk {
@@ -48,11 +50,10 @@ struct Chunk {
 };
 
 // q rows start .. end of chunk n (the chunks taken in order and made disjoint).
-__device__ __forceinline__ Chunk chunk_of(const ChunkWeightsParams& p, int n, int start, int end) {
+__device__ __forceinline__ Chunk chunk_of(const ChunkWeightsParams& p, int n, int start, int end, int len) {
   Chunk c;
   c.n = n;
   c.start = start;
-  const int len = max(p.seq_lens[(int64_t)n * p.sl_s], 0);
   const int rows = end - start;
   c.rows = p.observe > 0 ? min(rows, p.observe) : rows;
   c.row0 = end - c.rows;
@@ -60,6 +61,10 @@ __device__ __forceinline__ Chunk chunk_of(const ChunkWeightsParams& p, int n, in
   c.cap = min(len, p.Mb * 16);
   c.fresh = len - rows;
   return c;
+}
+
+__device__ __forceinline__ int len_of(const ChunkWeightsParams& p, int n) {
+  return max(p.seq_lens[(int64_t)n * p.sl_s], 0);
 }
 
 __device__ __forceinline__ int start_of(const ChunkWeightsParams& p, int n) {
@@ -71,68 +76,123 @@ __device__ __forceinline__ int visible(const Chunk& c, int end) { return min(max
 
 __device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
-// Units of a chunk and head: blocks of R rows times blocks of TB tokens.  A
-// causal chunk's first rows see few tokens and its last ones many, so row
-// block k shares a line of `width` units with block nb - 1 - k: the lines of a
-// chunk are then about equally long, and few of their units are empty.
-struct Grid {
-  int nb, width, units;
+// Units of a launch: (chunk, block of R rows, block of TB tokens that some of
+// the rows see, KV head), the head innermost.  A workgroup lists the chunks of a
+// window with their units before them once, so that a unit is found in LDS.
+constexpr int kWindow = 256;
+
+struct Window {
+  int start[kWindow], end[kWindow];  // q rows
+  int len[kWindow];                  // tokens of the sequence
+  int before[kWindow + 1];           // (row block, token block) pairs of the chunks before
 };
 
-__device__ __forceinline__ Grid grid_of(const Chunk& c, int R, int TB) {
-  Grid g;
-  g.nb = cdiv(c.rows, R);
-  if (g.nb <= 1) {
-    g.width = cdiv(visible(c, c.rows), TB);
-  } else {
-    const int64_t both = 2 * (int64_t)max(c.c0, 0) + (int64_t)(g.nb + 1) * R;
-    const int64_t most = 2 * (int64_t)cdiv(c.cap, TB);
-    g.width = (int)min((both + TB - 1) / TB + 1, most);
-  }
-  g.units = ((g.nb + 1) / 2) * g.width;
-  return g;
+__device__ __forceinline__ int token_blocks(const Chunk& c, int rb, int R, int TB) {
+  return cdiv(visible(c, (rb + 1) * R), TB);
 }
 
-// Unit u of a launch: its chunk, head, row block and token block.  False past
-// the last unit; empty (tb < 0) where a line ends early.
+// Lists chunks w0 .. w0 + kWindow - 1; `ends`: where the chunks before them end,
+// and then these.  Ends with a barrier.
+__device__ void list_chunks(const ChunkWeightsParams& p, Window* w, int w0, int R, int TB, int* ends) {
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int n_here = min(p.N - w0, kWindow);
+  int carry = *ends;
+  for (int base = 0; base < n_here; base += 64) {  // (every wave alike; wave 0 writes)
+    const int i = base + lane;
+    // a chunk starts where the ones before it end, if q_start has it earlier
+    const int start = max(wave_incl_max(i < n_here ? start_of(p, w0 + i) : 0, lane), carry);
+    const int end = i < n_here ? max(start_of(p, w0 + i + 1), start) : start;
+    if (wave == 0 && i < n_here) {
+      w->start[i] = start;
+      w->end[i] = end;
+      w->len[i] = len_of(p, w0 + i);
+    }
+    carry = wave_last(start);
+  }
+  *ends = carry;
+  __syncthreads();
+  for (int i = wave; i < n_here; i += 4) {
+    const Chunk c = chunk_of(p, w0 + i, w->start[i], w->end[i], w->len[i]);
+    const int nb = cdiv(c.rows, R);
+    int n = 0;
+    for (int rb = lane; rb < nb; rb += 64) n += token_blocks(c, rb, R, TB);
+    n = wave_last(wave_incl_scan(n, lane));
+    if (lane == 0) w->before[i + 1] = n;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int total = 0;
+    for (int base = 0; base < n_here; base += 64) {
+      const int i = base + lane;
+      const int incl = wave_incl_scan(i < n_here ? w->before[i + 1] : 0, lane) + total;
+      if (i < n_here) w->before[i + 1] = incl;
+      total = wave_last(incl);
+    }
+    if (lane == 0) w->before[0] = 0;
+  }
+  __syncthreads();
+}
+
 struct Unit {
   Chunk c;
   int h, rb, tb;
 };
 
-__device__ bool unit_of(const ChunkWeightsParams& p, int64_t u, int R, int TB, int lane, Unit* out) {
-  const int h = (int)(u % p.Hkv);
-  int64_t v = u / p.Hkv;
-  int before = 0;  // where the chunks before the lanes' end
-  for (int base = 0; base < p.N; base += 64) {
-    const int n = base + lane;
-    // a chunk starts where the ones before it end, if q_start has it earlier
-    const int start = max(wave_incl_max(n < p.N ? start_of(p, n) : 0, lane), before);
-    const int end = n < p.N ? max(start_of(p, n + 1), start) : start;
-    int units = 0;
-    if (n < p.N) units = grid_of(chunk_of(p, n, start, end), R, TB).units;
-    const int incl = wave_incl_scan(units, lane);
-    const uint64_t hit = __ballot(incl > v);
-    if (hit == 0) {
-      v -= wave_last(incl);
-      before = wave_last(start);
-      continue;
-    }
-    const int at = __ffsll((long long)hit) - 1;
-    v -= uniform(__shfl(incl - units, at, 64));
-    out->c = chunk_of(p, base + at, uniform(__shfl(start, at, 64)), uniform(__shfl(end, at, 64)));
-    const Grid g = grid_of(out->c, R, TB);
-    const int k = (int)v / g.width, t = (int)v - k * g.width;
-    const int first = cdiv(visible(out->c, (k + 1) * R), TB);
-    const int mate = g.nb - 1 - k;
-    out->h = h;
-    out->rb = t < first ? k : mate;
-    out->tb = t < first ? t : t - first;
-    if (t >= first && (mate == k || out->tb >= cdiv(visible(out->c, (mate + 1) * R), TB))) out->tb = -1;
-    return true;
+// Unit u of the window at w0 (0 <= u < units of the window).
+__device__ __forceinline__ Unit unit_of(const ChunkWeightsParams& p, const Window* w, int w0, int64_t u, int R, int TB,
+                                        int lane) {
+  Unit out;
+  out.h = (int)(u % p.Hkv);
+  int v = (int)(u / p.Hkv), i = 0;
+  for (int base = 0; base + w0 < p.N && base < kWindow; base += 64) {  // the last chunk with before[i] <= v
+    const uint64_t hit = __ballot(w0 + base + lane < p.N && w->before[base + lane] <= v);
+    if (hit == 0) break;
+    i = base + 63 - __builtin_clzll(hit);
   }
-  return false;
+  v -= uniform(w->before[i]);
+  out.c = chunk_of(p, w0 + i, uniform(w->start[i]), uniform(w->end[i]), uniform(w->len[i]));
+  const int nb = cdiv(out.c.rows, R);
+  for (int base = 0; base < nb; base += 64) {
+    const int rb = base + lane, n = rb < nb ? token_blocks(out.c, rb, R, TB) : 0;
+    const int incl = wave_incl_scan(n, lane);
+    const uint64_t hit = __ballot(incl > v);
+    if (hit != 0) {
+      const int at = __builtin_ctzll(hit);
+      out.rb = base + at;
+      out.tb = v - uniform(__shfl(incl - n, at, 64));
+      return out;
+    }
+    v -= wave_last(incl);
+  }
+  out.rb = out.tb = 0;  // (not reached: v is below the chunk's units)
+  return out;
 }
+
+// Where a chunk's observed row r lies in ws_ml, and its first row piece in ws_p:
+// by the chunk where a window of observers makes that shorter, else by the row
+// (chunks before it use at most one piece more than their rows fill).
+__device__ __forceinline__ int64_t stat_row(const ChunkWeightsParams& p, const Chunk& c, int r) {
+  return p.compact ? (int64_t)c.n * p.observe + r : (int64_t)c.row0 + r;
+}
+__device__ __forceinline__ int64_t piece0(const ChunkWeightsParams& p, const Chunk& c, int R) {
+  return p.compact ? (int64_t)c.n * cdiv(p.observe, R) : (int64_t)(c.start / R) + c.n;
+}
+
+// Waves of a SIMD that the registers are cut for: at head_dim 128 the operands
+// held (64 registers) leave room for two.
+template <int D>
+constexpr int waves_per_simd() {
+  return D == 64 ? 3 : 2;
+}
+
+// Columns to query rows: j / G for j below 1,024 and G up to 64, where
+// j * (G * ceil(2^16 / G) - 2^16) < 2^16 makes the rounded-up reciprocal exact.
+struct Columns {
+  uint32_t recip;
+  int G;
+  __device__ __forceinline__ explicit Columns(int group) : recip((65536u + (uint32_t)group - 1u) / (uint32_t)group), G(group) {}
+  __device__ __forceinline__ int row(int j) const { return (int)(((uint32_t)j * recip) >> 16); }
+};
 
 template <int D>
 constexpr int row_bytes() {
@@ -145,10 +205,10 @@ __device__ __forceinline__ int block_of(const ChunkWeightsParams& p, int n, int 
   return id >= 0 && id < p.NB ? id : -1;
 }
 
-// 16 bytes of operand (8 channels) of a K row: as stored, or converted (exactly).
+// 16 bytes of operand (8 channels) of a K row at element offset `at`: as stored,
+// or converted (exactly).
 template <int QT, int KT>
-__device__ __forceinline__ uint4 k_piece(const ChunkWeightsParams& p, int blk, int off, int h, int d) {
-  const int64_t at = (int64_t)blk * p.k_s[0] + (int64_t)off * p.k_s[1] + (int64_t)h * p.k_s[2] + d;
+__device__ __forceinline__ uint4 k_piece(const ChunkWeightsParams& p, int64_t at) {
   if constexpr (KT == kE4M3) {
     const uint2 v = *(const uint2*)((const uint8_t*)p.k + at);
     if constexpr (QT == kF16) return __builtin_bit_cast(uint4, e4m3x8_to_f16(v.x, v.y));
@@ -158,15 +218,24 @@ __device__ __forceinline__ uint4 k_piece(const ChunkWeightsParams& p, int blk, i
   }
 }
 
-// 16 bytes of a q row; `flip` changes the sign of every element.
-__device__ __forceinline__ uint4 q_piece(const ChunkWeightsParams& p, int row, int hq, int d, uint32_t flip) {
-  uint4 v = *(const uint4*)((const uint16_t*)p.q + (int64_t)row * p.q_sr + (int64_t)hq * p.q_sh + d);
-  v.x ^= flip;
-  v.y ^= flip;
-  v.z ^= flip;
-  v.w ^= flip;
-  return v;
-}
+// Rows of q from a unit's first on, for the heads of one KV head: offsets fit 32
+// bits (the launcher's bound on the strides).
+struct QRows {
+  const uint16_t* base;
+  int row, head;    // strides
+  uint32_t flip;    // changes the sign of every element
+  __device__ __forceinline__ QRows(const ChunkWeightsParams& p, int row0, int h, uint32_t sign)
+      : base((const uint16_t*)p.q + (int64_t)row0 * p.q_sr + (int64_t)(h * p.G) * p.q_sh), row((int)p.q_sr),
+        head((int)p.q_sh), flip(sign) {}
+  __device__ __forceinline__ uint4 piece(int r, int g, int d) const {
+    uint4 v = *(const uint4*)(base + (uint32_t)(r * row + g * head + d));
+    v.x ^= flip;
+    v.y ^= flip;
+    v.z ^= flip;
+    v.w ^= flip;
+    return v;
+  }
+};
 
 // Scores in log2 units are scale_of() times the products of K and Q, which
 // carry the scale's sign: the factor is never negative.
@@ -183,35 +252,57 @@ __device__ __forceinline__ Factor factor_of(const ChunkWeightsParams& p, int h) 
 // ---- rows: m and l of every (row, head) over a piece of its tokens --------------
 
 template <int QT, int KT, int D>
-__global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkWeightsParams p, int64_t max_units) {
+__global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_rows_kernel(ChunkWeightsParams p) {
   constexpr int NC = D / 32, RB = row_bytes<D>(), PPR = D / 8;  // MFMAs a tile, 16-byte pieces a row
   constexpr int LOADS = kStage * PPR / 256;
   __shared__ __align__(16) uint8_t stage[2][kStage * RB];
-  __shared__ int ids[2][kStage / 16];
+  __shared__ int64_t where[kMaxTP / 16];  // offsets of the unit's blocks (-1: none)
+  __shared__ Window win;
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lq = lane >> 4, wave = uniform(tid >> 6);
   const int R = kCols / p.G;
-  for (int64_t u = blockIdx.x; u < max_units; u += gridDim.x) {
-    Unit un;
-    if (!unit_of(p, u, R, p.TP, lane, &un)) return;
-    if (un.tb < 0) continue;
+  const Columns col(p.G);
+  // where a lane's pieces of a stage lie in their blocks
+  int64_t in_block[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int e = i * 256 + tid;
+    in_block[i] = (e / PPR & 15) * p.k_s[1] + e % PPR * 8;
+  }
+  int ends = 0, w0 = 0;
+  list_chunks(p, &win, 0, R, p.TP, &ends);
+  int64_t u = blockIdx.x, units = (int64_t)win.before[min(p.N, kWindow)] * p.Hkv;
+  for (;; u += gridDim.x) {
+    while (u >= units) {  // on to the next window
+      u -= units;
+      w0 += kWindow;
+      if (w0 >= p.N) return;
+      __syncthreads();
+      list_chunks(p, &win, w0, R, p.TP, &ends);
+      units = (int64_t)win.before[min(p.N - w0, kWindow)] * p.Hkv;
+    }
+    const Unit un = unit_of(p, &win, w0, u, R, p.TP, lane);
     const Chunk& c = un.c;
     const int r0 = un.rb * R, nr = min(R, c.rows - r0), ncol = nr * p.G;
     const int t_begin = un.tb * p.TP, t_end = min(t_begin + p.TP, visible(c, r0 + nr));
     const Factor f = factor_of(p, un.h);
+    for (int i = tid; t_begin + i * 16 < t_end; i += 256) {
+      const int blk = block_of(p, c.n, (t_begin >> 4) + i);
+      where[i] = blk < 0 ? -1 : (int64_t)blk * p.k_s[0] + (int64_t)un.h * p.k_s[2];
+    }
+    const QRows rows(p, c.row0 + r0, un.h, f.flip);
     // this wave's 64 columns: four tiles of 16
     QOp<QT> q[4][NC];
     int pos[4];  // last token that the lane's column of tile ct sees
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct) {
-      const int j = wave * 64 + ct * 16 + li, r = j / p.G, g = j - r * p.G;
+      const int j = wave * 64 + ct * 16 + li, r = col.row(j), g = j - r * p.G;
       pos[ct] = j < ncol ? c.c0 + r0 + r : -1;
 #pragma unroll
       for (int x = 0; x < NC; ++x)
-        q[ct][x] = as_qop<QT>(j < ncol ? q_piece(p, c.row0 + r0 + r, un.h * p.G + g, 32 * x + 8 * lq, f.flip)
-                                       : make_uint4(0, 0, 0, 0));
+        q[ct][x] = as_qop<QT>(j < ncol ? rows.piece(r, g, 32 * x + 8 * lq) : make_uint4(0, 0, 0, 0));
     }
     // positions of the wave's first and last column
-    const int w_lo = c.c0 + r0 + wave * 64 / p.G, w_hi = c.c0 + r0 + min(wave * 64 + 63, ncol - 1) / p.G;
+    const int w_lo = c.c0 + r0 + col.row(wave * 64), w_hi = c.c0 + r0 + col.row(min(wave * 64 + 63, ncol - 1));
     const bool busy = wave * 64 < ncol;
     float m[4], l[4];
 #pragma unroll
@@ -219,31 +310,36 @@ __global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkWeightsParams p, i
 
     uint4 reg[LOADS];
     auto fetch = [&](int t0) {  // tokens t0 .. + 63 (those past the end: the last one's block, masked)
+      const int last = (t_end - 1 - t_begin) >> 4, i0 = (t0 - t_begin) >> 4;
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int e = i * 256 + tid, t = t0 + e / PPR;
-        const int blk = block_of(p, c.n, min(t, t_end - 1) >> 4);
-        reg[i] = k_piece<QT, KT>(p, blk < 0 ? 0 : blk, t & 15, un.h, e % PPR * 8);
+        const int64_t at = where[min(i0 + (i * 256 + tid) / PPR / 16, last)];
+        reg[i] = k_piece<QT, KT>(p, (at < 0 ? (int64_t)un.h * p.k_s[2] : at) + in_block[i]);
       }
     };
-    auto store = [&](int t0, int buf) {
+    auto store = [&](int buf) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int e = i * 256 + tid;
         *(uint4*)(stage[buf] + e / PPR * RB + e % PPR * 16) = reg[i];
       }
-      if (tid < kStage / 16) ids[buf][tid] = t0 + tid * 16 < t_end ? block_of(p, c.n, (t0 >> 4) + tid) : -1;
     };
+    __syncthreads();
     fetch(t_begin);
-    store(t_begin, 0);
+    store(0);
     __syncthreads();
     for (int t0 = t_begin, buf = 0; t0 < t_end; t0 += kStage, buf ^= 1) {
       const bool more = t0 + kStage < t_end;
       if (more) fetch(t0 + kStage);
       if (busy && t0 <= w_hi) {
+        const int i0 = (t0 - t_begin) >> 4;
         bool whole = t0 + kStage - 1 <= w_lo && t0 + kStage <= t_end;
+        int valid[kStage / 16];  // whether a block is one of the cache
 #pragma unroll
-        for (int tt = 0; tt < kStage / 16; ++tt) whole = whole && uniform(ids[buf][tt]) >= 0;
+        for (int tt = 0; tt < kStage / 16; ++tt) {
+          valid[tt] = uniform((int)(t0 + tt * 16 < t_end ? where[i0 + tt] >> 32 : -1)) >= 0;
+          whole = whole && valid[tt];
+        }
         // (two bodies: the masks' selects would double the vector work of a tile
         // that needs none)
         auto tiles = [&](auto masked) {
@@ -262,7 +358,7 @@ __global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkWeightsParams p, i
             if constexpr (kMasked) {
 #pragma unroll
               for (int tt = 0; tt < 4; ++tt) {
-                const int last = ids[buf][tt] < 0 ? -1 : min(pos[ct], t_end - 1);
+                const int last = valid[tt] ? min(pos[ct], t_end - 1) : -1;
 #pragma unroll
                 for (int v = 0; v < 4; ++v)
                   if (t0 + tt * 16 + 4 * lq + v > last) s[tt][v] = -INFINITY;
@@ -292,7 +388,7 @@ __global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkWeightsParams p, i
         if (whole) tiles(std::false_type{});
         else tiles(std::true_type{});
       }
-      if (more) store(t0 + kStage, buf ^ 1);
+      if (more) store(buf ^ 1);
       __syncthreads();
     }
     // the four lanes of a column
@@ -304,9 +400,9 @@ __global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkWeightsParams p, i
       float L = l[ct] * (m[ct] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - M));
       L += __shfl_xor(L, 16, 64);
       L += __shfl_xor(L, 32, 64);
-      const int j = wave * 64 + ct * 16 + li, r = j / p.G, g = j - r * p.G;
+      const int j = wave * 64 + ct * 16 + li, r = col.row(j), g = j - r * p.G;
       if (lq == 0 && j < ncol)
-        p.ws_ml[((int64_t)un.tb * p.Tq + c.row0 + r0 + r) * p.Hq + un.h * p.G + g] = make_float2(M, L);
+        p.ws_ml[(un.tb * p.stat_rows + stat_row(p, c, r0 + r)) * p.Hq + un.h * p.G + g] = make_float2(M, L);
     }
     __syncthreads();  // the stage is filled anew
   }
@@ -314,22 +410,29 @@ __global__ __launch_bounds__(256) void chunk_rows_kernel(ChunkWeightsParams p, i
 
 // ---- tokens: sums over the rows of a piece -----------------------------------
 
-// Index of a chunk's first row piece of R rows in ws_p: chunks before it use at
-// most one piece more than their rows fill.
-__device__ __forceinline__ int64_t piece0(const Chunk& c, int R) { return (int64_t)(c.start / R) + c.n; }
-
 template <int QT, int KT, int D>
-__global__ __launch_bounds__(256) void chunk_tokens_kernel(ChunkWeightsParams p, int64_t max_units) {
+__global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_tokens_kernel(ChunkWeightsParams p) {
   constexpr int NC = D / 32, RB = row_bytes<D>(), PPR = D / 8;
   constexpr int LOADS = kStage * PPR / 256;
   __shared__ __align__(16) uint8_t stage[2][kStage * RB];
   __shared__ float2 fin[kMaxCB];  // (-m, 1 / l) of the unit's columns
+  __shared__ Window win;
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lq = lane >> 4, wave = uniform(tid >> 6);
   const int R = p.CB / p.G, RA = kCols / p.G;
-  for (int64_t u = blockIdx.x; u < max_units; u += gridDim.x) {
-    Unit un;
-    if (!unit_of(p, u, R, kCols, lane, &un)) return;
-    if (un.tb < 0) continue;
+  const Columns colm(p.G);
+  int ends = 0, w0 = 0;
+  list_chunks(p, &win, 0, R, kCols, &ends);
+  int64_t u = blockIdx.x, units = (int64_t)win.before[min(p.N, kWindow)] * p.Hkv;
+  for (;; u += gridDim.x) {
+    while (u >= units) {  // on to the next window
+      u -= units;
+      w0 += kWindow;
+      if (w0 >= p.N) return;
+      __syncthreads();
+      list_chunks(p, &win, w0, R, kCols, &ends);
+      units = (int64_t)win.before[min(p.N - w0, kWindow)] * p.Hkv;
+    }
+    const Unit un = unit_of(p, &win, w0, u, R, kCols, lane);
     const Chunk& c = un.c;
     const int r0 = un.rb * R, nr = min(R, c.rows - r0), ncol = nr * p.G;
     const int vis = visible(c, r0 + nr);
@@ -337,27 +440,6 @@ __global__ __launch_bounds__(256) void chunk_tokens_kernel(ChunkWeightsParams p,
     const Factor f = factor_of(p, un.h);
     // columns before the first row that sees the unit's tokens are left out
     const int j_begin = max(t0 - c.c0 - r0, 0) * p.G & ~(kStage - 1);
-
-    // the rows' references and sums, from their pieces
-    for (int j = j_begin + tid; j < cdiv(ncol, kStage) * kStage; j += 256) {
-      float2 v = make_float2(0.0f, 0.0f);
-      if (j < ncol) {
-        const int r = j / p.G, g = j - r * p.G, row = r0 + r;
-        const float2* ml = p.ws_ml + (int64_t)(c.row0 + row) * p.Hq + un.h * p.G + g;
-        const int64_t step = (int64_t)p.Tq * p.Hq;
-        const int np = cdiv(visible(c, (row / RA + 1) * RA), p.TP);  // pieces that the rows kernel wrote
-        float M = -INFINITY, L = 0.0f;
-        for (int i = 0; i < np; ++i) {
-          const float2 x = ml[i * step];
-          const float mn = fmaxf(M, x.x);
-          L = L * (M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - mn)) +
-              x.y * (x.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(x.x - mn));
-          M = mn;
-        }
-        v = make_float2(M == -INFINITY ? 0.0f : -M, L == 0.0f ? 0.0f : 1.0f / L);
-      }
-      fin[j] = v;
-    }
 
     // this wave's 64 tokens: four blocks of 16
     QOp<QT> k[4][NC];
@@ -369,7 +451,8 @@ __global__ __launch_bounds__(256) void chunk_tokens_kernel(ChunkWeightsParams p,
       live[tt] = blk < 0 ? 0 : min(vis - t, 16);
 #pragma unroll
       for (int x = 0; x < NC; ++x)
-        k[tt][x] = as_qop<QT>(k_piece<QT, KT>(p, blk < 0 ? 0 : blk, li, un.h, 32 * x + 8 * lq));
+        k[tt][x] = as_qop<QT>(k_piece<QT, KT>(p, (int64_t)(blk < 0 ? 0 : blk) * p.k_s[0] + (int64_t)un.h * p.k_s[2] +
+                                                      li * p.k_s[1] + 32 * x + 8 * lq));
     }
     const bool all_live = live[0] + live[1] + live[2] + live[3] == 64;
     float acc[4][4];
@@ -378,12 +461,13 @@ __global__ __launch_bounds__(256) void chunk_tokens_kernel(ChunkWeightsParams p,
 #pragma unroll
       for (int v = 0; v < 4; ++v) acc[tt][v] = 0.0f;
 
+    const QRows rows(p, c.row0 + r0, un.h, f.flip);
     uint4 reg[LOADS];
     auto fetch = [&](int j0) {  // columns j0 .. + 63 (zeros past the last)
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int e = i * 256 + tid, j = j0 + e / PPR, r = j / p.G, g = j - r * p.G;
-        reg[i] = j < ncol ? q_piece(p, c.row0 + r0 + r, un.h * p.G + g, e % PPR * 8, f.flip) : make_uint4(0, 0, 0, 0);
+        const int e = i * 256 + tid, j = j0 + e / PPR, r = colm.row(j), g = j - r * p.G;
+        reg[i] = j < ncol ? rows.piece(r, g, e % PPR * 8) : make_uint4(0, 0, 0, 0);
       }
     };
     auto store = [&](int buf) {
@@ -394,14 +478,43 @@ __global__ __launch_bounds__(256) void chunk_tokens_kernel(ChunkWeightsParams p,
       }
     };
     fetch(j_begin);
+    // the rows' references and sums, from their pieces: kBatch of them in
+    // flight at a time
+    for (int j = j_begin + tid; j < cdiv(ncol, kStage) * kStage; j += 256) {
+      float2 v = make_float2(0.0f, 0.0f);
+      if (j < ncol) {
+        const int r = colm.row(j), g = j - r * p.G, row = r0 + r;
+        const float2* ml = p.ws_ml + stat_row(p, c, row) * p.Hq + un.h * p.G + g;
+        const int64_t step = p.stat_rows * p.Hq;
+        const int np = cdiv(visible(c, (row / RA + 1) * RA), p.TP);  // pieces that the rows kernel wrote
+        float M = -INFINITY, L = 0.0f;
+        constexpr int kBatch = 8;
+        for (int i0 = 0; i0 < np; i0 += kBatch) {
+          float2 x[kBatch];
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) x[i] = ml[min(i0 + i, np - 1) * step];
+          float mn = M;
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) mn = fmaxf(mn, x[i].x);
+          L *= M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - mn);
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i)
+            if (i0 + i < np) L += x[i].y * (x[i].x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(x[i].x - mn));
+          M = mn;
+        }
+        v = make_float2(M == -INFINITY ? 0.0f : -M, L == 0.0f ? 0.0f : 1.0f / L);
+      }
+      fin[j] = v;
+    }
+
     store(0);
     __syncthreads();
     for (int j0 = j_begin, buf = 0; j0 < ncol; j0 += kStage, buf ^= 1) {
       const bool more = j0 + kStage < ncol;
       if (more) fetch(j0 + kStage);
       // the last of these columns sees the wave's first token, and the first its last
-      if (tw < vis && c.c0 + r0 + min(j0 + kStage - 1, ncol - 1) / p.G >= tw) {
-        const bool whole = all_live && c.c0 + r0 + j0 / p.G >= tw + 63;
+      if (tw < vis && c.c0 + r0 + colm.row(min(j0 + kStage - 1, ncol - 1)) >= tw) {
+        const bool whole = all_live && c.c0 + r0 + colm.row(j0) >= tw + 63;
         auto tiles = [&](auto masked) {
           constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll
@@ -411,7 +524,7 @@ __global__ __launch_bounds__(256) void chunk_tokens_kernel(ChunkWeightsParams p,
 #pragma unroll
             for (int x = 0; x < NC; ++x)
               q[x] = as_qop<QT>(*(const uint4*)(stage[buf] + (ct * 16 + li) * RB + x * 64 + lq * 16));
-            const int j = j0 + ct * 16 + li, last = !kMasked ? 0 : (j < ncol ? c.c0 + r0 + j / p.G : -1);
+            const int j = j0 + ct * 16 + li, last = !kMasked ? 0 : (j < ncol ? c.c0 + r0 + colm.row(j) : -1);
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) {
               f32x4_t s = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -446,7 +559,7 @@ __global__ __launch_bounds__(256) void chunk_tokens_kernel(ChunkWeightsParams p,
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) acc[tt][v] += __shfl_xor(acc[tt][v], o, 64);
     if (li == 0) {
-      float* out = p.ws_p + ((piece0(c, R) + un.rb) * p.Hkv + un.h) * (int64_t)p.Mb * 16;
+      float* out = p.ws_p + ((piece0(p, c, R) + un.rb) * p.Hkv + un.h) * (int64_t)p.Mb * 16;
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
         const int t = tw + tt * 16 + 4 * lq;
@@ -459,40 +572,72 @@ __global__ __launch_bounds__(256) void chunk_tokens_kernel(ChunkWeightsParams p,
 
 // ---- join --------------------------------------------------------------------
 
+// SPLIT: 64 tokens a workgroup, each wave summing every fourth piece, and the
+// four meet in LDS; else a token a thread.
+template <bool SPLIT>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkWeightsParams p) {
-  const int per = p.Mb * 16, chunks = cdiv(per, 256);
-  const int nh = blockIdx.x / chunks, n = nh / p.Hw, hw = nh - n * p.Hw;
-  const int t = (blockIdx.x - nh * chunks) * 256 + threadIdx.x;
+  constexpr int kTokens = SPLIT ? 64 : 256;
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = SPLIT ? uniform(threadIdx.x >> 6) : 0;
+  const int per = p.Mb * 16, groups = cdiv(per, kTokens);
+  const int nh = blockIdx.x / groups, n = nh / p.Hw, hw = nh - n * p.Hw;
+  const int t = (blockIdx.x - nh * groups) * kTokens + (SPLIT ? lane : (int)threadIdx.x);
   int start = 0;  // the end of the chunks before, and this one's own start
-  for (int i = (int)(threadIdx.x & 63); i <= n; i += 64) start = max(start, start_of(p, i));
+  for (int i = lane; i <= n; i += 64) start = max(start, start_of(p, i));
   start = wave_last(wave_incl_max(start, 0));
-  const Chunk c = chunk_of(p, n, start, max(start_of(p, n + 1), start));
-  if (c.rows == 0 || t >= c.cap) return;
+  const Chunk c = chunk_of(p, n, start, max(start_of(p, n + 1), start), len_of(p, n));
+  if (c.rows == 0) return;
   const int R = p.CB / p.G, nb = cdiv(c.rows, R), heads = p.Hkv / p.Hw;
-  // the first row block that sees token t
-  const int first = max(t - c.c0, 0) / R;
+  // the row blocks from the first that sees token t on, and their heads: one
+  // head's sums are Hkv rows apart, those of all heads follow each other
+  const int first = max(t - c.c0, 0) / R, count = t < c.cap ? (nb - first) * heads : 0;
+  const int64_t step = (int64_t)per * (p.Hw == 1 ? 1 : p.Hkv);
+  const float* part = p.ws_p + ((piece0(p, c, R) + first) * p.Hkv + hw * heads) * (int64_t)per + t;
   float sum = 0.0f;
-  for (int rb = first; rb < nb; ++rb)
-    for (int h = hw * heads; h < (hw + 1) * heads; ++h)
-      sum += p.ws_p[((piece0(c, R) + rb) * p.Hkv + h) * (int64_t)per + t];
+#pragma unroll 8
+  for (int i = wave; i < count; i += SPLIT ? 4 : 1) sum += part[i * step];
+  if constexpr (SPLIT) {
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0) return;
+    sum = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+  }
+  if (t >= c.cap) return;
   float* w = p.weights + (int64_t)n * p.w_sb + (int64_t)hw * p.w_sh + t;
   *w = t >= c.fresh || p.decay == 0.0f ? sum : __builtin_fmaf(*w, p.decay, sum);
 }
 
 // ---- launch ------------------------------------------------------------------
 
-int64_t row_pieces(int64_t Tq, int64_t N, int64_t G, int64_t CB) { return Tq / (CB / G) + N; }
+// How a call is cut, from its sizes alone: the workspace query and the launch
+// agree on it.
+struct Cut {
+  bool compact;         // rows stored by the chunk (a window of observers)
+  int64_t stat_rows;    // rows of ws_ml
+  int64_t row_pieces;   // of ws_p
+  int TP, CB;
+};
 
-// Columns of a tokens-kernel unit and tokens of a rows-kernel unit: long ones
-// reuse what they hold in registers more often, short ones spread a small call
-// over the GPU.
-int col_block(int64_t Tq, int64_t N, int64_t Hkv, int64_t G, int64_t cap) {
-  return row_pieces(Tq, N, G, kMaxCB) * Hkv * ceil_div(cap, kCols) / 2 >= 2 * (int64_t)device_cu_count() ? kMaxCB : kCols;
-}
-int token_piece(int64_t Tq, int64_t N, int64_t Hkv, int64_t G, int64_t cap) {
-  const int64_t few = row_pieces(Tq, N, G, kCols) * Hkv * ceil_div(cap, 1024) / 2 < 2 * (int64_t)device_cu_count();
-  const int64_t most = ceil_div(cap, 16);  // at most 16 pieces of a long row
-  return (int)std::max<int64_t>(few ? 256 : 1024, ceil_div(most, kStage) * kStage);
+// Long units reuse what they hold in registers more often, short ones even out
+// what the workgroups get: the longest that give each at least kUnitsEach, of
+// about half of the (row, token) blocks (causal).
+constexpr double kUnitsEach = 2.5;
+
+Cut cut_of(int64_t Tq, int64_t N, int64_t Hkv, int64_t G, int64_t D, int64_t cap, int64_t observe) {
+  Cut c;
+  c.compact = observe > 0 && N * observe < Tq;
+  c.stat_rows = c.compact ? N * observe : Tq;
+  const double want = kUnitsEach * (D == 64 ? 3 : 2) * device_cu_count();
+  const double seen = observe > 0 ? 1.0 : 0.5;
+  auto pieces = [&](int64_t cols) { return c.compact ? N * ceil_div(observe, cols / G) : Tq / (cols / G) + N; };
+  c.TP = 1024;
+  while (c.TP > 128 && (double)pieces(kCols) * Hkv * ceil_div(cap, c.TP) * seen < want) c.TP /= 2;
+  // (at most 64 pieces of a long row's tokens, as long as kMaxTP holds them)
+  c.TP = (int)std::min<int64_t>(kMaxTP, std::max<int64_t>(c.TP, ceil_div(ceil_div(cap, 64), kStage) * kStage));
+  c.CB = kMaxCB;
+  while (c.CB > kCols && (double)pieces(c.CB) * Hkv * ceil_div(cap, kCols) * seen < want) c.CB /= 2;
+  c.row_pieces = pieces(c.CB);
+  return c;
 }
 
 uint64_t pad(uint64_t x) { return (x + 255) & ~(uint64_t)255; }
@@ -500,22 +645,24 @@ uint64_t pad(uint64_t x) { return (x + 255) & ~(uint64_t)255; }
 template <int QT, int KT, int D>
 int32_t launch_d(const ChunkWeightsParams& p, hipStream_t stream) {
   const int64_t cap = (int64_t)p.Mb * 16;
-  // upper bounds of the units (a chunk's lines hold at most both of their blocks')
-  const int64_t ua = (row_pieces(p.Tq, p.N, p.G, kCols) + p.N) * p.Hkv * (ceil_div(cap, p.TP) + 1);
-  const int64_t ub = (row_pieces(p.Tq, p.N, p.G, p.CB) + p.N) * p.Hkv * (ceil_div(cap, kCols) + 1);
-  const int64_t most = 3 * (int64_t)device_cu_count();
+  // as many workgroups as are resident: each takes every grid-th unit
+  const dim3 grid((unsigned)(waves_per_simd<D>() * device_cu_count()));
   {
     ProfileScope prof("cf_chunk_rows", stream);
-    CF_LAUNCH((chunk_rows_kernel<QT, KT, D>), dim3((unsigned)std::min(ua, most)), dim3(256), 0, stream, p, ua);
+    CF_LAUNCH((chunk_rows_kernel<QT, KT, D>), grid, dim3(256), 0, stream, p);
     CF_HIP_CHECK(hipGetLastError());
   }
   {
     ProfileScope prof("cf_chunk_tokens", stream);
-    CF_LAUNCH((chunk_tokens_kernel<QT, KT, D>), dim3((unsigned)std::min(ub, most)), dim3(256), 0, stream, p, ub);
+    CF_LAUNCH((chunk_tokens_kernel<QT, KT, D>), grid, dim3(256), 0, stream, p);
     CF_HIP_CHECK(hipGetLastError());
   }
   ProfileScope prof("cf_chunk_join", stream);
-  CF_LAUNCH(chunk_join_kernel, dim3((unsigned)(ceil_div(cap, 256) * p.N * p.Hw)), dim3(256), 0, stream, p);
+  // (many pieces a token: more loads in flight)
+  if (ceil_div(p.Tq, p.N * (p.CB / p.G)) * (p.Hkv / p.Hw) >= 8)
+    CF_LAUNCH((chunk_join_kernel<true>), dim3((unsigned)(ceil_div(cap, 64) * p.N * p.Hw)), dim3(256), 0, stream, p);
+  else
+    CF_LAUNCH((chunk_join_kernel<false>), dim3((unsigned)(ceil_div(cap, 256) * p.N * p.Hw)), dim3(256), 0, stream, p);
   CF_HIP_CHECK(hipGetLastError());
   return CF_OK;
 }
@@ -532,6 +679,8 @@ bool chunk_weights_supported(const ChunkWeightsParams& p, int q_dt, int k_dt) {
     return false;
   if (p.D != 64 && p.D != 128) return false;
   if (p.G > 64 || p.NB < 1) return false;
+  // a unit's offsets into q: 1,024 rows and 64 heads
+  if (p.q_sr >= 1 << 20 || p.q_sh >= 1 << 20) return false;
   const int kb = k_dt == kE4M3 ? 1 : 2;
   if (p.k_s[3] != 1 || ((uintptr_t)p.k & 15) != 0 || ((uintptr_t)p.q & 15) != 0) return false;
   for (int i = 0; i < 3; ++i)
@@ -540,20 +689,22 @@ bool chunk_weights_supported(const ChunkWeightsParams& p, int q_dt, int k_dt) {
 }
 
 uint64_t chunk_weights_workspace_bytes(int64_t num_q_tokens, int64_t num_chunks, int64_t num_q_heads,
-                                       int64_t num_kv_heads, int64_t max_blocks) {
-  const int64_t cap = max_blocks * 16, G = num_q_heads / num_kv_heads;
-  const int64_t tp = token_piece(num_q_tokens, num_chunks, num_kv_heads, G, cap);
-  const int64_t cb = col_block(num_q_tokens, num_chunks, num_kv_heads, G, cap);
-  return pad((uint64_t)ceil_div(cap, tp) * num_q_tokens * num_q_heads * 8) +
-         pad((uint64_t)row_pieces(num_q_tokens, num_chunks, G, cb) * num_kv_heads * cap * 4);
+                                       int64_t num_kv_heads, int64_t head_dim, int64_t max_blocks, int64_t observe) {
+  const int64_t cap = max_blocks * 16;
+  const Cut c = cut_of(num_q_tokens, num_chunks, num_kv_heads, num_q_heads / num_kv_heads, head_dim, cap, observe);
+  return pad((uint64_t)ceil_div(cap, c.TP) * c.stat_rows * num_q_heads * 8) +
+         pad((uint64_t)c.row_pieces * num_kv_heads * cap * 4);
 }
 
 void chunk_weights_bind_workspace(ChunkWeightsParams& p, void* workspace) {
   const int64_t cap = (int64_t)p.Mb * 16;
-  p.TP = token_piece(p.Tq, p.N, p.Hkv, p.G, cap);
-  p.CB = col_block(p.Tq, p.N, p.Hkv, p.G, cap);
+  const Cut c = cut_of(p.Tq, p.N, p.Hkv, p.G, p.D, cap, p.observe);
+  p.compact = c.compact;
+  p.stat_rows = c.stat_rows;
+  p.TP = c.TP;
+  p.CB = c.CB;
   p.ws_ml = (float2*)workspace;
-  p.ws_p = (float*)((char*)workspace + pad((uint64_t)ceil_div(cap, p.TP) * p.Tq * p.Hq * 8));
+  p.ws_p = (float*)((char*)workspace + pad((uint64_t)ceil_div(cap, c.TP) * c.stat_rows * p.Hq * 8));
 }
 
 int32_t launch_chunk_weights(const ChunkWeightsParams& p, int q_dt, int k_dt, hipStream_t stream) {

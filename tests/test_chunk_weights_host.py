@@ -85,4 +85,7 @@ def test_the_workspace_is_checked():
     small = ops.chunk_weights_workspace_bytes(5, 2, 8, 2, 64, 3)
     assert 5 * 8 * 8 + 2 * 2 * 48 * 4 <= small <= 4096
     long = ops.chunk_weights_workspace_bytes(8192, 1, 32, 8, 128, 8192)
-    assert long <= 16 * 8192 * 32 * 8 + (8192 // 256 + 1) * 8 * 8192 * 16 * 4 + 512
+    assert long <= 64 * 8192 * 32 * 8 + (8192 * 4 // 256 + 1) * 8 * 8192 * 16 * 4 + 512
+    # a window of observers needs its rows only
+    few = ops.chunk_weights_workspace_bytes(8192, 1, 32, 8, 128, 8192, observe=64)
+    assert few <= 64 * 64 * 32 * 8 + 8 * 8192 * 16 * 4 + 512
