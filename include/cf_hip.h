@@ -559,6 +559,11 @@ int32_t cf_bp_prepare_writes(void* pool, int64_t n_requests, const char* const* 
                              int32_t* copies, int64_t copies_cap, int64_t* n_copies);
 /* Sets a request's token count (its device row length). */
 int32_t cf_bp_set_len(void* pool, const char* request_id, int64_t tokens);
+/* No reference counterpart: cuts a request to its first `tokens` tokens (at
+ * most what its blocks hold) and releases the blocks behind them, e.g. to
+ * cf_evict_select's new length once cf_evict_move is launched.  Work on a
+ * released block is ordered by the stream, as after cf_bp_free. */
+int32_t cf_bp_truncate(void* pool, const char* request_id, int64_t tokens);
 /* Device-resident tables (no reference counterpart; the reference builds
  * tables on the host every step).  cf_bp_bind_rows sizes the device table
  * [rows, cols] (initialised to -1 by the caller) and lengths [rows];

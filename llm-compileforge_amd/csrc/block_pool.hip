@@ -20,6 +20,8 @@
 //    cells that changed since the last call (col = -1: the row's length) for
 //    cf_block_tables_apply to scatter, instead of re-uploading every table
 //    each step.
+//  * truncate: a request cut to fewer tokens (after evictions from its cache)
+//    gives its last blocks back.
 //  * shared_prefix_lens over the rows, the statement the decode kernel takes
 //    (leading tokens a row shares, same physical blocks, with the row before).
 #include <algorithm>
@@ -409,6 +411,35 @@ int32_t cf_bp_set_len(void* h, const char* rid, int64_t tokens) {
     r->len = tokens;
     p->touch(r, kClean, true);
   }
+  return CF_OK;
+}
+
+// Cuts a request to its first `tokens` tokens: blocks behind them lose this
+// request's reference, in table order as cf_bp_free releases them.
+int32_t cf_bp_truncate(void* h, const char* rid, int64_t tokens) {
+  CF_CHECK(h && rid, "NULL argument");
+  CF_CHECK(tokens >= 0, "tokens must be non-negative");
+  Pool* p = pool_of(h);
+  Req* r = p->find(rid);
+  if (!r) {
+    set_error("Unknown request_id: %s", rid);
+    return CF_ERR_NOT_FOUND;
+  }
+  const int64_t held = (int64_t)r->table.size();
+  CF_CHECK(tokens <= held * p->block_size, "request %s holds %lld blocks of %lld, not %lld tokens", rid,
+           (long long)held, (long long)p->block_size, (long long)tokens);
+  const int64_t stay = p->ceil_blocks(tokens);
+  for (int64_t j = stay; j < held; ++j) {
+    const int32_t bid = r->table[j];
+    if (bid < 0 || bid >= p->num_blocks) continue;
+    const int64_t rc = p->rc[bid] > 0 ? p->rc[bid] - 1 : 0;
+    p->rc[bid] = rc;
+    if (rc == 0) p->free_list.push_back(bid);
+  }
+  r->table.resize(stay);
+  const bool moved = r->len != tokens;
+  r->len = tokens;
+  if (stay < held || moved) p->touch(r, stay < held ? (int32_t)stay : kClean, moved);
   return CF_OK;
 }
 

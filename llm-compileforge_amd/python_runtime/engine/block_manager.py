@@ -197,6 +197,13 @@ class BlockManager:
         """Sets a request's token count (its device row length)."""
         check(lib().cf_bp_set_len(self._h, _b(request_id), int(tokens)), "set_len")
 
+    def truncate(self, request_id: str, tokens: int) -> None:
+        """Cuts a request to its first `tokens` tokens and releases the blocks
+        behind them (shared ones only lose a reference), e.g. after
+        CacheManager.evict_rows; KeyError for an unknown id, ValueError for
+        more tokens than its blocks hold."""
+        check(lib().cf_bp_truncate(self._h, _b(request_id), int(tokens)), "truncate")
+
     @staticmethod
     def copy_blocks(copies: np.ndarray | torch.Tensor, caches: Iterable[torch.Tensor]) -> None:
         """Device copies of copy-on-write pairs into every cache tensor whose

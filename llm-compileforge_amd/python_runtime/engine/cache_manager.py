@@ -27,6 +27,11 @@ what moves them:
   (float32 result); attention reads the codes directly.
 - attend() (no reference counterpart) runs decode attention for one query
   row per request straight from the slabs.
+- Rotary positions, attention-weight accounts and eviction (no reference
+  counterpart): write_rotary rotates a step's queries and keys and writes the
+  keys and values in one launch; attend_rows and attend_chunks add each cached
+  token's attention weight to an account given to them; evict_rows cuts
+  requests to a budget of tokens by those accounts.
 
 Every I/O method runs on the GPU through libcf_hip.so and raises if the
 slab is not on a GPU or the library is missing; there is no CPU path.
@@ -523,16 +528,25 @@ class CacheManager:
         v_slab: str = "v",
         scale: float | None = None,
         out: torch.Tensor | None = None,
+        weights: torch.Tensor | None = None,
+        decay: float = 1.0,
     ) -> torch.Tensor:
         """Decode attention from the slabs with device-resident tables (e.g.
         BlockManager.sync_device): q [rows, q_heads, dim], block_tables int32
-        [rows, cols], seq_lens int32 [rows] (rows of length 0 give zeros)."""
+        [rows, cols], seq_lens int32 [rows] (rows of length 0 give zeros).
+        With `weights` (float32 [rows, heads or 1, slots], one account a row
+        and layer) each token's attention weight is added to it, after what it
+        held was multiplied by `decay` (kernels.paged_attention_weights)."""
         kv = self.layer_view(k_slab, layer_idx)
         vv = self.layer_view(v_slab, layer_idx)
         ks = self._scales[k_slab][layer_idx] if k_slab in self._scales else None
         vs = self._scales[v_slab][layer_idx] if v_slab in self._scales else None
         if scale is None:
             scale = 1.0 / math.sqrt(q.shape[-1])
+        if weights is not None:
+            return _ops.paged_decode_weights(q, kv, vv, block_tables, seq_lens, weights, float(scale),
+                                             self._block_size, decay, k_scale=ks, v_scale=vs, out=out,
+                                             shared_prefix_lens=shared_prefix_lens)
         return _ops.paged_decode(q, kv, vv, block_tables, seq_lens, float(scale), self._block_size, k_scale=ks,
                                  v_scale=vs, out=out, shared_prefix_lens=shared_prefix_lens)
 
@@ -547,20 +561,98 @@ class CacheManager:
         v_slab: str = "v",
         scale: float | None = None,
         out: torch.Tensor | None = None,
+        weights: torch.Tensor | None = None,
+        decay: float = 1.0,
+        observe: int = 0,
     ) -> torch.Tensor:
         """Chunked-prefill attention from the slabs: q [Tq, q_heads, dim]
         holds the rows of N chunks (chunk n owns rows [q_start[n],
         q_start[n+1])), whose K/V are already written; row i of a chunk of L
         rows sits at position seq_lens[n] - L + i and sees positions up to
-        it.  block_tables int32 [N, cols]; seq_lens int32 [N]."""
+        it.  block_tables int32 [N, cols]; seq_lens int32 [N].  With `weights`
+        (float32 [N, heads or 1, slots]) the chunks' attention weights are
+        added to it, those of every row or of each chunk's last `observe`
+        rows, after what it held was multiplied by `decay`
+        (kernels.chunk_attention_weights)."""
         kv = self.layer_view(k_slab, layer_idx)
         vv = self.layer_view(v_slab, layer_idx)
         ks = self._scales[k_slab][layer_idx] if k_slab in self._scales else None
         vs = self._scales[v_slab][layer_idx] if v_slab in self._scales else None
         if scale is None:
             scale = 1.0 / math.sqrt(q.shape[-1])
-        return _ops.prefill_chunk(q, kv, vv, block_tables, seq_lens, q_start, float(scale), self._block_size,
-                                  k_scale=ks, v_scale=vs, out=out)
+        out = _ops.prefill_chunk(q, kv, vv, block_tables, seq_lens, q_start, float(scale), self._block_size,
+                                 k_scale=ks, v_scale=vs, out=out)
+        if weights is not None:
+            _ops.chunk_weights(q, kv, block_tables, seq_lens, q_start, weights, float(scale), self._block_size, decay,
+                               observe, k_scale=ks)
+        return out
+
+    # Rotary writes and eviction over one layer of the slabs.
+
+    def write_rotary(
+        self,
+        q: torch.Tensor,
+        k_new: torch.Tensor,
+        v_new: torch.Tensor,
+        positions: torch.Tensor,
+        inv_freq: torch.Tensor,
+        slots: torch.Tensor | np.ndarray,
+        layer_idx: int,
+        *,
+        sections: tuple[int, ...] | None = None,
+        axis_order: str = "blocks",
+        interleaved: bool = False,
+        rotary_scale: float = 1.0,
+        k_slab: str = "k",
+        v_slab: str = "v",
+        out: torch.Tensor | None = None,
+    ) -> torch.Tensor:
+        """Rotates a step's queries (returned) and keys and writes the keys
+        and values at `slots`, in one launch: q [T, q_heads, dim], k_new and
+        v_new [T, heads, dim], slots [T] as BlockManager.prepare_writes
+        returns them (negative ones are skipped); the positions and the
+        rotary's form as in kernels.rotary.rotary_cache_write."""
+        if not (isinstance(slots, torch.Tensor) and slots.dim() == 1 and slots.device == self._device):
+            slots = torch.as_tensor(slots).reshape(-1).to(self._device)
+        kv = self.layer_view(k_slab, layer_idx)
+        vv = self.layer_view(v_slab, layer_idx)
+        ks = self._scales[k_slab][layer_idx] if k_slab in self._scales else None
+        vs = self._scales[v_slab][layer_idx] if v_slab in self._scales else None
+        return _ops.rotary_cache_write(q, k_new, v_new, positions, inv_freq, slots, kv, vv, sections, axis_order,
+                                       interleaved, rotary_scale, k_scale=ks, v_scale=vs, out=out)
+
+    def evict_rows(
+        self,
+        layer_idx: int,
+        weights: torch.Tensor,
+        block_tables: torch.Tensor,
+        seq_lens: torch.Tensor,
+        budget: int,
+        *,
+        sink: int = 0,
+        recent: int = 0,
+        positions: torch.Tensor | None = None,
+        kept: torch.Tensor | None = None,
+        seen: torch.Tensor | None = None,
+        k_slab: str = "k",
+        v_slab: str = "v",
+    ) -> torch.Tensor:
+        """Cuts layer `layer_idx` of every row with more than `budget` tokens
+        to that many, head by head: the first `sink` positions, the last
+        `recent` ones and the heaviest of the others, into the first slots of
+        the row's blocks; the slots' `weights` (attend_rows' account) and
+        `positions` move along (kernels.kv_eviction).  Returns the new lengths
+        int32 [rows], min(seq_lens, budget), the same in every layer: run all
+        layers with the old seq_lens, set `kept` to the new lengths, then cut
+        the requests with BlockManager.truncate.
+
+        Rows are written in place, so blocks that hold a row's first `budget`
+        slots and are shared must be made its own before:
+        BlockManager.prepare_writes([(request, 0, budget)]) and copy_blocks."""
+        keep, new_lens = _ops.evict_select(weights, seq_lens, budget, sink, recent, positions, kept, seen)
+        _ops.evict_move(keep, seq_lens, block_tables, self.layer_view(k_slab, layer_idx),
+                        self.layer_view(v_slab, layer_idx), weights, positions, kept, seen)
+        return new_lens
 
     def paged_slabs(self) -> list[torch.Tensor]:
         """Every paged slab (all layers), e.g. for BlockManager.copy_blocks."""

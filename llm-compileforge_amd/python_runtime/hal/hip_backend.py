@@ -42,6 +42,25 @@ Ops:
                       HIP decode kernels, reading key/value in place as
                       paged blocks; any other call goes to the fallback
                       executor unchanged.
+  rotary              inputs [x, positions, inv_freq]; kwargs sections,
+                      axis_order, interleaved, rotary_scale, out.  Returns
+                      the rotated rows [T, H, D].
+  rotary_cache_write  inputs [query, key, value, positions, inv_freq,
+                      slot_mapping, key_cache, value_cache]; rotary's kwargs,
+                      k_scale, v_scale.  Returns the rotated query.
+  paged_attention_weights
+                      inputs [query, key_cache, value_cache, block_table,
+                      seq_lens, weights]; kwargs block_size, scale, decay,
+                      k_scale, v_scale, shared_prefix_lens.  Adds the tokens'
+                      attention weights to `weights`; returns [B, Hq, D].
+  chunk_attention_weights
+                      inputs [query, key_cache, block_tables, seq_lens,
+                      q_start, weights]; kwargs block_size, scale, decay,
+                      observe, k_scale.  Returns weights.
+  cache_evict         inputs [weights, seq_lens, block_tables, key_cache,
+                      value_cache (, positions, kept, seen)]; kwargs budget,
+                      sink, recent.  Cuts every sequence to `budget` tokens
+                      in place; returns the new lengths [B].
   fp8_amax_scale      inputs [x]; per-head scales [H] (head axis -2).
   fp8_quantize        inputs [x, scales]; e4m3fn codes.
   fp8_dequantize      inputs [codes, scales]; float32 values.
@@ -67,6 +86,11 @@ _ARITY: dict[str, tuple[int, int]] = {
     "cache_write": (5, 5),
     "cache_read": (3, 3),
     "scaled_dot_product_attention": (3, 4),
+    "rotary": (3, 3),
+    "rotary_cache_write": (8, 8),
+    "paged_attention_weights": (6, 6),
+    "chunk_attention_weights": (6, 6),
+    "cache_evict": (5, 8),
     "fp8_amax_scale": (1, 1),
     "fp8_quantize": (2, 2),
     "fp8_dequantize": (2, 2),
@@ -93,6 +117,11 @@ class HipBackend(OpExecutor):
             "cache_write": self._cache_write,
             "cache_read": self._cache_read,
             "scaled_dot_product_attention": self._sdpa,
+            "rotary": self._rotary,
+            "rotary_cache_write": self._rotary_cache_write,
+            "paged_attention_weights": self._paged_attention_weights,
+            "chunk_attention_weights": self._chunk_attention_weights,
+            "cache_evict": self._cache_evict,
             "fp8_amax_scale": lambda inputs, **kw: _ops.fp8_amax_scale(inputs[0]),
             "fp8_quantize": lambda inputs, **kw: _ops.fp8_quantize(inputs[0], inputs[1]),
             "fp8_dequantize": lambda inputs, **kw: _ops.fp8_dequantize(inputs[0], inputs[1]),
@@ -187,6 +216,43 @@ class HipBackend(OpExecutor):
         _ops.paged_gather(k_cache, table, seq_len, scale=kw.get("k_scale"), out=out[0])
         _ops.paged_gather(v_cache, table, seq_len, scale=kw.get("v_scale"), out=out[1])
         return out
+
+    def _rotary(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
+        from kernels.rotary import rotary
+
+        return rotary(*inputs, **_given(kw, "sections", "axis_order", "interleaved", "rotary_scale", "out"))
+
+    def _rotary_cache_write(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
+        from kernels.rotary import rotary_cache_write
+
+        return rotary_cache_write(*inputs, **_given(kw, "sections", "axis_order", "interleaved", "rotary_scale",
+                                                    "k_scale", "v_scale", "out"))
+
+    def _paged_attention_weights(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
+        from kernels.paged_attention import paged_attention_weights
+
+        return paged_attention_weights(*inputs, int(kw.get("block_size", inputs[1].shape[1])), kw.get("scale"),
+                                       **_given(kw, "decay", "k_scale", "v_scale", "shared_prefix_lens"))
+
+    def _chunk_attention_weights(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
+        from kernels.paged_attention import chunk_attention_weights
+
+        return chunk_attention_weights(*inputs, int(kw.get("block_size", inputs[1].shape[1])), kw.get("scale"),
+                                       **_given(kw, "decay", "observe", "k_scale"))
+
+    def _cache_evict(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
+        from kernels.kv_eviction import evict_move, evict_select
+
+        weights, seq_lens, tables, k_cache, v_cache = inputs[:5]
+        state = dict(zip(("positions", "kept", "seen"), inputs[5:]))
+        keep, new_lens = evict_select(weights, seq_lens, int(kw["budget"]), sink=int(kw.get("sink", 0)),
+                                      recent=int(kw.get("recent", 0)), **state)
+        evict_move(keep, seq_lens, tables, k_cache, v_cache, weights=weights, **state)
+        return new_lens
+
+
+def _given(kw: dict[str, Any], *names: str) -> dict[str, Any]:
+    return {n: kw[n] for n in names if n in kw}
 
 
 def _dense_decode_plan(inputs: list[Any], kw: dict[str, Any]):

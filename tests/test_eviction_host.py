@@ -116,3 +116,117 @@ def test_the_plain_statement():
     assert oracle.select(np.array([1.0, np.nan, np.inf]), 3, 1)[0].tolist() == [1]
     # slot 0 holds the newest position: kept as recent
     assert oracle.select(np.zeros(4), 4, 2, recent=1, positions=np.array([9, 3, 4]), kept=3, seen=11)[0].tolist() == [0, 3]
+
+
+# ── the block pool behind an eviction ──────────────────────
+
+
+def test_truncate_gives_the_last_blocks_back():
+    from python_runtime.engine.block_manager import BlockManager
+
+    bm = BlockManager(16, 4)
+    bm.bind_rows(4, 8)
+    a = bm.allocate("a", 22)  # six blocks, the last half full
+    bm.set_len("a", 22)
+    bm.share_prefix("a", "b", 12)
+    bm.set_len("b", 12)
+    table, lens = np.full((4, 8), -1, np.int32), np.zeros(4, np.int32)
+
+    def sync():
+        for r, c, v, _ in bm.table_deltas():
+            if c < 0:
+                lens[r] = v
+            else:
+                table[r, c] = v
+
+    sync()
+    bm.truncate("a", 9)  # shared blocks 0-2 stay, 3-5 are free
+    assert bm.get_blocks("a") == a[:3] and bm.num_free_blocks() == 13
+    sync()
+    row = bm.row_of("a")
+    assert lens[row] == 9 and table[row].tolist() == a[:3] + [-1] * 5
+    bm.truncate("a", 4)  # b still holds blocks 1 and 2
+    assert bm.num_free_blocks() == 13 and bm.ref_count(a[1]) == 1 and bm.get_blocks("b") == a[:3]
+    bm.truncate("a", 4)
+    bm.truncate("b", 0)
+    assert bm.get_blocks("b") == [] and bm.num_free_blocks() == 15 and bm.ref_count(a[0]) == 1
+    sync()
+    assert lens[bm.row_of("b")] == 0 and (table[bm.row_of("b")] == -1).all()
+    slots, copies = bm.prepare_writes([("a", 4, 5)])  # a grows again from its new end
+    assert len(copies) == 0 and len(bm.get_blocks("a")) == 3 and len(slots) == 5
+    sync()
+    assert lens[row] == 9 and table[row, :3].tolist() == bm.get_blocks("a")
+    bm.free("a")
+    bm.free("b")
+    assert bm.num_free_blocks() == 16
+
+
+def test_truncate_refuses():
+    from python_runtime.engine.block_manager import BlockManager
+
+    bm = BlockManager(8, 4)
+    bm.allocate("a", 10)
+    with pytest.raises(KeyError):
+        bm.truncate("nobody", 1)
+    with pytest.raises(ValueError, match="not 13 tokens"):
+        bm.truncate("a", 13)
+    with pytest.raises(ValueError, match="non-negative"):
+        bm.truncate("a", -1)
+    assert len(bm.get_blocks("a")) == 3
+    bm.truncate("a", 12)
+    assert len(bm.get_blocks("a")) == 3
+
+
+def test_truncate_over_many_steps_keeps_the_pool_whole():
+    import random
+
+    from python_runtime.engine.block_manager import BlockManager
+
+    bm, rng, bs = BlockManager(64, 4), random.Random(2), 4
+    held: dict[str, int] = {}
+    for step in range(400):
+        rid = f"r{rng.randrange(6)}"
+        if rid not in held:
+            src = rng.choice(list(held)) if held and rng.random() < 0.5 else None
+            if src:
+                held[rid] = rng.randint(0, held[src])
+                bm.share_prefix(src, rid, held[rid])
+            else:
+                held[rid] = 0
+                bm.allocate(rid, 0)
+            bm.set_len(rid, held[rid])
+        elif rng.random() < 0.3:
+            held[rid] = rng.randint(0, held[rid])
+            bm.truncate(rid, held[rid])
+        elif rng.random() < 0.1:
+            bm.free(rid)
+            del held[rid]
+        elif held[rid] < 24:
+            n = rng.randint(1, 6)
+            bm.prepare_writes([(rid, held[rid], n)])
+            held[rid] += n
+        tables = [bm.get_blocks(r) for r in held]
+        assert [len(t) for t in tables] == [-(-n // bs) for n in held.values()]
+        used = {}
+        for t in tables:
+            assert len(set(t)) == len(t)
+            for blk in t:
+                used[blk] = used.get(blk, 0) + 1
+        assert bm.num_free_blocks() == 64 - len(used)
+        assert all(bm.ref_count(blk) == used.get(blk, 0) for blk in range(64))
+
+
+def test_backend_ops_check_their_inputs():
+    from python_runtime.hal.hip_backend import HipBackend
+
+    be, x = HipBackend(), torch.zeros(2, 2, 64)
+    names = {"rotary": 3, "rotary_cache_write": 8, "paged_attention_weights": 6, "chunk_attention_weights": 6,
+             "cache_evict": 5}
+    assert set(names) <= set(HipBackend.supported_ops())
+    for name, n in names.items():
+        with pytest.raises(ValueError, match=f"at least {n}"):
+            be.execute(name, [x] * (n - 1))
+        with pytest.raises(ValueError, match="at most"):
+            be.execute(name, [x] * 9)
+        with pytest.raises(ValueError, match="ROCm"):
+            be.execute(name, [x] * n, budget=4)
