@@ -81,6 +81,35 @@ struct Fp8Quant {
     if (__builtin_expect(!fast || needs_division(q), 0)) return e4m3_from_f32(x / s);
     return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false) & 0xFF);
   }
+  // 8 values -> 8 codes, element e in byte e % 4 of word e / 4.
+  __device__ __forceinline__ uint2 pack8(const float* f) const {
+    uint32_t w[2];
+    uint32_t redo = 0u;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      float q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        q[j] = f[4 * g + j] * r;
+        redo |= (uint32_t)needs_division(q[j]) << (4 * g + j);
+      }
+      int v = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+      v = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], v, true);
+      w[g] = (uint32_t)v;
+    }
+    if (!fast) redo = 0xFFu;
+    if (__builtin_expect(redo != 0u, 0)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if ((redo >> e) & 1u) {
+          const uint32_t c = e4m3_from_f32(f[e] / s);
+          const int sh = 8 * (e & 3);
+          w[e >> 2] = (w[e >> 2] & ~(0xFFu << sh)) | (c << sh);
+        }
+      }
+    }
+    return make_uint2(w[0], w[1]);
+  }
   // 16 values -> 16 codes, element e in byte e % 4 of word e / 4.
   __device__ __forceinline__ uint4 pack16(const float* f) const {
     uint32_t w[4];

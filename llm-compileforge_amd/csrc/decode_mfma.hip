@@ -583,22 +583,26 @@ __device__ __forceinline__ int stream_wave(int w, int Wtot, int Hkv) {
 // wave's last flush fills it): a branch around the stores would leave their
 // number open, and every wait for a tile's loads would wait for the stores that
 // followed them (64 sequences of 1,024 to 8,192 tokens: 140 us with the branch).
+// Rows of one head each, whose lines take several stores to fill, took 125 us
+// there, this order (score_at) takes 122.7; without the 38 MB of scores 90.
+template <bool F32>
 struct ScoreLane {
-  int64_t off = 0;  // of the column's row past its group leader's first row
+  int64_t off = 0;  // of the lane's first score past its tile's, in the column's sequence
   float* spare = nullptr;
 
   template <class P>
-  __device__ __forceinline__ ScoreLane(const P& p, int li, int w) {
+  __device__ __forceinline__ ScoreLane(const P& p, int li, int lq, int w) {
     if constexpr (kKeeps<P>) {
       const int m = li / p.G;
-      off = ((int64_t)m * p.Hq + (li - m * p.G)) * p.s_cap;
+      off = (int64_t)m * p.Hq * p.s_cap + score_at(F32 ? 4 * lq : 8 * lq, li - m * p.G, p.G);
       spare = p.ws_o + ((int64_t)w * 2 + 1) * kSlotCols * p.D;
     }
   }
-  // four scores, tokens `at` .. + 3 of the sequence that the column belongs to
+  // four scores of tile c.j: its tokens 8 lq + 4 x .. + 3 (F32: 16 x + 4 lq .. + 3)
   template <class P>
-  __device__ __forceinline__ void keep(const P& p, const Coord& c, int li, int at, float4 s) const {
-    float* to = p.ws_s + ((int64_t)c.b * p.Hq + c.h * p.G) * p.s_cap + off + at;
+  __device__ __forceinline__ void keep(const P& p, const Coord& c, int li, int x, float4 s) const {
+    float* to = p.ws_s + ((int64_t)c.b * p.Hq + c.h * p.G) * p.s_cap + (int64_t)c.j * 32 * p.G + off +
+                x * (F32 ? 8 : 16 * p.G);
     *(float4*)(li < c.ncols ? to : spare) = s;
   }
 };
@@ -618,7 +622,7 @@ __device__ __forceinline__ void stream_f32(const P& p, const Index& ix, const Se
                                            int64_t v_end, int64_t chunk, int w, int lane) {
   constexpr int NC = D / 16, NV = D / 16;
   const int li = lane & 15, lq = lane >> 4;
-  const ScoreLane scores(p, li, w);
+  const ScoreLane<true> scores(p, li, lq, w);
   (void)scores;
   TileF32<D> r;
   load_k_f32<D, VTOK>(r, kv, c0.blkA, c0.blkB, li, lq, c0.h);
@@ -718,8 +722,7 @@ __device__ __forceinline__ void stream_f32(const P& p, const Index& ix, const Se
     if constexpr (kKeeps<P>) {
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        scores.keep(p, c0, li, 32 * c0.j + 16 * x + 4 * lq,
-                    make_float4(sc[4 * x], sc[4 * x + 1], sc[4 * x + 2], sc[4 * x + 3]));
+        scores.keep(p, c0, li, x, make_float4(sc[4 * x], sc[4 * x + 1], sc[4 * x + 2], sc[4 * x + 3]));
     }
     float mt = sc[0];
 #pragma unroll
@@ -892,7 +895,7 @@ __global__ __launch_bounds__(256) void decode_stream_kernel(P p, const int32_t* 
   // token-major V: this wave's LDS staging rows, after the plan
   uint8_t* vstage = (uint8_t*)dyn_lds + (PL ? kPlanLdsBytes : 0) + wave * vtok_stage_bytes<D, KvTraits<KT>::kBytes>();
   (void)vstage;
-  const ScoreLane scores(p, li, w);
+  const ScoreLane<false> scores(p, li, lq, w);
   (void)scores;
   TileRegs<KT, D, VTOK> r0, r1;
   load_tile<KT, D, VTOK>(r0, kv, c0.blkA, c0.blkB, li, lq, c0.h, lane);
@@ -992,8 +995,7 @@ __global__ __launch_bounds__(256) void decode_stream_kernel(P p, const int32_t* 
     if constexpr (kKeeps<P>) {
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        scores.keep(p, c0, li, 32 * c0.j + 8 * lq + 4 * x,
-                    make_float4(sc[4 * x], sc[4 * x + 1], sc[4 * x + 2], sc[4 * x + 3]));
+        scores.keep(p, c0, li, x, make_float4(sc[4 * x], sc[4 * x + 1], sc[4 * x + 2], sc[4 * x + 3]));
     }
     float mt = sc[0];
 #pragma unroll

@@ -40,7 +40,7 @@ struct DecodeParams {
 // A decode call that also accounts for the weights: the kernels leave every
 // score and the rows' final (m, l), from which decode_weights_kernel forms them.
 struct DecodeWeightsParams : DecodeParams {
-  float* ws_s;    // scores [B, Hq, s_cap]: log2 units (MFMA path) or natural ones, -inf where masked
+  float* ws_s;    // scores [B, Hkv, s_cap / 32, 2, G, 16]: log2 units (MFMA path) or natural ones, -inf where masked
   float* ws_fin;  // [B, Hq, 2] final reference and sum of a row
   int64_t s_cap;  // tokens of a score row, a multiple of 32
   float* weights;  // [B, Hw, >= Mb * bs] f32, last stride 1
@@ -48,6 +48,14 @@ struct DecodeWeightsParams : DecodeParams {
   int Hw;  // Hkv, or 1
   float decay;
 };
+
+// Where a token's score lies among its tile's 32 * G: 16 floats a query head,
+// those of tokens 8 i .. 8 i + 3 in the first half and of 8 i + 4 .. 8 i + 7 in
+// the second.  A wave of the streaming kernel holds tokens 8 (lane / 16) + 4 x
+// .. + 3 of its heads, so each of its two stores fills whole lines.
+__device__ __forceinline__ int score_at(int t, int g, int G) {
+  return (t >> 5) * 32 * G + ((t >> 2) & 1) * 16 * G + g * 16 + ((t >> 3) & 3) * 4 + (t & 3);
+}
 
 // Launchers (return a CF_* status; kernels are enqueued on `stream`).
 int32_t launch_decode_generic(const DecodeParams& p, int q_dt, int kv_dt, hipStream_t stream);

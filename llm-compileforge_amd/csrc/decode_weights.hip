@@ -36,18 +36,21 @@ __global__ __launch_bounds__(256) void decode_weights_kernel(DecodeWeightsParams
   if (t0 >= len) return;
   const int heads = p.Hq / p.Hw;
   const float* fin = p.ws_fin + ((int64_t)b * p.Hq + hw * heads) * 2;
-  const float* s = p.ws_s + ((int64_t)b * p.Hq + hw * heads) * p.s_cap + t0;
+  const int first = hw * heads;
   float acc[kTokens] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int h0 = 0; h0 < heads; h0 += p.G) {  // KV heads
+    const float* s = p.ws_s + ((int64_t)b * p.Hq + first + h0) * p.s_cap + score_at(t0, 0, p.G);
 #pragma unroll 4
-  for (int h = 0; h < heads; ++h) {
-    const float m = fin[2 * h], l = fin[2 * h + 1];
-    const float mref = m == -INFINITY ? 0.0f : m;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (l NaN: so are the weights)
-    const float4 v = *(const float4*)(s + h * p.s_cap);
-    acc[0] += weight_of<LOG2>(v.x, mref, inv);
-    acc[1] += weight_of<LOG2>(v.y, mref, inv);
-    acc[2] += weight_of<LOG2>(v.z, mref, inv);
-    acc[3] += weight_of<LOG2>(v.w, mref, inv);
+    for (int g = 0; g < p.G; ++g) {
+      const float m = fin[2 * (h0 + g)], l = fin[2 * (h0 + g) + 1];
+      const float mref = m == -INFINITY ? 0.0f : m;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (l NaN: so are the weights)
+      const float4 v = *(const float4*)(s + g * 16);
+      acc[0] += weight_of<LOG2>(v.x, mref, inv);
+      acc[1] += weight_of<LOG2>(v.y, mref, inv);
+      acc[2] += weight_of<LOG2>(v.z, mref, inv);
+      acc[3] += weight_of<LOG2>(v.w, mref, inv);
+    }
   }
   float* w = p.weights + (int64_t)b * p.w_sb + (int64_t)hw * p.w_sh + t0;
   const bool keep = p.decay != 0.0f;  // (0: what was there is not read)

@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(P p) {
   if constexpr (kKeeps<P>) {
     for (int u = tid; u < G * count; u += kGenericThreads) {
       const int g = u / count, i = u - g * count;
-      p.ws_s[((int64_t)b * p.Hq + h * G + g) * p.s_cap + start + i] = sc[g * PT + i];
+      p.ws_s[((int64_t)b * p.Hq + h * G) * p.s_cap + score_at(start + i, g, G)] = sc[g * PT + i];
     }
     __syncthreads();
   }

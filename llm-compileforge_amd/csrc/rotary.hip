@@ -18,9 +18,11 @@
 // distance to the nearest whole number goes to sincospi.  A token's cosines
 // and sines are computed once for eight heads and kept in LDS.
 //
-// A workgroup takes a group of tokens and up to kHeads heads of the queries,
+// A workgroup takes one token or a group of 16 and some heads of the queries,
 // the keys or the values; a thread takes eight pairs (two 16-byte pieces of a
-// 16-bit row).  Bound by bytes for prompts, by the launch for a decode step.
+// 16-bit row).  Bound by bytes for prompts (about 4,900 rows of 32 + 8 + 8 heads
+// of 128, bf16 to e4m3 with channel-major values: 110 MB in 26.9 us, 4.1 TB/s),
+// by the launch for a decode step (32 rows: 4.3 us).
 #include <algorithm>
 
 #include "cf_device.hpp"
@@ -31,7 +33,10 @@ namespace cf {
 
 namespace {
 
-constexpr int kHeads = 8;     // heads of a workgroup
+constexpr int kHeads = 8;     // heads of a workgroup, for single tokens
+constexpr int kMostHeads = 16;  // ... and for groups of tokens, kLeast to kMostHeads
+constexpr int kLeast = 4;
+constexpr int kWorkgroups = 1024;
 constexpr int kTileD = 128;   // longest value row the transposing stage holds
 constexpr int kPiece = 8;     // channels of a piece
 
@@ -63,23 +68,39 @@ __device__ __forceinline__ typename Elem<DT>::T encode(float f, const Fp8Quant& 
   return v;
 }
 
+// kPiece elements as stored.
+template <int DT>
+union Encoded {
+  uint32_t w[kPiece * esize<DT>() / 4];
+  typename Elem<DT>::T e[kPiece];
+  __device__ __forceinline__ Encoded(const float* f, const Fp8Quant& qz) {
+    if constexpr (DT == kE4M3) {
+      const uint2 v = qz.pack8(f);
+      w[0] = v.x;
+      w[1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) e[i] = encode<DT>(f[i], qz);
+    }
+  }
+};
+
+// Elements of a staged value row: one bank past a whole number of them.
+template <int DT>
+constexpr int turned_row() {
+  return kTileD + 4 / esize<DT>();
+}
+
 template <int DT>
 __device__ __forceinline__ void store8(void* base, int64_t off, const float* f, const Fp8Quant& qz) {
-  using T = typename Elem<DT>::T;
-  constexpr int B = kPiece * esize<DT>();
-  union {
-    uint2 d[B / 8];
-    T e[kPiece];
-  } u;
-#pragma unroll
-  for (int i = 0; i < kPiece; ++i) u.e[i] = encode<DT>(f[i], qz);
-  T* dst = (T*)base + off;
-  if constexpr (B == 8) {
-    *(uint2*)dst = u.d[0];
+  const Encoded<DT> u(f, qz);
+  typename Elem<DT>::T* dst = (typename Elem<DT>::T*)base + off;
+  if constexpr (DT == kE4M3) {
+    *(uint2*)dst = make_uint2(u.w[0], u.w[1]);
   } else {
 #pragma unroll
-    for (int i = 0; i < B / 16; ++i)
-      ((uint4*)dst)[i] = make_uint4(u.d[2 * i].x, u.d[2 * i].y, u.d[2 * i + 1].x, u.d[2 * i + 1].y);
+    for (int i = 0; i < esize<DT>() / 2; ++i)
+      ((uint4*)dst)[i] = make_uint4(u.w[4 * i], u.w[4 * i + 1], u.w[4 * i + 2], u.w[4 * i + 3]);
   }
 }
 
@@ -114,7 +135,7 @@ __device__ __forceinline__ int64_t slot_offset(const RotaryParams& p, int64_t t,
   return blk * s[0] + (sl - blk * p.bs) * s[1];
 }
 
-// Rows of up to kHeads heads of the queries (WHAT 0) or keys (1): rotated
+// Rows of nh heads of the queries (WHAT 0) or keys (1): rotated
 // pieces, then the pieces that pass.
 template <int XT, int OT, int TT, int THREADS, int WHAT>
 __device__ __forceinline__ void rotate_rows(const RotaryParams& p, int64_t t0, int nt, int h0, int nh,
@@ -207,72 +228,69 @@ __device__ __forceinline__ void copy_values(const RotaryParams& p, int64_t t0, i
 }
 
 // Value rows into a channel-major tile (tokens of a channel side by side):
-// a wave turns one head's 16 rows over in LDS, so that both its reads and its
-// writes are whole runs; four tokens of a channel go out in one store where
-// their slots follow each other.
-template <int XT, int CT>
+// the heads' 16 rows are turned over in LDS, so that both reads and writes are
+// whole runs; four tokens of a channel go out in one store where their slots
+// follow each other.
+template <int XT, int CT, int THREADS>
 __device__ __forceinline__ void turn_values(const RotaryParams& p, int64_t t0, int nt, int h0, int nh,
                                             const int64_t* dst, uint8_t* stage_all) {
   using C = typename Elem<CT>::T;
-  constexpr int kRow = kTileD + 4 / esize<CT>();  // one bank past a whole number of them
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  C* stage = (C*)stage_all + wave * 16 * kRow;
+  constexpr int kRow = turned_row<CT>();
+  C* stage = (C*)stage_all;
   const int64_t *xs = p.x_s[2], *s = p.c_s[1];
   const int per = p.D / kPiece;
-  for (int hh = wave; hh < nh; hh += 4) {
-    const int h = h0 + hh;
+  for (int u = threadIdx.x; u < nh * 16 * per; u += THREADS) {
+    const int th = u / per, c = (u - th * per) * kPiece, t = th & 15, h = h0 + (th >> 4);
+    if (t >= nt) continue;
     const Fp8Quant qz(CT == kE4M3 ? p.scale[1][h * p.sc_s[1]] : 1.0f);
-    for (int u = lane; u < nt * per; u += 64) {
-      const int t = u / per, c = (u - t * per) * kPiece;
-      float f[kPiece];
-      load8<XT>(p.x[2], (t0 + t) * xs[0] + h * xs[1] + c, f);
+    float f[kPiece];
+    load8<XT>(p.x[2], (t0 + t) * xs[0] + h * xs[1] + c, f);
+    const Encoded<CT> v(f, qz);
+    uint32_t* row = (uint32_t*)(stage + th * kRow + c);  // (a row is a whole number of words)
 #pragma unroll
-      for (int i = 0; i < kPiece; ++i) stage[t * kRow + c + i] = encode<CT>(f[i], qz);
+    for (int i = 0; i < kPiece * esize<CT>() / 4; ++i) row[i] = v.w[i];
+  }
+  __syncthreads();
+  for (int u = threadIdx.x; u < nh * p.D * 4; u += THREADS) {
+    const int hc = u >> 2, hh = hc / p.D, c = hc - hh * p.D, t = (u & 3) * 4;
+    const C* from = stage + (hh * 16 + t) * kRow + c;
+    const int64_t at = dst[t];
+    C* to = (C*)p.cache[1] + (h0 + hh) * s[2] + c * s[3];
+    union {
+      uint32_t w[esize<CT>()];
+      C e[4];
+    } q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q.e[i] = from[i * kRow];
+    const bool run = t + 3 < nt && at >= 0 && dst[t + 1] == at + 1 && dst[t + 2] == at + 2 && dst[t + 3] == at + 3 &&
+                     ((uintptr_t)(to + at) & (4 * sizeof(C) - 1)) == 0;
+    if (run) {
+      if constexpr (sizeof(C) == 1) *(uint32_t*)(to + at) = q.w[0];
+      else if constexpr (sizeof(C) == 2) *(uint2*)(to + at) = make_uint2(q.w[0], q.w[1]);
+      else *(uint4*)(to + at) = make_uint4(q.w[0], q.w[1], q.w[2], q.w[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t + i < nt && dst[t + i] >= 0) to[dst[t + i]] = q.e[i];
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    for (int u = lane; u < p.D * 4; u += 64) {
-      const int c = u >> 2, t = (u & 3) * 4;
-      const int64_t at = dst[t];
-      C* to = (C*)p.cache[1] + h * s[2] + c * s[3];
-      union {
-        uint32_t w[esize<CT>()];
-        C e[4];
-      } q;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) q.e[i] = stage[(t + i) * kRow + c];
-      const bool run = t + 3 < nt && at >= 0 && dst[t + 1] == at + 1 && dst[t + 2] == at + 2 && dst[t + 3] == at + 3 &&
-                       ((uintptr_t)(to + at) & (4 * sizeof(C) - 1)) == 0;
-      if (run) {
-        if constexpr (sizeof(C) == 1) *(uint32_t*)(to + at) = q.w[0];
-        else if constexpr (sizeof(C) == 2) *(uint2*)(to + at) = make_uint2(q.w[0], q.w[1]);
-        else *(uint4*)(to + at) = make_uint4(q.w[0], q.w[1], q.w[2], q.w[3]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (t + i < nt && dst[t + i] >= 0) to[dst[t + i]] = q.e[i];
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
 }
 
 // TT tokens a workgroup.  Dynamic LDS: (cos, sin) [TT][pairs], or the stage
 // of turned values.
 template <int XT, int CT, int TT, int THREADS>
-__global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryParams p, int parts, int q_parts, int kv_parts) {
+__global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryParams p, int parts, int q_parts, int k_parts, int most,
+                                                         int v_most) {
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int64_t dst[TT];
   const int64_t group = blockIdx.x / parts;
   int part = (int)(blockIdx.x - group * parts);
   const int64_t t0 = group * TT;
   const int nt = (int)(p.T - t0 < TT ? p.T - t0 : TT);
-  const int what = part < q_parts ? 0 : (part < q_parts + kv_parts ? 1 : 2);
-  part -= what == 0 ? 0 : (what == 1 ? q_parts : q_parts + kv_parts);
-  const int heads = what == 0 ? p.Hq : p.Hkv, h0 = part * kHeads, nh = min(kHeads, heads - h0);
+  const int what = part < q_parts ? 0 : (part < q_parts + k_parts ? 1 : 2);
+  part -= what == 0 ? 0 : (what == 1 ? q_parts : q_parts + k_parts);
+  const int heads = what == 0 ? p.Hq : p.Hkv, each = what == 2 ? v_most : most;
+  const int h0 = part * each, nh = min(each, heads - h0);
   if (threadIdx.x < nt) {
     const int64_t t = t0 + threadIdx.x;
     dst[threadIdx.x] = what == 0 ? t * p.o_s[0] : slot_offset(p, t, p.c_s[what - 1]);
@@ -291,7 +309,7 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryParams p, int par
   } else {
     if constexpr (TT == 16) {
       if (p.v_tile) {
-        turn_values<XT, CT>(p, t0, nt, h0, nh, dst, lds);
+        turn_values<XT, CT, THREADS>(p, t0, nt, h0, nh, dst, lds);
         return;
       }
     }
@@ -301,25 +319,40 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryParams p, int par
 
 template <int XT, int CT, int TT, int THREADS>
 int32_t launch_tt(const RotaryParams& p, hipStream_t stream) {
-  const int q_parts = (p.Hq + kHeads - 1) / kHeads, kv_parts = (p.Hkv + kHeads - 1) / kHeads;
-  const int parts = q_parts + 2 * kv_parts;
-  const int64_t groups = ceil_div(p.T, TT) * parts;
+  // Heads of a workgroup: many share a token's cosines and sines, few make
+  // enough workgroups for the card.  Rows as above: 16 heads 26.9 us, 8 30.2,
+  // 32 42; 1,237 rows of 12 heads in f32: 4 heads 7.0 us, 16 8.1.  Values that
+  // are turned over have no cosines to share: of 4,900 rows 4 heads at a time
+  // take 27.2 us, 2 30.8; of 2,048 17.1 and 14.6; single ones are scattered by
+  // channel, a head a wave (64 rows: 4.8 us, by eight heads 10).
+  int most = TT == 1 ? kHeads : kMostHeads, v_most = most, q_parts, k_parts, parts;
+  int64_t groups;
+  for (;; most /= 2) {
+    v_most = p.vec[2] ? most : (TT == 1 ? 1 : std::max(most / 4, 2));
+    q_parts = (p.Hq + most - 1) / most;
+    k_parts = (p.Hkv + most - 1) / most;
+    parts = q_parts + k_parts + (p.Hkv + v_most - 1) / v_most;
+    groups = ceil_div(p.T, TT) * parts;
+    if (TT == 1 || most == kLeast || groups >= kWorkgroups) break;
+  }
   if (groups >= (int64_t)INT32_MAX) {
     set_error("rotary: too many rows");
     return CF_ERR_UNSUPPORTED;
   }
   size_t lds = (size_t)TT * p.pairs * sizeof(float2);
   if (TT == 16 && p.v_tile)
-    lds = std::max(lds, (size_t)4 * 16 * (kTileD + 4 / esize<CT>()) * esize<CT>());
+    lds = std::max(lds, (size_t)v_most * 16 * turned_row<CT>() * esize<CT>());
   ProfileScope prof("cf_rotary", stream);
   CF_LAUNCH((rotary_kernel<XT, CT, TT, THREADS>), dim3((unsigned)groups), dim3(THREADS), lds, stream, p, parts, q_parts,
-            kv_parts);
+            k_parts, most, v_most);
   CF_HIP_CHECK(hipGetLastError());
   return CF_OK;
 }
 
 template <int XT, int CT>
 int32_t launch_t(const RotaryParams& p, hipStream_t stream) {
+  // groups against single tokens, e4m3 caches of 8 heads of 128: 256 rows 6.9
+  // and 6.0 us, 512 rows 7.5 and 8.6, 2,048 rows 14.8 and 21.4
   if (p.T >= 512 && p.pairs <= 256) return launch_tt<XT, CT, 16, 256>(p, stream);
   return launch_tt<XT, CT, 1, 64>(p, stream);
 }
