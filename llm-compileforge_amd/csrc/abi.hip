@@ -800,7 +800,7 @@ int32_t cf_chunk_weights_workspace_bytes(int64_t num_q_tokens, int64_t num_chunk
   CF_CHECK(block_size == 16, "block_size must be 16, got %d", block_size);
   CF_CHECK(num_q_heads / num_kv_heads <= 64, "at most 64 query heads a KV head, got %lld",
            (long long)(num_q_heads / num_kv_heads));
-  *bytes_out = chunk_weights_workspace_bytes(num_q_tokens, num_chunks, num_q_heads, num_kv_heads, head_dim,
+  *bytes_out = chunk_weights_workspace_bytes(num_q_tokens, num_chunks, num_q_heads, num_kv_heads,
                                              max_blocks_per_seq, observe);
   return CF_OK;
 }
@@ -883,10 +883,12 @@ int32_t cf_chunk_weights(const CfTensor* q, const CfTensor* k_cache, const CfTen
     return CF_ERR_UNSUPPORTED;
   }
   if (Tq == 0 || N == 0 || cap == 0) return CF_OK;
-  CF_CHECK((Tq / (256 / p.G) + N) * ceil_div(cap, 128) < (int64_t)INT32_MAX &&
+  // (columns and steps are counted in 32 bits)
+  CF_CHECK(Tq * p.G < (int64_t)INT32_MAX && (Tq / (256 / p.G) + N) * ceil_div(cap, 64) < (int64_t)INT32_MAX &&
+               (Tq * p.G / 64 + N) * ceil_div(cap, 256) < (int64_t)INT32_MAX &&
                (Tq / 4 + 2 * N) * Hkv < (int64_t)INT32_MAX && ceil_div(cap, 64) * N * Hkv < (int64_t)INT32_MAX,
            "too many rows");
-  const uint64_t need = chunk_weights_workspace_bytes(Tq, N, Hq, Hkv, D, vt.size[1], observe);
+  const uint64_t need = chunk_weights_workspace_bytes(Tq, N, Hq, Hkv, vt.size[1], observe);
   if (workspace == nullptr || workspace_bytes < need) {
     set_error("workspace of %llu bytes needed, %llu given", (unsigned long long)need,
               (unsigned long long)workspace_bytes);

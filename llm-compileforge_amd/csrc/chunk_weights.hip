@@ -13,14 +13,21 @@
 //                  each column's (m, 1 / l), the sums per lane.
 // Both form S^T = K Q^T (v_mfma_f32_16x16x32; a lane's outputs are four tokens
 // of one column), so m, l, and 1 / l are lane-local and the tokens' sums meet
-// across the 16 lanes of a column group once a unit.  Work is cut into units
-// of 256 columns x TP tokens (rows kernel) and CB columns x 256 tokens (tokens
-// kernel), dealt out evenly to the resident workgroups; a unit leaves (m, l) or
-// sums of its piece in the workspace, joined in a fixed order, so there are no
-// atomics.  Per visible pair the kernels
-// issue a fused multiply-add, an exponential (four times the time of one) and
-// an addition next to 2 * D operations of the matrix pipe: the exponentials
-// bound them at head_dim 64, both about equally at 128.
+// across the 16 lanes of a column group once a run.  The work of a head is a
+// line of steps, 64 tokens for a block of 256 columns (rows kernel) or 64
+// columns for a block of 256 tokens (tokens kernel), block after block; every
+// resident workgroup takes an equal stretch of it, which is a run or two: it
+// leaves (m, l) or sums of each run in the workspace, joined in a fixed order,
+// so there are no atomics.  (Units of a fixed length, dealt out in turn, left
+// the busiest workgroup a third more steps than the mean.)  Per visible pair the
+// kernels issue a fused multiply-add, an exponential (almost three times the
+// time of one), an addition and half a maximum next to 2 * D operations of the
+// matrix pipe, which the vector pipe hardly overlaps: 64 by 64 pairs at head_dim
+// 64 take a SIMD 1,480 cycles with nothing else to do, and some 2,800 here, the
+// staging, masks and the end, when the older waves of a SIMD are done, included.
+// Two prompts of 1,500 to 4,000 rows, 32 heads of 64: rows 89 us, tokens 84
+// (3.6e10 operations of the matrix pipe each); 64 observers behind 4,000 to
+// 12,000 tokens, 4 sequences, 32 heads of 128, e4m3: 35 and 41 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -33,10 +40,10 @@ namespace cf {
 
 namespace {
 
-constexpr int kCols = 256;   // columns of a rows-kernel unit, tokens of a tokens-kernel unit
-constexpr int kStage = 64;   // tokens or columns staged at a time
-constexpr int kMaxCB = 1024;
-constexpr int kMaxTP = 16384;
+constexpr int kCols = 256;   // columns of a row block, tokens of a token block
+constexpr int kStage = 64;   // tokens or columns of a step
+constexpr int kSegment = 8192;  // tokens whose block offsets the rows kernel holds
+constexpr int kColumns = 960;   // columns whose (m, 1 / l) the tokens kernel holds
 
 // A chunk, as the kernels see it.  All wave-uniform.
 struct Chunk {
@@ -76,24 +83,41 @@ __device__ __forceinline__ int visible(const Chunk& c, int end) { return min(max
 
 __device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
-// Units of a launch: (chunk, block of R rows, block of TB tokens that some of
-// the rows see, KV head), the head innermost.  A workgroup lists the chunks of a
-// window with their units before them once, so that a unit is found in LDS.
+// The line of steps of one KV head: for each chunk its blocks, for each block its
+// steps.  A workgroup lists the chunks of a window with the steps before them
+// once, so that a step is found in LDS.
 constexpr int kWindow = 256;
 
 struct Window {
   int start[kWindow], end[kWindow];  // q rows
   int len[kWindow];                  // tokens of the sequence
-  int before[kWindow + 1];           // (row block, token block) pairs of the chunks before
+  int before[kWindow + 1];           // steps of the chunks before
 };
 
-__device__ __forceinline__ int token_blocks(const Chunk& c, int rb, int R, int TB) {
-  return cdiv(visible(c, (rb + 1) * R), TB);
-}
+// Blocks of R rows, steps of 64 tokens that some of the rows see.
+struct RowBlocks {
+  int R;
+  __device__ __forceinline__ int blocks(const Chunk& c) const { return cdiv(c.rows, R); }
+  __device__ __forceinline__ int steps(const Chunk& c, int b) const {
+    return (visible(c, (b + 1) * R) + kStage - 1) / kStage;
+  }
+};
+
+// Blocks of 256 tokens, steps of 64 columns from the first that sees the block's
+// first token on.
+struct TokenBlocks {
+  int G;
+  __device__ __forceinline__ int blocks(const Chunk& c) const { return (visible(c, c.rows) + kCols - 1) / kCols; }
+  __device__ __forceinline__ int first(const Chunk& c, int b) const { return max(b * kCols - c.c0, 0) * G / kStage; }
+  __device__ __forceinline__ int steps(const Chunk& c, int b) const {
+    return (c.rows * G + kStage - 1) / kStage - first(c, b);
+  }
+};
 
 // Lists chunks w0 .. w0 + kWindow - 1; `ends`: where the chunks before them end,
 // and then these.  Ends with a barrier.
-__device__ void list_chunks(const ChunkWeightsParams& p, Window* w, int w0, int R, int TB, int* ends) {
+template <class Blocks>
+__device__ void list_chunks(const ChunkWeightsParams& p, Window* w, int w0, const Blocks& blocks, int* ends) {
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n_here = min(p.N - w0, kWindow);
   int carry = *ends;
@@ -113,9 +137,9 @@ __device__ void list_chunks(const ChunkWeightsParams& p, Window* w, int w0, int 
   __syncthreads();
   for (int i = wave; i < n_here; i += 4) {
     const Chunk c = chunk_of(p, w0 + i, w->start[i], w->end[i], w->len[i]);
-    const int nb = cdiv(c.rows, R);
+    const int nb = blocks.blocks(c);
     int n = 0;
-    for (int rb = lane; rb < nb; rb += 64) n += token_blocks(c, rb, R, TB);
+    for (int b = lane; b < nb; b += 64) n += blocks.steps(c, b);
     n = wave_last(wave_incl_scan(n, lane));
     if (lane == 0) w->before[i + 1] = n;
   }
@@ -133,49 +157,83 @@ __device__ void list_chunks(const ChunkWeightsParams& p, Window* w, int w0, int 
   __syncthreads();
 }
 
-struct Unit {
+// Steps at .. at + n - 1 of a block, that one workgroup does.
+struct Run {
   Chunk c;
-  int h, rb, tb;
+  int block, at, n;
+  int piece, pieces;  // the run's number among the block's, and how many they are
+  bool last;
 };
 
-// Unit u of the window at w0 (0 <= u < units of the window).
-__device__ __forceinline__ Unit unit_of(const ChunkWeightsParams& p, const Window* w, int w0, int64_t u, int R, int TB,
-                                        int lane) {
-  Unit out;
-  out.h = (int)(u % p.Hkv);
-  int v = (int)(u / p.Hkv), i = 0;
-  for (int base = 0; base + w0 < p.N && base < kWindow; base += 64) {  // the last chunk with before[i] <= v
-    const uint64_t hit = __ballot(w0 + base + lane < p.N && w->before[base + lane] <= v);
-    if (hit == 0) break;
-    i = base + 63 - __builtin_clzll(hit);
-  }
-  v -= uniform(w->before[i]);
-  out.c = chunk_of(p, w0 + i, uniform(w->start[i]), uniform(w->end[i]), uniform(w->len[i]));
-  const int nb = cdiv(out.c.rows, R);
-  for (int base = 0; base < nb; base += 64) {
-    const int rb = base + lane, n = rb < nb ? token_blocks(out.c, rb, R, TB) : 0;
-    const int incl = wave_incl_scan(n, lane);
-    const uint64_t hit = __ballot(incl > v);
-    if (hit != 0) {
-      const int at = __builtin_ctzll(hit);
-      out.rb = base + at;
-      out.tb = v - uniform(__shfl(incl - n, at, 64));
-      return out;
-    }
-    v -= wave_last(incl);
-  }
-  out.rb = out.tb = 0;  // (not reached: v is below the chunk's units)
-  return out;
-}
+// The runs of a workgroup, one after the other.
+template <class Blocks>
+struct Runs {
+  const ChunkWeightsParams& p;
+  Window* win;
+  Blocks blocks;
+  int least;  // steps that a workgroup takes at least
+  int lane;
+  int x = 0, end = 0, share = 1;  // the stretch's steps left, and its length
+  int w0 = -kWindow, ends = 0;
 
-// Where a chunk's observed row r lies in ws_ml, and its first row piece in ws_p:
-// by the chunk where a window of observers makes that shorter, else by the row
-// (chunks before it use at most one piece more than their rows fill).
+  __device__ __forceinline__ Runs(const ChunkWeightsParams& params, Window* w, Blocks b, int least_steps)
+      : p(params), win(w), blocks(b), least(least_steps), lane(threadIdx.x & 63) {}
+
+  // The next one, false after the last.  Called by all threads, with a barrier
+  // between a run's use and the next call.
+  __device__ __forceinline__ bool next(Run* run) {
+    while (x >= end) {  // on to the next window
+      w0 += kWindow;
+      if (w0 >= p.N) return false;
+      __syncthreads();
+      list_chunks(p, win, w0, blocks, &ends);
+      const int total = uniform(win->before[min(p.N - w0, kWindow)]);
+      share = max(cdiv(total, (int)(gridDim.x / p.Hkv)), least);
+      x = min((int)(blockIdx.x / p.Hkv) * share, total);
+      end = min(x + share, total);
+    }
+    int v = x, i = 0;
+    for (int base = 0; base + w0 < p.N && base < kWindow; base += 64) {  // the last chunk with before[i] <= v
+      const uint64_t hit = __ballot(w0 + base + lane < p.N && win->before[base + lane] <= v);
+      if (hit == 0) break;
+      i = base + 63 - __builtin_clzll(hit);
+    }
+    v -= uniform(win->before[i]);
+    run->c = chunk_of(p, w0 + i, uniform(win->start[i]), uniform(win->end[i]), uniform(win->len[i]));
+    const int nb = blocks.blocks(run->c);
+    int steps = 0;
+    for (int base = 0; base < nb; base += 64) {
+      const int b = base + lane, n = b < nb ? blocks.steps(run->c, b) : 0;
+      const int incl = wave_incl_scan(n, lane);
+      const uint64_t hit = __ballot(incl > v);
+      if (hit != 0) {
+        const int at = __builtin_ctzll(hit);
+        run->block = base + at;
+        steps = uniform(__shfl(n, at, 64));
+        v -= uniform(__shfl(incl - n, at, 64));
+        break;
+      }
+      v -= wave_last(incl);
+    }
+    run->at = v;
+    run->n = min(end - x, steps - v);
+    run->last = v + run->n == steps;
+    const int first = (x - v) / share;  // the workgroup that has the block's first step
+    run->piece = x / share - first;
+    run->pieces = (x - v + steps - 1) / share - first + 1;
+    x += run->n;
+    return true;
+  }
+};
+
+// Where a chunk's observed row r lies in ws_ml, and its first piece in ws_p: by
+// the chunk where a window of observers makes that shorter, else by the row (a
+// chunk has at most two pieces more than its rows fill).
 __device__ __forceinline__ int64_t stat_row(const ChunkWeightsParams& p, const Chunk& c, int r) {
   return p.compact ? (int64_t)c.n * p.observe + r : (int64_t)c.row0 + r;
 }
-__device__ __forceinline__ int64_t piece0(const ChunkWeightsParams& p, const Chunk& c, int R) {
-  return p.compact ? (int64_t)c.n * cdiv(p.observe, R) : (int64_t)(c.start / R) + c.n;
+__device__ __forceinline__ int64_t piece0(const ChunkWeightsParams& p, const Chunk& c) {
+  return p.compact ? (int64_t)c.n * (cdiv(p.observe, p.piece_rows) + 1) : (int64_t)(c.start / p.piece_rows) + 2 * c.n;
 }
 
 // Waves of a SIMD that the registers are cut for: at head_dim 128 the operands
@@ -205,20 +263,25 @@ __device__ __forceinline__ int block_of(const ChunkWeightsParams& p, int n, int 
   return id >= 0 && id < p.NB ? id : -1;
 }
 
-// 16 bytes of operand (8 channels) of a K row at element offset `at`: as stored,
-// or converted (exactly).
-template <int QT, int KT>
-__device__ __forceinline__ uint4 k_piece(const ChunkWeightsParams& p, int64_t at) {
-  if constexpr (KT == kE4M3) {
-    const uint2 v = *(const uint2*)((const uint8_t*)p.k + at);
-    if constexpr (QT == kF16) return __builtin_bit_cast(uint4, e4m3x8_to_f16(v.x, v.y));
-    else return __builtin_bit_cast(uint4, e4m3x8_to_bf16(v.x, v.y));
-  } else {
-    return *(const uint4*)((const uint16_t*)p.k + at);
-  }
+// 8 channels of a K row at element offset `at`, as stored, and as 16 bytes of
+// operand (converted exactly).
+template <int KT>
+using Stored = typename std::conditional<KT == kE4M3, uint2, uint4>::type;
+
+template <int KT>
+__device__ __forceinline__ Stored<KT> k_piece(const ChunkWeightsParams& p, int64_t at) {
+  if constexpr (KT == kE4M3) return *(const uint2*)((const uint8_t*)p.k + at);
+  else return *(const uint4*)((const uint16_t*)p.k + at);
 }
 
-// Rows of q from a unit's first on, for the heads of one KV head: offsets fit 32
+template <int QT, int KT>
+__device__ __forceinline__ uint4 operand(const Stored<KT>& v) {
+  if constexpr (KT != kE4M3) return v;
+  else if constexpr (QT == kF16) return __builtin_bit_cast(uint4, e4m3x8_to_f16(v.x, v.y));
+  else return __builtin_bit_cast(uint4, e4m3x8_to_bf16(v.x, v.y));
+}
+
+// Rows of q from a block's or step's first on, for the heads of one KV head: offsets fit 32
 // bits (the launcher's bound on the strides).
 struct QRows {
   const uint16_t* base;
@@ -256,7 +319,7 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_rows_kernel(Ch
   constexpr int NC = D / 32, RB = row_bytes<D>(), PPR = D / 8;  // MFMAs a tile, 16-byte pieces a row
   constexpr int LOADS = kStage * PPR / 256;
   __shared__ __align__(16) uint8_t stage[2][kStage * RB];
-  __shared__ int64_t where[kMaxTP / 16];  // offsets of the unit's blocks (-1: none)
+  __shared__ int64_t where[kSegment / 16];  // offsets of the segment's blocks (-1: none)
   __shared__ Window win;
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lq = lane >> 4, wave = uniform(tid >> 6);
   const int R = kCols / p.G;
@@ -268,28 +331,15 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_rows_kernel(Ch
     const int e = i * 256 + tid;
     in_block[i] = (e / PPR & 15) * p.k_s[1] + e % PPR * 8;
   }
-  int ends = 0, w0 = 0;
-  list_chunks(p, &win, 0, R, p.TP, &ends);
-  int64_t u = blockIdx.x, units = (int64_t)win.before[min(p.N, kWindow)] * p.Hkv;
-  for (;; u += gridDim.x) {
-    while (u >= units) {  // on to the next window
-      u -= units;
-      w0 += kWindow;
-      if (w0 >= p.N) return;
-      __syncthreads();
-      list_chunks(p, &win, w0, R, p.TP, &ends);
-      units = (int64_t)win.before[min(p.N - w0, kWindow)] * p.Hkv;
-    }
-    const Unit un = unit_of(p, &win, w0, u, R, p.TP, lane);
+  const int h = (int)(blockIdx.x % (unsigned)p.Hkv);
+  Runs<RowBlocks> runs(p, &win, RowBlocks{R}, p.row_steps);
+  Run un;
+  while (runs.next(&un)) {
     const Chunk& c = un.c;
-    const int r0 = un.rb * R, nr = min(R, c.rows - r0), ncol = nr * p.G;
-    const int t_begin = un.tb * p.TP, t_end = min(t_begin + p.TP, visible(c, r0 + nr));
-    const Factor f = factor_of(p, un.h);
-    for (int i = tid; t_begin + i * 16 < t_end; i += 256) {
-      const int blk = block_of(p, c.n, (t_begin >> 4) + i);
-      where[i] = blk < 0 ? -1 : (int64_t)blk * p.k_s[0] + (int64_t)un.h * p.k_s[2];
-    }
-    const QRows rows(p, c.row0 + r0, un.h, f.flip);
+    const int r0 = un.block * R, nr = min(R, c.rows - r0), ncol = nr * p.G;
+    const int t_begin = un.at * kStage, t_end = min(t_begin + un.n * kStage, visible(c, r0 + nr));
+    const Factor f = factor_of(p, h);
+    const QRows rows(p, c.row0 + r0, h, f.flip);
     // this wave's 64 columns: four tiles of 16
     QOp<QT> q[4][NC];
     int pos[4];  // last token that the lane's column of tile ct sees
@@ -308,88 +358,104 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_rows_kernel(Ch
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct) m[ct] = -INFINITY, l[ct] = 0.0f;
 
-    uint4 reg[LOADS];
-    auto fetch = [&](int t0) {  // tokens t0 .. + 63 (those past the end: the last one's block, masked)
-      const int last = (t_end - 1 - t_begin) >> 4, i0 = (t0 - t_begin) >> 4;
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int64_t at = where[min(i0 + (i * 256 + tid) / PPR / 16, last)];
-        reg[i] = k_piece<QT, KT>(p, (at < 0 ? (int64_t)un.h * p.k_s[2] : at) + in_block[i]);
+    for (int seg = t_begin; seg < t_end; seg += kSegment) {
+      const int seg_end = min(seg + kSegment, t_end);
+      for (int i = tid; seg + i * 16 < seg_end; i += 256) {
+        const int blk = block_of(p, c.n, (seg >> 4) + i);
+        where[i] = blk < 0 ? -1 : (int64_t)blk * p.k_s[0] + (int64_t)h * p.k_s[2];
       }
-    };
-    auto store = [&](int buf) {
+      // A step's loads go out at the start of the one before it, from offsets
+      // looked up in the one before that.
+      Stored<KT> reg[LOADS];
+      int64_t at[LOADS];
+      uint32_t absent = 0, next_absent = 0;  // blocks of a step that are none of the cache's
+      auto locate = [&](int t0) {  // tokens t0 .. + 63 (those past the end: the last one's block, masked)
+        const int last = (seg_end - 1 - seg) >> 4, i0 = (t0 - seg) >> 4;
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int e = i * 256 + tid;
-        *(uint4*)(stage[buf] + e / PPR * RB + e % PPR * 16) = reg[i];
-      }
-    };
-    __syncthreads();
-    fetch(t_begin);
-    store(0);
-    __syncthreads();
-    for (int t0 = t_begin, buf = 0; t0 < t_end; t0 += kStage, buf ^= 1) {
-      const bool more = t0 + kStage < t_end;
-      if (more) fetch(t0 + kStage);
-      if (busy && t0 <= w_hi) {
-        const int i0 = (t0 - t_begin) >> 4;
-        bool whole = t0 + kStage - 1 <= w_lo && t0 + kStage <= t_end;
-        int valid[kStage / 16];  // whether a block is one of the cache
+        for (int i = 0; i < LOADS; ++i) at[i] = where[min(i0 + (i * 256 + tid) / PPR / 16, last)];
+        const bool none = t0 + li * 16 >= seg_end || where[min(i0 + li, last)] < 0;
+        next_absent = (uint32_t)__ballot(none) & 15u;
+      };
+      auto fetch = [&] {
 #pragma unroll
-        for (int tt = 0; tt < kStage / 16; ++tt) {
-          valid[tt] = uniform((int)(t0 + tt * 16 < t_end ? where[i0 + tt] >> 32 : -1)) >= 0;
-          whole = whole && valid[tt];
+        for (int i = 0; i < LOADS; ++i)
+          reg[i] = k_piece<KT>(p, (at[i] < 0 ? (int64_t)h * p.k_s[2] : at[i]) + in_block[i]);
+      };
+      auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int e = i * 256 + tid;
+          *(uint4*)(stage[buf] + e / PPR * RB + e % PPR * 16) = operand<QT, KT>(reg[i]);
         }
-        // (two bodies: the masks' selects would double the vector work of a tile
-        // that needs none)
-        auto tiles = [&](auto masked) {
-          constexpr bool kMasked = decltype(masked)::value;
+      };
+      __syncthreads();
+      locate(seg);
+      fetch();
+      absent = next_absent;
+      if (seg + kStage < seg_end) locate(seg + kStage);
+      store(0);
+      __syncthreads();
+      for (int t0 = seg, buf = 0; t0 < seg_end; t0 += kStage, buf ^= 1) {
+        const bool more = t0 + kStage < seg_end;
+        const uint32_t here = absent;
+        if (more) {
+          fetch();
+          absent = next_absent;
+          if (t0 + 2 * kStage < seg_end) locate(t0 + 2 * kStage);
+        }
+        if (busy && t0 <= w_hi) {
+          const bool whole = t0 + kStage - 1 <= w_lo && t0 + kStage <= t_end && here == 0;
+          // (two bodies: the masks' selects would double the vector work of a tile
+          // that needs none)
+          auto tiles = [&](auto masked) {
+            constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll
-          for (int ct = 0; ct < 4; ++ct) {
-            f32x4_t s[4];
-#pragma unroll
-            for (int tt = 0; tt < 4; ++tt) {
-              s[tt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-              for (int x = 0; x < NC; ++x)
-                s[tt] = mfma16(as_qop<QT>(*(const uint4*)(stage[buf] + (tt * 16 + li) * RB + x * 64 + lq * 16)),
-                               q[ct][x], s[tt]);
-            }
-            if constexpr (kMasked) {
+            for (int ct = 0; ct < 4; ++ct) {
+              f32x4_t s[4];
 #pragma unroll
               for (int tt = 0; tt < 4; ++tt) {
-                const int last = valid[tt] ? min(pos[ct], t_end - 1) : -1;
+                s[tt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int v = 0; v < 4; ++v)
-                  if (t0 + tt * 16 + 4 * lq + v > last) s[tt][v] = -INFINITY;
+                for (int x = 0; x < NC; ++x)
+                  s[tt] = mfma16(as_qop<QT>(*(const uint4*)(stage[buf] + (tt * 16 + li) * RB + x * 64 + lq * 16)),
+                                 q[ct][x], s[tt]);
               }
-            }
-            float mx = s[0][0];
+              if constexpr (kMasked) {
 #pragma unroll
-            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
-            mx = kMasked && mx == -INFINITY ? mx : mx * f.qk;
-            // the reference moves only when a score exceeds it by more than 8
-            // (log2 units): sums of e <= 256 are as exact in float32
-            if (mx > m[ct] + 8.0f) {
-              l[ct] *= __builtin_amdgcn_exp2f(m[ct] - mx);
-              m[ct] = mx;
-            }
-            const float ref = m[ct] == -INFINITY ? 0.0f : m[ct];
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int tt = 0; tt < 4; ++tt) {
+                  const int last = (here >> tt & 1) == 0 ? min(pos[ct], t_end - 1) : -1;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float sv = s[i >> 2][i & 3];
-              const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sv, f.qk, -ref));
-              sum[i & 3] += !kMasked || sv != -INFINITY ? e : 0.0f;
+                  for (int v = 0; v < 4; ++v)
+                    if (t0 + tt * 16 + 4 * lq + v > last) s[tt][v] = -INFINITY;
+                }
+              }
+              float mx = s[0][0];
+#pragma unroll
+              for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
+              mx = kMasked && mx == -INFINITY ? mx : mx * f.qk;
+              // the reference moves only when a score exceeds it by more than 8
+              // (log2 units): sums of e <= 256 are as exact in float32
+              if (mx > m[ct] + 8.0f) {
+                l[ct] *= __builtin_amdgcn_exp2f(m[ct] - mx);
+                m[ct] = mx;
+              }
+              const float ref = m[ct] == -INFINITY ? 0.0f : m[ct];
+              float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float sv = s[i >> 2][i & 3];
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sv, f.qk, -ref));
+                sum[i & 3] += !kMasked || sv != -INFINITY ? e : 0.0f;
+              }
+              l[ct] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
-            l[ct] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          }
-        };
-        if (whole) tiles(std::false_type{});
-        else tiles(std::true_type{});
+          };
+          if (whole) tiles(std::false_type{});
+          else tiles(std::true_type{});
+        }
+        if (more) store(buf ^ 1);
+        __syncthreads();
       }
-      if (more) store(buf ^ 1);
-      __syncthreads();
     }
     // the four lanes of a column
 #pragma unroll
@@ -402,44 +468,66 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_rows_kernel(Ch
       L += __shfl_xor(L, 32, 64);
       const int j = wave * 64 + ct * 16 + li, r = col.row(j), g = j - r * p.G;
       if (lq == 0 && j < ncol)
-        p.ws_ml[(un.tb * p.stat_rows + stat_row(p, c, r0 + r)) * p.Hq + un.h * p.G + g] = make_float2(M, L);
+        p.ws_ml[(un.piece * p.stat_rows + stat_row(p, c, r0 + r)) * p.Hq + h * p.G + g] = make_float2(M, L);
     }
-    __syncthreads();  // the stage is filled anew
+    if (un.last && h == 0 && tid < nr) p.ws_np[stat_row(p, c, r0 + tid)] = un.pieces;
   }
 }
 
-// ---- tokens: sums over the rows of a piece -----------------------------------
+// (-reference, 1 / sum) of a row and head from its runs, kBatch of them in flight
+// at a time.
+__device__ __forceinline__ float2 joined(const ChunkWeightsParams& p, int64_t row, int head) {
+  const float2* ml = p.ws_ml + row * p.Hq + head;
+  const int64_t step = p.stat_rows * p.Hq;
+  // (a row without tokens has no runs, and what is read for it goes nowhere)
+  const int np = min(max(p.ws_np[row], 0), p.ml_pieces);
+  float M = -INFINITY, L = 0.0f;
+  constexpr int kBatch = 8;
+  for (int i0 = 0; i0 < np; i0 += kBatch) {
+    float2 x[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) x[k] = ml[min(i0 + k, np - 1) * step];
+    float mn = M;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) mn = fmaxf(mn, x[k].x);
+    L *= M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - mn);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (i0 + k < np) L += x[k].y * (x[k].x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(x[k].x - mn));
+    M = mn;
+  }
+  return make_float2(M == -INFINITY ? 0.0f : -M, L == 0.0f ? 0.0f : 1.0f / L);
+}
+
+// In the place of the first run's, for calls whose tokens kernel would join a
+// row many times; one (row, head) a thread.  (Rows that no chunk has hold
+// anything, and nobody reads what comes of it.)
+__global__ __launch_bounds__(256) void chunk_stats_kernel(ChunkWeightsParams p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / p.Hq;
+  if (row < p.stat_rows) p.ws_ml[i] = joined(p, row, (int)(i - row * p.Hq));
+}
+
+// ---- tokens: sums over a run of columns ----------------------------------------
 
 template <int QT, int KT, int D>
 __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_tokens_kernel(ChunkWeightsParams p) {
   constexpr int NC = D / 32, RB = row_bytes<D>(), PPR = D / 8;
   constexpr int LOADS = kStage * PPR / 256;
   __shared__ __align__(16) uint8_t stage[2][kStage * RB];
-  __shared__ float2 fin[kMaxCB];  // (-m, 1 / l) of the unit's columns
+  __shared__ float2 fin[kColumns];  // (-m, 1 / l) of the segment's columns
   __shared__ Window win;
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lq = lane >> 4, wave = uniform(tid >> 6);
-  const int R = p.CB / p.G, RA = kCols / p.G;
   const Columns colm(p.G);
-  int ends = 0, w0 = 0;
-  list_chunks(p, &win, 0, R, kCols, &ends);
-  int64_t u = blockIdx.x, units = (int64_t)win.before[min(p.N, kWindow)] * p.Hkv;
-  for (;; u += gridDim.x) {
-    while (u >= units) {  // on to the next window
-      u -= units;
-      w0 += kWindow;
-      if (w0 >= p.N) return;
-      __syncthreads();
-      list_chunks(p, &win, w0, R, kCols, &ends);
-      units = (int64_t)win.before[min(p.N - w0, kWindow)] * p.Hkv;
-    }
-    const Unit un = unit_of(p, &win, w0, u, R, kCols, lane);
+  const int h = (int)(blockIdx.x % (unsigned)p.Hkv);
+  const TokenBlocks blocks{p.G};
+  Runs<TokenBlocks> runs(p, &win, blocks, p.col_steps);
+  Run un;
+  while (runs.next(&un)) {
     const Chunk& c = un.c;
-    const int r0 = un.rb * R, nr = min(R, c.rows - r0), ncol = nr * p.G;
-    const int vis = visible(c, r0 + nr);
-    const int t0 = un.tb * kCols, tw = t0 + wave * 64;  // the unit's and the wave's first token
-    const Factor f = factor_of(p, un.h);
-    // columns before the first row that sees the unit's tokens are left out
-    const int j_begin = max(t0 - c.c0 - r0, 0) * p.G & ~(kStage - 1);
+    const int ncol = c.rows * p.G, vis = visible(c, c.rows);
+    const int t0 = un.block * kCols, tw = t0 + wave * 64;  // the block's and the wave's first token
+    const int j_begin = (blocks.first(c, un.block) + un.at) * kStage, j_end = j_begin + un.n * kStage;
+    const Factor f = factor_of(p, h);
 
     // this wave's 64 tokens: four blocks of 16
     QOp<QT> k[4][NC];
@@ -451,8 +539,8 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_tokens_kernel(
       live[tt] = blk < 0 ? 0 : min(vis - t, 16);
 #pragma unroll
       for (int x = 0; x < NC; ++x)
-        k[tt][x] = as_qop<QT>(k_piece<QT, KT>(p, (int64_t)(blk < 0 ? 0 : blk) * p.k_s[0] + (int64_t)un.h * p.k_s[2] +
-                                                      li * p.k_s[1] + 32 * x + 8 * lq));
+        k[tt][x] = as_qop<QT>(operand<QT, KT>(k_piece<KT>(p, (int64_t)(blk < 0 ? 0 : blk) * p.k_s[0] +
+                                                                 (int64_t)h * p.k_s[2] + li * p.k_s[1] + 32 * x + 8 * lq)));
     }
     const bool all_live = live[0] + live[1] + live[2] + live[3] == 64;
     float acc[4][4];
@@ -461,13 +549,13 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_tokens_kernel(
 #pragma unroll
       for (int v = 0; v < 4; ++v) acc[tt][v] = 0.0f;
 
-    const QRows rows(p, c.row0 + r0, un.h, f.flip);
-    uint4 reg[LOADS];
-    auto fetch = [&](int j0) {  // columns j0 .. + 63 (zeros past the last)
+    uint4 reg[LOADS];  // a step's first column: head `head` of row `row`
+    auto fetch = [&](int j0, int row, int head) {  // columns j0 .. + 63 (zeros past the last)
+      const QRows rows(p, c.row0 + row, h, f.flip);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int e = i * 256 + tid, j = j0 + e / PPR, r = colm.row(j), g = j - r * p.G;
-        reg[i] = j < ncol ? rows.piece(r, g, e % PPR * 8) : make_uint4(0, 0, 0, 0);
+        const int e = i * 256 + tid, j = head + e / PPR, r = colm.row(j), g = j - r * p.G;
+        reg[i] = j0 + e / PPR < ncol ? rows.piece(r, g, e % PPR * 8) : make_uint4(0, 0, 0, 0);
       }
     };
     auto store = [&](int buf) {
@@ -477,79 +565,68 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_tokens_kernel(
         *(uint4*)(stage[buf] + e / PPR * RB + e % PPR * 16) = reg[i];
       }
     };
-    fetch(j_begin);
-    // the rows' references and sums, from their pieces: kBatch of them in
-    // flight at a time
-    for (int j = j_begin + tid; j < cdiv(ncol, kStage) * kStage; j += 256) {
-      float2 v = make_float2(0.0f, 0.0f);
-      if (j < ncol) {
-        const int r = colm.row(j), g = j - r * p.G, row = r0 + r;
-        const float2* ml = p.ws_ml + stat_row(p, c, row) * p.Hq + un.h * p.G + g;
-        const int64_t step = p.stat_rows * p.Hq;
-        const int np = cdiv(visible(c, (row / RA + 1) * RA), p.TP);  // pieces that the rows kernel wrote
-        float M = -INFINITY, L = 0.0f;
-        constexpr int kBatch = 8;
-        for (int i0 = 0; i0 < np; i0 += kBatch) {
-          float2 x[kBatch];
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) x[i] = ml[min(i0 + i, np - 1) * step];
-          float mn = M;
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) mn = fmaxf(mn, x[i].x);
-          L *= M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - mn);
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i)
-            if (i0 + i < np) L += x[i].y * (x[i].x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(x[i].x - mn));
-          M = mn;
-        }
-        v = make_float2(M == -INFINITY ? 0.0f : -M, L == 0.0f ? 0.0f : 1.0f / L);
+    int row = j_begin / p.G, head = j_begin - row * p.G;
+    for (int seg = j_begin; seg < j_end; seg += kColumns) {
+      const int seg_end = min(seg + kColumns, j_end);
+      fetch(seg, row, head);
+      for (int i = tid; i < seg_end - seg; i += 256) {
+        const int r = colm.row(head + i), g = head + i - r * p.G;
+        const int64_t at = stat_row(p, c, row + r);
+        fin[i] = seg + i >= ncol ? make_float2(0.0f, 0.0f)
+                                 : (p.joined ? p.ws_ml[at * p.Hq + h * p.G + g] : joined(p, at, h * p.G + g));
       }
-      fin[j] = v;
-    }
-
-    store(0);
-    __syncthreads();
-    for (int j0 = j_begin, buf = 0; j0 < ncol; j0 += kStage, buf ^= 1) {
-      const bool more = j0 + kStage < ncol;
-      if (more) fetch(j0 + kStage);
-      // the last of these columns sees the wave's first token, and the first its last
-      if (tw < vis && c.c0 + r0 + colm.row(min(j0 + kStage - 1, ncol - 1)) >= tw) {
-        const bool whole = all_live && c.c0 + r0 + colm.row(j0) >= tw + 63;
-        auto tiles = [&](auto masked) {
-          constexpr bool kMasked = decltype(masked)::value;
+      store(0);
+      __syncthreads();
+      for (int j0 = seg, buf = 0; j0 < seg_end; j0 += kStage, buf ^= 1) {
+        const bool more = j0 + kStage < seg_end;
+        const int on = colm.row(head + kStage), next_row = row + on, next_head = head + kStage - on * p.G;
+        if (more) fetch(j0 + kStage, next_row, next_head);
+        // the last of these columns sees the wave's first token, and the first its last
+        const int pos = c.c0 + row;
+        if (tw < vis && pos + colm.row(head + min(kStage - 1, ncol - 1 - j0)) >= tw) {
+          const bool whole = all_live && pos >= tw + 63;
+          auto tiles = [&](auto masked) {
+            constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll
-          for (int ct = 0; ct < 4; ++ct) {
-            const float2 col = fin[j0 + ct * 16 + li];
-            QOp<QT> q[NC];
+            for (int ct = 0; ct < 4; ++ct) {
+              const float2 col = fin[j0 - seg + ct * 16 + li];
+              QOp<QT> q[NC];
 #pragma unroll
-            for (int x = 0; x < NC; ++x)
-              q[x] = as_qop<QT>(*(const uint4*)(stage[buf] + (ct * 16 + li) * RB + x * 64 + lq * 16));
-            const int j = j0 + ct * 16 + li, last = !kMasked ? 0 : (j < ncol ? c.c0 + r0 + colm.row(j) : -1);
+              for (int x = 0; x < NC; ++x)
+                q[x] = as_qop<QT>(*(const uint4*)(stage[buf] + (ct * 16 + li) * RB + x * 64 + lq * 16));
+              const int j = ct * 16 + li, last = !kMasked ? 0 : (j0 + j < ncol ? pos + colm.row(head + j) : -1);
+              f32x4_t s[4];
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) {
-              f32x4_t s = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+              for (int tt = 0; tt < 4; ++tt) {
+                s[tt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-              for (int x = 0; x < NC; ++x) s = mfma16(k[tt][x], q[x], s);
+                for (int x = 0; x < NC; ++x) s[tt] = mfma16(k[tt][x], q[x], s[tt]);
+              }
 #pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], f.qk, col.x));
-                const float sum = __builtin_fmaf(e, col.y, acc[tt][v]);
-                if constexpr (kMasked) {
-                  // the block's tokens that exist, up to the column's own position
-                  const int end = min(live[tt], last + 1 - (tw + tt * 16));
-                  acc[tt][v] = 4 * lq + v < end ? sum : acc[tt][v];
-                } else {
-                  acc[tt][v] = sum;
+              for (int tt = 0; tt < 4; ++tt) {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                  const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][v], f.qk, col.x));
+                  const float sum = __builtin_fmaf(e, col.y, acc[tt][v]);
+                  if constexpr (kMasked) {
+                    // the block's tokens that exist, up to the column's own position
+                    const int end = min(live[tt], last + 1 - (tw + tt * 16));
+                    acc[tt][v] = 4 * lq + v < end ? sum : acc[tt][v];
+                  } else {
+                    acc[tt][v] = sum;
+                  }
                 }
               }
             }
-          }
-        };
-        if (whole) tiles(std::false_type{});
-        else tiles(std::true_type{});
+          };
+          if (whole) tiles(std::false_type{});
+          else tiles(std::true_type{});
+        }
+        if (more) store(buf ^ 1);
+        __syncthreads();
+        row = next_row;
+        head = next_head;
       }
-      if (more) store(buf ^ 1);
-      __syncthreads();
     }
     // the 16 columns of a lane group
 #pragma unroll
@@ -559,14 +636,14 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_tokens_kernel(
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) acc[tt][v] += __shfl_xor(acc[tt][v], o, 64);
     if (li == 0) {
-      float* out = p.ws_p + ((piece0(p, c, R) + un.rb) * p.Hkv + un.h) * (int64_t)p.Mb * 16;
+      float* out = p.ws_p + ((piece0(p, c) + un.piece) * p.Hkv + h) * (int64_t)p.Mb * 16;
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
         const int t = tw + tt * 16 + 4 * lq;
         if (t < p.Mb * 16) *(float4*)(out + t) = make_float4(acc[tt][0], acc[tt][1], acc[tt][2], acc[tt][3]);
       }
     }
-    __syncthreads();  // fin and the stage are filled anew
+    if (un.last && h == 0 && tid == 0) p.ws_tp[c.n * cdiv(p.Mb * 16, kCols) + un.block] = un.pieces;
   }
 }
 
@@ -587,12 +664,12 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkWeightsParams p) {
   start = wave_last(wave_incl_max(start, 0));
   const Chunk c = chunk_of(p, n, start, max(start_of(p, n + 1), start), len_of(p, n));
   if (c.rows == 0) return;
-  const int R = p.CB / p.G, nb = cdiv(c.rows, R), heads = p.Hkv / p.Hw;
-  // the row blocks from the first that sees token t on, and their heads: one
-  // head's sums are Hkv rows apart, those of all heads follow each other
-  const int first = max(t - c.c0, 0) / R, count = t < c.cap ? (nb - first) * heads : 0;
+  const int heads = p.Hkv / p.Hw;
+  // the pieces of the token's block and their heads: one head's sums are Hkv
+  // rows apart, those of all heads follow each other
+  const int seen = t < visible(c, c.rows) ? p.ws_tp[n * cdiv(per, kCols) + t / kCols] : 0, count = seen * heads;
   const int64_t step = (int64_t)per * (p.Hw == 1 ? 1 : p.Hkv);
-  const float* part = p.ws_p + ((piece0(p, c, R) + first) * p.Hkv + hw * heads) * (int64_t)per + t;
+  const float* part = p.ws_p + (piece0(p, c) * p.Hkv + hw * heads) * (int64_t)per + t;
   float sum = 0.0f;
 #pragma unroll 8
   for (int i = wave; i < count; i += SPLIT ? 4 : 1) sum += part[i * step];
@@ -614,42 +691,66 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkWeightsParams p) {
 struct Cut {
   bool compact;         // rows stored by the chunk (a window of observers)
   int64_t stat_rows;    // rows of ws_ml
-  int64_t row_pieces;   // of ws_p
-  int TP, CB;
+  int64_t ml_pieces;    // runs of a row's tokens, at most
+  int64_t pieces;       // of ws_p
+  int row_steps, col_steps, piece_rows;
 };
 
-// Long units reuse what they hold in registers more often, short ones even out
-// what the workgroups get: the longest that give each at least kUnitsEach, of
-// about half of the (row, token) blocks (causal).
-constexpr double kUnitsEach = 2.5;
-
-Cut cut_of(int64_t Tq, int64_t N, int64_t Hkv, int64_t G, int64_t D, int64_t cap, int64_t observe) {
+// The least that a workgroup takes bounds the runs of a block, and with them the
+// workspace: a row's tokens are at most 33 runs; a token's columns runs of 64
+// columns at least, or of more (up to 4,096) where the sums would exceed 32 MB.
+Cut cut_of(int64_t Tq, int64_t N, int64_t Hkv, int64_t G, int64_t cap, int64_t observe) {
   Cut c;
   c.compact = observe > 0 && N * observe < Tq;
   c.stat_rows = c.compact ? N * observe : Tq;
-  const double want = kUnitsEach * (D == 64 ? 3 : 2) * device_cu_count();
-  const double seen = observe > 0 ? 1.0 : 0.5;
-  auto pieces = [&](int64_t cols) { return c.compact ? N * ceil_div(observe, cols / G) : Tq / (cols / G) + N; };
-  c.TP = 1024;
-  while (c.TP > 128 && (double)pieces(kCols) * Hkv * ceil_div(cap, c.TP) * seen < want) c.TP /= 2;
-  // (at most 64 pieces of a long row's tokens, as long as kMaxTP holds them)
-  c.TP = (int)std::min<int64_t>(kMaxTP, std::max<int64_t>(c.TP, ceil_div(ceil_div(cap, 64), kStage) * kStage));
-  c.CB = kMaxCB;
-  while (c.CB > kCols && (double)pieces(c.CB) * Hkv * ceil_div(cap, kCols) * seen < want) c.CB /= 2;
-  c.row_pieces = pieces(c.CB);
+  const int64_t steps = std::max<int64_t>(ceil_div(cap, kStage), 1);
+  c.row_steps = (int)ceil_div(steps, 32);
+  c.ml_pieces = (steps - 1) / c.row_steps + 2;
+  for (c.col_steps = 1;; c.col_steps *= 2) {
+    c.piece_rows = (int)(c.col_steps * kStage / G);  // (G <= 64)
+    c.pieces = c.compact ? N * (ceil_div(observe, c.piece_rows) + 1) : Tq / c.piece_rows + 2 * N;
+    if (c.col_steps == 64 || c.pieces * Hkv * cap * 4 <= 32 << 20) break;
+  }
   return c;
 }
 
 uint64_t pad(uint64_t x) { return (x + 255) & ~(uint64_t)255; }
 
+// (row, head, token) triples from which a kernel of its own joins the rows'
+// runs: 256 observers of 32 heads over 12,000 tokens (9.8e7) take 41.1 us in the
+// tokens kernel and 4.0 before it, 48.0 where it joins them itself; 35 rows of
+// 64 heads over 4,200 (9.4e6) 13.6 in all.
+constexpr double kJoinFirst = 3.2e7;
+
+struct Layout {
+  Cut cut;
+  uint64_t p, np, tp, bytes;  // byte offsets behind ws_ml
+};
+
+Layout layout_of(int64_t Tq, int64_t N, int64_t Hq, int64_t Hkv, int64_t cap, int64_t observe) {
+  Layout w;
+  w.cut = cut_of(Tq, N, Hkv, Hq / Hkv, cap, observe);
+  w.p = pad((uint64_t)w.cut.ml_pieces * w.cut.stat_rows * Hq * 8);
+  w.np = w.p + pad((uint64_t)w.cut.pieces * Hkv * cap * 4);
+  w.tp = w.np + pad((uint64_t)w.cut.stat_rows * 4);
+  w.bytes = w.tp + pad((uint64_t)N * ceil_div(cap, kCols) * 4);
+  return w;
+}
+
 template <int QT, int KT, int D>
 int32_t launch_d(const ChunkWeightsParams& p, hipStream_t stream) {
   const int64_t cap = (int64_t)p.Mb * 16;
-  // as many workgroups as are resident: each takes every grid-th unit
-  const dim3 grid((unsigned)(waves_per_simd<D>() * device_cu_count()));
+  // as many workgroups as are resident, the same number for every head
+  const int resident = waves_per_simd<D>() * device_cu_count();
+  const dim3 grid((unsigned)(std::max(resident / p.Hkv, 1) * p.Hkv));
   {
     ProfileScope prof("cf_chunk_rows", stream);
     CF_LAUNCH((chunk_rows_kernel<QT, KT, D>), grid, dim3(256), 0, stream, p);
+    CF_HIP_CHECK(hipGetLastError());
+  }
+  if (p.joined) {
+    ProfileScope prof("cf_chunk_stats", stream);
+    CF_LAUNCH(chunk_stats_kernel, dim3((unsigned)ceil_div(p.stat_rows * p.Hq, 256)), dim3(256), 0, stream, p);
     CF_HIP_CHECK(hipGetLastError());
   }
   {
@@ -659,7 +760,7 @@ int32_t launch_d(const ChunkWeightsParams& p, hipStream_t stream) {
   }
   ProfileScope prof("cf_chunk_join", stream);
   // (many pieces a token: more loads in flight)
-  if (ceil_div(p.Tq, p.N * (p.CB / p.G)) * (p.Hkv / p.Hw) >= 8)
+  if (ceil_div(p.compact ? p.observe : ceil_div(p.Tq, p.N), p.piece_rows) * (p.Hkv / p.Hw) >= 8)
     CF_LAUNCH((chunk_join_kernel<true>), dim3((unsigned)(ceil_div(cap, 64) * p.N * p.Hw)), dim3(256), 0, stream, p);
   else
     CF_LAUNCH((chunk_join_kernel<false>), dim3((unsigned)(ceil_div(cap, 256) * p.N * p.Hw)), dim3(256), 0, stream, p);
@@ -679,7 +780,7 @@ bool chunk_weights_supported(const ChunkWeightsParams& p, int q_dt, int k_dt) {
     return false;
   if (p.D != 64 && p.D != 128) return false;
   if (p.G > 64 || p.NB < 1) return false;
-  // a unit's offsets into q: 1,024 rows and 64 heads
+  // a step's offsets into q: up to 256 rows and 64 heads
   if (p.q_sr >= 1 << 20 || p.q_sh >= 1 << 20) return false;
   const int kb = k_dt == kE4M3 ? 1 : 2;
   if (p.k_s[3] != 1 || ((uintptr_t)p.k & 15) != 0 || ((uintptr_t)p.q & 15) != 0) return false;
@@ -689,22 +790,23 @@ bool chunk_weights_supported(const ChunkWeightsParams& p, int q_dt, int k_dt) {
 }
 
 uint64_t chunk_weights_workspace_bytes(int64_t num_q_tokens, int64_t num_chunks, int64_t num_q_heads,
-                                       int64_t num_kv_heads, int64_t head_dim, int64_t max_blocks, int64_t observe) {
-  const int64_t cap = max_blocks * 16;
-  const Cut c = cut_of(num_q_tokens, num_chunks, num_kv_heads, num_q_heads / num_kv_heads, head_dim, cap, observe);
-  return pad((uint64_t)ceil_div(cap, c.TP) * c.stat_rows * num_q_heads * 8) +
-         pad((uint64_t)c.row_pieces * num_kv_heads * cap * 4);
+                                       int64_t num_kv_heads, int64_t max_blocks, int64_t observe) {
+  return layout_of(num_q_tokens, num_chunks, num_q_heads, num_kv_heads, max_blocks * 16, observe).bytes;
 }
 
 void chunk_weights_bind_workspace(ChunkWeightsParams& p, void* workspace) {
-  const int64_t cap = (int64_t)p.Mb * 16;
-  const Cut c = cut_of(p.Tq, p.N, p.Hkv, p.G, p.D, cap, p.observe);
-  p.compact = c.compact;
-  p.stat_rows = c.stat_rows;
-  p.TP = c.TP;
-  p.CB = c.CB;
+  const Layout w = layout_of(p.Tq, p.N, p.Hq, p.Hkv, (int64_t)p.Mb * 16, p.observe);
+  p.compact = w.cut.compact;
+  p.stat_rows = w.cut.stat_rows;
+  p.ml_pieces = (int)w.cut.ml_pieces;
+  p.row_steps = w.cut.row_steps;
+  p.col_steps = w.cut.col_steps;
+  p.piece_rows = w.cut.piece_rows;
+  p.joined = (double)p.stat_rows * p.Hq * p.Mb * 16 >= kJoinFirst;
   p.ws_ml = (float2*)workspace;
-  p.ws_p = (float*)((char*)workspace + pad((uint64_t)ceil_div(cap, c.TP) * c.stat_rows * p.Hq * 8));
+  p.ws_p = (float*)((char*)workspace + w.p);
+  p.ws_np = (int*)((char*)workspace + w.np);
+  p.ws_tp = (int*)((char*)workspace + w.tp);
 }
 
 int32_t launch_chunk_weights(const ChunkWeightsParams& p, int q_dt, int k_dt, hipStream_t stream) {

@@ -27,18 +27,22 @@ struct ChunkWeightsParams {
   int observe;  // last rows of a chunk that count; 0: all of them
   int N, Tq, Hq, Hkv, Hw, G, D, Mb, NB;
   // set by chunk_weights_bind_workspace
-  float2* ws_ml;  // [token pieces, stat_rows, Hq] (reference, sum) of a row over a piece of its tokens
-  float* ws_p;    // [row pieces, Hkv, Mb * 16] sums over the rows of a piece
+  float2* ws_ml;  // [ml_pieces, stat_rows, Hq] (reference, sum) of a row over a run of its tokens
+  float* ws_p;    // [pieces, Hkv, Mb * 16] sums over a run of columns
+  int* ws_np;     // [stat_rows] runs of the row's tokens
+  int* ws_tp;     // [N, blocks of 256 tokens] runs of the block's columns
   int64_t stat_rows;
-  bool compact;   // rows and row pieces are numbered by the chunk's observers
-  int TP;         // tokens of a piece
-  int CB;         // columns (query rows x heads of the group) of a row piece
+  bool compact;   // rows and pieces are numbered by the chunk's observers
+  bool joined;    // the rows' runs are joined before the tokens kernel
+  int ml_pieces;
+  int row_steps, col_steps;  // steps that a workgroup takes at least
+  int piece_rows;            // rows of col_steps steps
 };
 
 bool chunk_weights_supported(const ChunkWeightsParams& p, int q_dt, int k_dt);
 // Workspace of a call; chunk_weights_bind_workspace lays it out.
 uint64_t chunk_weights_workspace_bytes(int64_t num_q_tokens, int64_t num_chunks, int64_t num_q_heads,
-                                       int64_t num_kv_heads, int64_t head_dim, int64_t max_blocks, int64_t observe);
+                                       int64_t num_kv_heads, int64_t max_blocks, int64_t observe);
 void chunk_weights_bind_workspace(ChunkWeightsParams& p, void* workspace);
 int32_t launch_chunk_weights(const ChunkWeightsParams& p, int q_dt, int k_dt, hipStream_t stream);
 

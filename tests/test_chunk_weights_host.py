@@ -81,11 +81,12 @@ def test_the_workspace_is_checked():
         ops.chunk_weights_workspace_bytes(5, 2, 8, 2, 64, 3, 8)
     with pytest.raises(ValueError, match="64 query heads"):
         ops.chunk_weights_workspace_bytes(5, 2, 130, 2, 64, 3)
-    # 8 bytes a row, head and piece, 4 a token and head for each row piece
+    # 8 bytes a row, head and run of its tokens, 4 a token and head for each run
+    # of columns, 4 a row and 4 a block of 256 tokens
     small = ops.chunk_weights_workspace_bytes(5, 2, 8, 2, 64, 3)
     assert 5 * 8 * 8 + 2 * 2 * 48 * 4 <= small <= 4096
     long = ops.chunk_weights_workspace_bytes(8192, 1, 32, 8, 128, 8192)
     assert long <= 64 * 8192 * 32 * 8 + (8192 * 4 // 256 + 1) * 8 * 8192 * 16 * 4 + 512
     # a window of observers needs its rows only
     few = ops.chunk_weights_workspace_bytes(8192, 1, 32, 8, 128, 8192, observe=64)
-    assert few <= 64 * 64 * 32 * 8 + 8 * 8192 * 16 * 4 + 512
+    assert few <= 33 * 64 * 32 * 8 + 5 * 8 * 8192 * 16 * 4 + 64 * 4 + 512 * 4 + 1024

@@ -2,9 +2,11 @@
 
 Tolerance: a weight p is within 1.2e-5 p of the exact one for log2 scores up to
 16 (tests/test_gpu_decode_weights.py has the terms); an account adds them in
-float32, at most 64 in a chain, then 16 lanes, then the pieces and heads one by
-one (32 at most here), half a step each: 112 * 2^-24 < 7e-6 of the sum, and a
-step of the whole for the old value."""
+float32, four a step of a workgroup's stretch (84 in a chain at most here), then
+16 lanes in four steps and the runs in five, half a step each: 93 * 2^-24 =
+5.6e-6 of the sum; l is a sum of 35 roundings at most, 1.2e-6 more than the
+2^-20 counted there: below 7e-6 together, and a step of the whole for the old
+value."""
 
 from __future__ import annotations
 
