@@ -38,6 +38,7 @@ namespace {
 // lane of one wave; if they are too many, a histogram of the bin's next ten
 // bits comes first.  A workgroup is bound by its instructions a key (some 80)
 // and the latency of its barriers and LDS steps.
+// 64 sequences of 8 heads and 2,064 slots: 14 us (12.6 MB); four of 30,000: 28 us.
 
 __device__ __forceinline__ uint32_t key_of(float w) {
   if (w != w) return 0xFFFFFFFEu;
@@ -398,21 +399,30 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictSelectParams
 
 // ---- move --------------------------------------------------------------------
 //
-// Weights and positions move with a lane a slot.  K and V rows: where channels
-// are contiguous a row moves as 16-byte pieces.  Where a channel's tokens are
-// contiguous (channel-major V) it is D single elements; when most slots of a
-// 16-token run change, as when a prompt is cut, a lane takes a channel instead,
-// reads its 16 tokens from where each belongs, and writes the run whole
-// (unmoved tokens with their own value).  Two kernels: a wave a run of 16
-// slots, everything it moves in flight at once, for calls that may move much;
-// and 256 slots scanned a workgroup for those that move few (a decode batch
-// evicting its latest block), whose time is the scan.
+// A workgroup looks 256 slots up, moves their weights and positions with a lane
+// a slot, and lists the slots that move.  Rows whose channels are contiguous move
+// as 16-byte pieces.  Where a channel's tokens are contiguous (channel-major V) a
+// row is D single elements; when many of the 256 move, as when a prompt is cut, a
+// lane takes a channel of a 16-token run instead and writes the run whole.
+constexpr int kSlots = 256;
+constexpr int kRuns = kSlots / 16;
+// (2,048 slots of 16 sequences and 8 heads of 128 in bf16, of 256 slots 51, 93
+// and 128 moving: element by element 34, 51 and 86 us, by runs 68, 70 and 74; in
+// e4m3 25, 34 and 46 against 36, 37 and 37.)
+constexpr int kTileMoves = 112;
 
 enum MoveMode : int { kRows = 0, kTile = 1, kElements = 2 };
 
-// Element offset of a slot in a cache, without head and channel.
-__device__ __forceinline__ int64_t slot_at(const int64_t* s, int blk, int off) {
-  return (int64_t)blk * s[0] + (int64_t)off * s[1];
+// A cache's strides, by value (pointers into the kernel's arguments would put
+// them into scratch memory).
+struct Strides {
+  int64_t block, token, head, channel;
+  // Element offset of a slot, without head and channel.
+  __device__ __forceinline__ int64_t slot(int blk, int off) const { return (int64_t)blk * block + (int64_t)off * token; }
+};
+template <int WHICH>
+__device__ __forceinline__ Strides strides_of(const EvictMoveParams& p) {
+  return Strides{p.c_s[WHICH][0], p.c_s[WHICH][1], p.c_s[WHICH][2], p.c_s[WHICH][3]};
 }
 
 // Slot j of sequence b, account head h: its source, and where both lie.
@@ -454,133 +464,114 @@ __device__ __forceinline__ MoveSlot move_slot(const EvictMoveParams& p, int b, i
 
 __device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
-// A wave's 16 slots (lanes 0..15): rows as pieces.  Loads first, kRowsInFlight
-// pieces a lane, then stores.
-template <class T>
-__device__ __forceinline__ void move_rows(const EvictMoveParams& p, int which, int h, const MoveSlot& m, uint32_t bits,
-                                          int lane) {
-  constexpr int kInFlight = 4, kElems = 16 / (int)sizeof(T);
-  const int64_t* s = p.c_s[which];
-  T* base = (T*)p.cache[which] + (int64_t)h * s[2];
-  const int per = p.D / kElems, n = 16 * per;
-  for (int u0 = 0; u0 < n; u0 += 64 * kInFlight) {
-    uint4 v[kInFlight];
-    T* to[kInFlight];
-    bool live[kInFlight];
+// (the compiler keeps arrays of uint4 that are stored under a condition in
+// scratch memory, and arrays of this in registers)
+typedef uint32_t Bytes16 __attribute__((ext_vector_type(4)));
+
+// kN pieces a thread of the listed rows' `total` from `from` on, by pieces
+// (E = Bytes16) or elements; past the end the last one again, not stored.
+template <int kN, class E, class T>
+__device__ __forceinline__ void copy_pieces(const Strides& s, T* base, int h0, int per, int row, const int4* list,
+                                            int from, int total) {
+  constexpr int kElems = (int)(sizeof(E) / sizeof(T));
+  E v[kN];
+  T* to[kN];
 #pragma unroll
-    for (int i = 0; i < kInFlight; ++i) {
-      const int u = u0 + i * 64 + lane, l = min(u, n - 1) / per, c = u - l * per;
-      live[i] = u < n && ((bits >> l) & 1u) != 0;
-      const int sb = __shfl(m.src_blk, l, 64), so = __shfl(m.src_off, l, 64);
-      const int db = __shfl(m.dst_blk, l, 64), dof = __shfl(m.dst_off, l, 64);
-      to[i] = base + slot_at(s, db, dof) + c * kElems;
-      if (live[i]) v[i] = *(const uint4*)(base + slot_at(s, sb, so) + c * kElems);
-    }
-#pragma unroll
-    for (int i = 0; i < kInFlight; ++i)
-      if (live[i]) *(uint4*)to[i] = v[i];
+  for (int i = 0; i < kN; ++i) {
+    const uint32_t u = (uint32_t)min(from + i * 256 + (int)threadIdx.x, total - 1);
+    const uint32_t k = u / (uint32_t)row, r = u - k * (uint32_t)row;
+    const uint32_t hh = r / (uint32_t)per, c = r - hh * (uint32_t)per;
+    const int4 m = list[k];
+    const int64_t at = (int64_t)(h0 + (int)hh) * s.head + (int64_t)(c * kElems) * s.channel;
+    v[i] = *(const E*)(base + s.slot(m.x, m.y) + at);
+    to[i] = base + s.slot(m.z, m.w) + at;
   }
+#pragma unroll
+  for (int i = 0; i < kN; ++i)
+    if (from + i * 256 + (int)threadIdx.x < total) *(E*)to[i] = v[i];
 }
 
-// The same for 16 tokens of a block in channel-major storage.
+// The listed rows of heads [h0, h0 + nh): eight pieces a thread in flight, the
+// rest two at a time (a few moves must not load eight).
+template <int WHICH, class E, class T>
+__device__ __forceinline__ void copy_listed(const EvictMoveParams& p, int h0, int nh, const int4* list, int n) {
+  constexpr int kElems = (int)(sizeof(E) / sizeof(T));
+  const Strides s = strides_of<WHICH>(p);
+  T* base = (T*)p.cache[WHICH];
+  const int per = p.D / kElems, row = nh * per, total = n * row;
+  int from = 0;
+  for (; from + 8 * 256 <= total; from += 8 * 256)
+    copy_pieces<8, E, T>(s, base, h0, per, row, list, from, total);
+  for (; from < total; from += 2 * 256) copy_pieces<2, E, T>(s, base, h0, per, row, list, from, total);
+}
+
+// Channel-major V of heads [h0, h0 + nh) by runs of 16 slots in which some move:
+// a wave takes 64 channels of a run, a lane reads its 16 tokens from where each
+// belongs (unmoved ones from their own place: a load that may be left out would
+// have to be waited for where the ways meet) and writes them whole.
 template <class T>
-__device__ __forceinline__ void move_tile(const EvictMoveParams& p, int which, int h, const MoveSlot& m, uint32_t bits,
-                                          int lane) {
-  const int64_t* s = p.c_s[which];
-  T* base = (T*)p.cache[which] + (int64_t)h * s[2];
-  const int l0 = __builtin_ctz(bits);
-  const int64_t run = slot_at(s, lane_value(m.dst_blk, l0), lane_value(m.dst_off, l0) - l0);
-  for (int d = lane; d < p.D; d += 64) {
-    T* dst = base + run + (int64_t)d * s[3];
+__device__ __forceinline__ void copy_tiles(const EvictMoveParams& p, int h0, int nh, const int4* slots,
+                                           const uint64_t* moved) {
+  const Strides s = strides_of<1>(p);
+  const int lane = threadIdx.x & 63, parts = (p.D + 63) >> 6, items = nh * kRuns * parts;
+  for (int u = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < items; u += 4) {
+    const int run = u & (kRuns - 1), hp = u / kRuns, hh = hp / parts, d = (hp - hh * parts) * 64 + lane;
+    const uint32_t bits = (uint32_t)__builtin_amdgcn_readfirstlane((int)(moved[run >> 2] >> (run & 3) * 16)) & 0xFFFFu;
+    if (bits == 0u) continue;
+    const int4 m = slots[run * 16 + (lane & 15)];
+    const int l0 = __builtin_ctz(bits);
+    // the place of the run's slot 0, from the first that moves
+    const int64_t first = s.slot(lane_value(m.z, l0), lane_value(m.w, l0) - l0);
+    const int64_t own = (bits >> (lane & 15)) & 1u ? s.slot(m.x, m.y) : first + (lane & 15);
+    const int lo = (int)own, hi = (int)(own >> 32);
+    if (d >= p.D) continue;
+    T* base = (T*)p.cache[1] + (int64_t)(h0 + hh) * s.head + (int64_t)d * s.channel;
+    T e[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      e[i] = base[(int64_t)((uint64_t)(uint32_t)lane_value(hi, i) << 32 | (uint32_t)lane_value(lo, i))];
     union {
       uint4 q[sizeof(T)];
       T e[16];
     } r;
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T); ++i) r.q[i] = ((const uint4*)dst)[i];
+    for (int i = 0; i < 16; ++i) r.e[i] = e[i];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if ((bits >> i) & 1u)
-        r.e[i] = base[slot_at(s, lane_value(m.src_blk, i), lane_value(m.src_off, i)) + (int64_t)d * s[3]];
-    }
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T); ++i) ((uint4*)dst)[i] = r.q[i];
+    for (int i = 0; i < (int)sizeof(T); ++i) ((uint4*)(base + first))[i] = r.q[i];
   }
 }
 
-// A wave a run of 16 slots of one sequence and KV head (K in rows, V in rows or
-// tiles, blocks of a multiple of 16 tokens).
+// kSlots slots a workgroup; any strides.
 template <class T>
-__global__ __launch_bounds__(256) void evict_move_run_kernel(EvictMoveParams p, int64_t waves) {
-  const int lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (w >= waves) return;
-  const int per = (p.budget + 15) >> 4;
-  const int bh = (int)(w / per), b = bh / p.Hkv, hk = bh - b * p.Hkv;
-  const int j = ((int)(w - (int64_t)bh * per) << 4) + lane;
-  MoveSlot m{0, 0, 0, 0, false};
-  if (lane < 16) m = move_slot(p, b, p.Hw == 1 ? 0 : hk, j, p.Hw > 1 || hk == 0);
-  const uint32_t bits = (uint32_t)__ballot(m.moved);
-  if (bits == 0u) return;
-  move_rows<T>(p, 0, hk, m, bits, lane);
-  if (p.mode[1] == kRows) move_rows<T>(p, 1, hk, m, bits, lane);
-  else move_tile<T>(p, 1, hk, m, bits, lane);
-}
-
-// The listed rows of heads [h0, h0 + nh), by pieces (E = uint4) or elements.
-template <class E, class T>
-__device__ __forceinline__ void copy_listed(const EvictMoveParams& p, int which, int h0, int nh, const int4* list,
-                                            int n) {
-  constexpr int kInFlight = 8, kElems = (int)(sizeof(E) / sizeof(T));
-  const int64_t* s = p.c_s[which];
-  T* base = (T*)p.cache[which];
-  const int per = p.D / kElems, row = nh * per, total = n * row;
-  for (int base0 = 0; base0 < total; base0 += 256 * kInFlight) {
-    E v[kInFlight];
-    T* to[kInFlight];
-#pragma unroll
-    for (int i = 0; i < kInFlight; ++i) {
-      if (base0 + i * 256 < total) {
-      const uint32_t u = (uint32_t)min(base0 + i * 256 + (int)threadIdx.x, total - 1), k = u / (uint32_t)row, r = u - k * (uint32_t)row;
-      const uint32_t hh = r / (uint32_t)per, c = r - hh * (uint32_t)per;
-      const int4 m = list[k];
-      const int64_t at = (int64_t)(h0 + (int)hh) * s[2] + (int64_t)(c * kElems) * s[3];
-      v[i] = *(const E*)(base + slot_at(s, m.x, m.y) + at);
-      to[i] = base + slot_at(s, m.z, m.w) + at;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kInFlight; ++i)
-      if (base0 + i * 256 + (int)threadIdx.x < total) *(E*)to[i] = v[i];
-  }
-}
-
-// 256 slots a workgroup; any strides.
-template <class T>
-__global__ __launch_bounds__(256) void evict_move_list_kernel(EvictMoveParams p) {
-  __shared__ int4 list[256];  // source block and offset, destination block and offset
-  __shared__ int count[4];
+__global__ __launch_bounds__(256) void evict_move_kernel(EvictMoveParams p) {
+  __shared__ int4 list[kSlots];  // source block and offset, destination block and offset of the slots that move
+  __shared__ int4 slots[kSlots];  // the same by slot
+  __shared__ uint64_t moved[4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int per = (p.budget + 255) >> 8;
+  const int per = (p.budget + kSlots - 1) / kSlots;
   const int bh = blockIdx.x / per, b = bh / p.Hw, h = bh - b * p.Hw;
-  const MoveSlot m = move_slot(p, b, h, (int)(blockIdx.x - bh * per) * 256 + (int)threadIdx.x, true);
+  const MoveSlot m = move_slot(p, b, h, (int)(blockIdx.x - bh * per) * kSlots + (int)threadIdx.x, true);
   const uint64_t bits = __ballot(m.moved);
-  if (lane == 0) count[wave] = __popcll(bits);
+  if (lane == 0) moved[wave] = bits;
   __syncthreads();
   int at = 0, n = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    at += i < wave ? count[i] : 0;
-    n += count[i];
+    const int count = __popcll(moved[i]);
+    at += i < wave ? count : 0;
+    n += count;
   }
   if (n == 0) return;
-  if (m.moved) list[at + rank_in(bits)] = make_int4(m.src_blk, m.src_off, m.dst_blk, m.dst_off);
+  const int4 x = make_int4(m.src_blk, m.src_off, m.dst_blk, m.dst_off);
+  if (m.moved) list[at + rank_in(bits)] = x;
+  slots[threadIdx.x] = x;
   __syncthreads();
   const int nh = p.Hw == 1 ? p.Hkv : 1, h0 = p.Hw == 1 ? 0 : h;
-  for (int c = 0; c < 2; ++c) {
-    if (p.mode[c] == kRows) copy_listed<uint4, T>(p, c, h0, nh, list, n);
-    else copy_listed<T, T>(p, c, h0, nh, list, n);
-  }
+  if (p.mode[0] == kRows) copy_listed<0, Bytes16, T>(p, h0, nh, list, n);
+  else copy_listed<0, T, T>(p, h0, nh, list, n);
+  if (p.mode[1] == kRows) copy_listed<1, Bytes16, T>(p, h0, nh, list, n);
+  else if (p.mode[1] == kTile && n >= kTileMoves) copy_tiles<T>(p, h0, nh, slots, moved);
+  else copy_listed<1, T, T>(p, h0, nh, list, n);
 }
 
 template <int THREADS, int E>
@@ -594,8 +585,13 @@ int32_t launch_select_t(const EvictSelectParams& p, hipStream_t stream) {
 }  // namespace
 
 int32_t launch_evict_select(const EvictSelectParams& p, hipStream_t stream) {
+  // Few threads with many keys leave room for other heads' workgroups, many
+  // with few shorten a lone one's chain.  64 sequences of 8 heads: 2,064 slots 12
+  // us on 256 threads, 17 on 512, 24 on 1,024; 8,000 slots 18 on 512, 27 on 1,024
+  // (four sequences: 13 both); 16,000 slots 38 on 1,024, 49 on 512.
   if (p.S <= 256 * 4) return launch_select_t<256, 4>(p, stream);
   if (p.S <= 256 * 16) return launch_select_t<256, 16>(p, stream);
+  if (p.S <= 512 * 16) return launch_select_t<512, 16>(p, stream);
   if (p.S <= 1024 * 16) return launch_select_t<1024, 16>(p, stream);
   if (p.S <= 1024 * 32) return launch_select_t<1024, 32>(p, stream);
   return launch_select_t<1024, 0>(p, stream);
@@ -611,25 +607,12 @@ int32_t launch_evict_move(const EvictMoveParams& q, int elem_bytes, hipStream_t 
     else if (base && s[1] == 1 && whole(s[3]) && p.bs % 16 == 0) p.mode[c] = kTile;
     else p.mode[c] = kElements;
   }
-  // Runs of 16 where many slots of a sequence may move: up to S - budget of
-  // them, the tokens past the new end.
-  const bool runs = p.mode[0] == kRows && p.mode[1] != kElements && p.bs % 16 == 0 && (int64_t)(p.S - p.budget) * 4 > p.budget;
   ProfileScope prof("cf_evict_move", stream);
-  if (runs) {
-    const int64_t waves = ceil_div(p.budget, 16) * p.Hkv * p.B;
-    const dim3 grid((unsigned)ceil_div(waves, 4));
-    switch (elem_bytes) {
-      case 1: CF_LAUNCH((evict_move_run_kernel<uint8_t>), grid, dim3(256), 0, stream, p, waves); break;
-      case 2: CF_LAUNCH((evict_move_run_kernel<uint16_t>), grid, dim3(256), 0, stream, p, waves); break;
-      default: CF_LAUNCH((evict_move_run_kernel<uint32_t>), grid, dim3(256), 0, stream, p, waves); break;
-    }
-  } else {
-    const dim3 grid((unsigned)(ceil_div(p.budget, 256) * p.Hw * p.B));
-    switch (elem_bytes) {
-      case 1: CF_LAUNCH((evict_move_list_kernel<uint8_t>), grid, dim3(256), 0, stream, p); break;
-      case 2: CF_LAUNCH((evict_move_list_kernel<uint16_t>), grid, dim3(256), 0, stream, p); break;
-      default: CF_LAUNCH((evict_move_list_kernel<uint32_t>), grid, dim3(256), 0, stream, p); break;
-    }
+  const dim3 grid((unsigned)(ceil_div(p.budget, kSlots) * p.Hw * p.B));
+  switch (elem_bytes) {
+    case 1: CF_LAUNCH((evict_move_kernel<uint8_t>), grid, dim3(256), 0, stream, p); break;
+    case 2: CF_LAUNCH((evict_move_kernel<uint16_t>), grid, dim3(256), 0, stream, p); break;
+    default: CF_LAUNCH((evict_move_kernel<uint32_t>), grid, dim3(256), 0, stream, p); break;
   }
   CF_HIP_CHECK(hipGetLastError());
   return CF_OK;

@@ -149,6 +149,29 @@ def test_move(gpu, dtype, layout, bs, d, hw):
     assert torch.equal(_raw(k), want[0]) and torch.equal(_raw(v), want[1]) and torch.equal(w, ww)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("layout", ["paired", "native", "token_major"])
+@pytest.mark.parametrize("bs, d, hw", [(16, 64, 2), (32, 40, 1), (16, 144, 1)])
+def test_move_of_many(gpu, dtype, layout, bs, d, hw):
+    """Most slots of a sequence move, few of another's, none of a third's; runs
+    that end at the budget, and blocks that the cache does not have."""
+    h, lens, budget = 2, [1100, 320, 296, 700], 297
+    mb = -(-1120 // bs)
+    nb = len(lens) * mb + 3
+    k, v = _caches(gpu, nb, bs, h, d, dtype, layout)
+    w = _weights(gpu, len(lens), hw, mb * bs, 23, "plain")
+    perm = torch.randperm(nb, generator=torch.Generator().manual_seed(2)).to(torch.int32)
+    tables = perm[: len(lens) * mb].view(len(lens), mb).to(gpu)
+    tables[0, 1], tables[0, mb // 2], tables[3, mb // 3] = -1, nb, 1 << 30
+    tl = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    keep, _ = evict_select(w, tl, budget, sink=2, recent=8)
+    moved = (keep != torch.arange(budget, device=gpu)) & (keep >= 0)
+    assert int(moved[0, 0, :256].sum()) > 150 and int(moved[1, 0].sum()) < 30 and not bool(moved[2].any())
+    want = [_expected(_raw(c), keep, tables, hw) for c in (k, v)]
+    evict_move(keep, tl, tables, k, v)
+    assert torch.equal(_raw(k), want[0]) and torch.equal(_raw(v), want[1])
+
+
 def test_move_of_positions(gpu):
     """Stored positions move, appended slots get theirs, nothing past the new end is written."""
     lens, kept, seen, budget = [80, 64, 30], [64, 64, 20], [500, 64, 45], 64
