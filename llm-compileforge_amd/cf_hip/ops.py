@@ -75,6 +75,13 @@ def _cached_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return ws
 
 
+def _captured() -> bool:
+    """Whether a graph captures the call.  It then takes a workspace from the
+    graph's own memory: the cached one may be replaced by a larger call's, and
+    graphs that share it could not run side by side."""
+    return torch.cuda.is_current_stream_capturing()
+
+
 # The native call path (_fastcall.cpp): each wrapper below tries it first and
 # goes on by itself where it returns None (arguments that are not plain
 # tensors on the current device), which raises or handles the case.
@@ -279,8 +286,11 @@ def paged_decode_weights(
     [B, Hkv or 1, S] (float32, S >= the tables' tokens), in place: decay times
     what the entry held (nothing for the newest token) plus the weights of its
     query heads.  workspace: decode_weights_workspace_bytes() bytes, by default
-    a cached one per (device, stream)."""
+    a cached one per (device, stream), a captured call's own under capture."""
     if _on_gpu(q):
+        if workspace is None and _captured():
+            workspace = new_workspace(decode_weights_workspace_bytes(
+                q.shape[0], q.shape[1], k_cache.shape[2], q.shape[2], block_tables.shape[1], block_size), q.device)
         r = _fast().paged_decode_weights(q, k_cache, v_cache, block_tables, seq_lens, weights, float(scale),
                                          int(block_size), float(decay), k_scale, v_scale, out, workspace,
                                          shared_prefix_lens)
@@ -410,8 +420,12 @@ def chunk_weights(
     tables, lengths and q_start) to weights [N, Hkv or 1, S], in place; with
     observe > 0 only each chunk's last `observe` rows count.  workspace:
     chunk_weights_workspace_bytes() bytes, by default a cached one per
-    (device, stream)."""
+    (device, stream), a captured call's own under capture."""
     if _on_gpu(q):
+        if workspace is None and _captured():
+            workspace = new_workspace(chunk_weights_workspace_bytes(
+                q.shape[0], block_tables.shape[0], q.shape[1], k_cache.shape[2], q.shape[2], block_tables.shape[1],
+                block_size, _int32("observe", int(observe))), q.device)
         r = _fast().chunk_weights(q, k_cache, block_tables, seq_lens, q_start, weights, float(scale), int(block_size),
                                   float(decay), int(observe), k_scale, workspace)
         if r is not None:

@@ -204,7 +204,10 @@ int32_t account_view(const CfTensor* t, const char* name, int dtype, View* v) {
   for (int i = 0; i < 2; ++i)
     CF_CHECK(v->size[i] <= 1 || v->stride[i] >= v->size[2], "%s: rows overlap (stride %lld on dim %d)", name,
              (long long)v->stride[i], i);
-  CF_CHECK(v->size[0] <= 1 || v->size[1] <= 1 || v->stride[0] != v->stride[1], "%s: rows overlap", name);
+  if (v->size[0] > 1 && v->size[1] > 1) {  // the rows of one dim all lie between two of the other's
+    const int in = v->stride[0] < v->stride[1] ? 0 : 1;
+    CF_CHECK((v->size[in] - 1) * v->stride[in] + v->size[2] <= v->stride[1 - in], "%s: rows overlap", name);
+  }
   CF_CHECK(v->size[2] < (int64_t)INT32_MAX - (1 << 20), "%s: too many slots", name);
   return CF_OK;
 }

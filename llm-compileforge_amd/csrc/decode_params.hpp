@@ -53,8 +53,8 @@ struct DecodeWeightsParams : DecodeParams {
 // those of tokens 8 i .. 8 i + 3 in the first half and of 8 i + 4 .. 8 i + 7 in
 // the second.  A wave of the streaming kernel holds tokens 8 (lane / 16) + 4 x
 // .. + 3 of its heads, so each of its two stores fills whole lines.
-__device__ __forceinline__ int score_at(int t, int g, int G) {
-  return (t >> 5) * 32 * G + ((t >> 2) & 1) * 16 * G + g * 16 + ((t >> 3) & 3) * 4 + (t & 3);
+__device__ __forceinline__ int64_t score_at(int t, int g, int G) {
+  return (int64_t)(t >> 5) * (32 * G) + (((t >> 2) & 1) * 16 * G + g * 16 + ((t >> 3) & 3) * 4 + (t & 3));
 }
 
 // Launchers (return a CF_* status; kernels are enqueued on `stream`).

@@ -286,7 +286,8 @@ def paged_attention_weights(
         decay: what the account keeps of earlier steps; 0 leaves this step's
             weights alone, whatever was there.
         workspace: cf_hip.ops.decode_weights_workspace_bytes() bytes, by
-            default a cached one per (device, stream).
+            default a cached one per (device, stream), under graph capture one of
+            the graph's.
 
     The other arguments and the result are those of `paged_attention_tensors`.
     """

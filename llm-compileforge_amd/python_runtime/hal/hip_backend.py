@@ -243,6 +243,8 @@ class HipBackend(OpExecutor):
     def _cache_evict(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
         from kernels.kv_eviction import evict_move, evict_select
 
+        if "budget" not in kw:
+            raise ValueError("cache_evict needs a budget")
         weights, seq_lens, tables, k_cache, v_cache = inputs[:5]
         state = dict(zip(("positions", "kept", "seen"), inputs[5:]))
         keep, new_lens = evict_select(weights, seq_lens, int(kw["budget"]), sink=int(kw.get("sink", 0)),

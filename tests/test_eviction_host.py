@@ -44,6 +44,8 @@ def _select(**change):
     (dict(weights=torch.zeros(2, 4)), "weights: expected rank 3"),
     (dict(weights=torch.zeros(2, 4, 128)[:, :, ::2]), "the last stride must be 1"),
     (dict(weights=torch.zeros(2, 1, 64).expand(2, 4, 64)), "rows overlap"),
+    (dict(weights=torch.as_strided(torch.zeros(1024), (2, 4, 64), (96, 64, 1))), "rows overlap"),
+    (dict(weights=torch.as_strided(torch.zeros(1024), (2, 4, 64), (64, 96, 1))), "rows overlap"),
     (dict(seq_lens=_i32(3)), "seq_lens has 3 entries"),
     (dict(seq_lens=torch.zeros(2, dtype=torch.int64)), "seq_lens: expected i32"),
     (dict(positions=None), "go together"),
@@ -230,3 +232,5 @@ def test_backend_ops_check_their_inputs():
             be.execute(name, [x] * 9)
         with pytest.raises(ValueError, match="ROCm"):
             be.execute(name, [x] * n, budget=4)
+    with pytest.raises(ValueError, match="budget"):
+        be.execute("cache_evict", [x] * 5)

@@ -188,6 +188,41 @@ def test_two_graphs_of_the_whole_step(gpu):
                 assert torch.equal(t, u), (turn, i, name)
 
 
+def test_captured_calls_have_workspaces_of_their_own(gpu):
+    """Two graphs captured without workspaces, replayed side by side, after a
+    larger eager call has replaced the cached ones."""
+    xs = [Inputs(gpu, torch.bfloat16, 20 + i) for i in range(2)]
+    eager = [Inputs(gpu, torch.bfloat16, 20 + i) for i in range(2)]
+
+    def step(x, out):
+        paged_attention_weights(x.q, x.kc, x.vc, x.tables, x.lens, x.w, out=out)
+        chunk_attention_weights(x.q, x.kc, x.tables, x.lens, x.start, x.w)
+
+    step(Inputs(gpu, torch.bfloat16, 99), torch.empty_like(xs[0].q))
+    outs, graphs = [torch.empty_like(x.q) for x in xs], []
+    torch.cuda.synchronize()
+    for x, o in zip(xs, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step(x, o)
+        graphs.append(graph)
+    big = Inputs(gpu, torch.bfloat16, 30)
+    wide = torch.zeros(3, 400, dtype=torch.int32, device=gpu)
+    paged_attention_weights(big.q, big.kc, big.vc, wide, big.lens, torch.zeros(3, 2, 6400, device=gpu))
+    chunk_attention_weights(big.q, big.kc, wide, big.lens, big.start, torch.zeros(3, 2, 6400, device=gpu))
+    streams = [torch.cuda.Stream(device=gpu) for _ in xs]
+    for turn in range(4):
+        want = [torch.empty_like(o) for o in outs]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for x, e, o, w in zip(xs, eager, outs, want):
+            step(e, w)
+            assert torch.equal(o, w) and torch.equal(x.w, e.w), turn
+
+
 def test_int64_tables_and_lengths_are_taken(gpu):
     x, y = Inputs(gpu, torch.bfloat16), Inputs(gpu, torch.bfloat16)
     a = paged_attention_weights(x.q, x.kc, x.vc, x.tables, x.lens, x.w)
