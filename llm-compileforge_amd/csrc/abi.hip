@@ -603,9 +603,12 @@ static int32_t decode_call(const CfTensor* q, const CfTensor* k_cache, const CfT
   }
   if (mfma) {
     if ((rc = launch_decode_mfma(p, vq.dtype, vk.dtype, st))) return rc;
+    if (accounts_with_rows(p)) return CF_OK;
   } else {
     if ((rc = launch_decode_generic(p, vq.dtype, vk.dtype, st))) return rc;
-    if (p.max_parts > 1 && (rc = launch_decode_reduce(p, vq.dtype, st))) return rc;
+    if (p.max_parts > 1) {
+      if ((rc = launch_decode_reduce(p, vq.dtype, st)) || accounts_with_rows(p)) return rc;
+    }
   }
   return launch_decode_weights(p, mfma, st);
 }

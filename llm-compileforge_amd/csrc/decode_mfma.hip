@@ -34,6 +34,7 @@
 // merge of its prefix partial and its own-run partial.
 #include "cf_device.hpp"
 #include "cf_host.hpp"
+#include "decode_account.hpp"
 #include "decode_params.hpp"
 #include "mfma_tile.hpp"
 
@@ -1136,10 +1137,9 @@ __device__ __forceinline__ float merge_weight(float m, float M) {
 // registers, all four waves of each otherwise.  Partial rows hold the G
 // heads of h in consecutive rows.
 template <int QT, int D, int G, int NSL, class P>
-__global__ __launch_bounds__(256) void decode_merge_kernel(P p) {
+__device__ __forceinline__ void merge_rows(const P& p, int h, int b, int slice) {
   constexpr int E = G * D / 64;  // output elements per lane
   constexpr int kWaves = 4;
-  const int h = blockIdx.x, b = blockIdx.y;
   const int lane = threadIdx.x & 63;
   const int wave = uniform((int)threadIdx.x >> 6);
   const int2 dn = p.own_desc[(int64_t)b * p.Hkv + h];
@@ -1150,7 +1150,7 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(P p) {
   if (nsrc == 0) return;  // written whole by the decode kernel (or empty)
   constexpr int KMAX = 64 / E;  // partials the register path holds
   if (nsrc <= KMAX) {
-    if (wave != 0 || blockIdx.z != 0) return;
+    if (wave != 0 || slice != 0) return;
     // Few partials (the usual case): every load is issued at once -- each
     // lane's slice of every partial row and every (m, l) -- so the merge
     // costs one round trip after the descriptors.
@@ -1244,7 +1244,7 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(P p) {
   int fs[FPT], gs[FPT];
 #pragma unroll
   for (int j = 0; j < FPT; ++j) {
-    fs[j] = (int)blockIdx.z * NF4 + (FPT == 1 ? tid % NF4 : tid + 256 * j);
+    fs[j] = slice * NF4 + (FPT == 1 ? tid % NF4 : tid + 256 * j);
     gs[j] = 4 * fs[j] / D;
   }
   if (tid < G) {
@@ -1327,7 +1327,7 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(P p) {
     __syncthreads();  // the next chunk restages sm, sl, srow
   }
   if constexpr (kKeeps<P>) {
-    if (blockIdx.z == 0 && tid < G) {
+    if (slice == 0 && tid < G) {
       float* fin = p.ws_fin + ((int64_t)b * p.Hq + h * G + tid) * 2;
       fin[0] = run_m[tid];
       fin[1] = run_l[tid];
@@ -1354,6 +1354,38 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(P p) {
     auto nrm = [&](float a) { return lg > 0.0f ? a / lg : a * 0.0f; };
     store_out4<QT>(p.out, out + (int64_t)(h * G + g) * p.o_sh + d, nrm(acc[j].x), nrm(acc[j].y), nrm(acc[j].z),
                    nrm(acc[j].w));
+  }
+}
+
+template <int QT, int D, int G, int NSL, class P>
+__global__ __launch_bounds__(256) void decode_merge_kernel(P p) {
+  merge_rows<QT, D, G, NSL>(p, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
+// The partials of a (sequence, KV head), for account_block.
+struct RunParts {
+  const float* ws_ml;
+  int2 own, pre;
+  int nown, count;
+  __device__ __forceinline__ RunParts(const DecodeWeightsParams& p, int b, int h)
+      : ws_ml(p.ws_ml), own(p.own_desc[(int64_t)b * p.Hkv + h]), pre(p.pre_desc[(int64_t)b * p.Hkv + h]),
+        nown(own.y < 0 ? 1 : own.y), count(nown + (pre.y < 0 ? 1 : pre.y)) {}
+  __device__ __forceinline__ float2 ml(int g, int k) const {
+    const int64_t row = k < nown ? part_row(own, k) : part_row(pre, k - nown);
+    return *(const float2*)(ws_ml + (row + g) * 2);
+  }
+};
+
+// The merge and the accounts in one launch: `merges` workgroups join rows, the
+// others form accounts.
+template <int QT, int D, int G, int NSL>
+__global__ __launch_bounds__(256) void decode_finish_kernel(DecodeWeightsParams p, int merges, bool vec) {
+  __shared__ float2 fin[G];
+  if ((int)blockIdx.x < merges) {
+    const int x = blockIdx.x, y = x / p.Hkv, z = y / p.B;
+    merge_rows<QT, D, G, NSL>(p, x - y * p.Hkv, y - z * p.B, z);
+  } else {
+    account_block<true, RunParts>(p, (int)blockIdx.x - merges, fin, vec);
   }
 }
 
@@ -1428,8 +1460,28 @@ int32_t launch_t(const P& p, hipStream_t stream) {
   const bool split = (int64_t)p.B * p.Hkv < kMergeSplitBelow;
   const dim3 grid(p.Hkv, p.B, split ? 4 : 1);
   ProfileScope prof("cf_decode_merge", stream);
-#define CF_MERGE(G)                                                                         \
-  if (split) CF_LAUNCH((decode_merge_kernel<QT, D, G, 4, P>), grid, dim3(256), 0, stream, p); \
+  bool finish = false;  // with accounts
+  int64_t merges = 0, all = 0;
+  if constexpr (kKeeps<P>) {
+    finish = accounts_with_rows(p);
+    merges = (int64_t)p.Hkv * p.B * (split ? 4 : 1);
+    all = merges + account_blocks(p);
+    if (finish && all >= (int64_t)INT32_MAX) {
+      set_error("decode weights: too many accounts");
+      return CF_ERR_UNSUPPORTED;
+    }
+  }
+#define CF_MERGE(G)                                                                                              \
+  if constexpr (kKeeps<P>) {                                                                                     \
+    if (finish) {                                                                                                \
+      if (split) CF_LAUNCH((decode_finish_kernel<QT, D, G, 4>), dim3((unsigned)all), dim3(256), 0, stream, p,    \
+                           (int)merges, accounts_aligned(p));                                                    \
+      else CF_LAUNCH((decode_finish_kernel<QT, D, G, 1>), dim3((unsigned)all), dim3(256), 0, stream, p,          \
+                     (int)merges, accounts_aligned(p));                                                          \
+      break;                                                                                                     \
+    }                                                                                                            \
+  }                                                                                                              \
+  if (split) CF_LAUNCH((decode_merge_kernel<QT, D, G, 4, P>), grid, dim3(256), 0, stream, p);                    \
   else CF_LAUNCH((decode_merge_kernel<QT, D, G, 1, P>), grid, dim3(256), 0, stream, p);
   switch (p.G) {
     case 1: CF_MERGE(1) break;

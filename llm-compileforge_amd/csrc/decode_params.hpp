@@ -49,6 +49,21 @@ struct DecodeWeightsParams : DecodeParams {
   float decay;
 };
 
+// Workgroups that form the accounts, 1,024 tokens each.
+inline int64_t account_blocks(const DecodeWeightsParams& p) {
+  return ((int64_t)p.Mb * p.bs + 1023) / 1024 * p.B * p.Hw;
+}
+// Accounts of one KV head each are formed in the launch that joins the rows, if
+// they are few: the joining kernel's registers leave fewer waves to hide the
+// scores' latency.  4 requests of 512 f32 tokens: 4.1 us against 4.3 and 4.0 in
+// two launches; 29 sequences of 2,928 tokens (696 workgroups) 7.3 against 4.4 and
+// 4.4; 79 of 1,073 (1,264) 9.0 against 4.2 and 5.5; 64 of 8,192 (4,096) 22.6
+// against 4.3 and 13.8.
+inline bool accounts_with_rows(const DecodeWeightsParams& p) { return p.Hw == p.Hkv && account_blocks(p) <= 1024; }
+inline bool accounts_aligned(const DecodeWeightsParams& p) {
+  return ((uintptr_t)p.weights & 15) == 0 && p.w_sb % 4 == 0 && p.w_sh % 4 == 0;
+}
+
 // Where a token's score lies among its tile's 32 * G: 16 floats a query head,
 // those of tokens 8 i .. 8 i + 3 in the first half and of 8 i + 4 .. 8 i + 7 in
 // the second.  A wave of the streaming kernel holds tokens 8 (lane / 16) + 4 x

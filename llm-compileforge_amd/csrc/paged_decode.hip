@@ -22,6 +22,7 @@
 
 #include "cf_device.hpp"
 #include "cf_host.hpp"
+#include "decode_account.hpp"
 #include "decode_params.hpp"
 
 namespace cf {
@@ -253,10 +254,9 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(P p) {
 // the weighted sum takes the partitions in 256 / D interleaved groups (all
 // their loads independent), whose sums meet in LDS.
 template <int OT, class P>
-__global__ __launch_bounds__(256) void decode_reduce_kernel(P p) {
+__device__ __forceinline__ void reduce_row(const P& p, int hq, int b) {
   __shared__ float red[8];
   __shared__ float part_acc[256];
-  const int hq = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
   const int ctx = effective_len(p, b);
   const int nparts = (ctx + p.PT - 1) / p.PT;
@@ -318,6 +318,32 @@ __global__ __launch_bounds__(256) void decode_reduce_kernel(P p) {
     for (int g = 0; g < ng; ++g) s += part_acc[g * p.D + tid];
     OutE::store(o + tid, s * inv);
   }
+}
+
+template <int OT, class P>
+__global__ __launch_bounds__(256) void decode_reduce_kernel(P p) {
+  reduce_row<OT>(p, blockIdx.x, blockIdx.y);
+}
+
+// The partitions of a (sequence, KV head), for account_block.
+struct PartitionParts {
+  const float* ml0;
+  int64_t stride;
+  int count;
+  __device__ __forceinline__ PartitionParts(const DecodeWeightsParams& p, int b, int h)
+      : ml0(p.ws_ml + ((int64_t)b * p.Hq + h * p.G) * p.max_parts * 2), stride((int64_t)p.max_parts * 2),
+        count((effective_len(p, b) + p.PT - 1) / p.PT) {}
+  __device__ __forceinline__ float2 ml(int g, int k) const { return *(const float2*)(ml0 + g * stride + k * 2); }
+};
+
+// The reduction and the accounts in one launch: workgroups below B * Hq reduce a
+// row, the others form accounts.  Dynamic LDS: G pairs.
+template <int OT>
+__global__ __launch_bounds__(256) void decode_reduce_finish_kernel(DecodeWeightsParams p, bool vec) {
+  extern __shared__ float smem[];
+  const int rows = p.B * p.Hq, x = blockIdx.x;
+  if (x < rows) reduce_row<OT>(p, x % p.Hq, x / p.Hq);
+  else account_block<false, PartitionParts>(p, x - rows, (float2*)smem, vec);
 }
 
 template <int QT, int KT, class P>
@@ -397,7 +423,24 @@ int32_t launch_decode_reduce(const DecodeParams& p, int q_dt, hipStream_t stream
 }
 
 int32_t launch_decode_reduce(const DecodeWeightsParams& p, int q_dt, hipStream_t stream) {
-  return launch_reduce_any(p, q_dt, stream);
+  if (!accounts_with_rows(p)) return launch_reduce_any(p, q_dt, stream);
+  const int64_t blocks = (int64_t)p.B * p.Hq + account_blocks(p);
+  if (blocks >= (int64_t)INT32_MAX) {
+    set_error("decode weights: too many accounts");
+    return CF_ERR_UNSUPPORTED;
+  }
+  const dim3 grid((unsigned)blocks);
+  const size_t lds = (size_t)p.G * 8;
+  const bool vec = accounts_aligned(p);
+  ProfileScope prof("cf_decode_reduce", stream);
+  switch (q_dt) {
+    case kF32: CF_LAUNCH((decode_reduce_finish_kernel<kF32>), grid, dim3(256), lds, stream, p, vec); break;
+    case kF16: CF_LAUNCH((decode_reduce_finish_kernel<kF16>), grid, dim3(256), lds, stream, p, vec); break;
+    case kBF16: CF_LAUNCH((decode_reduce_finish_kernel<kBF16>), grid, dim3(256), lds, stream, p, vec); break;
+    default: set_error("unsupported output dtype %d", q_dt); return CF_ERR_UNSUPPORTED;
+  }
+  CF_HIP_CHECK(hipGetLastError());
+  return CF_OK;
 }
 
 size_t generic_lds_bytes(int64_t G, int64_t D, int64_t PT, int64_t bs) {

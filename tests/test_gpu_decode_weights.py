@@ -169,6 +169,19 @@ def test_shared_prefixes(gpu, d, hq, h):
     _check(case, shared_prefix_lens=shared)
 
 
+def test_accounts_in_a_launch_of_their_own(gpu):
+    """Tables so wide that the rows are joined first: a shared prefix, and the partitioned kernel."""
+    case = Case(gpu, 6, 16, 4, 64, [300, 290, 160, 0, 64, 5000], torch.bfloat16, torch.float8_e4m3fn, seed=12, mb=2800)
+    case.tables[1:3, :10] = case.tables[0, :10]
+    shared = torch.tensor([0, 160, 160, 0, 0, 0], dtype=torch.int32, device=gpu)
+    _check(case, shared_prefix_lens=shared)
+    _check(Case(gpu, 3, 6, 2, 40, [1000, 1, 3000], torch.float32, torch.float32, "token_major", seed=13, mb=11000))
+
+
+def test_many_partitions(gpu):
+    _check(Case(gpu, 1, 6, 2, 40, [40000], torch.float32, torch.bfloat16, "token_major", seed=14))
+
+
 def test_lengths_at_the_edges_and_invalid_blocks(gpu):
     case = Case(gpu, 6, 8, 2, 64, [0, -3, 48, 90, 33, 48], torch.bfloat16, torch.bfloat16, seed=7, mb=3)
     case.tables[4, 1] = -1
