@@ -491,8 +491,8 @@ __device__ __forceinline__ void copy_pieces(const Strides& s, T* base, int h0, i
     if (from + i * 256 + (int)threadIdx.x < total) *(E*)to[i] = v[i];
 }
 
-// The listed rows of heads [h0, h0 + nh): eight pieces a thread in flight, the
-// rest two at a time (a few moves must not load eight).
+// The listed rows of heads [h0, h0 + nh): four pieces a thread in flight, the
+// rest two at a time (a few moves must not load four).
 template <int WHICH, class E, class T>
 __device__ __forceinline__ void copy_listed(const EvictMoveParams& p, int h0, int nh, const int4* list, int n) {
   constexpr int kElems = (int)(sizeof(E) / sizeof(T));
@@ -500,8 +500,8 @@ __device__ __forceinline__ void copy_listed(const EvictMoveParams& p, int h0, in
   T* base = (T*)p.cache[WHICH];
   const int per = p.D / kElems, row = nh * per, total = n * row;
   int from = 0;
-  for (; from + 8 * 256 <= total; from += 8 * 256)
-    copy_pieces<8, E, T>(s, base, h0, per, row, list, from, total);
+  for (; from + 4 * 256 <= total; from += 4 * 256)
+    copy_pieces<4, E, T>(s, base, h0, per, row, list, from, total);
   for (; from < total; from += 2 * 256) copy_pieces<2, E, T>(s, base, h0, per, row, list, from, total);
 }
 
