@@ -507,6 +507,28 @@ __global__ __launch_bounds__(256) void chunk_stats_kernel(ChunkWeightsParams p) 
   if (row < p.stat_rows) p.ws_ml[i] = joined(p, row, (int)(i - row * p.Hq));
 }
 
+// A wave's sums of tokens tw .. + 63 over the run's columns: the 16 columns of a
+// lane group, then the run's place.
+__device__ __forceinline__ void leave_sums(const ChunkWeightsParams& p, const Chunk& c, const Run& un, int h, int tw,
+                                           float acc[4][4]) {
+  const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) acc[tt][v] += __shfl_xor(acc[tt][v], o, 64);
+  if (li == 0) {
+    float* out = p.ws_p + ((piece0(p, c) + un.piece) * p.Hkv + h) * (int64_t)p.Mb * 16;
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+      const int t = tw + tt * 16 + 4 * lq;
+      if (t < p.Mb * 16) *(float4*)(out + t) = make_float4(acc[tt][0], acc[tt][1], acc[tt][2], acc[tt][3]);
+    }
+  }
+  if (un.last && h == 0 && threadIdx.x == 0) p.ws_tp[c.n * cdiv(p.Mb * 16, kCols) + un.block] = un.pieces;
+}
+
 // ---- tokens: sums over a run of columns ----------------------------------------
 
 template <int QT, int KT, int D>
@@ -628,22 +650,147 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_tokens_kernel(
         head = next_head;
       }
     }
-    // the 16 columns of a lane group
+    leave_sums(p, c, un, h, tw, acc);
+  }
+}
+
+// ---- short sequences: rows and tokens at once -----------------------------------
+
+// Tables of at most 256 tokens: a workgroup that holds them all (64 a wave) has a
+// column's whole row of scores, so one pass does: the scores of 64 columns stay in
+// registers, the waves' maxima and sums of a column meet in LDS, and the weights
+// are added up as in the tokens kernel.
+constexpr int kShortPerCU = 2;  // workgroups: the scores held leave room for two waves a SIMD
+
+template <int QT, int KT, int D>
+__global__ __launch_bounds__(256, kShortPerCU) void chunk_short_kernel(ChunkWeightsParams p) {
+  constexpr int NC = D / 32, RB = row_bytes<D>(), PPR = D / 8;
+  constexpr int LOADS = kStage * PPR / 256;
+  __shared__ __align__(16) uint8_t stage[2][kStage * RB];
+  __shared__ float wave_m[4][kStage], wave_l[4][kStage];
+  __shared__ Window win;
+  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lq = lane >> 4, wave = uniform(tid >> 6);
+  const Columns colm(p.G);
+  const int h = (int)(blockIdx.x % (unsigned)p.Hkv);
+  const TokenBlocks blocks{p.G};
+  Runs<TokenBlocks> runs(p, &win, blocks, p.col_steps);
+  Run un;
+  while (runs.next(&un)) {
+    const Chunk& c = un.c;
+    const int ncol = c.rows * p.G, vis = visible(c, c.rows), tw = wave * 64;
+    const int j_begin = (blocks.first(c, un.block) + un.at) * kStage, j_end = j_begin + un.n * kStage;
+    const Factor f = factor_of(p, h);
+    QOp<QT> k[4][NC];
+    int live[4];  // tokens of the block that exist
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+      const int t = tw + tt * 16;
+      const int blk = t < vis ? block_of(p, c.n, t >> 4) : -1;
+      live[tt] = blk < 0 ? 0 : min(vis - t, 16);
+#pragma unroll
+      for (int x = 0; x < NC; ++x)
+        k[tt][x] = as_qop<QT>(operand<QT, KT>(k_piece<KT>(p, (int64_t)(blk < 0 ? 0 : blk) * p.k_s[0] +
+                                                                 (int64_t)h * p.k_s[2] + li * p.k_s[1] + 32 * x + 8 * lq)));
+    }
+    float acc[4][4];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
+      for (int v = 0; v < 4; ++v) acc[tt][v] = 0.0f;
+
+    uint4 reg[LOADS];
+    auto fetch = [&](int j0, int row, int head) {  // columns j0 .. + 63, the first head `head` of row `row`
+      const QRows rows(p, c.row0 + row, h, f.flip);
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) acc[tt][v] += __shfl_xor(acc[tt][v], o, 64);
-    if (li == 0) {
-      float* out = p.ws_p + ((piece0(p, c) + un.piece) * p.Hkv + h) * (int64_t)p.Mb * 16;
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const int t = tw + tt * 16 + 4 * lq;
-        if (t < p.Mb * 16) *(float4*)(out + t) = make_float4(acc[tt][0], acc[tt][1], acc[tt][2], acc[tt][3]);
+      for (int i = 0; i < LOADS; ++i) {
+        const int e = i * 256 + tid, j = head + e / PPR, r = colm.row(j), g = j - r * p.G;
+        reg[i] = j0 + e / PPR < ncol ? rows.piece(r, g, e % PPR * 8) : make_uint4(0, 0, 0, 0);
       }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int e = i * 256 + tid;
+        *(uint4*)(stage[buf] + e / PPR * RB + e % PPR * 16) = reg[i];
+      }
+    };
+    int row = j_begin / p.G, head = j_begin - row * p.G;
+    fetch(j_begin, row, head);
+    store(0);
+    __syncthreads();
+    for (int j0 = j_begin, buf = 0; j0 < j_end; j0 += kStage, buf ^= 1) {
+      const bool more = j0 + kStage < j_end;
+      const int on = colm.row(head + kStage), next_row = row + on, next_head = head + kStage - on * p.G;
+      if (more) fetch(j0 + kStage, next_row, next_head);
+      f32x4_t s[4][4];
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        const int j = ct * 16 + li;
+        // the lane's column sees this many of the wave's tokens
+        const int seen = (j0 + j < ncol ? c.c0 + row + colm.row(head + j) + 1 : 0) - tw;
+        QOp<QT> q[NC];
+#pragma unroll
+        for (int x = 0; x < NC; ++x)
+          q[x] = as_qop<QT>(*(const uint4*)(stage[buf] + j * RB + x * 64 + lq * 16));
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          s[ct][tt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int x = 0; x < NC; ++x) s[ct][tt] = mfma16(k[tt][x], q[x], s[ct][tt]);
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          const int end = min(live[tt], seen - tt * 16);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            if (4 * lq + v >= end) s[ct][tt][v] = -INFINITY;
+            mx = fmaxf(mx, s[ct][tt][v]);
+          }
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        if (lq == 0) wave_m[wave][j] = mx;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        const int j = ct * 16 + li;
+        const float mx = fmaxf(fmaxf(wave_m[0][j], wave_m[1][j]), fmaxf(wave_m[2][j], wave_m[3][j]));
+        const float ref = mx == -INFINITY ? 0.0f : mx * f.qk;
+        float sum = 0.0f;
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float sv = s[ct][tt][v], e = __builtin_amdgcn_exp2f(__builtin_fmaf(sv, f.qk, -ref));
+            s[ct][tt][v] = sv != -INFINITY ? e : -1.0f;  // (-1: masked)
+            sum += sv != -INFINITY ? e : 0.0f;
+          }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (lq == 0) wave_l[wave][j] = sum;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        const int j = ct * 16 + li;
+        const float L = (wave_l[0][j] + wave_l[1][j]) + (wave_l[2][j] + wave_l[3][j]);
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {  // (a NaN reaches the row's own tokens only)
+            const float e = s[ct][tt][v];
+            acc[tt][v] = e != -1.0f ? __builtin_fmaf(e, inv, acc[tt][v]) : acc[tt][v];
+          }
+      }
+      if (more) store(buf ^ 1);
+      __syncthreads();
+      row = next_row;
+      head = next_head;
     }
-    if (un.last && h == 0 && tid == 0) p.ws_tp[c.n * cdiv(p.Mb * 16, kCols) + un.block] = un.pieces;
+    leave_sums(p, c, un, h, tw, acc);
   }
 }
 
@@ -743,20 +890,27 @@ int32_t launch_d(const ChunkWeightsParams& p, hipStream_t stream) {
   // as many workgroups as are resident, the same number for every head
   const int resident = waves_per_simd<D>() * device_cu_count();
   const dim3 grid((unsigned)(std::max(resident / p.Hkv, 1) * p.Hkv));
-  {
-    ProfileScope prof("cf_chunk_rows", stream);
-    CF_LAUNCH((chunk_rows_kernel<QT, KT, D>), grid, dim3(256), 0, stream, p);
+  if (cap <= kCols) {
+    const dim3 few((unsigned)(std::max(kShortPerCU * device_cu_count() / p.Hkv, 1) * p.Hkv));
+    ProfileScope prof("cf_chunk_short", stream);
+    CF_LAUNCH((chunk_short_kernel<QT, KT, D>), few, dim3(256), 0, stream, p);
     CF_HIP_CHECK(hipGetLastError());
-  }
-  if (p.joined) {
-    ProfileScope prof("cf_chunk_stats", stream);
-    CF_LAUNCH(chunk_stats_kernel, dim3((unsigned)ceil_div(p.stat_rows * p.Hq, 256)), dim3(256), 0, stream, p);
-    CF_HIP_CHECK(hipGetLastError());
-  }
-  {
-    ProfileScope prof("cf_chunk_tokens", stream);
-    CF_LAUNCH((chunk_tokens_kernel<QT, KT, D>), grid, dim3(256), 0, stream, p);
-    CF_HIP_CHECK(hipGetLastError());
+  } else {
+    {
+      ProfileScope prof("cf_chunk_rows", stream);
+      CF_LAUNCH((chunk_rows_kernel<QT, KT, D>), grid, dim3(256), 0, stream, p);
+      CF_HIP_CHECK(hipGetLastError());
+    }
+    if (p.joined) {
+      ProfileScope prof("cf_chunk_stats", stream);
+      CF_LAUNCH(chunk_stats_kernel, dim3((unsigned)ceil_div(p.stat_rows * p.Hq, 256)), dim3(256), 0, stream, p);
+      CF_HIP_CHECK(hipGetLastError());
+    }
+    {
+      ProfileScope prof("cf_chunk_tokens", stream);
+      CF_LAUNCH((chunk_tokens_kernel<QT, KT, D>), grid, dim3(256), 0, stream, p);
+      CF_HIP_CHECK(hipGetLastError());
+    }
   }
   ProfileScope prof("cf_chunk_join", stream);
   // (many pieces a token: more loads in flight)
