@@ -11,7 +11,9 @@
 //                  through LDS, an online softmax per lane;
 //   tokens kernel  K of 256 tokens in registers, Q streamed through LDS with
 //                  each column's (m, 1 / l), the sums per lane.
-// Both form S^T = K Q^T (v_mfma_f32_16x16x32; a lane's outputs are four tokens
+//   short kernel   both at once, for tables of a workgroup's tokens: the scores of
+//                  64 columns in registers, their maxima and sums joined in LDS.
+// All form S^T = K Q^T (v_mfma_f32_16x16x32; a lane's outputs are four tokens
 // of one column), so m, l, and 1 / l are lane-local and the tokens' sums meet
 // across the 16 lanes of a column group once a run.  The work of a head is a
 // line of steps, 64 tokens for a block of 256 columns (rows kernel) or 64
@@ -103,12 +105,13 @@ struct RowBlocks {
   }
 };
 
-// Blocks of 256 tokens, steps of 64 columns from the first that sees the block's
-// first token on.
+// Blocks of TOKENS tokens, steps of 64 columns from the first that sees the
+// block's first token on.
+template <int TOKENS>
 struct TokenBlocks {
   int G;
-  __device__ __forceinline__ int blocks(const Chunk& c) const { return (visible(c, c.rows) + kCols - 1) / kCols; }
-  __device__ __forceinline__ int first(const Chunk& c, int b) const { return max(b * kCols - c.c0, 0) * G / kStage; }
+  __device__ __forceinline__ int blocks(const Chunk& c) const { return (visible(c, c.rows) + TOKENS - 1) / TOKENS; }
+  __device__ __forceinline__ int first(const Chunk& c, int b) const { return max(b * TOKENS - c.c0, 0) * G / kStage; }
   __device__ __forceinline__ int steps(const Chunk& c, int b) const {
     return (c.rows * G + kStage - 1) / kStage - first(c, b);
   }
@@ -526,7 +529,9 @@ __device__ __forceinline__ void leave_sums(const ChunkWeightsParams& p, const Ch
       if (t < p.Mb * 16) *(float4*)(out + t) = make_float4(acc[tt][0], acc[tt][1], acc[tt][2], acc[tt][3]);
     }
   }
-  if (un.last && h == 0 && threadIdx.x == 0) p.ws_tp[c.n * cdiv(p.Mb * 16, kCols) + un.block] = un.pieces;
+  // (a short sequence's one block of 512 tokens is two of the join's)
+  const int blocks = cdiv(p.Mb * 16, kCols), own = blockDim.x == 256 ? 1 : blocks;
+  if (un.last && h == 0 && (int)threadIdx.x < own) p.ws_tp[c.n * blocks + un.block + threadIdx.x] = un.pieces;
 }
 
 // ---- tokens: sums over a run of columns ----------------------------------------
@@ -541,8 +546,8 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_tokens_kernel(
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lq = lane >> 4, wave = uniform(tid >> 6);
   const Columns colm(p.G);
   const int h = (int)(blockIdx.x % (unsigned)p.Hkv);
-  const TokenBlocks blocks{p.G};
-  Runs<TokenBlocks> runs(p, &win, blocks, p.col_steps);
+  const TokenBlocks<kCols> blocks{p.G};
+  Runs<TokenBlocks<kCols>> runs(p, &win, blocks, p.col_steps);
   Run un;
   while (runs.next(&un)) {
     const Chunk& c = un.c;
@@ -656,24 +661,31 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_tokens_kernel(
 
 // ---- short sequences: rows and tokens at once -----------------------------------
 
-// Tables of at most 256 tokens: a workgroup that holds them all (64 a wave) has a
+// Tables of at most 256 or 512 tokens: a workgroup of four or eight waves that
+// holds them all (64 a wave) has a
 // column's whole row of scores, so one pass does: the scores of 64 columns stay in
 // registers, the waves' maxima and sums of a column meet in LDS, and the weights
 // are added up as in the tokens kernel.
-constexpr int kShortPerCU = 2;  // workgroups: the scores held leave room for two waves a SIMD
+// It forms masked scores, too, so eight waves are for few rows: of 500 rows and
+// tokens and 32 heads of 64, one chunk takes 20.5 us against 29.4, eight (6.6e7
+// row, head and token triples) 65.9 and 67.7, 32 209 and 159; of 12 heads eight
+// 36.5 and 53.1, 32 (9.8e7) 106 both.  Of 253 rows and tokens 64 chunks take 114 and
+// 123, one 15 and 24.
+constexpr double kShortMost = 1e8;
+constexpr int kShortWaves = 2;  // of a SIMD: the scores held leave room for no more
 
-template <int QT, int KT, int D>
-__global__ __launch_bounds__(256, kShortPerCU) void chunk_short_kernel(ChunkWeightsParams p) {
+template <int QT, int KT, int D, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, kShortWaves) void chunk_short_kernel(ChunkWeightsParams p) {
   constexpr int NC = D / 32, RB = row_bytes<D>(), PPR = D / 8;
-  constexpr int LOADS = kStage * PPR / 256;
+  constexpr int THREADS = WAVES * 64, LOADS = kStage * PPR / THREADS;
   __shared__ __align__(16) uint8_t stage[2][kStage * RB];
-  __shared__ float wave_m[4][kStage], wave_l[4][kStage];
+  __shared__ float wave_m[WAVES][kStage], wave_l[WAVES][kStage];
   __shared__ Window win;
   const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lq = lane >> 4, wave = uniform(tid >> 6);
   const Columns colm(p.G);
   const int h = (int)(blockIdx.x % (unsigned)p.Hkv);
-  const TokenBlocks blocks{p.G};
-  Runs<TokenBlocks> runs(p, &win, blocks, p.col_steps);
+  const TokenBlocks<WAVES * 64> blocks{p.G};
+  Runs<TokenBlocks<WAVES * 64>> runs(p, &win, blocks, p.col_steps);
   Run un;
   while (runs.next(&un)) {
     const Chunk& c = un.c;
@@ -703,14 +715,14 @@ __global__ __launch_bounds__(256, kShortPerCU) void chunk_short_kernel(ChunkWeig
       const QRows rows(p, c.row0 + row, h, f.flip);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int e = i * 256 + tid, j = head + e / PPR, r = colm.row(j), g = j - r * p.G;
+        const int e = i * THREADS + tid, j = head + e / PPR, r = colm.row(j), g = j - r * p.G;
         reg[i] = j0 + e / PPR < ncol ? rows.piece(r, g, e % PPR * 8) : make_uint4(0, 0, 0, 0);
       }
     };
     auto store = [&](int buf) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int e = i * 256 + tid;
+        const int e = i * THREADS + tid;
         *(uint4*)(stage[buf] + e / PPR * RB + e % PPR * 16) = reg[i];
       }
     };
@@ -756,7 +768,9 @@ __global__ __launch_bounds__(256, kShortPerCU) void chunk_short_kernel(ChunkWeig
 #pragma unroll
       for (int ct = 0; ct < 4; ++ct) {
         const int j = ct * 16 + li;
-        const float mx = fmaxf(fmaxf(wave_m[0][j], wave_m[1][j]), fmaxf(wave_m[2][j], wave_m[3][j]));
+        float mx = wave_m[0][j];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) mx = fmaxf(mx, wave_m[i][j]);
         const float ref = mx == -INFINITY ? 0.0f : mx * f.qk;
         float sum = 0.0f;
 #pragma unroll
@@ -775,7 +789,9 @@ __global__ __launch_bounds__(256, kShortPerCU) void chunk_short_kernel(ChunkWeig
 #pragma unroll
       for (int ct = 0; ct < 4; ++ct) {
         const int j = ct * 16 + li;
-        const float L = (wave_l[0][j] + wave_l[1][j]) + (wave_l[2][j] + wave_l[3][j]);
+        float L = wave_l[0][j];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) L += wave_l[i][j];
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
@@ -890,10 +906,16 @@ int32_t launch_d(const ChunkWeightsParams& p, hipStream_t stream) {
   // as many workgroups as are resident, the same number for every head
   const int resident = waves_per_simd<D>() * device_cu_count();
   const dim3 grid((unsigned)(std::max(resident / p.Hkv, 1) * p.Hkv));
+  const auto few = [&](int waves) {
+    return dim3((unsigned)(std::max(kShortWaves * 4 / waves * device_cu_count() / p.Hkv, 1) * p.Hkv));
+  };
   if (cap <= kCols) {
-    const dim3 few((unsigned)(std::max(kShortPerCU * device_cu_count() / p.Hkv, 1) * p.Hkv));
     ProfileScope prof("cf_chunk_short", stream);
-    CF_LAUNCH((chunk_short_kernel<QT, KT, D>), few, dim3(256), 0, stream, p);
+    CF_LAUNCH((chunk_short_kernel<QT, KT, D, 4>), few(4), dim3(256), 0, stream, p);
+    CF_HIP_CHECK(hipGetLastError());
+  } else if (cap <= 2 * kCols && (double)p.stat_rows * p.Hq * cap <= kShortMost) {
+    ProfileScope prof("cf_chunk_short", stream);
+    CF_LAUNCH((chunk_short_kernel<QT, KT, D, 8>), few(8), dim3(512), 0, stream, p);
     CF_HIP_CHECK(hipGetLastError());
   } else {
     {

@@ -95,6 +95,9 @@ def _check(case, **more):
     assert bool((err <= bound).all()), (float((err / bound).max()), int((err > bound).sum()))
 
 
+# blocks of the tables: as many as the tokens take, and the widths at which four
+# waves, eight, or kernels for rows and tokens apart take them
+WIDTHS = pytest.mark.parametrize("mb", [None, 24, 40])
 TYPES = [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float8_e4m3fn), (torch.float16, torch.float16),
          (torch.float16, torch.float8_e4m3fn)]
 
@@ -102,13 +105,15 @@ TYPES = [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float8_e4m3fn)
 @pytest.mark.parametrize("q, kv", TYPES)
 @pytest.mark.parametrize("layout", ["paired", "native", "token_major"])
 @pytest.mark.parametrize("hq, h, d", [(4, 4, 64), (8, 1, 64), (32, 8, 128), (16, 1, 128)])
-def test_types_and_heads(gpu, q, kv, layout, hq, h, d):
-    _check(Case(gpu, [(1, 0), (17, 30), (130, 0), (64, 300)], hq, h, d, q, kv, layout, seed=1))
+@pytest.mark.parametrize("mb, most", [(None, 150), (None, 300), (40, 300)])
+def test_types_and_heads(gpu, q, kv, layout, hq, h, d, mb, most):
+    _check(Case(gpu, [(1, 0), (17, 30), (130, 0), (64, most)], hq, h, d, q, kv, layout, seed=1, mb=mb))
 
 
 @pytest.mark.parametrize("hq, h", [(6, 2), (3, 1), (64, 1), (20, 4), (1, 1)])
-def test_groups_that_are_no_power_of_two(gpu, hq, h):
-    _check(Case(gpu, [(100, 45), (7, 0)], hq, h, 64, torch.bfloat16, torch.bfloat16, seed=2))
+@WIDTHS
+def test_groups_that_are_no_power_of_two(gpu, hq, h, mb):
+    _check(Case(gpu, [(100, 45), (7, 0)], hq, h, 64, torch.bfloat16, torch.bfloat16, seed=2, mb=mb))
 
 
 @pytest.mark.parametrize("rows, cached", [(1, 0), (1, 999), (15, 1), (16, 16), (255, 1), (256, 0), (257, 255), (1000, 24),
@@ -126,8 +131,9 @@ def test_observers(gpu, observe, hw):
 
 @pytest.mark.parametrize("decay", [0.0, 0.5, -2.0])
 @pytest.mark.parametrize("hw", [None, 1])
-def test_decay(gpu, decay, hw):
-    case = Case(gpu, [(33, 64), (5, 100)], 8, 4, 64, torch.float16, torch.float16, seed=5, hw=hw)
+@WIDTHS
+def test_decay(gpu, decay, hw, mb):
+    case = Case(gpu, [(33, 64), (5, 100)], 8, 4, 64, torch.float16, torch.float16, seed=5, hw=hw, mb=mb)
     want, add = case.expected(decay=decay)
     for n, (r, c) in enumerate(case.chunks):  # entries without history are not read
         case.w[n, :, c: r + c] = float("nan")
@@ -146,36 +152,41 @@ def test_large_units_and_many_pieces(gpu):
     _check(Case(gpu, [(2500, 0), (1024, 2000), (2000, 70)], 32, 8, 64, torch.bfloat16, torch.bfloat16, seed=6))
 
 
-def test_many_chunks(gpu):
-    _check(Case(gpu, [(1 + i % 5, i * 7 % 90) for i in range(150)], 4, 2, 64, torch.bfloat16, torch.bfloat16, seed=7,
-                gaps=3))
+@WIDTHS
+def test_many_chunks(gpu, mb):
+    _check(Case(gpu, [(1 + i % 5, i * 7 % 90) for i in range(270)], 4, 2, 64, torch.bfloat16, torch.bfloat16, seed=7,
+                gaps=3, mb=mb))
 
 
-def test_chunks_without_rows_and_odd_starts(gpu):
-    case = Case(gpu, [(10, 20), (0, 50), (30, 0), (5, 5)], 8, 2, 64, torch.bfloat16, torch.bfloat16, seed=8)
+@WIDTHS
+def test_chunks_without_rows_and_odd_starts(gpu, mb):
+    case = Case(gpu, [(10, 20), (0, 50), (30, 0), (5, 5)], 8, 2, 64, torch.bfloat16, torch.bfloat16, seed=8, mb=mb)
     before = case.w[1].clone()
     _check(case)
     assert torch.equal(case.w[1], before)
     # a start before the previous chunk's end starts there; ends past q are cut
-    case = Case(gpu, [(10, 20), (6, 50), (24, 10)], 8, 2, 64, torch.bfloat16, torch.bfloat16, seed=9)
+    case = Case(gpu, [(10, 20), (6, 50), (24, 10)], 8, 2, 64, torch.bfloat16, torch.bfloat16, seed=9, mb=mb)
     case.start = torch.tensor([0, 10, 4, 999], dtype=torch.int32, device=gpu)
     case.starts = [0, 10, 10, 40]
     case.lens = [30, 56, 34]
     _check(case)
 
 
-def test_lengths_at_the_edges_and_invalid_blocks(gpu):
+@pytest.mark.parametrize("mb", [3, 24, 40])
+def test_lengths_at_the_edges_and_invalid_blocks(gpu, mb):
     case = Case(gpu, [(40, 8), (20, 0), (20, 28), (48, 0), (48, 0)], 8, 2, 64, torch.bfloat16, torch.bfloat16, seed=10,
-                mb=3)
-    case.lens = [100, 7, 0, 48, 48]  # past the table, shorter than the chunk, empty
+                mb=mb)
+    case.lens = [mb * 16 + 52, 7, 0, 48, 48]  # past the table, shorter than the chunk, empty
     case.seq = torch.tensor(case.lens, dtype=torch.int32, device=gpu)
     case.tables[3, 1] = -1
     case.tables[4, :] = case.k.shape[0]
     _check(case)
 
 
-def test_nan_scores_stay_in_their_rows(gpu):
-    bad, clean = (Case(gpu, [(64, 0), (64, 0)], 8, 2, 64, torch.bfloat16, torch.bfloat16, seed=11) for _ in range(2))
+@WIDTHS
+def test_nan_scores_stay_in_their_rows(gpu, mb):
+    bad, clean = (Case(gpu, [(64, 0), (64, 0)], 8, 2, 64, torch.bfloat16, torch.bfloat16, seed=11, mb=mb)
+                  for _ in range(2))
     bad.q[20, 1] = float("nan")  # chunk 0, KV head 0
     bad.run()
     clean.run()
@@ -184,8 +195,9 @@ def test_nan_scores_stay_in_their_rows(gpu):
 
 
 @pytest.mark.parametrize("scale", [-0.125, 0.0])
-def test_negative_and_zero_scales(gpu, scale):
-    case = Case(gpu, [(70, 20), (9, 0)], 8, 2, 64, torch.float16, torch.float8_e4m3fn, seed=12)
+@WIDTHS
+def test_negative_and_zero_scales(gpu, scale, mb):
+    case = Case(gpu, [(70, 20), (9, 0)], 8, 2, 64, torch.float16, torch.float8_e4m3fn, seed=12, mb=mb)
     _check(case, scale=scale)
 
 
