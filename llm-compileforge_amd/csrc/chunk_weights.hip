@@ -935,7 +935,9 @@ int32_t launch_d(const ChunkWeightsParams& p, hipStream_t stream) {
     }
   }
   ProfileScope prof("cf_chunk_join", stream);
-  // (many pieces a token: more loads in flight)
+  // Many pieces a token: more loads in flight.  Two prompts of 4,000 rows 4.0 us
+  // against 4.6, 469 rows of 64 heads into one account 4.0 and 7.6; 64 observers
+  // of four sequences, whose pieces are few, 8.2 and 4.4.
   if (ceil_div(p.compact ? p.observe : ceil_div(p.Tq, p.N), p.piece_rows) * (p.Hkv / p.Hw) >= 8)
     CF_LAUNCH((chunk_join_kernel<true>), dim3((unsigned)(ceil_div(cap, 64) * p.N * p.Hw)), dim3(256), 0, stream, p);
   else
