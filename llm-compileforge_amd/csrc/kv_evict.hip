@@ -524,8 +524,8 @@ __device__ __forceinline__ void copy_tiles(const EvictMoveParams& p, int h0, int
     const int64_t first = s.slot(lane_value(m.z, l0), lane_value(m.w, l0) - l0);
     const int64_t own = (bits >> (lane & 15)) & 1u ? s.slot(m.x, m.y) : first + (lane & 15);
     const int lo = (int)own, hi = (int)(own >> 32);
-    if (d >= p.D) continue;
-    T* base = (T*)p.cache[1] + (int64_t)(h0 + hh) * s.head + (int64_t)d * s.channel;
+    // (lanes past the last channel read it again: every lane stays for the shuffles)
+    T* base = (T*)p.cache[1] + (int64_t)(h0 + hh) * s.head + (int64_t)min(d, p.D - 1) * s.channel;
     T e[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -536,8 +536,10 @@ __device__ __forceinline__ void copy_tiles(const EvictMoveParams& p, int h0, int
     } r;
 #pragma unroll
     for (int i = 0; i < 16; ++i) r.e[i] = e[i];
+    if (d < p.D) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T); ++i) ((uint4*)(base + first))[i] = r.q[i];
+      for (int i = 0; i < (int)sizeof(T); ++i) ((uint4*)(base + first))[i] = r.q[i];
+    }
   }
 }
 

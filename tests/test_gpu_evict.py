@@ -151,7 +151,7 @@ def test_move(gpu, dtype, layout, bs, d, hw):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float8_e4m3fn])
 @pytest.mark.parametrize("layout", ["paired", "native", "token_major"])
-@pytest.mark.parametrize("bs, d, hw", [(16, 64, 2), (32, 40, 1), (16, 144, 1)])
+@pytest.mark.parametrize("bs, d, hw", [(16, 64, 2), (32, 40, 1), (16, 136, 1), (16, 8, 2)])
 def test_move_of_many(gpu, dtype, layout, bs, d, hw):
     """Most slots of a sequence move, few of another's, none of a third's; runs
     that end at the budget, and blocks that the cache does not have."""
