@@ -262,9 +262,10 @@ int32_t cf_prefill_chunk_fp8(const CfTensor* q, const CfTensor* k_cache,
                              void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Workspace of cf_chunk_weights for tables of max_blocks_per_seq blocks: 8
- * bytes a counted row, query head and piece of 1,024 tokens (down to 128 in
- * small calls; at most 64 pieces up to a million tokens), and 4 bytes a KV head
- * and token for each 1,024 (down to 256) counted rows x heads of the group. */
+ * bytes a counted row, query head and run of its tokens (at most 33 runs); 4
+ * bytes a KV head and token for each run of 64 counted rows x heads of the group
+ * (up to 4,096 where the sums would exceed 32 MB; two runs a chunk more); and 4
+ * bytes a counted row and a block of 256 tokens. */
 int32_t cf_chunk_weights_workspace_bytes(int64_t num_q_tokens, int64_t num_chunks, int64_t num_q_heads,
                                          int64_t num_kv_heads, int64_t head_dim, int64_t max_blocks_per_seq,
                                          int32_t block_size, int32_t observe, uint64_t* bytes_out);
