@@ -168,8 +168,10 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictSelectParams
     }
   };
 
-  // the range of the unprotected keys, and how many are protected
-  // (0 and kSafe step aside: one below 0 and one above kSafe wrap round)
+  // the range of the unprotected keys, and how many are protected (0 and kSafe
+  // step aside: one below 0 and one above kSafe wrap round; the steps are taken
+  // back once, after the workgroup's least and greatest are known, since lanes and
+  // waves of nothing but 0 or kSafe hold the wrapped values until then)
   uint32_t lo = 0xFFFFFFFFu, hi = 0u;
   int safe = 0;
   each([&](int, uint32_t k) {
@@ -177,8 +179,6 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictSelectParams
     hi = max(hi, k + 1u);
     safe += k == kSafe ? 1 : 0;
   });
-  lo += 1u;
-  hi -= 1u;
   safe = wave_last(wave_incl_scan(safe, lane));
   lo = ~wave_umax(~lo);
   hi = wave_umax(hi);
@@ -186,8 +186,8 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(EvictSelectParams
   __syncthreads();
   {
     const int4 v = votes[0][lane & (WAVES - 1)];
-    lo = ~wave_umax(~(uint32_t)v.x);
-    hi = wave_umax((uint32_t)v.y);
+    lo = ~wave_umax(~(uint32_t)v.x) + 1u;
+    hi = wave_umax((uint32_t)v.y) - 1u;
     safe = ring_sum<WAVES>(v.z);
   }
   // the greatest key that at least `budget` keys reach, how many keys are

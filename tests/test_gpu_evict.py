@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from cf_hip import layout as L
+from cf_hip import ops
 from kernels.kv_eviction import evict_move, evict_select
 from oracle import kv_eviction as oracle
 
@@ -222,3 +223,31 @@ def test_weights_a_few_last_bits_apart(gpu, budget):
     w = 1.0 + steps[torch.randint(0, 8, (1, 2, 4000), generator=g, device=gpu)] * 2.0**-23
     w[0, 1, ::2] = 5.0
     _check_select(w.float(), [4000], budget, 2, 30)
+
+
+def _select_ms(w, lens, budget):
+    """Median time of the kernel."""
+    tl = torch.tensor(lens, dtype=torch.int32, device=w.device)
+    for _ in range(5):
+        evict_select(w, tl, budget, sink=4, recent=256)
+    torch.cuda.synchronize()
+    ops.KernelTimer.reset()
+    with ops.KernelTimer() as timer:
+        for _ in range(31):
+            evict_select(w, tl, budget, sink=4, recent=256)
+        torch.cuda.synchronize()
+    return sorted(timer.durations("cf_evict_select"))[15]
+
+
+@pytest.mark.parametrize("s, b, budget", [(30000, 4, 4096), (16000, 4, 4096)])
+def test_slots_past_the_sequence_do_not_slow_the_search(gpu, s, b, budget):
+    """The histogram's bins come from the keys of the sequence: a sequence that
+    ends before its buffer, whose last waves hold nothing, is searched as one that
+    fills it.  Weights of one binade: with a range that took in the empty slots
+    their leading bits, all alike, chose one bin for all of them, and a shorter
+    sequence took half as long again."""
+    w = 1.0 + torch.rand(b, 8, s, generator=torch.Generator(device=gpu).manual_seed(8), device=gpu)
+    _check_select(w[:1, :2], [s * 9 // 10], budget, 4, 256)
+    whole = _select_ms(w, [s] * b, budget)
+    for n in (s * 9 // 10, s * 7 // 10, s // 2):
+        assert _select_ms(w, [n] * b, budget) <= 1.3 * whole, n
