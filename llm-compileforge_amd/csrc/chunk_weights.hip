@@ -611,7 +611,8 @@ __global__ __launch_bounds__(256, waves_per_simd<D>()) void chunk_tokens_kernel(
         // the last of these columns sees the wave's first token, and the first its last
         const int pos = c.c0 + row;
         if (tw < vis && pos + colm.row(head + min(kStage - 1, ncol - 1 - j0)) >= tw) {
-          const bool whole = all_live && pos >= tw + 63;
+          // (columns past the last are zeros, which make NaN of an infinity of K)
+          const bool whole = all_live && pos >= tw + 63 && j0 + kStage <= ncol;
           auto tiles = [&](auto masked) {
             constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll

@@ -194,6 +194,19 @@ def test_nan_scores_stay_in_their_rows(gpu, mb):
     assert torch.equal(bad.w[0, 1], clean.w[0, 1]) and torch.equal(bad.w[1], clean.w[1])
 
 
+@pytest.mark.parametrize("kv", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [64, 70, 83])  # x 4 heads: whole steps of columns, and not
+@WIDTHS
+def test_infinite_keys_that_no_row_attends_to(gpu, kv, rows, mb):
+    """A key channel of +inf that every query meets with a negative value: its token's score is
+    -inf and its weight 0, whatever the last step's columns past the rows hold."""
+    case = Case(gpu, [(rows, 200), (9, 0)], 8, 2, 64, kv, kv, seed=16, mb=mb)
+    case.q[:, :, 5] = -case.q[:, :, 5].abs() - 0.5
+    for t in (10, 130):
+        case.k[int(case.tables[0, t // 16]), t % 16, :, 5] = math.inf
+    _check(case)
+
+
 @pytest.mark.parametrize("scale", [-0.125, 0.0])
 @WIDTHS
 def test_negative_and_zero_scales(gpu, scale, mb):
