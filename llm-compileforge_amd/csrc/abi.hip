@@ -631,6 +631,7 @@ static int32_t default_partition(int32_t bs) {
 int32_t cf_paged_decode_weights_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
                                                 int64_t head_dim, int64_t max_blocks_per_seq, int32_t block_size,
                                                 uint64_t* bytes_out) {
+  CF_CHECK(bytes_out != nullptr, "bytes_out is NULL");
   CF_CHECK(block_size > 0, "block_size must be positive");
   uint64_t plain = 0;
   const int32_t rc = cf_paged_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, max_blocks_per_seq,

@@ -70,3 +70,8 @@ def test_the_workspace_holds_a_score_a_head_and_token():
     assert lib.cf_paged_decode_weights_workspace_bytes(1, 5, 2, 64, 3, 16, ctypes.byref(n)) == _abi.CF_ERR_INVALID
     assert lib.cf_paged_decode_weights_workspace_bytes(1, 4, 2, 64, 3, 0, ctypes.byref(n)) == _abi.CF_ERR_INVALID
     assert lib.cf_paged_decode_weights_workspace_bytes(1, 4, 2, 64, 3, 1000, ctypes.byref(n)) == 0
+
+
+def test_the_workspace_query_refuses_a_null_result():
+    assert _abi.lib().cf_paged_decode_weights_workspace_bytes(1, 4, 2, 64, 3, 16, None) == _abi.CF_ERR_INVALID
+    assert "bytes_out is NULL" in _abi.last_error()
