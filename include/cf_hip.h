@@ -479,7 +479,7 @@ int32_t cf_rotary_cache_write(const CfTensor* q, const CfTensor* k_new, const Cf
  *   positions  [B, H, S]        i32, S stride 1, or NULL
  *   seq_lens, kept, seen  [B]   i32
  *   keep       [B, H, budget]   i32, last stride 1 (output)
- *   new_lens   [B]              i32: n (output)
+ *   new_lens   [B]              i32: n (output; not seq_lens, kept or seen themselves)
  * budget >= 1, sink, recent >= 0, sink + recent <= budget. */
 int32_t cf_evict_select(const CfTensor* weights, const CfTensor* seq_lens, const CfTensor* positions,
                         const CfTensor* kept, const CfTensor* seen, int32_t sink, int32_t recent, CfTensor* keep,

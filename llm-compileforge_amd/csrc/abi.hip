@@ -195,6 +195,16 @@ int32_t row_view(const CfTensor* t, const char* name, int64_t B, const int32_t**
   return CF_OK;
 }
 
+// Whether two rows of n i32 entries (strides in elements) have an entry in common.
+bool rows_meet(const int32_t* a, int64_t a_s, const int32_t* b, int64_t b_s, int64_t n) {
+  if (n == 0 || a > b + (n - 1) * b_s || b > a + (n - 1) * a_s) return false;
+  for (int64_t i = 0; i < n; ++i) {
+    const int64_t d = a + i * a_s - b;
+    if (d >= 0 && d <= (n - 1) * b_s && (b_s == 0 || d % b_s == 0)) return true;
+  }
+  return false;
+}
+
 // An account or its positions: [B, H, S] with unit S stride, rows apart.
 int32_t account_view(const CfTensor* t, const char* name, int dtype, View* v) {
   int32_t rc = view_of(t, name, 3, v);
@@ -1301,6 +1311,13 @@ int32_t cf_evict_select(const CfTensor* weights, const CfTensor* seq_lens, const
            (long long)S);
   if ((rc = view_of(new_lens, "new_lens", 1, &vn))) return rc;
   CF_CHECK(vn.dtype == CF_I32 && vn.size[0] == B, "new_lens must be i32 [%lld]", (long long)B);
+  CF_CHECK(B <= 1 || vn.stride[0] != 0, "new_lens: rows overlap (stride 0 on dim 0)");
+  // (a row's heads are workgroups of their own, each of which reads these)
+  const int32_t* n0 = (const int32_t*)vn.base;
+  CF_CHECK(!rows_meet(n0, vn.stride[0], p.lens, p.l_s, B) &&
+               (positions == nullptr || (!rows_meet(n0, vn.stride[0], p.kept, p.kept_s, B) &&
+                                         !rows_meet(n0, vn.stride[0], p.seen, p.seen_s, B))),
+           "new_lens must not share entries with seq_lens, kept or seen, which every head of a row reads");
   CF_CHECK(B * H < (int64_t)INT32_MAX, "too many rows");
   if (B * H == 0) return CF_OK;
   p.weights = (const float*)vw.base;

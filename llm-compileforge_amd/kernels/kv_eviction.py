@@ -52,7 +52,9 @@ def evict_select(
             sink + recent <= budget.
         positions, kept, seen: int32 [B, H, S], [B], [B]; none of them as
             long as nothing was evicted (a slot's index is its position).
-        keep, new_lens: outputs, allocated if not given.
+        keep, new_lens: outputs, allocated if not given; memory of their own
+            (new_lens over seq_lens, kept or seen is refused: every head of a
+            sequence reads them, and so does evict_move afterwards).
 
     Returns:
         (keep int32 [B, H, budget], new_lens int32 [B]): keep[b, h, j] is the

@@ -66,6 +66,37 @@ def test_select_refuses(change, message):
     assert message in _abi.last_error()
 
 
+LENS, STATE = _i32(2), _i32(2, 3)
+
+
+@pytest.mark.parametrize("change", [
+    dict(seq_lens=LENS, new_lens=LENS),
+    dict(kept=LENS, new_lens=LENS),
+    dict(seen=LENS, new_lens=LENS),
+    dict(seen=STATE[:, 1], new_lens=STATE[:, 1]),
+    dict(kept=STATE.view(-1)[:2], new_lens=STATE.view(-1)[1:3]),  # one entry in common
+    dict(seq_lens=STATE.view(-1)[::3], new_lens=STATE.view(-1)[3:5]),
+    dict(seq_lens=LENS[:1].expand(2), new_lens=LENS),
+    dict(seq_lens=LENS, new_lens=LENS, positions=None, kept=None, seen=None),
+])
+def test_select_refuses_new_lengths_over_what_its_heads_read(change):
+    """One head's workgroup would write a length before another's has read the old one."""
+    assert _select(**change) == _abi.CF_ERR_INVALID
+    assert "new_lens must not share" in _abi.last_error()
+
+
+def test_select_refuses_new_lengths_that_are_one():
+    assert _select(new_lens=_i32(1).expand(2)) == _abi.CF_ERR_INVALID
+    assert "new_lens: rows overlap" in _abi.last_error()
+
+
+def test_select_takes_columns_of_one_tensor():
+    """Lengths side by side in one tensor share no entry (no heads: nothing is launched)."""
+    no_heads = dict(weights=torch.zeros(2, 0, 64), positions=_i32(2, 0, 64), keep=_i32(2, 0, 16))
+    assert _select(seq_lens=STATE[:, 0], kept=STATE[:, 1], new_lens=STATE[:, 2], **no_heads) == 0, _abi.last_error()
+    assert _select(seen=STATE.view(-1)[::3], new_lens=STATE.view(-1)[1:3], **no_heads) == 0, _abi.last_error()
+
+
 def _move(**change):
     a = dict(keep=_i32(2, 4, 16), seq_lens=_i32(2), tables=_i32(2, 3), k=torch.zeros(9, 16, 4, 64),
              v=torch.zeros(9, 16, 4, 64), weights=torch.zeros(2, 4, 48), positions=_i32(2, 4, 48), kept=_i32(2),
