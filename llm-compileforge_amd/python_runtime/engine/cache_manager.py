@@ -573,7 +573,13 @@ class CacheManager:
         (float32 [N, heads or 1, slots]) the chunks' attention weights are
         added to it, those of every row or of each chunk's last `observe`
         rows, after what it held was multiplied by `decay`
-        (kernels.chunk_attention_weights)."""
+        (kernels.chunk_attention_weights); row n of `weights` is chunk n's, as
+        row n of `block_tables` is (a caller with accounts in the order of
+        other rows gathers and scatters them), and `out` must not be q, from
+        which the accounts are formed after the attention."""
+        if weights is not None and out is not None and out.data_ptr() == q.data_ptr():
+            raise ValueError("out must not be q in a call with weights: the accounts are formed from the queries "
+                             "after the attention has been written")
         kv = self.layer_view(k_slab, layer_idx)
         vv = self.layer_view(v_slab, layer_idx)
         ks = self._scales[k_slab][layer_idx] if k_slab in self._scales else None

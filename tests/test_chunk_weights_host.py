@@ -7,6 +7,7 @@ import torch
 
 from cf_hip import _abi, ops
 from kernels.paged_attention import chunk_attention_weights
+from python_runtime.engine.cache_manager import CacheManager
 
 
 def _i32(*shape):
@@ -90,3 +91,15 @@ def test_the_workspace_is_checked():
     # a window of observers needs its rows only
     few = ops.chunk_weights_workspace_bytes(8192, 1, 32, 8, 128, 8192, observe=64)
     assert few <= 33 * 64 * 32 * 8 + 5 * 8 * 8192 * 16 * 4 + 64 * 4 + 512 * 4 + 1024
+
+
+def test_attention_over_its_own_queries_leaves_none_for_the_accounts():
+    slabs = [{"slab_id": n, "storage": "paged", "dims": {"layers": 1, "heads": 2, "dim": 64}, "layout": "BNLD",
+              "dtype": "bfloat16"} for n in "kv"]
+    mgr = CacheManager({"slabs": slabs, "intercepts": [], "block_size": 16}, num_blocks=4, device="cpu")
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    args = (q, 0, _i32(1, 2), _i32(1), _i32(2))
+    with pytest.raises(ValueError, match="out must not be q"):
+        mgr.attend_chunks(*args, weights=torch.zeros(1, 2, 32), out=q)
+    with pytest.raises(ValueError, match="ROCm"):  # (without accounts the call goes on to the kernels)
+        mgr.attend_chunks(*args, out=q)
