@@ -88,6 +88,47 @@ def test_select_with_positions_and_strides(gpu):
     _check_select(w, lens, budget, 0, 90, pos, kept, seen)
 
 
+@pytest.mark.parametrize("kind", ["plain", "ties"])
+@pytest.mark.parametrize("s, budget", [(900, 300), (2000, 700), (6000, 2048), (12000, 2500), (30000, 4096), (40000, 9000)])
+def test_select_with_positions_at_every_width(gpu, kind, s, budget):
+    """Stored positions with each kernel: sequences near their buffer's end and far from it, whose last
+    waves hold nothing, some of whose protected tokens lie anywhere in their slots."""
+    g = torch.Generator(device=gpu).manual_seed(s)
+    h = 2 if s < 10000 else 1
+    lens = [s, s - s // 10 - 3, s // 2 + 1, budget + 1]
+    kept = [s // 2, budget, s // 3, budget]
+    seen = [3 * n for n in lens]
+    w = _weights(gpu, len(lens), h, s, 15, kind)
+    pos = torch.full((len(lens), h, s), -7, dtype=torch.int32, device=gpu)  # (unused past kept)
+    for i in range(len(lens)):
+        for j in range(h):
+            at = torch.randperm(seen[i] - (lens[i] - kept[i]), generator=g, device=gpu)[: kept[i]]
+            pos[i, j, : kept[i]] = at.to(torch.int32)
+        # the text's first tokens and some of its latest, wherever they are
+        pos[i, :, kept[i] // 3: kept[i] // 3 + 4] = torch.arange(4, dtype=torch.int32, device=gpu)
+    _check_select(w, lens, budget, 4, budget // 2, pos, kept, seen)
+    _check_select(w, lens, budget, 4, min(budget - 4, s // 20), pos, kept, seen)
+
+
+def test_select_takes_columns_of_one_tensor(gpu):
+    """Lengths side by side in one tensor, the new ones among them."""
+    w = _weights(gpu, 3, 2, 300, 16, "plain")
+    state = torch.tensor([[300, 64, 500], [150, 100, 150], [40, 0, 40]], dtype=torch.int32, device=gpu)
+    new = torch.zeros(3, 4, dtype=torch.int32, device=gpu)
+    new[:, 1:] = state
+    pos = torch.arange(300, dtype=torch.int32, device=gpu).expand(3, 2, 300).contiguous()
+    want = evict_select(w, state[:, 0], 64, sink=2, recent=9, positions=pos, kept=state[:, 1], seen=state[:, 2])
+    got = evict_select(w, new[:, 1], 64, sink=2, recent=9, positions=pos, kept=new[:, 2], seen=new[:, 3],
+                       new_lens=new[:, 0])
+    assert torch.equal(got[0], want[0]) and torch.equal(new[:, 0], want[1]) and torch.equal(new[:, 1:], state)
+    for shared in (1, 2, 3):
+        with pytest.raises(ValueError, match="new_lens must not share"):
+            evict_select(w, new[:, 1], 64, sink=2, recent=9, positions=pos, kept=new[:, 2], seen=new[:, 3],
+                         new_lens=new[:, shared])
+    with pytest.raises(ValueError, match="new_lens must not share"):
+        evict_select(w, new[:, 1], 64, new_lens=new[:, 1])
+
+
 def _fill(t, seed):
     g = torch.Generator(device=t.device).manual_seed(seed)
     raw = {1: torch.uint8, 2: torch.int16, 4: torch.int32}[t.element_size()]
