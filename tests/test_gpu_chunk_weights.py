@@ -207,6 +207,24 @@ def test_infinite_keys_that_no_row_attends_to(gpu, kv, rows, mb):
     _check(case)
 
 
+@pytest.mark.parametrize("observe", [0, 16])
+@pytest.mark.parametrize("hw", [None, 1])
+@pytest.mark.parametrize("chunks", [[(77, 0), (1, 30), (38, 12)], [(500, 0)] * 8, [(40, 1900), (300, 100)]])
+def test_tables_and_accounts_much_wider_than_the_sequences(gpu, chunks, hw, observe):
+    """The engine's own tables: 2,048 columns for sequences of a few blocks, no block past their end."""
+    case = Case(gpu, chunks, 8, 2, 64, torch.bfloat16, torch.bfloat16, seed=17, hw=hw)
+    n = len(chunks)
+    tables = torch.full((n, 2048), -1, dtype=torch.int32, device=gpu)
+    w = torch.rand(n, case.w.shape[1], 2048 * 16 + 5, device=gpu)
+    for i, m in enumerate(case.lens):
+        tables[i, : -(-m // 16)] = case.tables[i, : -(-m // 16)]
+    case.tables, case.w = tables, w
+    rest = w.clone()
+    _check(case, observe=observe)
+    for i, m in enumerate(case.lens):
+        assert torch.equal(w[i, :, m:], rest[i, :, m:])
+
+
 @pytest.mark.parametrize("scale", [-0.125, 0.0])
 @WIDTHS
 def test_negative_and_zero_scales(gpu, scale, mb):

@@ -261,3 +261,19 @@ def test_capture_and_replay(gpu):
         want = eager.run()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(cap.w, eager.w), i
+
+
+@pytest.mark.parametrize("hw", [None, 1])
+@pytest.mark.parametrize("q, kv", [(torch.bfloat16, torch.float8_e4m3fn), (torch.float32, torch.float32)])
+def test_tables_and_accounts_much_wider_than_the_sequences(gpu, q, kv, hw):
+    """The engine's own tables: 2,048 columns for sequences of a few blocks, rows without a request among them."""
+    case = Case(gpu, 5, 8, 2, 64, [40, 0, 1, 511, 200], q, kv, seed=31, hw=hw)
+    tables = torch.full((5, 2048), -1, dtype=torch.int32, device=gpu)
+    w = torch.rand(5, case.w.shape[1], 2048 * 16 + 3, device=gpu)
+    for i, m in enumerate(case.lens):
+        tables[i, : -(-m // 16)] = case.tables[i, : -(-m // 16)]
+    case.tables, case.w = tables, w
+    rest = w.clone()
+    _check(case, decay=0.5)
+    for i, m in enumerate(case.lens):
+        assert torch.equal(w[i, :, m:], rest[i, :, m:])

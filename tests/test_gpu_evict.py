@@ -110,6 +110,14 @@ def test_select_with_positions_at_every_width(gpu, kind, s, budget):
     _check_select(w, lens, budget, 4, min(budget - 4, s // 20), pos, kept, seen)
 
 
+@pytest.mark.parametrize("s", [4096, 12000, 32000, 40000])
+def test_accounts_much_wider_than_the_sequences(gpu, s):
+    """A bounded cache's accounts, as wide as the longest prompt: sequences near the budget, and one
+    that has no token."""
+    w = _weights(gpu, 5, 2, s, 18, "plain")
+    _check_select(w, [2064, 2049, 2048, 17, 0], 2048, 4, 256)
+
+
 def test_select_takes_columns_of_one_tensor(gpu):
     """Lengths side by side in one tensor, the new ones among them."""
     w = _weights(gpu, 3, 2, 300, 16, "plain")
