@@ -18,8 +18,8 @@ After a sequence's first eviction its slots no longer follow its text.  Its
 `positions` then say where each slot's token stands (they decide what is first
 and what is latest), for the slots below `kept`; slots from there on hold the
 tokens appended since, the last of them at position seen - 1.  A caller keeps
-positions int32 [B, heads, slots], kept and seen int32 [B], and sets kept to
-new_lens after each eviction.
+positions int32 [B, heads, slots], kept and seen int32 [B], sets kept to
+new_lens after each eviction, and starts a new sequence in a row with kept 0.
 """
 
 from __future__ import annotations

@@ -652,9 +652,11 @@ class CacheManager:
         layers with the old seq_lens, set `kept` to the new lengths, then cut
         the requests with BlockManager.truncate.
 
-        Rows are written in place, so blocks that hold a row's first `budget`
-        slots and are shared must be made its own before:
-        BlockManager.prepare_writes([(request, 0, budget)]) and copy_blocks."""
+        Rows over the budget are written in place, so blocks that hold such a
+        row's first `budget` slots and are shared must be made its own before:
+        BlockManager.prepare_writes([(request, 0, budget)]) and copy_blocks, for
+        those requests alone (others keep what they share).  After truncate the
+        request's next token goes to slot `budget`."""
         keep, new_lens = _ops.evict_select(weights, seq_lens, budget, sink, recent, positions, kept, seen)
         _ops.evict_move(keep, seq_lens, block_tables, self.layer_view(k_slab, layer_idx),
                         self.layer_view(v_slab, layer_idx), weights, positions, kept, seen)

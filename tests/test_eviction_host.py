@@ -194,6 +194,37 @@ def test_truncate_gives_the_last_blocks_back():
     assert bm.num_free_blocks() == 16
 
 
+def test_only_requests_over_the_budget_give_up_what_they_share():
+    """The order of an eviction on the pool: copy-on-write for the requests that are cut, no others, and
+    the next token in the slot behind the budget."""
+    from python_runtime.engine.block_manager import BlockManager
+
+    bm, budget = BlockManager(32, 4), 8
+    bm.allocate("a", 0)
+    bm.prepare_writes([("a", 0, 8)])
+    for r in ("b", "c"):
+        bm.share_prefix("a", r, 8)
+        bm.set_len(r, 8)
+    length = {"a": 8, "b": 8, "c": 8}
+    bm.prepare_writes([("c", 8, 6)])
+    length["c"] = 14
+    free = bm.num_free_blocks()
+    over = [r for r, n in length.items() if n > budget]
+    assert over == ["c"]
+    _, copies = bm.prepare_writes([(r, 0, budget) for r in over])
+    assert len(copies) == 2 and bm.num_free_blocks() == free - 2  # c's two shared blocks
+    assert bm.get_blocks("a") == bm.get_blocks("b")               # these two still share theirs
+    assert not set(bm.get_blocks("c")) & set(bm.get_blocks("a"))
+    for r in over:
+        bm.truncate(r, budget)
+        length[r] = budget
+    assert bm.num_free_blocks() == free  # two blocks taken, two given back
+    slots, copies = bm.prepare_writes([(r, length[r], 1) for r in over])
+    assert len(copies) == 0 and slots.tolist() == [bm.get_blocks("c")[2] * 4]
+    # at the length from before the cut it would be a gap of five slots
+    assert len(bm.get_blocks("c")) == 3
+
+
 def test_truncate_refuses():
     from python_runtime.engine.block_manager import BlockManager
 
