@@ -199,7 +199,10 @@ int32_t cf_paged_decode_weights_workspace_bytes(int64_t batch, int64_t num_q_hea
  *                       + sum over the query heads of hw of softmax weight t
  * for the tokens t that sequence b attends to; other entries are left as they
  * were.  The newest token, at seq_lens[b] - 1, has no history: what its entry
- * held is not read, nor is any entry's with decay 0.
+ * held is not read, nor is any entry's with decay 0.  The output is that of
+ * cf_paged_decode_shared bit for bit, so over e4m3fn and f16 caches 16-bit
+ * queries have their softmax weights rounded to 11 bits before the product with
+ * V (2e-4 of an output in the mean square); the accounts take the float32 ones.
  *   weights  [B, Hw, S]  f32, S stride 1, S >= Mb * bs; Hw = Hkv (an account a
  *                        KV head), or 1 (one for all query heads)
  * Tokens in blocks outside [0, NB) draw nothing.
@@ -418,7 +421,8 @@ int32_t cf_paged_gather(const CfTensor* cache, const CfTensor* block_tables,
  * follow axis 0, the next sections[1] axis 1 and so on, or with
  * CF_ROTARY_CYCLED pair j follows axis a = j % axes while j < axes *
  * sections[a], and axis 0 after that; the sections sum to the pairs.  Angles
- * are exact to about 1e-7 of a turn for any position; results are computed in
+ * are formed in 64 bits: exact to about 1e-7 of a turn while |position *
+ * inv_freq| stays below 2^31, and to 6e-17 of it beyond; results are computed in
  * float32 and rounded once. */
 #define CF_ROTARY_MAX_AXES 4
 enum {

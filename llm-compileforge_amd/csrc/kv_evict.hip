@@ -38,7 +38,9 @@ namespace {
 // lane of one wave; if they are too many, a histogram of the bin's next ten
 // bits comes first.  A workgroup is bound by its instructions a key (some 80)
 // and the latency of its barriers and LDS steps.
-// 64 sequences of 8 heads and 2,064 slots: 14 us (12.6 MB); four of 30,000: 28 us.
+// 64 sequences of 8 heads and 2,064 slots: 12.4 us, 13.6 with positions (8.4 and
+// 12.6 MB); four of 30,000: 29.0 and 31.4.  What lies past a sequence's end in its
+// buffer costs its loads: 2,064 tokens in 32,000 slots take 52 us.
 
 __device__ __forceinline__ uint32_t key_of(float w) {
   if (w != w) return 0xFFFFFFFEu;
@@ -588,9 +590,11 @@ int32_t launch_select_t(const EvictSelectParams& p, hipStream_t stream) {
 
 int32_t launch_evict_select(const EvictSelectParams& p, hipStream_t stream) {
   // Few threads with many keys leave room for other heads' workgroups, many
-  // with few shorten a lone one's chain.  64 sequences of 8 heads: 2,064 slots 12
-  // us on 256 threads, 17 on 512, 24 on 1,024; 8,000 slots 18 on 512, 27 on 1,024
-  // (four sequences: 13 both); 16,000 slots 38 on 1,024, 49 on 512.
+  // with few shorten a lone one's chain.  64 sequences of 8 heads without
+  // positions (with them), <threads, keys>: 2,064 slots 12.4 us (13.6) on <256, 16>,
+  // 12.9 (14.0) on <512, 16>, 22.6 (24.4) on <1024, 16>; 8,000 slots 20.7 (24.7) on
+  // <512, 16>, 32.5 (37.2) on <1024, 16> (four sequences: 15.4 and 15.8); 16,000
+  // slots 40.6 (49.8) on <1024, 16>, 49.4 (67.9) on <512, 32>.
   if (p.S <= 256 * 4) return launch_select_t<256, 4>(p, stream);
   if (p.S <= 256 * 16) return launch_select_t<256, 16>(p, stream);
   if (p.S <= 512 * 16) return launch_select_t<512, 16>(p, stream);

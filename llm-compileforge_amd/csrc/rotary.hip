@@ -21,8 +21,10 @@
 // A workgroup takes one token or a group of 16 and some heads of the queries,
 // the keys or the values; a thread takes eight pairs (two 16-byte pieces of a
 // 16-bit row).  Bound by bytes for prompts (about 4,900 rows of 32 + 8 + 8 heads
-// of 128, bf16 to e4m3 with channel-major values: 110 MB in 26.9 us, 4.1 TB/s),
-// by the launch for a decode step (32 rows: 4.3 us).
+// of 128, bf16 to e4m3 with channel-major values: 110 MB in 26.3 us, 4.2 TB/s,
+// with two sets of inputs in turn, of which the last-level cache still holds some,
+// and 30.7 us, 3.6 TB/s, with three), by the launch for a decode step (32 rows:
+// 4.3 us).
 #include <algorithm>
 
 #include "cf_device.hpp"

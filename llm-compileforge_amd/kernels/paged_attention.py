@@ -289,7 +289,10 @@ def paged_attention_weights(
             default a cached one per (device, stream), under graph capture one of
             the graph's.
 
-    The other arguments and the result are those of `paged_attention_tensors`.
+    The other arguments and the result are those of `paged_attention_tensors`,
+    bit for bit: over FP8 and float16 caches 16-bit queries have their softmax
+    weights rounded to 11 bits ahead of the product with V (2e-4 of an output in
+    the mean square), while the accounts add up the float32 weights.
     """
     _require_rocm(q)
     if scale is None:

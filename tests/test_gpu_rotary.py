@@ -78,6 +78,16 @@ def test_far_and_negative_positions(gpu):
         _check(rotary(x, p, f), want, size * (1 + 4 * 2.0**31 * 2.0**-53 / TURN), torch.float32)
 
 
+def test_positions_past_32_bits(gpu):
+    """The float64 turns are off by three roundings (the product, 1 / (2 pi) and its product); frequencies
+    that are powers of two leave the oracle's own product exact."""
+    pos = torch.tensor([2**33 + 1, 2**40 - 3, -(2**45) + 7, 2**52 - 1], device=gpu)
+    x, f = _rows(gpu, (4, 2, 64), torch.float32, 6), (0.5 ** torch.arange(32, dtype=torch.float64)).float().to(gpu)
+    want, size = oracle.rotate(_f64(x), [pos.cpu().numpy()], f.cpu().numpy(), [32])
+    angle = np.abs(pos.cpu().numpy()[:, None].astype(np.float64) * np.tile(f.cpu().numpy(), 2))[:, None]
+    _check(rotary(x, pos, f), want, size * (1 + angle * 3 * 2.0**-53 / TURN), torch.float32)
+
+
 def test_strides_in_place_and_zero_rows(gpu):
     f, pos = _freq(gpu, 24), torch.arange(40, device=gpu)
     big = _rows(gpu, (2, 60, 5, 130), torch.float16, 5)
