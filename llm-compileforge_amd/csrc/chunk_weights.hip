@@ -27,9 +27,9 @@
 // matrix pipe, which the vector pipe hardly overlaps: 64 by 64 pairs at head_dim
 // 64 take a SIMD 1,480 cycles with nothing else to do, and some 2,800 here, the
 // staging, masks and the end, when the older waves of a SIMD are done, included.
-// Two prompts of 1,500 to 4,000 rows, 32 heads of 64: rows 89 us, tokens 84
+// Two prompts of 1,500 to 4,000 rows, 32 heads of 64: rows 90 us, tokens 85
 // (3.6e10 operations of the matrix pipe each); 64 observers behind 4,000 to
-// 12,000 tokens, 4 sequences, 32 heads of 128, e4m3: 35 and 41 us.
+// 12,000 tokens, 4 sequences, 32 heads of 128, e4m3: 35 and 42 us.
 #include <algorithm>
 #include <type_traits>
 

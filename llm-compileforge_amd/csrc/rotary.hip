@@ -23,8 +23,8 @@
 // 16-bit row).  Bound by bytes for prompts (about 4,900 rows of 32 + 8 + 8 heads
 // of 128, bf16 to e4m3 with channel-major values: 110 MB in 26.3 us, 4.2 TB/s,
 // with two sets of inputs in turn, of which the last-level cache still holds some,
-// and 30.7 us, 3.6 TB/s, with three), by the launch for a decode step (32 rows:
-// 4.3 us).
+// and 30.7 us, 3.6 TB/s, with three; launch-stamped events), by the launch for a
+// decode step (32 rows: 4.2 us).
 #include <algorithm>
 
 #include "cf_device.hpp"
