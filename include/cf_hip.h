@@ -497,7 +497,8 @@ int32_t cf_evict_select(const CfTensor* weights, const CfTensor* seq_lens, const
  * the rows stay.
  *   keep          [B, Hw, budget]   i32, last stride 1: cf_evict_select's, Hw = Hkv,
  *                                   or 1 (all heads move together)
- *   seq_lens      [B]               i32, as given to cf_evict_select
+ *   seq_lens      [B]               i32, as given to cf_evict_select, and no more
+ *                                   than the tables' tokens
  *   block_tables  [B, Mb]           i32
  *   k_cache, v_cache  [NB, bs, Hkv, D]  of one dtype, any strides
  *   weights       [B, Hw, S]        f32, S stride 1, or NULL
