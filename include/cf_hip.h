@@ -1,6 +1,6 @@
 /*
  * cf_hip.h -- C ABI of libcf_hip.so: paged decode attention over a paged
- * KV cache (bf16 / fp32 / OCP FP8 e4m3) and FP8 KV quantization on MI355X
+ * KV cache (bf16 / fp32 / OCP FP8 e4m3 / int8) and its quantization on MI355X
  * (gfx950).
  *
  * Conventions (all entry points):
@@ -96,7 +96,10 @@ int32_t cf_paged_decode_workspace_bytes(int64_t batch, int64_t num_q_heads,
  *   block_tables [B, Mb]               i32, physical block ids
  *   seq_lens     [B]                   i32
  *   k_scale,     [Hkv] or [1]          f32 dequant scales (e4m3fn caches
- *   v_scale                            only; NULL otherwise)
+ *   v_scale                            only; NULL otherwise), or
+ *                [NB, Hkv]             a scale for each block and head (both;
+ *                                      e4m3fn and i8 caches): see
+ *                                      cf_kv_write_blocks
  *   scale        softmax scale (the reference default 1/sqrt(D) is applied
  *                by the caller)
  *   out          [B, Hq, D]            dtype of q
@@ -114,7 +117,8 @@ int32_t cf_paged_decode_workspace_bytes(int64_t batch, int64_t num_q_heads,
  * (token stride 1: the layout cf_hip.layout calls "native") or token-major, all
  * 16-byte aligned, with
  *     q bf16 over bf16 or e4m3fn caches,   q f16 over f16 or e4m3fn caches,
- *     q f32 over bf16, e4m3fn or f32 caches.
+ *     q f32 over bf16, e4m3fn or f32 caches,   any of them over e4m3fn or i8
+ *     caches with block scales.
  * The other, for every other input, splits sequences into partitions of
  * partition_tokens tokens (a multiple of bs; shortened where the call is small)
  * merged by a log-sum-exp reduce.  partition_tokens is unused by the first, with
@@ -206,6 +210,7 @@ int32_t cf_paged_decode_weights_workspace_bytes(int64_t batch, int64_t num_q_hea
  *   weights  [B, Hw, S]  f32, S stride 1, S >= Mb * bs; Hw = Hkv (an account a
  *                        KV head), or 1 (one for all query heads)
  * Tokens in blocks outside [0, NB) draw nothing.
+ * Caches with block scales return CF_ERR_UNSUPPORTED.
  * workspace: cf_paged_decode_weights_workspace_bytes() bytes, 256-byte aligned. */
 int32_t cf_paged_decode_weights(const CfTensor* q, const CfTensor* k_cache, const CfTensor* v_cache,
                                 const CfTensor* block_tables, const CfTensor* seq_lens,
@@ -246,7 +251,8 @@ int32_t cf_prefill_chunk_workspace_bytes(int64_t num_q_tokens, int64_t num_chunk
  *                                      the chunk
  *   q_start      [N + 1]               i32, chunk n owns q rows
  *                                      [q_start[n], q_start[n+1])
- *   k_scale, v_scale                   as cf_paged_decode
+ *   k_scale, v_scale                   as cf_paged_decode ([NB, Hkv]: bf16 or
+ *                                      f16 q over e4m3fn or i8 caches)
  *   out          [Tq, Hq, D]           q's dtype
  *
  * Chunk n has L = q_start[n+1] - q_start[n] rows; row i sits at position
@@ -379,6 +385,41 @@ int32_t cf_kv_write_fp8(const CfTensor* k_new, const CfTensor* v_new,
                         CfTensor* v_cache, const CfTensor* k_scale,
                         const CfTensor* v_scale, void* stream);
 
+/* ---- Caches with a scale for each block of tokens and head -----------------
+ * No counterpart in the reference, whose FP8 caches have one scale a tensor
+ * (compiler/quantize/fp8_kv_cache.py:66-93).  Codes are e4m3fn or i8, the value of
+ * a code of block b and head h is code * scale[b, h].  cf_paged_decode*,
+ * cf_prefill_chunk_fp8 and cf_paged_gather read such a cache where they are given
+ * scales [NB, H] (rank 2, any strides; scales positive); what writes by slots with
+ * given scales, moves single rows or keeps accounts does not take it.
+ *
+ * Writes the new rows of N sequences at their last positions: row i of sequence
+ * n's L rows goes to position seq_lens[n] - L + i of block_tables[n] (the operands
+ * of the attention calls that follow).  For each block that takes rows and each
+ * head, with m the largest magnitude of those rows and s0 the block's scale (0 if
+ * the first of them is at offset 0: what the block held before is then dropped):
+ *     need = m / 127 (i8), or the least power of two >= m / 448 (e4m3fn);
+ *     s1 = max(s0, need, 2^-40);
+ *     codes of the new rows: x / s1 rounded to the nearest code, ties to even;
+ *     if s1 is not s0, codes of the rows before them: code * s0 / s1, rounded.
+ * Codes behind the new rows stay.  A NaN or infinity among a block's values makes
+ * its scale NaN, with which all of its values read as NaN, until the block starts
+ * anew.
+ *   k_new, v_new      [T, H, D]        f32 | f16 | bf16, one dtype, any strides
+ *   block_tables      [N, Mb]          i32
+ *   seq_lens          [N]              i32, the new rows included
+ *   q_start           [N + 1] i32, ascending: sequence n owns rows [q_start[n],
+ *                     q_start[n + 1]); NULL: T = N and row n is sequence n's (none
+ *                     where seq_lens[n] is 0)
+ *   k_cache, v_cache  [NB, bs, H, D]   e4m3fn | i8, one dtype, any strides
+ *   k_scale, v_scale  [NB, H]          f32, any strides
+ * Rows at negative positions or past Mb * bs are skipped, and those of blocks
+ * outside [0, NB).  The blocks written to must be their sequence's own
+ * (cf_bp_prepare_writes): two sequences with rows for one block race. */
+int32_t cf_kv_write_blocks(const CfTensor* k_new, const CfTensor* v_new, const CfTensor* block_tables,
+                           const CfTensor* seq_lens, const CfTensor* q_start, CfTensor* k_cache, CfTensor* v_cache,
+                           CfTensor* k_scale, CfTensor* v_scale, void* stream);
+
 /* Writes new rows into one paged tensor (a K or a V cache, any layout):
  * row i goes to block slot_mapping[i] / bs, offset slot_mapping[i] % bs
  * (reference CacheManager.write_paged placement,
@@ -405,7 +446,9 @@ int32_t cf_paged_write(const CfTensor* x_new, const CfTensor* slot_mapping,
  * _kv_cache.py:106-132).
  *   cache         [NB, bs, H, D]   f32 | f16 | bf16 | e4m3fn, any strides
  *   block_tables  [R, Mb]          i32
- *   scale         [H] or [1] f32   (e4m3fn caches; NULL otherwise)
+ *   scale         [H] or [1] f32   (e4m3fn caches; NULL otherwise), or [NB, H]
+ *                                  f32, a scale for each block and head
+ *                                  (e4m3fn and i8 caches)
  *   out           [R, S, H, D]     f32 | f16 | bf16, any strides */
 int32_t cf_paged_gather(const CfTensor* cache, const CfTensor* block_tables,
                         const CfTensor* scale, CfTensor* out, void* stream);
@@ -570,6 +613,20 @@ int32_t cf_bp_set_len(void* pool, const char* request_id, int64_t tokens);
  * cf_evict_select's new length once cf_evict_move is launched.  Work on a
  * released block is ordered by the stream, as after cf_bp_free. */
 int32_t cf_bp_truncate(void* pool, const char* request_id, int64_t tokens);
+/* No reference counterpart: n requests dst[i] (new ones) that continue src's
+ * first `tokens` tokens.  They share its whole blocks, and each gets a fresh block
+ * for a partial last one: (old, fresh) goes to copies ([copies_cap][2]) for
+ * cf_move_blocks, so that all can be written to at once.  All-or-nothing. */
+int32_t cf_bp_fork(void* pool, const char* src_request_id, int64_t n, const char* const* dst_request_ids,
+                   int64_t tokens, int32_t* copies, int64_t copies_cap, int64_t* n_copies);
+/* No reference counterpart: gives the blocks in use new ids from 0 on, each
+ * request's one after the other in table order (requests by device row, then by
+ * id; a block that several share at the first of them; blocks that only a
+ * reference count holds behind, by id).  moves [cap][2] receives (old, new) for
+ * cf_move_blocks, all to be taken at once; NULL only counts and changes nothing.
+ * Tables follow; who keeps ids elsewhere (a prefix cache) has to map them.  The
+ * free block with the lowest id is then the next one taken. */
+int32_t cf_bp_compact(void* pool, int32_t* moves, int64_t cap, int64_t* n_moves);
 /* Device-resident tables (no reference counterpart; the reference builds
  * tables on the host every step).  cf_bp_bind_rows sizes the device table
  * [rows, cols] (initialised to -1 by the caller) and lengths [rows];
@@ -590,6 +647,16 @@ int32_t cf_block_tables_apply(CfTensor* table, CfTensor* lens, const CfTensor* d
  * elements contiguous, E stride 1): block pairs[i][1] <- pairs[i][0], for
  * copy-on-write.  A destination must not be another pair's source. */
 int32_t cf_copy_blocks(CfTensor* cache, const CfTensor* pairs, void* stream);
+/* Moves whole blocks of several paged tensors, each viewed as [NB, E] as
+ * cf_copy_blocks takes it (K and V of all layers, their scales): in every tensor
+ * block moves[i][1] takes what block moves[i][0] held before the call.  A source
+ * may be given to several destinations, and a destination may be a source of other
+ * moves (chains and cycles are taken in place); a destination is given once.
+ *   caches  n_caches descriptors; of different dtypes and sizes, any count
+ *   moves   [n_moves][2] i32 on the host, ids within every tensor's blocks; read
+ *           by the call (a captured call replays these moves)
+ * In one launch for up to 16 tensors and about 300 moves. */
+int32_t cf_move_blocks(const CfTensor* caches, int32_t n_caches, const int32_t* moves, int64_t n_moves, void* stream);
 
 /* Kernel timing hook for benchmarks (no reference counterpart).  While
  * enabled, every kernel this library launches carries a pair of HIP events

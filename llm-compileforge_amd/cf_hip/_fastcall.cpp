@@ -44,6 +44,7 @@ struct Lib {
   decltype(&cf_rotary_cache_write) rotary_write = nullptr;
   decltype(&cf_evict_select) evict_select = nullptr;
   decltype(&cf_evict_move) evict_move = nullptr;
+  decltype(&cf_kv_write_blocks) write_blocks = nullptr;
 };
 Lib g_lib;
 PyObject* g_raw_stream = nullptr;        // device index -> hipStream_t of the current stream
@@ -330,10 +331,15 @@ PyObject* paged_gather(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t seq = as_int(a[2]);
     if (seq < 0) throw Slow{};
     CfTensor dsc{}, dout;
-    if (a[4] != Py_None) dsc = call.flat(a[4]);
+    // (2-D: a scale for each block and head)
+    if (a[4] != Py_None) {
+      const at::Tensor& sc = tensor_of(a[4]);
+      dsc = sc.dim() == 2 && sc.size(0) == cache.size(0) && sc.size(1) == cache.size(2) ? call.in(a[4]) : call.flat(a[4]);
+    }
     at::Tensor fresh;
     if (a[5] == Py_None) {
-      at::ScalarType dtype = cache.scalar_type() == at::kFloat8_e4m3fn ? at::kFloat : cache.scalar_type();
+      const bool codes = cache.scalar_type() == at::kFloat8_e4m3fn || cache.scalar_type() == at::kChar;
+      at::ScalarType dtype = codes ? at::kFloat : cache.scalar_type();
       if (a[3] != Py_None) {
         if (!THPDtype_Check(a[3])) throw Slow{};
         dtype = reinterpret_cast<THPDtype*>(a[3])->scalar_type;
@@ -659,6 +665,21 @@ PyObject* evict_move(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// (k_new, v_new, block_tables, seq_lens, q_start, k_cache, v_cache, k_scale,
+// v_scale) -> 0
+PyObject* kv_write_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(args, n, 9, [](PyObject* const* a) -> PyObject* {
+    const Call call(tensor_of(a[0]));
+    const CfTensor dk = call.in(a[0]), dv = call.in(a[1]), dt = call.in(a[2]), dl = call.in(a[3]);
+    CfTensor dq{};
+    if (a[4] != Py_None) dq = call.in(a[4]);
+    CfTensor dkc = call.in(a[5]), dvc = call.in(a[6]), dks = call.in(a[7]), dvs = call.in(a[8]);
+    return PyLong_FromLong(without_gil([&] {
+      return g_lib.write_blocks(&dk, &dv, &dt, &dl, opt(a[4], dq), &dkc, &dvc, &dks, &dvs, call.stream);
+    }));
+  });
+}
+
 template <class T>
 bool take_address(PyObject* addrs, const char* name, T* fn) {
   PyObject* v = PyDict_GetItemString(addrs, name);
@@ -692,7 +713,8 @@ PyObject* bind(PyObject*, PyObject* args) {
       !take_address(addrs, "cf_rotary", &l.rotary) ||
       !take_address(addrs, "cf_rotary_cache_write", &l.rotary_write) ||
       !take_address(addrs, "cf_evict_select", &l.evict_select) ||
-      !take_address(addrs, "cf_evict_move", &l.evict_move))
+      !take_address(addrs, "cf_evict_move", &l.evict_move) ||
+      !take_address(addrs, "cf_kv_write_blocks", &l.write_blocks))
     return nullptr;
   g_lib = l;
   for (auto [slot, obj] : {std::pair{&g_raw_stream, raw}, std::pair{&g_current_device, cur},
@@ -721,6 +743,7 @@ PyMethodDef kMethods[] = {
     CF_FAST(rotary_cache_write),
     CF_FAST(evict_select),
     CF_FAST(evict_move),
+    CF_FAST(kv_write_blocks),
     {nullptr, nullptr, 0, nullptr},
 };
 #undef CF_FAST

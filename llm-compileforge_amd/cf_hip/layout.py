@@ -62,6 +62,16 @@ def alloc_kv_cache(
     raise ValueError(f"unknown KV layout {layout!r}; expected one of {LAYOUTS}")
 
 
+def alloc_kv_scales(
+    num_blocks: int, num_kv_heads: int, device: torch.device | str
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """(k_scale, v_scale) of an 8-bit cache with a scale for each block and head,
+    each viewed as float32 [NB, Hkv]; a block's K and V scales lie side by side, as
+    the paired layout's tiles do."""
+    buf = torch.zeros(num_blocks, 2, num_kv_heads, dtype=torch.float32, device=device)
+    return buf[:, 0], buf[:, 1]
+
+
 def to_layout(logical: torch.Tensor, layout: str, is_value: bool) -> torch.Tensor:
     """Copies a logical [NB, bs, Hkv, D] tensor into `layout` storage."""
     if logical.dim() != 4:

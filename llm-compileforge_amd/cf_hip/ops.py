@@ -10,10 +10,11 @@ from __future__ import annotations
 import contextlib
 import ctypes
 
+import numpy as np
 import torch
 
 from . import _abi
-from ._abi import check, descriptor, lib, ref, stream_handle
+from ._abi import CfTensor, check, descriptor, lib, ref, stream_handle
 
 DEFAULT_PARTITION_TOKENS = 512  # CF_DEFAULT_PARTITION_TOKENS
 
@@ -105,6 +106,11 @@ def _fast():
     return _FAST
 
 
+def _block_scaled(scale) -> bool:
+    """Whether a call's scales are one for each block and head [NB, H]."""
+    return isinstance(scale, torch.Tensor) and scale.dim() == 2
+
+
 def _on_gpu(t) -> bool:
     return isinstance(t, torch.Tensor) and t.is_cuda
 
@@ -165,12 +171,17 @@ def paged_decode(
 
     block_tables: int32 [B, Mb]; seq_lens: int32 [B]; caches [NB, bs, Hkv, D]
     with any strides (f32/f16/bf16/e4m3fn); e4m3fn caches need per-KV-head
-    fp32 k_scale/v_scale of shape [Hkv] or [1].
+    fp32 k_scale/v_scale of shape [Hkv] or [1], or [NB, Hkv]: a scale for each
+    block and head, which int8 caches may have too (kv_write_blocks).
 
     partition_tokens: partition length of the calls that the partitioned kernel
     takes.  Over float32 caches any other value than the default asks for that
     kernel (2 to 4 times as long on large calls).
     """
+    if _block_scaled(k_scale) and workspace is None and _on_gpu(q) and _captured():
+        workspace = new_workspace(decode_workspace_bytes(
+            q.shape[0], q.shape[1], k_cache.shape[2], q.shape[2], block_tables.shape[1], block_size,
+            partition_tokens), q.device)
     if _on_gpu(q):
         r = _fast().paged_decode(q, k_cache, v_cache, block_tables, seq_lens, float(scale), int(block_size), k_scale,
                                  v_scale, int(partition_tokens), out, workspace, shared_prefix_lens)
@@ -357,11 +368,15 @@ def prefill_chunk(
     cache positions [0, seq_lens[n] - L + i].  Caches: bf16 or e4m3fn under
     bf16 q, fp16 or e4m3fn under fp16 q, block_size 16, in the native or
     paired tile layout or the reference's token-major rows ([NB, 16, Hkv,
-    D] contiguous).
+    D] contiguous).  k_scale, v_scale: [Hkv] or [1] over e4m3fn caches, or [NB,
+    Hkv] over e4m3fn and int8 ones (kv_write_blocks).
 
     workspace: optional buffer, by default a cached one per (device, stream);
     prefill_workspace_bytes() of this call or of a larger one.
     """
+    if _block_scaled(k_scale) and workspace is None and _on_gpu(q) and _captured():
+        workspace = new_workspace(prefill_workspace_bytes(
+            q.shape[0], block_tables.shape[0], q.shape[1], k_cache.shape[2], q.shape[2], block_size), q.device)
     if _on_gpu(q):
         r = _fast().prefill_chunk(q, k_cache, v_cache, block_tables, seq_lens, q_start, float(scale), int(block_size),
                                   k_scale, v_scale, out, workspace)
@@ -673,6 +688,39 @@ def kv_write_fp8(
     check(rc, "cf_kv_write_fp8")
 
 
+def kv_write_blocks(
+    k_new: torch.Tensor,
+    v_new: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    q_start: torch.Tensor | None = None,
+) -> None:
+    """Writes new K/V rows [T, H, D] at the last positions of their sequences into
+    e4m3fn or int8 caches with a scale for each block and head [NB, H], widening
+    the scales of the blocks they go to (see cf_hip.h).  Sequence n owns rows
+    [q_start[n], q_start[n+1]) of seq_lens[n] tokens; without q_start one row each."""
+    if _on_gpu(k_new):
+        r = _fast().kv_write_blocks(k_new, v_new, block_tables, seq_lens, q_start, k_cache, v_cache, k_scale, v_scale)
+        if r is not None:
+            _result(r, "cf_kv_write_blocks")
+            return
+    given = [("k_new", k_new), ("v_new", v_new), ("block_tables", block_tables), ("seq_lens", seq_lens),
+             ("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale), ("v_scale", v_scale)]
+    given += [("q_start", q_start)] if q_start is not None else []
+    for name, t in given:
+        _require_device(name, t)
+    dev = _same_device(*(t for _, t in given))
+    d = [descriptor(t) if t is not None else None
+         for t in (k_new, v_new, block_tables, seq_lens, q_start, k_cache, v_cache, k_scale, v_scale)]
+    with _on(dev):
+        rc = lib().cf_kv_write_blocks(*(ref(x) for x in d), stream_handle(dev))
+    check(rc, "cf_kv_write_blocks")
+
+
 def paged_write(
     x_new: torch.Tensor, slot_mapping: torch.Tensor, cache: torch.Tensor, scale: torch.Tensor | None = None
 ) -> None:
@@ -708,7 +756,8 @@ def paged_gather(
 ) -> torch.Tensor:
     """Dense [R, seq_len, H, D] rows of the tables' first seq_len tokens
     (e4m3fn caches dequantized with `scale`, returned as float32 unless
-    out_dtype says otherwise); table entries < 0 give zero rows."""
+    out_dtype says otherwise; so are int8 ones, whose scale is [NB, H], one for
+    each block and head); table entries < 0 give zero rows."""
     if _on_gpu(cache):
         r = _fast().paged_gather(cache, block_tables, seq_len, out_dtype, scale, out)
         if r is not None:
@@ -717,12 +766,13 @@ def paged_gather(
     _require_device("block_tables", block_tables)
     dev = _same_device(cache, block_tables)
     if out is None:
-        dt = out_dtype or (torch.float32 if cache.dtype == torch.float8_e4m3fn else cache.dtype)
+        dt = out_dtype or (torch.float32 if cache.dtype in (torch.float8_e4m3fn, torch.int8) else cache.dtype)
         out = torch.empty(block_tables.shape[0], seq_len, cache.shape[2], cache.shape[3], dtype=dt, device=dev)
     dsc = None
     if scale is not None:
         _require_device("scale", scale)
-        dsc = descriptor(scale.reshape(-1))
+        dsc = descriptor(scale if _block_scaled(scale) and scale.shape == (cache.shape[0], cache.shape[2])
+                         else scale.reshape(-1))
     dc, dt_, do = descriptor(cache), descriptor(block_tables), descriptor(out)
     with _on(dev):
         rc = lib().cf_paged_gather(ref(dc), ref(dt_), ref(dsc), ref(do), stream_handle(dev))
@@ -991,6 +1041,35 @@ def copy_blocks(cache: torch.Tensor, pairs: torch.Tensor) -> None:
     check(rc, "cf_copy_blocks")
 
 
+def move_blocks(caches, moves) -> None:
+    """Moves whole blocks of paged tensors (dim 0 = block, one device), in place: in
+    each of them block moves[i, 1] takes what block moves[i, 0] held before.  A
+    source may go to several blocks, and a destination may be a source of other
+    moves; each destination is given once.  moves: [n, 2] on the host (a list, numpy
+    array or CPU tensor); it is part of the launch, nothing is uploaded."""
+    caches = list(caches)
+    if isinstance(moves, torch.Tensor) and moves.device.type != "cpu":
+        raise ValueError(f"moves must be on the host (got device {moves.device})")
+    m = np.asarray(moves)
+    if m.size == 0:
+        m = np.empty((0, 2), dtype=np.int32)
+    if m.ndim != 2 or m.shape[1] != 2 or m.dtype.kind not in "iu":
+        raise ValueError(f"moves must be whole numbers [n, 2], got {m.dtype} {m.shape}")
+    if m.size and (int(m.min()) < 0 or int(m.max()) >= 1 << 31):
+        raise ValueError("moves: block ids must be within the caches")
+    m = np.ascontiguousarray(m, dtype=np.int32)
+    for c in caches:
+        _require_device("cache", c)
+    if not caches:
+        return
+    dev = _same_device(*caches)
+    # (descriptors of bytes: any element type)
+    d = (CfTensor * len(caches))(*(descriptor(block_span_view(c).view(torch.uint8)) for c in caches))
+    with _on(dev):
+        rc = lib().cf_move_blocks(d, len(caches), m.ctypes.data, m.shape[0], stream_handle(dev))
+    check(rc, "cf_move_blocks")
+
+
 # ---- side-by-side work on one device ------------------------------------------
 # Decode attention is bound by HBM and chunked prefill by the MFMA pipes.  The
 # decode kernel keeps one workgroup per CU (166 VGPRs a wave), which leaves
@@ -1099,7 +1178,9 @@ __all__ = [
     "fp8_scale_quantize",
     "fp8_quantize",
     "fp8_quantize_kv",
+    "kv_write_blocks",
     "kv_write_fp8",
+    "move_blocks",
     "paged_decode",
     "paged_decode_noalloc",
     "paged_decode_weights",

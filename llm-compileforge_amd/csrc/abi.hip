@@ -13,6 +13,7 @@
 #include "cf_host.hpp"
 #include "chunk_weights.hpp"
 #include "decode_params.hpp"
+#include "kv_blocks.hpp"
 #include "kv_evict.hpp"
 #include "kv_fp8.hpp"
 #include "paged_io.hpp"
@@ -162,6 +163,24 @@ int32_t scale_view(const CfTensor* t, const char* name, int64_t H, const float**
            (long long)v.size[0]);
   *ptr = (const float*)v.base;
   *stride = v.size[0] == 1 ? 0 : v.stride[0];
+  return CF_OK;
+}
+
+// Whether the caller gives a scale for each block and head, [NB, H].
+bool has_block_scales(const CfTensor* t) { return t != nullptr && t->t.rank == 2; }
+
+// [NB, H] f32.
+int32_t block_scale_view(const CfTensor* t, const char* name, int64_t NB, int64_t H, const float** ptr, int64_t* sb,
+                         int64_t* sh) {
+  View v;
+  const int32_t rc = view_of(t, name, 2, &v);
+  if (rc) return rc;
+  CF_CHECK(v.dtype == CF_F32, "%s: expected f32, got %s", name, dtype_name(v.dtype));
+  CF_CHECK(v.size[0] == NB && v.size[1] == H, "%s: expected [%lld, %lld] (a scale for each block and head), got "
+           "[%lld, %lld]", name, (long long)NB, (long long)H, (long long)v.size[0], (long long)v.size[1]);
+  *ptr = (const float*)v.base;
+  *sb = v.stride[0];
+  *sh = v.stride[1];
   return CF_OK;
 }
 
@@ -465,14 +484,19 @@ static int32_t decode_call(const CfTensor* q, const CfTensor* k_cache, const CfT
   if ((rc = view_of(out, "out", 3, &vo))) return rc;
 
   CF_CHECK(is_float_dtype(vq.dtype), "q: dtype must be f32, f16 or bf16, got %s", dtype_name(vq.dtype));
-  CF_CHECK(is_float_dtype(vk.dtype) || vk.dtype == CF_F8E4M3FN,
-           "k_cache: dtype must be f32, f16, bf16 or f8e4m3fn, got %s", dtype_name(vk.dtype));
+  const bool blocks = has_block_scales(k_scale);
+  CF_CHECK(is_float_dtype(vk.dtype) || vk.dtype == CF_F8E4M3FN || (blocks && vk.dtype == CF_I8),
+           "k_cache: dtype must be f32, f16, bf16 or f8e4m3fn, or i8 with block scales, got %s", dtype_name(vk.dtype));
   CF_CHECK(vv.dtype == vk.dtype, "v_cache dtype %s differs from k_cache dtype %s", dtype_name(vv.dtype),
            dtype_name(vk.dtype));
   CF_CHECK(vt.dtype == CF_I32, "block_tables: expected i32, got %s", dtype_name(vt.dtype));
   CF_CHECK(vs.dtype == CF_I32, "seq_lens: expected i32, got %s", dtype_name(vs.dtype));
   CF_CHECK(vo.dtype == vq.dtype, "out dtype %s differs from q dtype %s", dtype_name(vo.dtype),
            dtype_name(vq.dtype));
+  if (blocks && weights != nullptr) {
+    set_error("accounts of attention weight are not kept over caches with block scales");
+    return CF_ERR_UNSUPPORTED;
+  }
 
   const int64_t B = vq.size[0], Hq = vq.size[1], D = vq.size[2];
   const int64_t NB = vk.size[0], bs = vk.size[1], Hkv = vk.size[2];
@@ -537,7 +561,12 @@ static int32_t decode_call(const CfTensor* q, const CfTensor* k_cache, const CfT
   p.PT = generic_partition(B, Hq, Hkv, D, vt.size[1], block_size, partition_tokens);
   p.max_parts = (int)decode_max_parts(vt.size[1], block_size, p.PT);
 
-  if (vk.dtype == CF_F8E4M3FN) {
+  int64_t ks_b = 0, vs_b = 0;
+  if (blocks) {
+    CF_CHECK(vk.dtype == CF_F8E4M3FN || vk.dtype == CF_I8, "block scales apply to f8e4m3fn and i8 caches only");
+    if ((rc = block_scale_view(k_scale, "k_scale", NB, Hkv, &p.k_scale, &ks_b, &p.ks_s))) return rc;
+    if ((rc = block_scale_view(v_scale, "v_scale", NB, Hkv, &p.v_scale, &vs_b, &p.vs_s))) return rc;
+  } else if (vk.dtype == CF_F8E4M3FN) {
     CF_CHECK(k_scale != nullptr && v_scale != nullptr, "f8e4m3fn caches need k_scale and v_scale");
     if ((rc = scale_view(k_scale, "k_scale", Hkv, &p.k_scale, &p.ks_s))) return rc;
     if ((rc = scale_view(v_scale, "v_scale", Hkv, &p.v_scale, &p.vs_s))) return rc;
@@ -604,6 +633,16 @@ static int32_t decode_call(const CfTensor* q, const CfTensor* k_cache, const CfT
   }
 
   hipStream_t st = as_stream(stream);
+  if (blocks) {
+    DecodeBlockParams bp{};
+    static_cast<DecodeParams&>(bp) = plain;
+    bp.ks_b = ks_b;
+    bp.vs_b = vs_b;
+    if (mfma) return launch_decode_mfma(bp, vq.dtype, vk.dtype, st);
+    rc = launch_decode_generic(bp, vq.dtype, vk.dtype, st);
+    if (rc) return rc;
+    return p.max_parts > 1 ? launch_decode_reduce(plain, vq.dtype, st) : CF_OK;
+  }
   if (weights == nullptr) {
     if (mfma) return launch_decode_mfma(plain, vq.dtype, vk.dtype, st);
     rc = launch_decode_generic(plain, vq.dtype, vk.dtype, st);
@@ -713,8 +752,9 @@ int32_t cf_prefill_chunk_fp8(const CfTensor* q, const CfTensor* k_cache, const C
   if ((rc = view_of(out, "out", 3, &vo))) return rc;
 
   CF_CHECK(vq.dtype == CF_BF16 || vq.dtype == CF_F16, "q: dtype must be bf16 or f16, got %s", dtype_name(vq.dtype));
-  CF_CHECK(vk.dtype == CF_BF16 || vk.dtype == CF_F16 || vk.dtype == CF_F8E4M3FN,
-           "k_cache: dtype must be bf16, f16 or f8e4m3fn, got %s", dtype_name(vk.dtype));
+  const bool blocks = has_block_scales(k_scale);
+  CF_CHECK(vk.dtype == CF_BF16 || vk.dtype == CF_F16 || vk.dtype == CF_F8E4M3FN || (blocks && vk.dtype == CF_I8),
+           "k_cache: dtype must be bf16, f16 or f8e4m3fn, or i8 with block scales, got %s", dtype_name(vk.dtype));
   CF_CHECK(vv.dtype == vk.dtype, "v_cache dtype %s differs from k_cache dtype %s", dtype_name(vv.dtype),
            dtype_name(vk.dtype));
   CF_CHECK(vt.dtype == CF_I32, "block_tables: expected i32, got %s", dtype_name(vt.dtype));
@@ -748,7 +788,7 @@ int32_t cf_prefill_chunk_fp8(const CfTensor* q, const CfTensor* k_cache, const C
   CF_CHECK(Hkv < 65536, "too many KV heads");
   CF_CHECK(std::isfinite(scale), "scale must be finite");
 
-  PrefillParams p{};
+  PrefillBlockParams p{};
   p.q = vq.base;
   p.q_sr = vq.stride[0];
   p.q_sh = vq.stride[1];
@@ -777,7 +817,11 @@ int32_t cf_prefill_chunk_fp8(const CfTensor* q, const CfTensor* k_cache, const C
   p.D = (int)D;
   p.Mb = (int)vt.size[1];
   p.NB = (int)NB;
-  if (vk.dtype == CF_F8E4M3FN) {
+  if (blocks) {
+    CF_CHECK(vk.dtype == CF_F8E4M3FN || vk.dtype == CF_I8, "block scales apply to f8e4m3fn and i8 caches only");
+    if ((rc = block_scale_view(k_scale, "k_scale", NB, Hkv, &p.k_scale, &p.ks_b, &p.ks_s))) return rc;
+    if ((rc = block_scale_view(v_scale, "v_scale", NB, Hkv, &p.v_scale, &p.vs_b, &p.vs_s))) return rc;
+  } else if (vk.dtype == CF_F8E4M3FN) {
     CF_CHECK(k_scale != nullptr && v_scale != nullptr, "f8e4m3fn caches need k_scale and v_scale");
     if ((rc = scale_view(k_scale, "k_scale", Hkv, &p.k_scale, &p.ks_s))) return rc;
     if ((rc = scale_view(v_scale, "v_scale", Hkv, &p.v_scale, &p.vs_s))) return rc;
@@ -785,7 +829,7 @@ int32_t cf_prefill_chunk_fp8(const CfTensor* q, const CfTensor* k_cache, const C
     CF_CHECK(k_scale == nullptr && v_scale == nullptr, "k_scale/v_scale apply to f8e4m3fn caches only");
   }
   if (!prefill_supported(p, vq.dtype, vk.dtype)) {
-    set_error("prefill: needs bf16 q over bf16/e4m3 caches or f16 q over f16/e4m3 caches, head_dim 64/128, "
+    set_error("prefill: needs bf16 q over bf16/e4m3 caches or f16 q over f16/e4m3 caches (or int8 with block scales), head_dim 64/128, "
               "GQA group 1/2/4/8/16, native or token-major caches with 16-byte aligned blocks, heads and token "
               "rows, and 16-byte aligned q rows");
     return CF_ERR_UNSUPPORTED;
@@ -801,6 +845,9 @@ int32_t cf_prefill_chunk_fp8(const CfTensor* q, const CfTensor* k_cache, const C
     return CF_ERR_WORKSPACE;
   }
   CF_CHECK(((uintptr_t)workspace & 255) == 0, "workspace must be 256-byte aligned");
+  if (blocks)
+    return vk.dtype == CF_I8 ? launch_prefill_i8(p, vq.dtype, as_stream(stream))
+                             : launch_prefill_e4m3(p, vq.dtype, as_stream(stream));
   return launch_prefill(p, vq.dtype, vk.dtype, as_stream(stream));
 }
 
@@ -1108,6 +1155,80 @@ int32_t cf_kv_write_fp8(const CfTensor* k_new, const CfTensor* v_new, const CfTe
   return launch_kv_write_fp8(p, vk.dtype, vsl.dtype, as_stream(stream));
 }
 
+int32_t cf_kv_write_blocks(const CfTensor* k_new, const CfTensor* v_new, const CfTensor* block_tables,
+                           const CfTensor* seq_lens, const CfTensor* q_start, CfTensor* k_cache, CfTensor* v_cache,
+                           CfTensor* k_scale, CfTensor* v_scale, void* stream) {
+  const CfTensor* in[2] = {k_new, v_new};
+  const CfTensor* ca[2] = {k_cache, v_cache};
+  const CfTensor* sc[2] = {k_scale, v_scale};
+  const char* in_names[2] = {"k_new", "v_new"};
+  const char* ca_names[2] = {"k_cache", "v_cache"};
+  const char* sc_names[2] = {"k_scale", "v_scale"};
+  View vx[2], vc[2], vs[2], vt;
+  int32_t rc;
+  for (int i = 0; i < 2; ++i) {
+    if ((rc = view_of(in[i], in_names[i], 3, &vx[i]))) return rc;
+    if ((rc = view_of(ca[i], ca_names[i], 4, &vc[i]))) return rc;
+    if ((rc = view_of(sc[i], sc_names[i], 2, &vs[i]))) return rc;
+    CF_CHECK(is_float_dtype(vx[i].dtype), "%s: dtype must be f32, f16 or bf16, got %s", in_names[i],
+             dtype_name(vx[i].dtype));
+    CF_CHECK(vx[i].dtype == vx[0].dtype, "v_new dtype %s differs from k_new dtype %s", dtype_name(vx[i].dtype),
+             dtype_name(vx[0].dtype));
+    CF_CHECK(vc[i].dtype == CF_F8E4M3FN || vc[i].dtype == CF_I8, "%s: dtype must be f8e4m3fn or i8, got %s", ca_names[i],
+             dtype_name(vc[i].dtype));
+    CF_CHECK(vc[i].dtype == vc[0].dtype, "v_cache dtype %s differs from k_cache dtype %s", dtype_name(vc[i].dtype),
+             dtype_name(vc[0].dtype));
+    for (int d = 0; d < 3; ++d)
+      CF_CHECK(vx[i].size[d] == vx[0].size[d], "v_new shape differs from k_new on dim %d", d);
+    for (int d = 0; d < 4; ++d)
+      CF_CHECK(vc[i].size[d] == vc[0].size[d], "v_cache shape differs from k_cache shape on dim %d", d);
+    CF_CHECK(vs[i].dtype == CF_F32, "%s: expected f32, got %s", sc_names[i], dtype_name(vs[i].dtype));
+    CF_CHECK(vs[i].size[0] == vc[0].size[0] && vs[i].size[1] == vc[0].size[2],
+             "%s: expected [%lld, %lld] (a scale for each block and head), got [%lld, %lld]", sc_names[i],
+             (long long)vc[0].size[0], (long long)vc[0].size[2], (long long)vs[i].size[0], (long long)vs[i].size[1]);
+    if ((rc = check_apart(vc[i], ca_names[i])) || (rc = check_apart(vs[i], sc_names[i]))) return rc;
+  }
+  if ((rc = view_of(block_tables, "block_tables", 2, &vt))) return rc;
+  CF_CHECK(vt.dtype == CF_I32, "block_tables: expected i32, got %s", dtype_name(vt.dtype));
+  const int64_t T = vx[0].size[0], H = vx[0].size[1], D = vx[0].size[2], N = vt.size[0];
+  const int64_t NB = vc[0].size[0], bs = vc[0].size[1];
+  CF_CHECK(vc[0].size[2] == H && vc[0].size[3] == D, "cache [NB, bs, %lld, %lld] does not match new rows [T, %lld, %lld]",
+           (long long)vc[0].size[2], (long long)vc[0].size[3], (long long)H, (long long)D);
+  CF_CHECK(bs > 0, "cache block size must be positive");
+  CF_CHECK(H < 65536 && D < 65536 && bs < 65536, "dims too large");
+  CF_CHECK(N < (int64_t)INT32_MAX / 4 && vt.size[1] < (int64_t)INT32_MAX && T < (int64_t)INT32_MAX,
+           "too many rows or sequences");
+  KvBlocksParams p{};
+  if ((rc = row_view(seq_lens, "seq_lens", N, &p.lens, &p.l_s))) return rc;
+  if (q_start != nullptr) {
+    if ((rc = row_view(q_start, "q_start", N + 1, &p.start, &p.st_s))) return rc;
+  } else {
+    CF_CHECK(T == N, "%lld rows for %lld sequences (without q_start each has one)", (long long)T, (long long)N);
+  }
+  for (int i = 0; i < 2; ++i) {
+    p.x[i] = vx[i].base;
+    p.cache[i] = vc[i].base;
+    p.scale[i] = (float*)vs[i].base;
+    for (int d = 0; d < 3; ++d) p.x_s[i][d] = vx[i].stride[d];
+    for (int d = 0; d < 4; ++d) p.c_s[i][d] = vc[i].stride[d];
+    for (int d = 0; d < 2; ++d) p.s_s[i][d] = vs[i].stride[d];
+  }
+  p.tables = (const int32_t*)vt.base;
+  p.t_sn = vt.stride[0];
+  p.t_sm = vt.stride[1];
+  p.T = T;
+  p.NB = NB;
+  p.N = (int)N;
+  p.Mb = (int)vt.size[1];
+  p.H = (int)H;
+  p.D = (int)D;
+  p.bs = (int)bs;
+  p.units = q_start != nullptr ? T / bs + 2 * N : N;
+  CF_CHECK(p.units < (int64_t)INT32_MAX, "too many blocks");
+  if (T == 0 || N == 0 || H == 0 || D == 0 || NB == 0 || p.Mb == 0) return CF_OK;
+  return launch_kv_blocks(p, vx[0].dtype, vc[0].dtype, as_stream(stream));
+}
+
 int32_t cf_paged_write(const CfTensor* x_new, const CfTensor* slot_mapping, CfTensor* cache, const CfTensor* scale,
                        void* stream) {
   View vx, vsl, vc;
@@ -1154,8 +1275,9 @@ int32_t cf_paged_gather(const CfTensor* cache, const CfTensor* block_tables, con
   if ((rc = view_of(cache, "cache", 4, &vc))) return rc;
   if ((rc = view_of(block_tables, "block_tables", 2, &vt))) return rc;
   if ((rc = view_of(out, "out", 4, &vo))) return rc;
-  CF_CHECK(is_float_dtype(vc.dtype) || vc.dtype == CF_F8E4M3FN,
-           "cache: dtype must be f32, f16, bf16 or f8e4m3fn, got %s", dtype_name(vc.dtype));
+  const bool blocks = has_block_scales(scale);
+  CF_CHECK(is_float_dtype(vc.dtype) || vc.dtype == CF_F8E4M3FN || (blocks && vc.dtype == CF_I8),
+           "cache: dtype must be f32, f16, bf16 or f8e4m3fn, or i8 with block scales, got %s", dtype_name(vc.dtype));
   CF_CHECK(vt.dtype == CF_I32, "block_tables: expected i32, got %s", dtype_name(vt.dtype));
   CF_CHECK(is_float_dtype(vo.dtype), "out: dtype must be f32, f16 or bf16, got %s", dtype_name(vo.dtype));
   const int64_t R = vt.size[0];
@@ -1166,7 +1288,10 @@ int32_t cf_paged_gather(const CfTensor* cache, const CfTensor* block_tables, con
                vc.size[2] < 65536 && vc.size[3] < 65536 && vc.size[1] < 65536,
            "gather dims too large");
   PagedGatherParams p{};
-  if (vc.dtype == CF_F8E4M3FN) {
+  if (blocks) {
+    CF_CHECK(vc.dtype == CF_F8E4M3FN || vc.dtype == CF_I8, "block scales apply to f8e4m3fn and i8 caches only");
+    if ((rc = block_scale_view(scale, "scale", vc.size[0], vc.size[2], &p.scale, &p.sc_b, &p.sc_s))) return rc;
+  } else if (vc.dtype == CF_F8E4M3FN) {
     CF_CHECK(scale != nullptr, "f8e4m3fn caches need a scale");
     if ((rc = scale_view(scale, "scale", vc.size[2], &p.scale, &p.sc_s))) return rc;
   } else {

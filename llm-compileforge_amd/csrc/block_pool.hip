@@ -20,6 +20,9 @@
 //    cells that changed since the last call (col = -1: the row's length) for
 //    cf_block_tables_apply to scatter, instead of re-uploading every table
 //    each step.
+//  * fork: requests that continue another one, sharing its whole blocks, each
+//    with a copy of its own of the partial last one.
+//  * compact: blocks get new ids, so that each request's follow each other.
 //  * truncate: a request cut to fewer tokens (after evictions from its cache)
 //    gives its last blocks back.
 //  * shared_prefix_lens over the rows, the statement the decode kernel takes
@@ -440,6 +443,129 @@ int32_t cf_bp_truncate(void* h, const char* rid, int64_t tokens) {
   const bool moved = r->len != tokens;
   r->len = tokens;
   if (stay < held || moved) p->touch(r, stay < held ? (int32_t)stay : kClean, moved);
+  return CF_OK;
+}
+
+// Requests that continue src's first `tokens` tokens: the whole blocks are shared,
+// a partial last one is copied for each (src, fresh) so that all can write at once.
+int32_t cf_bp_fork(void* h, const char* src, int64_t n, const char* const* dst, int64_t tokens, int32_t* copies,
+                   int64_t copies_cap, int64_t* n_copies) {
+  CF_CHECK(h && src && (n == 0 || dst), "NULL argument");
+  CF_CHECK(n >= 0 && tokens >= 0, "the number of requests and tokens must be non-negative");
+  Pool* p = pool_of(h);
+  Req* s = p->find(src);
+  if (!s) {
+    set_error("Unknown request_id: %s", src);
+    return CF_ERR_NOT_FOUND;
+  }
+  const int64_t bs = p->block_size, held = (int64_t)s->table.size(), full = tokens / bs;
+  CF_CHECK(tokens <= held * bs, "request %s holds %lld blocks of %lld, not %lld tokens", src, (long long)held,
+           (long long)bs, (long long)tokens);
+  const bool part = tokens % bs != 0;
+  const int64_t need = part ? n : 0;
+  try {
+    std::vector<std::string> ids;
+    for (int64_t i = 0; i < n; ++i) {
+      CF_CHECK(dst[i] != nullptr, "request id %lld is NULL", (long long)i);
+      CF_CHECK(!p->find(dst[i]), "request '%s' already has blocks", dst[i]);
+      ids.push_back(dst[i]);
+    }
+    std::sort(ids.begin(), ids.end());
+    const auto twice = std::adjacent_find(ids.begin(), ids.end());
+    CF_CHECK(twice == ids.end(), "request %s listed twice", twice == ids.end() ? "" : twice->c_str());
+    if (need > p->free_count()) return out_of_blocks(p, need);
+    CF_CHECK(copies == nullptr || need <= copies_cap, "copies holds %lld pairs, %lld needed", (long long)copies_cap,
+             (long long)need);
+    CF_CHECK(need == 0 || copies != nullptr, "copies needed but no buffer given");
+    // (everything that may throw comes before the first change)
+    std::vector<std::unique_ptr<Req>> fresh;
+    for (int64_t i = 0; i < n; ++i) {
+      fresh.emplace_back(new Req());
+      fresh.back()->table.reserve(full + 1);
+      fresh.back()->table.assign(s->table.begin(), s->table.begin() + full);
+    }
+    p->reqs.reserve(p->reqs.size() + n);
+    if (p->rows > 0) p->dirty.reserve(p->dirty.size() + n);
+    for (int64_t i = 0; i < n; ++i) {
+      Req* r = (p->reqs[dst[i]] = std::move(fresh[i])).get();
+      for (const int32_t bid : r->table)
+        if (bid >= 0 && bid < p->num_blocks) p->rc[bid] += 1;
+      if (part) {
+        copies[2 * i] = s->table[full];
+        copies[2 * i + 1] = p->pop_block();
+        r->table.push_back(copies[2 * i + 1]);
+      }
+      r->len = tokens;
+      p->touch(r, 0, true);
+    }
+  } catch (...) {
+    set_error("cf_bp_fork: out of host memory");
+    return CF_ERR_INVALID;
+  }
+  if (n_copies) *n_copies = need;
+  return CF_OK;
+}
+
+// New ids for every block in use: the requests' blocks in table order from 0 on, by
+// device row and then by request id, a shared one where it comes first; then the
+// blocks that only reference counts hold, by id.  moves [n][2]: (old, new) of every
+// block whose id changes, to be taken at once (cf_move_blocks).  NULL: only counts.
+int32_t cf_bp_compact(void* h, int32_t* moves, int64_t cap, int64_t* n_moves) {
+  CF_CHECK(h && n_moves, "NULL argument");
+  Pool* p = pool_of(h);
+  try {
+    std::vector<std::pair<const std::string*, Req*>> order;
+    for (auto& kv : p->reqs) order.emplace_back(&kv.first, kv.second.get());
+    std::sort(order.begin(), order.end(), [](const auto& a, const auto& b) {
+      const int64_t ra = a.second->row < 0 ? INT64_MAX : a.second->row, rb = b.second->row < 0 ? INT64_MAX : b.second->row;
+      return ra != rb ? ra < rb : *a.first < *b.first;
+    });
+    std::vector<int32_t> now(p->num_blocks, -1);
+    int32_t next = 0;
+    auto place = [&](int32_t bid) {
+      // (ids outside the pool, and free blocks that a table still names, stay)
+      if (bid >= 0 && bid < p->num_blocks && p->rc[bid] > 0 && now[bid] < 0) now[bid] = next++;
+    };
+    for (const auto& r : order)
+      for (const int32_t bid : r.second->table) place(bid);
+    for (int64_t b = 0; b < p->num_blocks; ++b) place((int32_t)b);
+    int64_t n = 0;
+    for (int64_t b = 0; b < p->num_blocks; ++b) n += now[b] >= 0 && now[b] != b;
+    *n_moves = n;
+    if (moves == nullptr) return CF_OK;
+    CF_CHECK(n <= cap, "moves holds %lld pairs, %lld needed", (long long)cap, (long long)n);
+    std::vector<int64_t> rc(p->num_blocks, 0);
+    std::vector<int32_t> free_list;
+    for (int64_t b = p->num_blocks - 1; b >= next; --b) free_list.push_back((int32_t)b);  // the lowest is taken next
+    free_list.reserve(p->num_blocks);
+    if (p->rows > 0) p->dirty.reserve(p->reqs.size());
+    int64_t k = 0;
+    for (int64_t b = 0; b < p->num_blocks; ++b) {
+      if (now[b] < 0) continue;
+      rc[now[b]] = p->rc[b];
+      if (now[b] != b) {
+        moves[2 * k] = (int32_t)b;
+        moves[2 * k + 1] = now[b];
+        ++k;
+      }
+    }
+    p->rc.swap(rc);
+    p->free_list.swap(free_list);
+    for (const auto& r : order) {
+      int32_t from = kClean;
+      auto& table = r.second->table;
+      for (size_t j = 0; j < table.size(); ++j) {
+        const int32_t bid = table[j];
+        if (bid < 0 || bid >= p->num_blocks || now[bid] < 0 || now[bid] == bid) continue;
+        table[j] = now[bid];
+        from = std::min(from, (int32_t)j);
+      }
+      if (from != kClean) p->touch(r.second, from, false);
+    }
+  } catch (...) {
+    set_error("cf_bp_compact: out of host memory");
+    return CF_ERR_INVALID;
+  }
   return CF_OK;
 }
 

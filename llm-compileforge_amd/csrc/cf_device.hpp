@@ -169,7 +169,7 @@ __device__ __forceinline__ uint16_t bf16_bits_from_f32(float f) {
 }
 
 // Element access by dtype code (CfDtype numbering).
-enum : int { kF32 = 0, kF16 = 1, kBF16 = 2, kI64 = 3, kI32 = 4, kE4M3 = 7 };
+enum : int { kF32 = 0, kF16 = 1, kBF16 = 2, kI64 = 3, kI32 = 4, kI8 = 5, kE4M3 = 7 };
 
 template <int DT> struct Elem;
 template <> struct Elem<kF32> {
@@ -192,6 +192,10 @@ template <> struct Elem<kE4M3> {
   static __device__ __forceinline__ float load(const T* p) { return f32_from_e4m3(*p); }
   static __device__ __forceinline__ void store(T* p, float v) { *p = e4m3_from_f32(v); }
 };
+template <> struct Elem<kI8> {
+  using T = int8_t;
+  static __device__ __forceinline__ float load(const T* p) { return (float)*p; }
+};
 
 // 16 consecutive elements of dtype code XT (16-byte aligned) as floats.
 template <int XT>
@@ -211,6 +215,11 @@ __device__ __forceinline__ void load16(const void* src, float* f) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 16; ++j) f[j] = f32_from_e4m3((w[j >> 2] >> (8 * (j & 3))) & 0xFFu);
+  } else if constexpr (XT == kI8) {
+    const uint4 u = s[0];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 16; ++j) f[j] = (float)(int8_t)(w[j >> 2] >> (8 * (j & 3)));
   } else {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {

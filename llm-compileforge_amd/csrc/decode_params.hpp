@@ -37,6 +37,11 @@ struct DecodeParams {
   int NB;  // cache blocks; a block id outside [0, NB) contributes no tokens
 };
 
+// A decode call over a cache with a scale for each block and head.
+struct DecodeBlockParams : DecodeParams {
+  int64_t ks_b, vs_b;  // strides over blocks of k_scale and v_scale [NB, Hkv] (ks_s, vs_s: over heads)
+};
+
 // A decode call that also accounts for the weights: the kernels leave every
 // score and the rows' final (m, l), from which decode_weights_kernel forms them.
 struct DecodeWeightsParams : DecodeParams {
@@ -75,6 +80,8 @@ __device__ __forceinline__ int64_t score_at(int t, int g, int G) {
 // Launchers (return a CF_* status; kernels are enqueued on `stream`).
 int32_t launch_decode_generic(const DecodeParams& p, int q_dt, int kv_dt, hipStream_t stream);
 int32_t launch_decode_mfma(const DecodeParams& p, int q_dt, int kv_dt, hipStream_t stream);
+int32_t launch_decode_generic(const DecodeBlockParams& p, int q_dt, int kv_dt, hipStream_t stream);
+int32_t launch_decode_mfma(const DecodeBlockParams& p, int q_dt, int kv_dt, hipStream_t stream);
 // The same with scores and final (m, l) written (the call is one that the
 // plain launcher takes), and the accounts formed from them.
 int32_t launch_decode_generic(const DecodeWeightsParams& p, int q_dt, int kv_dt, hipStream_t stream);

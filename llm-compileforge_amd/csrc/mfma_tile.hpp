@@ -59,6 +59,10 @@ struct KvTraits<kE4M3> {
   static constexpr int kBytes = 1;
 };
 template <>
+struct KvTraits<kI8> {
+  static constexpr int kBytes = 1;
+};
+template <>
 struct KvTraits<kBF16> {
   static constexpr int kBytes = 2;
 };
@@ -284,11 +288,43 @@ __device__ __forceinline__ uint4 mask_tokens(uint4 v, int n_valid) {
   return make_uint4(lo.x, lo.y, hi.x, hi.y);
 }
 
+// 8 int8 codes -> 8 bf16, exact: a float of one byte's range has nothing below its
+// upper half.
+__device__ __forceinline__ bf16x8_t i8x8_to_bf16(uint32_t lo, uint32_t hi) {
+  const uint32_t w[2] = {lo, hi};
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = w[i >> 1] >> (16 * (i & 1));
+    const float x = (float)(int8_t)a, y = (float)(int8_t)(a >> 8);
+    r[i] = __builtin_amdgcn_perm(f2u(y), f2u(x), 0x07060302u);
+  }
+  return as_bf16x8(make_uint4(r[0], r[1], r[2], r[3]));
+}
+
+// 8 int8 codes -> 8 fp16, exact: with its sign bit flipped a byte u = x + 128 is the
+// low byte of the fp16 number 1024 + u.
+__device__ __forceinline__ f16x8_t i8x8_to_f16(uint32_t lo, uint32_t hi) {
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+  const uint32_t w[2] = {lo ^ 0x80808080u, hi ^ 0x80808080u};
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = __builtin_amdgcn_perm(0x64646464u, w[i >> 1], (i & 1) ? 0x04030402u : 0x04010400u);
+    const f16x2_t f = __builtin_bit_cast(f16x2_t, u) - f16x2_t{(_Float16)1152.0f, (_Float16)1152.0f};
+    r[i] = __builtin_bit_cast(uint32_t, f);
+  }
+  return __builtin_bit_cast(f16x8_t, make_uint4(r[0], r[1], r[2], r[3]));
+}
+
 template <int KT>
 __device__ __forceinline__ bf16x8_t k_operand(const uint4* raw, int c) {
   if constexpr (KT == kE4M3) {
     const uint4 u = raw[c >> 1];
     return (c & 1) ? e4m3x8_to_bf16(u.z, u.w) : e4m3x8_to_bf16(u.x, u.y);
+  } else if constexpr (KT == kI8) {
+    const uint4 u = raw[c >> 1];
+    return (c & 1) ? i8x8_to_bf16(u.z, u.w) : i8x8_to_bf16(u.x, u.y);
   } else {
     return as_bf16x8(raw[c]);
   }
@@ -324,6 +360,9 @@ __device__ __forceinline__ QOp<QT> k_operand_q(const uint4* raw, int c) {
     if constexpr (KT == kE4M3) {
       const uint4 u = raw[c >> 1];
       return (c & 1) ? e4m3x8_to_f16(u.z, u.w) : e4m3x8_to_f16(u.x, u.y);
+    } else if constexpr (KT == kI8) {
+      const uint4 u = raw[c >> 1];
+      return (c & 1) ? i8x8_to_f16(u.z, u.w) : i8x8_to_f16(u.x, u.y);
     } else {
       return __builtin_bit_cast(f16x8_t, raw[c]);
     }

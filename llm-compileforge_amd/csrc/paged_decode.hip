@@ -41,6 +41,9 @@ __device__ __forceinline__ int effective_len(const DecodeParams& p, int b) {
 // P: DecodeParams, or DecodeWeightsParams for a call that also keeps its scores.
 template <class P>
 constexpr bool kKeeps = std::is_same<P, DecodeWeightsParams>::value;
+// DecodeBlockParams: a cache with a scale for each block and head.
+template <class P>
+constexpr bool kBlocks = std::is_same<P, DecodeBlockParams>::value;
 
 template <int QT, int KT, bool DIRECT, class P>
 __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(P p) {
@@ -82,8 +85,8 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(P p) {
     sblk[i] = p.tables[(int64_t)b * p.t_sb + (int64_t)(blk0 + i) * p.t_sm];
   __syncthreads();
 
-  const float ks = p.k_scale ? p.k_scale[h * p.ks_s] : 1.0f;
-  const float vs = p.v_scale ? p.v_scale[h * p.vs_s] : 1.0f;
+  const float ks = !kBlocks<P> && p.k_scale ? p.k_scale[h * p.ks_s] : 1.0f;
+  const float vs = !kBlocks<P> && p.v_scale ? p.v_scale[h * p.vs_s] : 1.0f;
   const float qk_scale = p.scale * ks;
 
   // scores: token i on the 16 lanes of slot i % 16, channels sub, sub + 16, ...
@@ -132,8 +135,12 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(P p) {
         }
       }
     }
+    float row_scale = qk_scale;
+    if constexpr (kBlocks<P>) {
+      if (blk_ok) row_scale *= p.k_scale[blk * p.ks_b + h * p.ks_s];
+    }
     if (sub == 0 && tok_ok)
-      for (int g = 0; g < G; ++g) sc[g * PT + i] = blk_ok ? sc[g * PT + i] * qk_scale : -INFINITY;
+      for (int g = 0; g < G; ++g) sc[g * PT + i] = blk_ok ? sc[g * PT + i] * row_scale : -INFINITY;
   }
   __syncthreads();
   if constexpr (kKeeps<P>) {
@@ -195,6 +202,14 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(P p) {
         float v16[16];
         load16<KT>(vbase + blk * p.v_s[0] + (int64_t)h * p.v_s[2] + (int64_t)d * p.v_s[3], v16);
         const int t0 = bi * 16;
+        if constexpr (kBlocks<P>) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (t0 + e < count) sum = fmaf(sc[g * PT + t0 + e], v16[e], sum);
+          acc = fmaf(sum, p.v_scale[blk * p.vs_b + h * p.vs_s], acc);
+          continue;
+        }
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (t0 + e < count) acc = fmaf(sc[g * PT + t0 + e], v16[e], acc);
@@ -217,6 +232,9 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(P p) {
           const float x = KE::load(vrow + (int64_t)d * p.v_s[3]);
           vv[u] = ok ? x : 0.0f;
           ww[u] = ok ? sc[g * PT + tt] : 0.0f;
+          if constexpr (kBlocks<P>) {
+            if (ok) vv[u] *= p.v_scale[blk * p.vs_b + h * p.vs_s];
+          }
         }
 #pragma unroll
         for (int u = 0; u < kU; ++u) acc = fmaf(ww[u], vv[u], acc);
@@ -416,6 +434,13 @@ int32_t launch_decode_generic(const DecodeParams& p, int q_dt, int kv_dt, hipStr
 
 int32_t launch_decode_generic(const DecodeWeightsParams& p, int q_dt, int kv_dt, hipStream_t stream) {
   return launch_generic_any(p, q_dt, kv_dt, stream);
+}
+
+int32_t launch_decode_generic(const DecodeBlockParams& p, int q_dt, int kv_dt, hipStream_t stream) {
+  const bool i8 = kv_dt == kI8;
+  if (q_dt == kF32) return i8 ? launch_generic_t<kF32, kI8>(p, stream) : launch_generic_t<kF32, kE4M3>(p, stream);
+  if (q_dt == kF16) return i8 ? launch_generic_t<kF16, kI8>(p, stream) : launch_generic_t<kF16, kE4M3>(p, stream);
+  return i8 ? launch_generic_t<kBF16, kI8>(p, stream) : launch_generic_t<kBF16, kE4M3>(p, stream);
 }
 
 int32_t launch_decode_reduce(const DecodeParams& p, int q_dt, hipStream_t stream) {

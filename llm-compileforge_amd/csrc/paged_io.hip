@@ -9,7 +9,8 @@
 // [0, NB * bs) are skipped.
 //
 // paged_gather: out[r, s] = the row of token s of table r (block
-// tables[r][s / bs], offset s % bs), dequantized (e4m3fn: code * scale[h]);
+// tables[r][s / bs], offset s % bs), dequantized (e4m3fn: code * scale[h], or with
+// a scale for each block and head, as int8 too, code * scale[block, h]);
 // a table entry outside [0, NB) gives zeros (the reference gathers a
 // request's blocks in table order and leaves positions past its table zero,
 // cache_manager.py:173-197).
@@ -50,6 +51,10 @@ template <int DT>
 constexpr int esize() {
   return (int)sizeof(typename Elem<DT>::T);
 }
+// Dtypes whose values are codes times a scale.
+template <int DT>
+constexpr bool kScaled = DT == kE4M3 || DT == kI8;
+
 template <int A, int B>
 constexpr int piece_channels() {
   return 16 / (esize<A>() > esize<B>() ? esize<A>() : esize<B>());
@@ -278,8 +283,8 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(PagedGatherParams p, 
     if constexpr (N == 1) f[0] = load_as_f32<CT>(p.cache, co);
     else if (VEC || cvec) load_piece<CT, N>(p.cache, co, f);
     else load_strided<CT, N>(p.cache, co, p.c_s[3], f);
-    if constexpr (CT == kE4M3) {
-      const float sc = p.scale[h * p.sc_s];
+    if constexpr (kScaled<CT>) {
+      const float sc = p.scale[blk * p.sc_b + h * p.sc_s];
 #pragma unroll
       for (int e = 0; e < N; ++e) f[e] *= sc;
     }
@@ -333,7 +338,7 @@ __global__ __launch_bounds__(256) void paged_gather_tile_kernel(PagedGatherParam
 #pragma unroll
       for (int q = 0; q < esize<CT>(); ++q) in.q[k][q] = ((const uint4*)(src + k * p.c_s[3]))[q];
   }
-  const float sc = CT == kE4M3 ? p.scale[h * p.sc_s] : 1.0f;
+  const float sc = kScaled<CT> && blk >= 0 ? p.scale[blk * p.sc_b + h * p.sc_s] : 1.0f;
   const int ns = min(16, p.S - s0);
   O* out = (O*)p.out + (int64_t)r * p.o_s[0] + (int64_t)s0 * p.o_s[1] + (int64_t)h * p.o_s[2] + d;
 #pragma unroll
@@ -343,7 +348,7 @@ __global__ __launch_bounds__(256) void paged_gather_tile_kernel(PagedGatherParam
 #pragma unroll
       for (int k = 0; k < P; ++k) {
         float f = blk >= 0 ? Elem<CT>::load(&in.c[k][t]) : 0.0f;
-        if constexpr (CT == kE4M3) f = blk >= 0 ? f * sc : 0.0f;
+        if constexpr (kScaled<CT>) f = blk >= 0 ? f * sc : 0.0f;
         Elem<OT>::store(&v[k], f);
       }
       if constexpr (P * sizeof(O) == 4) *(uint32_t*)(out + (int64_t)t * p.o_s[1]) = __builtin_bit_cast(uint32_t, v);
@@ -491,7 +496,7 @@ int32_t launch_gather_t(const PagedGatherParams& p, hipStream_t stream) {
   // Channels per thread of the tile kernel: 4 bytes of output, but one of
   // e4m3fn codes, whose conversion is the thread's time (4,000 rows of 8 heads
   // of 128 to bf16: 7.9 us by two channels, 7.1 by one; 32 rows 6.6, 4.7).
-  constexpr int P = esize<OT>() == 4 || CT == kE4M3 ? 1 : 2;
+  constexpr int P = esize<OT>() == 4 || kScaled<CT> ? 1 : 2;
   if (values >= tile_gather_values<CT>() && channel_tiles(p.cache, p.c_s, p.bs, esize<CT>()) && p.D % P == 0 &&
       (int64_t)p.H * p.D < INT32_MAX && rows_aligned(p.out, p.o_s, 3, p.o_s[3], esize<OT>(), P * esize<OT>())) {
     const int64_t bpr = ceil_div(p.S, 16), blocks = blocks_of((int64_t)p.R * bpr * (p.H * p.D / P));
@@ -536,6 +541,7 @@ int32_t launch_paged_gather(const PagedGatherParams& p, int cache_dt, int out_dt
     case kF16: return launch_gather_o<kF16>(p, out_dt, stream);
     case kBF16: return launch_gather_o<kBF16>(p, out_dt, stream);
     case kE4M3: return launch_gather_o<kE4M3>(p, out_dt, stream);
+    case kI8: return launch_gather_o<kI8>(p, out_dt, stream);
   }
   set_error("paged gather: unsupported cache dtype %d", cache_dt);
   return CF_ERR_UNSUPPORTED;

@@ -39,6 +39,11 @@ struct PrefillParams {
   int workers;      // direct launches: resident workgroups of the item kernel, at most the slots
 };
 
+// A call over a cache with a scale for each block and head.
+struct PrefillBlockParams : PrefillParams {
+  int64_t ks_b, vs_b;  // strides over blocks of k_scale and v_scale [NB, Hkv] (ks_s, vs_s: over heads)
+};
+
 // Query rows per work item for GQA group G.
 int prefill_rows_per_item(int G);
 bool prefill_supported(const PrefillParams& p, int q_dt, int kv_dt);
@@ -47,5 +52,7 @@ uint64_t prefill_workspace_bytes(int64_t Tq, int64_t N, int64_t Hq, int64_t Hkv,
 // more.  Less than prefill_workspace_bytes() is a queued launch.
 uint64_t prefill_bind_workspace(PrefillParams& p, void* workspace, uint64_t bytes);
 int32_t launch_prefill(PrefillParams& p, int q_dt, int kv_dt, hipStream_t stream);
+int32_t launch_prefill_e4m3(PrefillBlockParams& p, int q_dt, hipStream_t stream);
+int32_t launch_prefill_i8(PrefillBlockParams& p, int q_dt, hipStream_t stream);
 
 }  // namespace cf

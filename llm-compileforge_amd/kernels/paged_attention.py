@@ -178,7 +178,9 @@ def paged_attention_tensors(
             min(seq_lens[b], Mb*block_size) tokens (0 gives a zero row).
         block_size: tokens per block (must equal k_cache.shape[1]).
         scale: softmax scale, default 1/sqrt(D).
-        k_scale, v_scale: dequant scales for float8_e4m3fn caches.
+        k_scale, v_scale: dequant scales for float8_e4m3fn caches, [Hkv] or
+            [1]; or [num_blocks, Hkv], one for each block and head, for
+            float8_e4m3fn and int8 caches (kernels.block_scaled_kv).
         shared_prefix_lens: optional int32 [B]; entry b = leading tokens of
             sequence b held in the same physical blocks as sequence b - 1's
             (cf_hip.ops.shared_prefix_lens computes it from host tables).
@@ -225,7 +227,8 @@ def paged_attention(
         seq_lens: request_id -> current sequence length.
         block_size: Tokens per KV block (default 16).
         scale: Attention scale (default 1/sqrt(head_dim)).
-        k_scale, v_scale: FP8 dequant scales (float8_e4m3fn caches only).
+        k_scale, v_scale: dequant scales of float8_e4m3fn caches, or of int8 ones
+            (as paged_attention_tensors takes them).
 
     Returns:
         dict mapping request_id -> output tensor [num_heads, head_dim].
@@ -335,6 +338,8 @@ def chunked_prefill_attention(
         seq_lens: int32 [N], tokens of each sequence including its chunk.
         q_start: int32 [N + 1]; chunk n owns q rows [q_start[n], q_start[n+1]).
         scale: softmax scale, default 1/sqrt(D).
+        k_scale, v_scale: as paged_attention_tensors, [num_blocks, Hkv] over
+            float8_e4m3fn or int8 caches under either type of queries.
 
     Row i of a chunk of L rows is the token at position seq_lens[n] - L + i
     and attends to positions [0, seq_lens[n] - L + i] (bottom-right causal;

@@ -17,6 +17,12 @@ Additions for the GPU path (no reference counterparts):
   returns the new tokens' slots plus the (old, new) copy-on-write pairs.
   `copy_blocks(pairs, caches)` performs those copies on the device for every
   cache tensor (each layer's K and V, or CacheManager slabs).
+- `fork(request, [new ids])` makes requests that continue another one (samples of
+  one prompt, beams): whole blocks shared, the partial last one copied for each.
+- `compact()` gives the blocks in use the lowest ids, each request's one after the
+  other, so that the pool's end is free and a request's blocks are read in order.
+- `move_blocks(moves, caches)` does what those two, and copy-on-write, ask for, over
+  every cache tensor at once and in place.
 - `bind_device(rows, cols)` keeps an int32 block table [rows, cols] and
   lengths [rows] on the GPU; `sync_device()` uploads only the cells that
   changed since the last sync (one small copy and one scatter kernel)
@@ -216,6 +222,42 @@ class BlockManager:
         pairs = torch.as_tensor(np.asarray(copies, dtype=np.int32)).to(dev)
         for c in caches:
             _ops.copy_blocks(c, pairs)
+
+    @staticmethod
+    def move_blocks(moves: np.ndarray | torch.Tensor, caches: Iterable[torch.Tensor]) -> None:
+        """Moves blocks of every cache tensor whose dim 0 is the block (as
+        copy_blocks takes them; one device), in place: moves [n, 2] of (source,
+        destination), on the host.  Each destination takes what its source held
+        before the call, also where it is a source itself; it is given once."""
+        _ops.move_blocks(caches, moves)
+
+    # ── fork and compaction ────────────────────────────────
+
+    def fork(self, request_id: str, new_ids: Iterable[str], tokens: int) -> np.ndarray:
+        """Requests `new_ids` that continue the first `tokens` tokens of another one:
+        they share its whole blocks, and each has a block of its own for a partial
+        last one.  Returns int32 [n, 2] of (old, new) blocks for move_blocks (or
+        copy_blocks).  KeyError for an unknown request, ValueError for an id that has
+        blocks already or more tokens than the request's blocks hold, RuntimeError
+        when the pool is exhausted (nothing is changed)."""
+        batch = RequestBatch(new_ids)
+        copies = np.empty((max(len(batch), 1), 2), dtype=np.int32)
+        n = ctypes.c_int64(0)
+        check(lib().cf_bp_fork(self._h, _b(request_id), len(batch), batch.c_ids, int(tokens), copies.ctypes.data,
+                               copies.shape[0], ctypes.byref(n)), "fork")
+        return copies[: n.value]
+
+    def compact(self) -> np.ndarray:
+        """New ids for the blocks in use: 0, 1, 2, ... along the requests' tables, by
+        device row and then by id; blocks that only a prefix cache holds come last.
+        Returns int32 [n, 2] of (old, new), for move_blocks over every cache before
+        anything reads or writes by the new tables (sync_device), and for
+        RadixCache.relocate."""
+        n = ctypes.c_int64(0)
+        check(lib().cf_bp_compact(self._h, None, 0, ctypes.byref(n)), "compact")
+        moves = np.empty((max(n.value, 1), 2), dtype=np.int32)
+        check(lib().cf_bp_compact(self._h, moves.ctypes.data, moves.shape[0], ctypes.byref(n)), "compact")
+        return moves[: n.value]
 
     # ── device-resident tables ─────────────────────────────
 

@@ -18,6 +18,8 @@ Block accounting, kept identical because callers depend on it:
   (the shared head keeps the first ceil(common / block_size) blocks, the
   tail the rest); the unmatched remainder becomes a leaf owning the
   remaining new blocks, each gaining one block-manager reference.
+- relocate maps the nodes' blocks after BlockManager.compact (no reference
+  counterpart).
 - evict frees, depth first and children before parents, nodes whose
   reference count is 0 until the target is met.
 """
@@ -137,6 +139,15 @@ class RadixCache:
             if freed >= target_blocks:
                 break
         return freed
+
+    def relocate(self, moves: Any) -> None:
+        """Follows moves [n, 2] of (old, new) block ids, all at once."""
+        now = {int(old): int(new) for old, new in moves}
+        stack = [self.root]
+        while stack:
+            node = stack.pop()
+            node.kv_blocks = [now.get(b, b) for b in node.kv_blocks]
+            stack += node.children.values()
 
     def _add_leaf(self, parent: RadixTreeNode, token_ids: tuple[int, ...], kv_blocks: list[int]) -> None:
         node = RadixTreeNode(token_ids)

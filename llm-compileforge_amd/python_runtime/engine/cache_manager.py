@@ -33,6 +33,10 @@ what moves them:
   token's attention weight to an account given to them; evict_rows cuts
   requests to a budget of tokens by those accounts.
 
+- With block_scaled (no reference counterpart) the paged slabs are held in 8 bits
+  with a scale for each block, layer and head: write_rows quantizes a step's rows
+  by them, the attention methods read them, and nothing is calibrated.
+
 Every I/O method runs on the GPU through libcf_hip.so and raises if the
 slab is not on a GPU or the library is missing; there is no CPU path.
 """
@@ -118,6 +122,10 @@ def _dtype_from_str(name: str) -> torch.dtype:
         "fp8_e4m3": torch.float8_e4m3fn,
     }
     return mapping.get(name, torch.float32)
+
+
+# Types of paged slabs with a scale for each block, layer and head.
+_BLOCK_SCALED = {"float8_e4m3fn": torch.float8_e4m3fn, "int8": torch.int8}
 
 
 # Host-side addressing: pure functions, no device work.
@@ -257,10 +265,18 @@ class CacheManager:
             FP8 slabs take their scales from it (1.0 where absent).
         num_blocks: physical blocks per paged slab.
         device: where the slabs live (default: the current GPU).
+        block_scaled: "float8_e4m3fn" or "int8" holds the paged slabs in that
+            type, whatever the policy's, with a scale for each block, layer and
+            head (kernels.block_scaled_kv).  Rows are then written by write_rows,
+            which widens the scales; the methods that write single slots, move
+            rows or keep accounts refuse such slabs.
     """
 
-    def __init__(self, policy: Any, num_blocks: int, device: torch.device | str | None = None) -> None:
+    def __init__(self, policy: Any, num_blocks: int, device: torch.device | str | None = None, *,
+                 block_scaled: str | None = None) -> None:
         policy = _as_policy(policy)
+        if block_scaled is not None and block_scaled not in _BLOCK_SCALED:
+            raise ValueError(f"block_scaled must be one of {sorted(_BLOCK_SCALED)}, got {block_scaled!r}")
         if device is None:
             if not torch.cuda.is_available():
                 raise RuntimeError("CacheManager needs a GPU (no device given and none is visible)")
@@ -275,6 +291,8 @@ class CacheManager:
         self._specs: dict[str, Any] = {}
         self._roles: dict[str, str] = {}
         self._scales: dict[str, torch.Tensor] = {}
+        self._block_scaled = block_scaled
+        self._block_scales: dict[str, torch.Tensor] = {}  # [NB, L, H] of each paged slab
         self._layer_counters: dict[str, int] = {}
         self._block_tables: dict[str, list[int]] = {}
         self._cover: np.ndarray | None = None
@@ -287,6 +305,10 @@ class CacheManager:
             self._roles[spec.name] = _slab_role(spec, intercepts)
             self._slabs[spec.name] = self._allocate_slab(spec)
             self._layer_counters[spec.name] = 0
+            if block_scaled is not None and spec.slab_type == "paged":
+                self._block_scales[spec.name] = torch.zeros(self._num_blocks, spec.num_layers, spec.num_heads,
+                                                            dtype=torch.float32, device=self._device)
+                continue
             if self._slabs[spec.name].dtype == torch.float8_e4m3fn:
                 shape = (max(spec.num_layers, 1), max(spec.num_heads, 1))
                 stored = list(getattr(spec, "scales", []))
@@ -302,6 +324,8 @@ class CacheManager:
 
     def _allocate_slab(self, spec: Any) -> torch.Tensor:
         dtype = _dtype_from_str(spec.dtype)
+        if self._block_scaled is not None and spec.slab_type == "paged":
+            dtype = _BLOCK_SCALED[self._block_scaled]
         nb, L, bs, H, D = self._num_blocks, spec.num_layers, self._block_size, spec.num_heads, spec.head_dim
         if spec.slab_type == "paged":
             role = self._roles[spec.name]
@@ -351,7 +375,7 @@ class CacheManager:
     def kv_scales(self, slab_id: str) -> torch.Tensor:
         """Per-(layer, head) float32 dequant scales [L, H] of an FP8 slab."""
         if slab_id not in self._scales:
-            raise ValueError(f"slab {slab_id!r} is not an FP8 slab")
+            raise ValueError(f"slab {slab_id!r} is not an FP8 slab with a scale for each head")
         return self._scales[slab_id]
 
     def set_kv_scales(self, slab_id: str, scales: torch.Tensor, layer_idx: int | None = None) -> None:
@@ -376,6 +400,23 @@ class CacheManager:
         self.kv_scales(slab_id)[layer_idx].copy_(sc.reshape(-1))
         return sc
 
+    def block_scales(self, slab_id: str) -> torch.Tensor:
+        """Scales [num_blocks, L, H] (float32) of a block-scaled slab."""
+        if slab_id not in self._block_scales:
+            raise ValueError(f"slab {slab_id!r} has no block scales")
+        return self._block_scales[slab_id]
+
+    def _layer_scales(self, slab_id: str, layer_idx: int) -> torch.Tensor | None:
+        """A layer's scales as the attention takes them: [H], [num_blocks, H] or None."""
+        if slab_id in self._block_scales:
+            return self._block_scales[slab_id][:, layer_idx]
+        return self._scales[slab_id][layer_idx] if slab_id in self._scales else None
+
+    def _no_block_scales(self, what: str, *slab_ids: str) -> None:
+        for slab_id in slab_ids:
+            if slab_id in self._block_scales:
+                raise NotImplementedError(f"{what} does not take block-scaled slabs ({slab_id!r})")
+
     # Writing and reading K/V rows through block tables.
 
     def layer_view(self, slab_id: str, layer_idx: int) -> torch.Tensor:
@@ -390,6 +431,7 @@ class CacheManager:
         positions raise ValueError); positions already on the GPU are
         resolved there, and uncovered or negative ones are skipped without a
         warning, which would need a device sync."""
+        self._no_block_scales("write_paged", slab_id)
         slab = self._slabs[slab_id]
         bt = self._block_tables
         if not bt or slab is None:
@@ -419,7 +461,7 @@ class CacheManager:
     def read_paged(self, slab_id: str, layer_idx: int, max_seq_len: int) -> torch.Tensor:
         """Dense [requests, max_seq_len, heads, dim] rows of this step's
         requests (sorted request-id order, zeros past a table), in the slab
-        dtype (float32 for an FP8 slab)."""
+        dtype (float32 for an FP8 or block-scaled slab)."""
         slab = self._slabs[slab_id]
         if slab is None or not self._block_tables:
             raise RuntimeError("Paged slab read requested without active block tables")
@@ -433,7 +475,7 @@ class CacheManager:
             valid = (ids >= 0) & (s // bs < tables.shape[1])
             rows = view[ids.clamp(min=0), (s % bs).expand_as(ids)]
             return torch.where(valid[..., None, None], rows, torch.zeros((), dtype=rows.dtype, device=rows.device))
-        sc = self._scales[slab_id][layer_idx] if slab_id in self._scales else None
+        sc = self._layer_scales(slab_id, layer_idx)
         return _ops.paged_gather(view, tables, int(max_seq_len), scale=sc)
 
     # Decode and chunked-prefill attention straight over the slabs.
@@ -473,8 +515,8 @@ class CacheManager:
                 raise ValueError(f"attend: sequence length {s} outside the table's {n * bs} slots")
         kv = self.layer_view(k_slab, layer_idx)
         vv = self.layer_view(v_slab, layer_idx)
-        ks = self._scales[k_slab][layer_idx] if k_slab in self._scales else None
-        vs = self._scales[v_slab][layer_idx] if v_slab in self._scales else None
+        ks = self._layer_scales(k_slab, layer_idx)
+        vs = self._layer_scales(v_slab, layer_idx)
         if scale is None:
             scale = 1.0 / math.sqrt(q.shape[-1])
         dev = self._device
@@ -497,6 +539,7 @@ class CacheManager:
         """Writes token rows at explicit slots (block * block_size + offset),
         e.g. those BlockManager.prepare_writes returns; negative slots are
         skipped."""
+        self._no_block_scales("write_slots", slab_id)
         spec = self._specs[slab_id]
         rows = normalize_kv(data, spec.num_heads, spec.head_dim)
         if rows.dim() != 3:
@@ -516,6 +559,30 @@ class CacheManager:
             return
         sc = self._scales[slab_id][layer_idx] if slab_id in self._scales else None
         _ops.paged_write(rows, slots, view, sc)
+
+    def write_rows(
+        self,
+        k_new: torch.Tensor,
+        v_new: torch.Tensor,
+        layer_idx: int,
+        block_tables: torch.Tensor,
+        seq_lens: torch.Tensor,
+        q_start: torch.Tensor | None = None,
+        k_slab: str = "k",
+        v_slab: str = "v",
+    ) -> None:
+        """Writes a step's new rows into block-scaled slabs: k_new, v_new [T, heads,
+        dim] at the last positions of their sequences, over the tables and lengths
+        that attend_rows or attend_chunks then takes (BlockManager.prepare_writes
+        first makes the blocks the requests' own).  q_start int32 [rows + 1] says
+        which rows are whose; without it row n is table row n's, none where its
+        length is 0 (kernels.block_scaled_kv.write_kv_blocks)."""
+        for slab in (k_slab, v_slab):
+            if slab not in self._block_scales:
+                raise ValueError(f"write_rows: slab {slab!r} is not block-scaled (write_slots writes it)")
+        _ops.kv_write_blocks(k_new, v_new, block_tables, seq_lens, self.layer_view(k_slab, layer_idx),
+                             self.layer_view(v_slab, layer_idx), self._layer_scales(k_slab, layer_idx),
+                             self._layer_scales(v_slab, layer_idx), q_start)
 
     def attend_rows(
         self,
@@ -539,11 +606,12 @@ class CacheManager:
         held was multiplied by `decay` (kernels.paged_attention_weights)."""
         kv = self.layer_view(k_slab, layer_idx)
         vv = self.layer_view(v_slab, layer_idx)
-        ks = self._scales[k_slab][layer_idx] if k_slab in self._scales else None
-        vs = self._scales[v_slab][layer_idx] if v_slab in self._scales else None
+        ks = self._layer_scales(k_slab, layer_idx)
+        vs = self._layer_scales(v_slab, layer_idx)
         if scale is None:
             scale = 1.0 / math.sqrt(q.shape[-1])
         if weights is not None:
+            self._no_block_scales("attend_rows with weights", k_slab, v_slab)
             return _ops.paged_decode_weights(q, kv, vv, block_tables, seq_lens, weights, float(scale),
                                              self._block_size, decay, k_scale=ks, v_scale=vs, out=out,
                                              shared_prefix_lens=shared_prefix_lens)
@@ -577,13 +645,15 @@ class CacheManager:
         row n of `block_tables` is (a caller with accounts in the order of
         other rows gathers and scatters them), and `out` must not be q, from
         which the accounts are formed after the attention."""
+        if weights is not None:
+            self._no_block_scales("attend_chunks with weights", k_slab, v_slab)
         if weights is not None and out is not None and out.data_ptr() == q.data_ptr():
             raise ValueError("out must not be q in a call with weights: the accounts are formed from the queries "
                              "after the attention has been written")
         kv = self.layer_view(k_slab, layer_idx)
         vv = self.layer_view(v_slab, layer_idx)
-        ks = self._scales[k_slab][layer_idx] if k_slab in self._scales else None
-        vs = self._scales[v_slab][layer_idx] if v_slab in self._scales else None
+        ks = self._layer_scales(k_slab, layer_idx)
+        vs = self._layer_scales(v_slab, layer_idx)
         if scale is None:
             scale = 1.0 / math.sqrt(q.shape[-1])
         out = _ops.prefill_chunk(q, kv, vv, block_tables, seq_lens, q_start, float(scale), self._block_size,
@@ -618,12 +688,13 @@ class CacheManager:
         v_new [T, heads, dim], slots [T] as BlockManager.prepare_writes
         returns them (negative ones are skipped); the positions and the
         rotary's form as in kernels.rotary.rotary_cache_write."""
+        self._no_block_scales("write_rotary", k_slab, v_slab)
         if not (isinstance(slots, torch.Tensor) and slots.dim() == 1 and slots.device == self._device):
             slots = torch.as_tensor(slots).reshape(-1).to(self._device)
         kv = self.layer_view(k_slab, layer_idx)
         vv = self.layer_view(v_slab, layer_idx)
-        ks = self._scales[k_slab][layer_idx] if k_slab in self._scales else None
-        vs = self._scales[v_slab][layer_idx] if v_slab in self._scales else None
+        ks = self._layer_scales(k_slab, layer_idx)
+        vs = self._layer_scales(v_slab, layer_idx)
         return _ops.rotary_cache_write(q, k_new, v_new, positions, inv_freq, slots, kv, vv, sections, axis_order,
                                        interleaved, rotary_scale, k_scale=ks, v_scale=vs, out=out)
 
@@ -657,14 +728,17 @@ class CacheManager:
         BlockManager.prepare_writes([(request, 0, budget)]) and copy_blocks, for
         those requests alone (others keep what they share).  After truncate the
         request's next token goes to slot `budget`."""
+        self._no_block_scales("evict_rows", k_slab, v_slab)
         keep, new_lens = _ops.evict_select(weights, seq_lens, budget, sink, recent, positions, kept, seen)
         _ops.evict_move(keep, seq_lens, block_tables, self.layer_view(k_slab, layer_idx),
                         self.layer_view(v_slab, layer_idx), weights, positions, kept, seen)
         return new_lens
 
     def paged_slabs(self) -> list[torch.Tensor]:
-        """Every paged slab (all layers), e.g. for BlockManager.copy_blocks."""
-        return [t for name, t in self._slabs.items() if self._specs[name].slab_type == "paged"]
+        """Every paged slab (all layers) and, of block-scaled ones, the scales: what
+        goes with a block, e.g. for BlockManager.copy_blocks and move_blocks."""
+        slabs = [t for name, t in self._slabs.items() if self._specs[name].slab_type == "paged"]
+        return slabs + list(self._block_scales.values())
 
     # Fixed-size (per-slot) state slabs: [slots, layers, ...] rows.
 

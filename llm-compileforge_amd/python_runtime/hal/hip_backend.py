@@ -21,6 +21,12 @@ Ops:
                       k_scale, v_scale.  Returns [Tq, Hq, D].
   kv_cache_write_fp8  inputs [k_new, v_new, slot_mapping, key_cache,
                       value_cache, k_scale, v_scale]; returns key_cache.
+  kv_cache_write_blocks
+                      inputs [k_new, v_new, block_tables, seq_lens, key_cache,
+                      value_cache, k_scale, v_scale (, q_start)]: rows into caches
+                      with a scale for each block and head (paged_attention,
+                      chunked_prefill_attention and cache_read take those scales
+                      as k_scale / v_scale); returns key_cache.
   cache_write         the planned hal.cache_write (HALOps.td:195-199):
                       inputs [key, value, slot_mapping, key_cache,
                       value_cache]; caches of any float dtype and layout,
@@ -83,6 +89,7 @@ _ARITY: dict[str, tuple[int, int]] = {
     "paged_attention": (4, 5),
     "chunked_prefill_attention": (6, 6),
     "kv_cache_write_fp8": (7, 7),
+    "kv_cache_write_blocks": (8, 9),
     "cache_write": (5, 5),
     "cache_read": (3, 3),
     "scaled_dot_product_attention": (3, 4),
@@ -114,6 +121,7 @@ class HipBackend(OpExecutor):
             "paged_attention": self._paged_attention,
             "chunked_prefill_attention": self._chunked_prefill,
             "kv_cache_write_fp8": self._kv_cache_write_fp8,
+            "kv_cache_write_blocks": self._kv_cache_write_blocks,
             "cache_write": self._cache_write,
             "cache_read": self._cache_read,
             "scaled_dot_product_attention": self._sdpa,
@@ -200,6 +208,11 @@ class HipBackend(OpExecutor):
         _ops.kv_write_fp8(k_new, v_new, slots, k_cache, v_cache, k_scale, v_scale)
         return k_cache
 
+    def _kv_cache_write_blocks(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
+        from kernels.block_scaled_kv import write_kv_blocks
+
+        write_kv_blocks(*inputs[:8], q_start=inputs[8] if len(inputs) > 8 else kw.get("q_start"))
+        return inputs[4]
 
     def _cache_write(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
         key, value, slots, k_cache, v_cache = inputs
@@ -210,7 +223,8 @@ class HipBackend(OpExecutor):
     def _cache_read(self, inputs: list[Any], **kw: Any) -> torch.Tensor:
         k_cache, v_cache, table = inputs
         seq_len = int(kw.get("seq_len", table.shape[1] * k_cache.shape[1]))
-        dt = kw.get("out_dtype") or (torch.float32 if k_cache.dtype == torch.float8_e4m3fn else k_cache.dtype)
+        codes = k_cache.dtype in (torch.float8_e4m3fn, torch.int8)
+        dt = kw.get("out_dtype") or (torch.float32 if codes else k_cache.dtype)
         out = torch.empty(2, table.shape[0], seq_len, k_cache.shape[2], k_cache.shape[3], dtype=dt,
                           device=k_cache.device)
         _ops.paged_gather(k_cache, table, seq_len, scale=kw.get("k_scale"), out=out[0])
