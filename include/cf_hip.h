@@ -398,7 +398,8 @@ int32_t cf_kv_write_fp8(const CfTensor* k_new, const CfTensor* v_new,
  * of the attention calls that follow).  For each block that takes rows and each
  * head, with m the largest magnitude of those rows and s0 the block's scale (0 if
  * the first of them is at offset 0: what the block held before is then dropped):
- *     need = m / 127 (i8), or the least power of two >= m / 448 (e4m3fn);
+ *     need = m / 127 (i8), or the least power of two >= m / 448 (e4m3fn; both
+ *            quotients as float32 products with the rounded reciprocal);
  *     s1 = max(s0, need, 2^-40);
  *     codes of the new rows: x / s1 rounded to the nearest code, ties to even;
  *     if s1 is not s0, codes of the rows before them: code * s0 / s1, rounded.

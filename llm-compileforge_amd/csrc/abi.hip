@@ -603,7 +603,11 @@ static int32_t decode_call(const CfTensor* q, const CfTensor* k_cache, const CfT
   if (B == 0) return CF_OK;
 
   const DecodeParams& plain = p;
-  bool mfma = decode_mfma_supported(p, vq.dtype, vk.dtype);
+  DecodeBlockParams bp{};
+  static_cast<DecodeParams&>(bp) = plain;
+  bp.ks_b = ks_b;
+  bp.vs_b = vs_b;
+  bool mfma = decode_mfma_supported(p, vq.dtype, vk.dtype) && (!blocks || decode_mfma_block_scales(bp));
   // fp32 caches also run on the generic kernel.  It takes the calls that it is
   // faster for, those that ask for a partition length of their own (the MFMA
   // kernel has no partitions), and those whose workspace, or the fixed scratch,
@@ -634,10 +638,7 @@ static int32_t decode_call(const CfTensor* q, const CfTensor* k_cache, const CfT
 
   hipStream_t st = as_stream(stream);
   if (blocks) {
-    DecodeBlockParams bp{};
-    static_cast<DecodeParams&>(bp) = plain;
-    bp.ks_b = ks_b;
-    bp.vs_b = vs_b;
+    static_cast<DecodeParams&>(bp) = plain;  // (with its workspace)
     if (mfma) return launch_decode_mfma(bp, vq.dtype, vk.dtype, st);
     rc = launch_decode_generic(bp, vq.dtype, vk.dtype, st);
     if (rc) return rc;

@@ -4,7 +4,7 @@
 //
 // The scale of a block that holds values up to amax is the least that its codes
 // can reach them with: amax / 127 for int8, and for e4m3fn the next power of two
-// from amax / 448 on.  A floating-point code loses no precision by it (its steps
+// from amax / 448 on (quotients as products with the rounded reciprocal).  A floating-point code loses no precision by it (its steps
 // are relative; the smallest normal one is 2^14 below amax in either case), the
 // division by it is exact, and where a later row widens the block's scale, the
 // codes already there move by whole exponents and are exact still, unless they
@@ -27,11 +27,9 @@ template <int CT>
 __device__ __forceinline__ float least_scale(uint32_t amax) {
   if (amax >= 0x7F800000u) return u2f(0x7FC00000u);
   if constexpr (CT == kI8) {
-    return fmaxf(u2f(amax) / 127.0f, kLeastScale);
+    return fmaxf(u2f(amax) * (1.0f / 127.0f), kLeastScale);
   } else {
-    // (the quotient is above a power of two exactly where amax / 448 is: 448 *
-    // 2^k and its neighbours are 2^-23 / 1.75 apart, more than half a step of 1)
-    const uint32_t a = f2u(fmaxf(u2f(amax) / 448.0f, kLeastScale));
+    const uint32_t a = f2u(fmaxf(u2f(amax) * (1.0f / 448.0f), kLeastScale));
     return u2f((a + 0x7FFFFFu) & 0x7F800000u);
   }
 }

@@ -2,8 +2,14 @@
 //
 // A tile of 32 tokens is two blocks, and the QK^T product leaves a lane the scores
 // of 8 tokens of one of them: its K scale multiplies them, its V scale their
-// weights ahead of the product with V.  Two 4-byte loads a lane and tile, and 8
-// multiplications.
+// weights ahead of the product with V: two 4-byte loads a lane and tile, 8
+// multiplications, and P in two bf16 terms.  Bound by HBM as the kernel with a scale
+// a head: 64 sequences of 1,024 to 8,192 tokens, half of them on a shared prefix
+// (528 MB, e4m3, 32 / 8 heads of 128), DECODE_FP8 us against 93 without scales to
+// load; int8, whose codes take 12 instructions where 8 e4m3 codes take 4, DECODE_I8
+// us for 456 MB.
+#include <algorithm>
+
 #include "decode_stream.hpp"
 
 namespace cf {
@@ -17,6 +23,11 @@ int32_t launch_kt(const DecodeBlockParams& p, int q_dt, hipStream_t stream) {
 }
 
 }  // namespace
+
+bool decode_mfma_block_scales(const DecodeBlockParams& p) {
+  const int64_t most = std::max((p.NB - 1) * p.ks_b + (p.Hkv - 1) * p.ks_s, (p.NB - 1) * p.vs_b + (p.Hkv - 1) * p.vs_s);
+  return most < ((int64_t)1 << 31);
+}
 
 int32_t launch_decode_mfma(const DecodeBlockParams& p, int q_dt, int kv_dt, hipStream_t stream) {
   return kv_dt == kI8 ? launch_kt<kI8>(p, q_dt, stream) : launch_kt<kE4M3>(p, q_dt, stream);

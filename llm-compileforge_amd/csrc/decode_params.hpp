@@ -88,6 +88,8 @@ int32_t launch_decode_generic(const DecodeWeightsParams& p, int q_dt, int kv_dt,
 int32_t launch_decode_mfma(const DecodeWeightsParams& p, int q_dt, int kv_dt, hipStream_t stream);
 int32_t launch_decode_weights(const DecodeWeightsParams& p, bool log2_units, hipStream_t stream);
 bool decode_mfma_supported(const DecodeParams& p, int q_dt, int kv_dt);
+// Whether its scales' offsets are what the MFMA kernel takes (32 bits).
+bool decode_mfma_block_scales(const DecodeBlockParams& p);
 // Workspace of the MFMA path: two (m, l, o) partial slots per launched wave.
 uint64_t decode_mfma_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim);
 void decode_mfma_bind_workspace(DecodeParams& p, void* workspace);

@@ -537,16 +537,25 @@ __device__ __forceinline__ uint4 codes_to_16(uint32_t lo, uint32_t hi) {
     return F16 ? __builtin_bit_cast(uint4, e4m3x8_to_f16(lo, hi)) : __builtin_bit_cast(uint4, e4m3x8_to_bf16(lo, hi));
 }
 
+// The V operands of 8 codes: fp16, with block scales (BLK) times the power of two g.
+template <int KT, bool BLK>
+__device__ __forceinline__ uint4 v_to_16(uint32_t lo, uint32_t hi, float g) {
+  if constexpr (!BLK) return codes_to_16<KT, true>(lo, hi);
+  else if constexpr (KT == kI8) return __builtin_bit_cast(uint4, i8x8_to_f16(lo, hi, g));
+  else return __builtin_bit_cast(uint4, e4m3x8_to_f16(lo, hi, g));
+}
+
 // Converts the staged registers and writes them in operand order: K entry
 // (chain s, step c, lane) = the 8 channels lane (li, lq) feeds step c of
 // chain s; V entry (step t, lane) = channel 16 t + li, tokens 8 lq .. 8 lq + 7.
 // V tokens at or past `valid` (tile-relative) or in an invalid block become
 // zero (cache slots there may hold any bits, NaN codes included).
-// BLK: a cache with block scales, whose V operands are bf16 (fp16 otherwise).
+// BLK: a cache with block scales, whose V codes are staged times ga (the tile's
+// first block) and gb.
 // FULL: the caller knows every token of the tile is valid.
 template <int QT, int KT, int D, bool VTOK, bool BLK, bool FULL = false>
 __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const uint4* vr, const TileIds& t,
-                                            int valid, int tid) {
+                                            int valid, int tid, float ga = 1.0f, float gb = 1.0f) {
   using Gm = Geo<KT, D>;
 #pragma unroll
   for (int i = 0; i < Gm::KPT; ++i) {
@@ -584,8 +593,8 @@ __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const u
         const uint4 v = make_uint4(vr[i].x & km, vr[i].y & km, vr[i].z & km, vr[i].w & km);
         uint8_t* row = rows + vtok_slot(16 * X + r) * Gm::VRS;
         if constexpr (Gm::KB == 1) {
-          *(uint4*)(row + 32 * c) = codes_to_16<KT, !BLK>(v.x, v.y);
-          *(uint4*)(row + 32 * c + 16) = codes_to_16<KT, !BLK>(v.z, v.w);
+          *(uint4*)(row + 32 * c) = v_to_16<KT, BLK>(v.x, v.y, uniform(X) ? gb : ga);
+          *(uint4*)(row + 32 * c + 16) = v_to_16<KT, BLK>(v.z, v.w, uniform(X) ? gb : ga);
         } else {
           *(uint4*)(row + 16 * c) = v;
         }
@@ -603,8 +612,8 @@ __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const u
       const int li = d & 15, tt = d >> 4;
       if (full) {
         if constexpr (Gm::KB == 1) {
-          vl[tt * 64 + 32 * X + li] = codes_to_16<KT, !BLK>(vr[i].x, vr[i].y);
-          vl[tt * 64 + 32 * X + 16 + li] = codes_to_16<KT, !BLK>(vr[i].z, vr[i].w);
+          vl[tt * 64 + 32 * X + li] = v_to_16<KT, BLK>(vr[i].x, vr[i].y, uniform(X) ? gb : ga);
+          vl[tt * 64 + 32 * X + 16 + li] = v_to_16<KT, BLK>(vr[i].z, vr[i].w, uniform(X) ? gb : ga);
         } else {
           vl[tt * 64 + 32 * X + 16 * part + li] = vr[i];
         }
@@ -612,8 +621,8 @@ __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const u
         const int n0 = ok ? valid - 16 * X : 0;  // valid tokens among this load's 16
         const uint2 lo = keep_bytes(make_uint2(vr[i].x, vr[i].y), n0);
         const uint2 hi = keep_bytes(make_uint2(vr[i].z, vr[i].w), n0 - 8);
-        vl[tt * 64 + 32 * X + li] = codes_to_16<KT, !BLK>(lo.x, lo.y);
-        vl[tt * 64 + 32 * X + 16 + li] = codes_to_16<KT, !BLK>(hi.x, hi.y);
+        vl[tt * 64 + 32 * X + li] = v_to_16<KT, BLK>(lo.x, lo.y, uniform(X) ? gb : ga);
+        vl[tt * 64 + 32 * X + 16 + li] = v_to_16<KT, BLK>(hi.x, hi.y, uniform(X) ? gb : ga);
       } else {
         const int n0 = ok ? valid - 16 * X - 8 * part : 0;
         vl[tt * 64 + 32 * X + 16 * part + li] = mask_tokens(vr[i], n0);
@@ -685,6 +694,21 @@ __device__ __forceinline__ LaneScales load_scales(const Pm& p, const float* __re
 __device__ __forceinline__ bool finite_scales(const LaneScales& s) {
   return __builtin_fmaxf(__builtin_fabsf(s.k), __builtin_fabsf(s.v)) < INFINITY && s.k == s.k && s.v == s.v;
 }
+// A V scale is 2^e * f with f in [1, 2).  2^e goes to the codes as they are staged,
+// against a reference 2^eref that is the largest of the item's blocks so far (O is
+// in its units and follows it), kVHead binades below fp16's largest: a block of 2^-21
+// (e4m3; int8 2^-28) of the largest before it keeps every bit of its codes.  f goes
+// to the exponent of the tile's weights, and the row sums take 1 / f of it back: the
+// P.V product against a channel of ones has 1 / f in their place, as two fp16 terms
+// in rows 0 and 1.  So a weight is rounded to fp16 once, as without block scales, and
+// a tile costs about 14 vector instructions more (V's scale multiplied into P, P in
+// two bf16 terms and row sums by addition: CHUNK_V1 us for eight 512-row chunks
+// over int8 against CHUNK_V2).
+template <int KT>
+constexpr int kVHead = KT == kI8 ? 5 : 7;
+__device__ __forceinline__ int exponent_of(float v) { return (int)((f2u(v) >> 23) & 0xFFu) - 127; }
+__device__ __forceinline__ float power_of_two(int e) { return u2f((uint32_t)min(max(e + 127, 0), 254) << 23); }
+
 // The tile's blocks that are valid and have finite scales, as bits.
 __device__ __forceinline__ int finite_blocks(const TileIds& t, const LaneScales& s) {
   const unsigned long long bad = __ballot(!finite_scales(s));
@@ -806,8 +830,6 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
     if (qk_scale == 0.0f) qk_scale = 1.17549435e-38f;
 
     float m[2] = {-INFINITY, -INFINITY};
-    float lsum[2] = {0.0f, 0.0f};  // block scales: row sums by lane
-    (void)lsum;
     f32x4_t o[2][NV];
     // Row sums come from the PV MFMAs: an extra V tile whose channel 0 is all
     // ones gives O[column][0] = sum of P (lane (li, lq = 0), element 0).
@@ -834,18 +856,34 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
     LaneScales sc0 = load_scales(p, kscale, vscale, id0, h, lq), sc1 = load_scales(p, kscale, vscale, id1, h, lq);
     (void)sc0;
     (void)sc1;
+    // V's reference exponent of tiles j and j + 1 (eref0, eref1), and O's (eo)
+    int eref0 = -127, eo = -127;
+    auto stage_scales = [&](const TileIds& idv, const LaneScales& sc, int& eref, float& ga, float& gb) {
+      const float va = u2f(__builtin_amdgcn_readlane(f2u(sc.v), 0)), vb = u2f(__builtin_amdgcn_readlane(f2u(sc.v), 32));
+      const int ea = (idv.ok & 1) ? exponent_of(va) : -127, eb = (idv.ok & 2) ? exponent_of(vb) : -127;
+      eref = max(eref, max(ea, eb));
+      ga = power_of_two(ea - eref + kVHead<KT>);
+      gb = power_of_two(eb - eref + kVHead<KT>);
+    };
+    (void)stage_scales;
     if (jt0 < nt) {
       stage_load<KT, D, VTOK>(kr, vr, p, id0, h, tid);
       TileIds idv = id0;
-      if constexpr (kBlocks<Pm>) idv.ok = finite_blocks(id0, sc0);
-      stage_write<QT, KT, D, VTOK, kBlocks<Pm>>(lds[0], kr, vr, idv, kvlen - 32 * jt0, tid);
+      float ga = 1.0f, gb = 1.0f;
+      if constexpr (kBlocks<Pm>) {
+        idv.ok = finite_blocks(id0, sc0);
+        stage_scales(idv, sc0, eref0, ga, gb);
+        eo = eref0;
+      }
+      stage_write<QT, KT, D, VTOK, kBlocks<Pm>>(lds[0], kr, vr, idv, kvlen - 32 * jt0, tid, ga, gb);
     }
+    int eref1 = eref0;
     if (jt0 + 1 < nt) stage_load<KT, D, VTOK>(kr, vr, p, id1, h, tid);
     __syncthreads();
 
     // P in fp16 against fp16 V operands (e4m3 V converts exactly; fp16 V as
     // is); against bf16 V as bf16 hi + lo
-    using POp = typename std::conditional<KT == kBF16 || kBlocks<Pm>, bf16x8_t, f16x8_t>::type;
+    using POp = typename std::conditional<KT == kBF16, bf16x8_t, f16x8_t>::type;
     using KOp = QOp<QT>;
 
     // The tile's math per column tile k, in pieces the step below orders so
@@ -896,8 +934,7 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
       const float mnew = mt > m[k] + 8.0f ? mt : m[k];
       const float alpha = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[k] - mnew);
-      if constexpr (kBlocks<Pm>) lsum[k] *= alpha;
-      else ol[k] = ol[k] * alpha;
+      ol[k] = ol[k] * alpha;
 #pragma unroll
       for (int t = 0; t < NV; ++t) o[k][t] = o[k][t] * alpha;
       m[k] = mnew;
@@ -908,20 +945,13 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       constexpr int k = decltype(kc)::value;
       return m[k] == -INFINITY ? 0.0f : m[k];
     };
-    auto probs = [&](auto kc, const f32x4_t& s1, const f32x4_t& s2, float qk_scale, float mref, POp& pk, POp& pl) {
-      constexpr int k = decltype(kc)::value;
-      (void)k;
+    // (mref: less log2 f with block scales)
+    auto probs = [&](const f32x4_t& s1, const f32x4_t& s2, float qk_scale, float mref, POp& pk, POp& pl) {
 #pragma unroll
       for (int v = 0; v < 8; ++v) {
         const float sv = v < 4 ? s1[v] : s2[v - 4];
         const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(sv, qk_scale, -mref));
-        if constexpr (kBlocks<Pm>) {
-          lsum[k] += pv;
-          const float ps = pv * sc0.v;
-          const __bf16 hi = (__bf16)ps;
-          pk[v] = hi;
-          pl[v] = (__bf16)(ps - (float)hi);
-        } else if constexpr (KT != kBF16) {
+        if constexpr (KT != kBF16) {
           pk[v] = (_Float16)pv;
         } else {
           const __bf16 hi = (__bf16)pv;
@@ -948,17 +978,13 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
     (void)not_finite;
     // O^T += V^T P^T for column tile k; the row sums come out of the same
     // pipe as O[column][0] against a V tile whose channel 0 is all ones.
+    _Float16 finv = (_Float16)0.0f;  // block scales: a term of 1 / f in rows 0 and 1, 0 in the others
+    (void)finv;
     auto pv = [&](auto kc, const uint4* vraw, const POp& pk, const POp& pl) {
       constexpr int k = decltype(kc)::value;
-      if constexpr (kBlocks<Pm>) {
-#pragma unroll
-        for (int t = 0; t < NV; ++t) {
-          const bf16x8_t vop = as_bf16x8(vraw[t]);
-          o[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, pk, o[k][t], 0, 0, 0);
-          o[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, pl, o[k][t], 0, 0, 0);
-        }
-      } else if constexpr (KT != kBF16) {
-        const _Float16 one = li == 0 ? (_Float16)1.0f : (_Float16)0.0f;
+      if constexpr (KT != kBF16) {
+        _Float16 one = li == 0 ? (_Float16)1.0f : (_Float16)0.0f;
+        if constexpr (kBlocks<Pm>) one = finv;
         const f16x8_t ones = {one, one, one, one, one, one, one, one};
         ol[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pk, ol[k], 0, 0, 0);
 #pragma unroll
@@ -978,7 +1004,7 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       }
     };
     // MFMAs of one column tile's P.V (or QK^T) product per batch below.
-    constexpr int kPvMfma = kBlocks<Pm> ? 2 * NV : (KT != kBF16 ? NV + 1 : 2 * NV + 2);
+    constexpr int kPvMfma = KT != kBF16 ? NV + 1 : 2 * NV + 2;
     constexpr int kQkMfma = 2 * NC;
 
     // One step: the next tile's registers go to the other LDS buffer and
@@ -996,8 +1022,10 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       TileIds idv = id1;
       LaneScales sc2;
       (void)sc2;
+      float ga = 1.0f, gb = 1.0f;
       if constexpr (kBlocks<Pm>) {
         idv.ok = finite_blocks(id1, sc1);
+        stage_scales(idv, sc1, eref1, ga, gb);
         sc2 = load_scales(p, kscale, vscale, id2, h, lq);
       }
       if (!(j + 2 <= nfull && idv.ok == 3)) mask_staged_v<KT, D, VTOK>(vr, idv, valid_next, tid);
@@ -1018,9 +1046,22 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
         a2[c] = as_qop<QT>(kl[(NC + c) * 64 + lane]);
       }
       // block scales: a lane's own factor (1e-30 where the product is 0, as above)
-      float qk0 = qk_scale;
+      float qk0 = qk_scale, lf = 0.0f;
       if constexpr (kBlocks<Pm>) {
         if (__any(!finite_scales(sc0))) not_finite(32 * j + 8 * lq);
+        if (eo != eref0) {  // V's reference has grown
+          const float down = eo - eref0 < -126 ? 0.0f : power_of_two(eo - eref0);
+#pragma unroll
+          for (int t = 0; t < NV; ++t) {
+            o[0][t] = o[0][t] * down;
+            o[1][t] = o[1][t] * down;
+          }
+          eo = eref0;
+        }
+        const float f = u2f((f2u(sc0.v) & 0x007FFFFFu) | 0x3F800000u), inv = __builtin_amdgcn_rcpf(f);
+        const _Float16 hi = (_Float16)inv, lo = (_Float16)(inv - (float)hi);
+        finv = li == 0 ? hi : (li == 1 ? lo : (_Float16)0.0f);
+        lf = __builtin_amdgcn_logf(f);
         qk0 = qk_scale * sc0.k;
         qk0 = qk0 == 0.0f ? 1e-30f : qk0;
       }
@@ -1032,7 +1073,7 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       POp pa, pla, pb, plb;
       // QK^T of column tile 0 beside the next tile's conversion into LDS
       qk(K0, a1, a2, s1a, s2a);
-      stage_write<QT, KT, D, VTOK, kBlocks<Pm>, true>(lds[1 - P], kr, vr, id1, valid_next, tid);
+      stage_write<QT, KT, D, VTOK, kBlocks<Pm>, true>(lds[1 - P], kr, vr, id1, valid_next, tid, ga, gb);
       stage_load<KT, D, VTOK>(kr, vr, p, id2, h, tid);
       __builtin_amdgcn_sched_group_barrier(0x100, 2 * NC, 0);
 #pragma unroll
@@ -1069,9 +1110,9 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       }
       // exponentials of column tile 0, then its P.V beside the exponentials
       // of column tile 1, then column tile 1's P.V
-      probs(K0, s1a, s2a, qk0, mref_of(K0), pa, pla);
+      probs(s1a, s2a, qk0, kBlocks<Pm> ? mref_of(K0) - lf : mref_of(K0), pa, pla);
       pv(K0, vraw, pa, pla);
-      probs(K1, s1b, s2b, qk0, mref_of(K1), pb, plb);
+      probs(s1b, s2b, qk0, kBlocks<Pm> ? mref_of(K1) - lf : mref_of(K1), pb, plb);
       pv(K1, vraw, pb, plb);
       __builtin_amdgcn_sched_group_barrier(0x002, 20, 2);
 #pragma unroll
@@ -1084,6 +1125,7 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       if constexpr (kBlocks<Pm>) {
         sc0 = sc1;
         sc1 = sc2;
+        eref0 = eref1;
       }
       id0 = id1;
       id1 = id2;
@@ -1095,11 +1137,14 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
     }
 
     if constexpr (kBlocks<Pm>) {
+      // the two terms of the row sums, and O out of V's reference
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        lsum[k] += __shfl_xor(lsum[k], 16, 64);
-        lsum[k] += __shfl_xor(lsum[k], 32, 64);
-        ol[k][0] = lsum[k];
+        ol[k][0] += ol[k][1];
+#pragma unroll
+        for (int t = 0; t < NV; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[k][t][e] = __builtin_amdgcn_ldexpf(o[k][t][e], eo - kVHead<KT>);
       }
     }
     // ---- a piece: its used columns' (m, l) and o, in register order ---------

@@ -15,7 +15,7 @@ def least_scale(amax: float, dtype: torch.dtype) -> float:
     """The least scale of values up to amax (float32 arithmetic), NaN where they are not finite."""
     if not math.isfinite(amax):
         return math.nan
-    a = torch.tensor(amax, dtype=torch.float32) / MOST[dtype]
+    a = torch.tensor(amax, dtype=torch.float32) * (torch.ones(()) / torch.tensor(MOST[dtype], dtype=torch.float32))
     if dtype == torch.int8:
         return max(float(a), LEAST)
     frac, exp = math.frexp(max(float(a), LEAST))
@@ -79,35 +79,40 @@ def dense(codes, scales, table, n, bs):
 
 def attend_ref(q, k_codes, k_scales, v_codes, v_scales, table, n, scale, bs=16):
     """One query row [Hq, D] over a sequence's first n tokens, in float64: (output, sum of p |v|, largest sum of
-    |q k| of a score)."""
+    |q k| of a score, sum of |v|)."""
     hq, d = q.shape
     hkv = k_codes.shape[2]
     g = hq // hkv
     n = min(n, len(table) * bs)
     if n <= 0:
-        return torch.zeros(hq, d).double(), torch.zeros(hq, d).double(), 0.0
+        return torch.zeros(hq, d).double(), torch.zeros(hq, d).double(), 0.0, torch.zeros(hq, d).double()
     (k, ok), (v, _) = dense(k_codes, k_scales, table, n, bs), dense(v_codes, v_scales, table, n, bs)
     k, v, idx = k[:, ok], v[:, ok], torch.arange(hq) // g
     if not bool(ok.any()):
-        return torch.zeros(hq, d).double(), torch.zeros(hq, d).double(), 0.0
+        return torch.zeros(hq, d).double(), torch.zeros(hq, d).double(), 0.0, torch.zeros(hq, d).double()
     qd = q.double()
     s = (qd[:, None] * k[idx]).sum(-1) * scale
     size = float(((qd.abs()[:, None] * k[idx].abs()).sum(-1) * abs(scale)).max())
     p = torch.softmax(s, -1)
-    return (p[..., None] * v[idx]).sum(1), (p[..., None] * v[idx].abs()).sum(1), size
+    return (p[..., None] * v[idx]).sum(1), (p[..., None] * v[idx].abs()).sum(1), size, v[idx].abs().sum(1)
 
 
-def assert_attended(got, refs, out_dtype, dim, tokens, p_round, what):
+def assert_attended(got, refs, out_dtype, dim, tokens, p_round, what, p_least=0.0):
     """Every element within what the kernels' roundings can add up to: the output's own half step; of the sum of
     p |v|, the rounding of p ahead of the product with V (p_round), float32 sums over the tokens (one rounding a
     tile of 32 and its tree of 5), and what an error of a score does to every weight, twice (numerator and sum): a
     score is a float32 sum of dim / 32 + 5 roundings of terms of `size` in all, times a factor (2 roundings), and
-    its exponential is good to 2^-21."""
+    its exponential is good to 2^-21.
+
+    p_least: the absolute rounding of a small weight.  In fp16 it is half of the smallest step, 2^-25, where p is
+    below 2^-14; p is relative to a reference that is at most the row's largest score, so the sum of all is 1 or
+    more, and a token's |v| enters the output by at most 2^-25 too much or too little."""
     ref = torch.stack([r[0] for r in refs])
     size = max(r[2] for r in refs)
     weight = 2.0 * (size * (dim / 32 + 7) * 2.0**-23 + 2.0**-21)
     per = p_round + (tokens / 32 + 6) * 2.0**-23 + weight
     tol = torch.finfo(out_dtype).eps / 2 * ref.abs() * (1 + per) + per * torch.stack([r[1] for r in refs])
+    tol = tol + p_least * torch.stack([r[3] for r in refs])
     # (results below the smallest normal number are rounded to its last bit)
     tol = tol + torch.finfo(out_dtype).smallest_normal * torch.finfo(out_dtype).eps
     err = (got.double().cpu() - ref).abs()

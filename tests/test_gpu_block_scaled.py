@@ -378,8 +378,8 @@ def _check_prefill(qt, dtype, layout, chunks, hq, hkv, dim, seed=0, spread=1.0, 
         for i in sorted({0, 1, r // 2, r - 2, r - 1} & set(range(r))) if r > 12 else range(r):
             rows.append(start[n] + i)
             refs.append(attend_ref(q[start[n] + i], k, ks, v, vs, tables[n], c + i + 1, scale))
-    # P in fp16 ahead of the product with V, and its subnormals (2^-25 of up to 2^8 tokens' weight)
-    assert_attended(got[rows], refs, qt, dim, max(lens), 2.0**-11 + 2.0**-16, f"prefill {qt} {dtype} {layout} {chunks}")
+    # P in fp16 ahead of the product with V, and its subnormals
+    assert_attended(got[rows], refs, qt, dim, max(lens), 2.0**-11 + 2.0**-16, f"prefill {qt} {dtype} {layout} {chunks}", 2.0**-25)
     return got
 
 

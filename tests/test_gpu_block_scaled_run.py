@@ -108,7 +108,7 @@ class Run:
                 for k in sorted({0, new[r] // 2, new[r] - 1}):
                     pick.append(first + k)
                     refs.append(self.refs(layer, r, q[first + k], n - new[r] + k + 1))
-            assert_attended(out[pick], refs, torch.bfloat16, D, 250, 2.0**-11 + 2.0**-16, f"prefill layer {layer}")
+            assert_attended(out[pick], refs, torch.bfloat16, D, 250, 2.0**-11 + 2.0**-16, f"prefill layer {layer}", 2.0**-25)
 
     def fork(self, src, new_ids):
         copies = self.bm.fork(src, new_ids, len(self.text[src][0][0]))
