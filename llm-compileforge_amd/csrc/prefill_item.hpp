@@ -550,12 +550,12 @@ __device__ __forceinline__ uint4 v_to_16(uint32_t lo, uint32_t hi, float g) {
 // chain s; V entry (step t, lane) = channel 16 t + li, tokens 8 lq .. 8 lq + 7.
 // V tokens at or past `valid` (tile-relative) or in an invalid block become
 // zero (cache slots there may hold any bits, NaN codes included).
-// BLK: a cache with block scales, whose V codes are staged times ga (the tile's
-// first block) and gb.
+// BLK: a cache with block scales, whose V codes are staged times g, this thread's
+// block's power of two.
 // FULL: the caller knows every token of the tile is valid.
 template <int QT, int KT, int D, bool VTOK, bool BLK, bool FULL = false>
 __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const uint4* vr, const TileIds& t,
-                                            int valid, int tid, float ga = 1.0f, float gb = 1.0f) {
+                                            int valid, int tid, float g = 1.0f) {
   using Gm = Geo<KT, D>;
 #pragma unroll
   for (int i = 0; i < Gm::KPT; ++i) {
@@ -593,8 +593,8 @@ __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const u
         const uint4 v = make_uint4(vr[i].x & km, vr[i].y & km, vr[i].z & km, vr[i].w & km);
         uint8_t* row = rows + vtok_slot(16 * X + r) * Gm::VRS;
         if constexpr (Gm::KB == 1) {
-          *(uint4*)(row + 32 * c) = v_to_16<KT, BLK>(v.x, v.y, uniform(X) ? gb : ga);
-          *(uint4*)(row + 32 * c + 16) = v_to_16<KT, BLK>(v.z, v.w, uniform(X) ? gb : ga);
+          *(uint4*)(row + 32 * c) = v_to_16<KT, BLK>(v.x, v.y, g);
+          *(uint4*)(row + 32 * c + 16) = v_to_16<KT, BLK>(v.z, v.w, g);
         } else {
           *(uint4*)(row + 16 * c) = v;
         }
@@ -612,8 +612,8 @@ __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const u
       const int li = d & 15, tt = d >> 4;
       if (full) {
         if constexpr (Gm::KB == 1) {
-          vl[tt * 64 + 32 * X + li] = v_to_16<KT, BLK>(vr[i].x, vr[i].y, uniform(X) ? gb : ga);
-          vl[tt * 64 + 32 * X + 16 + li] = v_to_16<KT, BLK>(vr[i].z, vr[i].w, uniform(X) ? gb : ga);
+          vl[tt * 64 + 32 * X + li] = v_to_16<KT, BLK>(vr[i].x, vr[i].y, g);
+          vl[tt * 64 + 32 * X + 16 + li] = v_to_16<KT, BLK>(vr[i].z, vr[i].w, g);
         } else {
           vl[tt * 64 + 32 * X + 16 * part + li] = vr[i];
         }
@@ -621,8 +621,8 @@ __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const u
         const int n0 = ok ? valid - 16 * X : 0;  // valid tokens among this load's 16
         const uint2 lo = keep_bytes(make_uint2(vr[i].x, vr[i].y), n0);
         const uint2 hi = keep_bytes(make_uint2(vr[i].z, vr[i].w), n0 - 8);
-        vl[tt * 64 + 32 * X + li] = v_to_16<KT, BLK>(lo.x, lo.y, uniform(X) ? gb : ga);
-        vl[tt * 64 + 32 * X + 16 + li] = v_to_16<KT, BLK>(hi.x, hi.y, uniform(X) ? gb : ga);
+        vl[tt * 64 + 32 * X + li] = v_to_16<KT, BLK>(lo.x, lo.y, g);
+        vl[tt * 64 + 32 * X + 16 + li] = v_to_16<KT, BLK>(hi.x, hi.y, g);
       } else {
         const int n0 = ok ? valid - 16 * X - 8 * part : 0;
         vl[tt * 64 + 32 * X + 16 * part + li] = mask_tokens(vr[i], n0);
@@ -673,46 +673,81 @@ __device__ __forceinline__ void mask_staged_v(uint4* vr, const TileIds& t, int v
 template <class Pm>
 constexpr bool kBlocks = std::is_same<Pm, PrefillBlockParams>::value;
 
-// The K and V scale of the block that a lane's 8 tokens of a tile lie in (lanes lq
-// 0-1: block a, 2-3: block b).  What stands in for an invalid block may hold
-// anything: 1 and 0 take its place.
-struct LaneScales {
-  float k, v;
+// Block scales.  A lane's 8 tokens of a tile lie in one block (lanes lq 0-1: block a,
+// 2-3: block b).  Its K scale is the factor of the lane's scores.  Its V scale is
+// 2^e * f with f in [1, 2): 2^e goes to the codes as they are staged, against a
+// reference 2^eref that is the largest of the item's tiles so far (O is in its units
+// and follows it), kVHead binades below fp16's largest, so that a block of 2^-21
+// (e4m3; int8 2^-28) of the largest before it keeps every bit of its codes; f goes to
+// the exponent of the tile's weights, and the row sums take 1 / f of it back: the P.V
+// product against a channel of ones has 1 / f in their place, as two fp16 terms in
+// rows 0 and 1.  A weight is rounded to fp16 once, as without block scales.
+//
+// What the tiles need of their scales is formed kScaleTiles tiles at a time, a thread
+// a block, and kept in LDS; a step then takes three LDS reads and about ten other
+// instructions for it.  Eight 512-row chunks behind 0-4,096 tokens, e4m3 under bf16:
+// 211 us; with every wave loading and forming its tile's own a step ahead
+// 218-220 (some 60 instructions a step), one scale a head 183; int8 223 and
+// 230-237.  V's scales multiplied into P, P in two bf16 terms and row sums by
+// addition took 264 (int8, fp16 queries).
+constexpr int kScaleTiles = 128;              // of a pass
+constexpr int kScaleSlots = 2 * kScaleTiles;  // tiles held
+struct alignas(16) BlockScale {
+  float k;       // the scores' factor
+  float lf;      // log2 f
+  uint32_t inv;  // 1 / f as two fp16 terms
+  float g;       // the power of two of the V codes
 };
-template <class Pm>
-__device__ __forceinline__ LaneScales load_scales(const Pm& p, const float* __restrict__ kscale,
-                                                  const float* __restrict__ vscale, const TileIds& t, int h, int lq) {
-  LaneScales s{1.0f, 1.0f};
-  if constexpr (kBlocks<Pm>) {
-    const int64_t b = lq < 2 ? t.a : t.b;
-    s.k = kscale[b * p.ks_b + h * p.ks_s];
-    s.v = vscale[b * p.vs_b + h * p.vs_s];
-    if (!((t.ok >> (lq >> 1)) & 1)) s = LaneScales{1.0f, 0.0f};
-  }
-  return s;
-}
-__device__ __forceinline__ bool finite_scales(const LaneScales& s) {
-  return __builtin_fmaxf(__builtin_fabsf(s.k), __builtin_fabsf(s.v)) < INFINITY && s.k == s.k && s.v == s.v;
-}
-// A V scale is 2^e * f with f in [1, 2).  2^e goes to the codes as they are staged,
-// against a reference 2^eref that is the largest of the item's blocks so far (O is
-// in its units and follows it), kVHead binades below fp16's largest: a block of 2^-21
-// (e4m3; int8 2^-28) of the largest before it keeps every bit of its codes.  f goes
-// to the exponent of the tile's weights, and the row sums take 1 / f of it back: the
-// P.V product against a channel of ones has 1 / f in their place, as two fp16 terms
-// in rows 0 and 1.  So a weight is rounded to fp16 once, as without block scales, and
-// a tile costs about 14 vector instructions more (V's scale multiplied into P, P in
-// two bf16 terms and row sums by addition: CHUNK_V1 us for eight 512-row chunks
-// over int8 against CHUNK_V2).
+struct ScaleWindow {
+  BlockScale at[kScaleSlots][2];
+  int word[kScaleSlots];  // eref (with a float's bias) << 4 | blocks with NaN or infinite scales << 2 | valid blocks
+  int top[4];
+};
 template <int KT>
 constexpr int kVHead = KT == kI8 ? 5 : 7;
-__device__ __forceinline__ int exponent_of(float v) { return (int)((f2u(v) >> 23) & 0xFFu) - 127; }
-__device__ __forceinline__ float power_of_two(int e) { return u2f((uint32_t)min(max(e + 127, 0), 254) << 23); }
+__device__ __forceinline__ float power_of_two(int e) { return u2f((uint32_t)max(e + 127, 0) << 23); }  // e < 128
 
-// The tile's blocks that are valid and have finite scales, as bits.
-__device__ __forceinline__ int finite_blocks(const TileIds& t, const LaneScales& s) {
-  const unsigned long long bad = __ballot(!finite_scales(s));
-  return t.ok & ~(((uint32_t)bad != 0 ? 1 : 0) | ((bad >> 32) != 0 ? 2 : 0));
+// The tiles first .. + kScaleTiles - 1 of an item (whose own first one is jt0) into
+// their slots; eref: the reference of the tile before.  All 256 threads.
+template <int KT>
+__device__ __forceinline__ void fill_scales(const PrefillBlockParams& p, ScaleWindow* w, const float* __restrict__ kscale,
+                                            const float* __restrict__ vscale, const int32_t* __restrict__ trow, int jt0,
+                                            int first, int nt, int nblk, int h, float qk_scale, int& eref, int tid) {
+  const int j = first + (tid >> 1), X = tid & 1, jb = 2 * j + X;
+  int id = -1;
+  if (j < nt && jb < nblk) id = trow[(int64_t)jb * p.t_sm];
+  const bool valid = (unsigned)id < (unsigned)p.NB;
+  float k = 1.0f, v = 0.0f;
+  if (valid) {
+    k = kscale[id * p.ks_b + h * p.ks_s];
+    v = vscale[id * p.vs_b + h * p.vs_s];
+  }
+  const bool bad = !(__builtin_fabsf(k) < INFINITY && __builtin_fabsf(v) < INFINITY);
+  if (bad) k = 1.0f, v = 0.0f;
+  const int e = (int)((f2u(v) >> 23) & 0xFFu), pair = max(e, __shfl_xor(e, 1, 64));
+  const int incl = wave_incl_max(pair, 0);
+  const int mine = (valid ? 1 : 0) << X | (bad ? 1 : 0) << (2 + X), flags = mine | __shfl_xor(mine, 1, 64);
+  if ((tid & 63) == 63) w->top[tid >> 6] = incl;
+  __syncthreads();
+  int before = eref, all = eref;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < (tid >> 6)) before = max(before, w->top[i]);
+    all = max(all, w->top[i]);
+  }
+  const int own = max(before, incl);
+  const float f = u2f((f2u(v) & 0x007FFFFFu) | 0x3F800000u), r = 1.0f / f;
+  const _Float16 hi = (_Float16)r, lo = (_Float16)(r - (float)hi);
+  const int slot = (j - jt0) & (kScaleSlots - 1);
+  BlockScale s;
+  s.k = fmaxf(qk_scale * k, 1e-30f);  // (a product of 0: as for one scale a head)
+  s.lf = __builtin_amdgcn_logf(f);
+  s.inv = (uint32_t)__builtin_bit_cast(uint16_t, hi) | ((uint32_t)__builtin_bit_cast(uint16_t, lo) << 16);
+  s.g = power_of_two(e - own + kVHead<KT>);
+  w->at[slot][X] = s;
+  if (X == 0) w->word[slot] = own << 4 | flags;
+  eref = all;
+  __syncthreads();
 }
 
 // DIRECT: one piece per workgroup (direct_piece), otherwise the queue's items;
@@ -729,6 +764,8 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
   constexpr int RB = kCols / G;
   __shared__ uint4 lds[2][Gm::KENT + (VTOK ? Gm::VENT_TOK : Gm::VENT)];
   __shared__ int s_item;
+  __shared__ typename std::conditional<kBlocks<Pm>, ScaleWindow, int>::type s_scales;
+  (void)s_scales;
   const int xcd = blockIdx.x % kXcds;
   bool own_list = true;  // (thread 0) this XCD's list still has items
   const int tid = threadIdx.x, lane = tid & 63;
@@ -853,31 +890,39 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
     TileIds id0 = tile_ids(p, trow, jt0, kvlen);
     TileIds id1 = jt0 + 1 < nt ? tile_ids(p, trow, jt0 + 1, kvlen) : id0;
     TileIds id2 = jt0 + 2 < nt ? tile_ids(p, trow, jt0 + 2, kvlen) : id1;
-    LaneScales sc0 = load_scales(p, kscale, vscale, id0, h, lq), sc1 = load_scales(p, kscale, vscale, id1, h, lq);
-    (void)sc0;
-    (void)sc1;
-    // V's reference exponent of tiles j and j + 1 (eref0, eref1), and O's (eo)
-    int eref0 = -127, eo = -127;
-    auto stage_scales = [&](const TileIds& idv, const LaneScales& sc, int& eref, float& ga, float& gb) {
-      const float va = u2f(__builtin_amdgcn_readlane(f2u(sc.v), 0)), vb = u2f(__builtin_amdgcn_readlane(f2u(sc.v), 32));
-      const int ea = (idv.ok & 1) ? exponent_of(va) : -127, eb = (idv.ok & 2) ? exponent_of(vb) : -127;
-      eref = max(eref, max(ea, eb));
-      ga = power_of_two(ea - eref + kVHead<KT>);
-      gb = power_of_two(eb - eref + kVHead<KT>);
-    };
-    (void)stage_scales;
+    // Block scales: the lane's of tile j (sc), the staging's of tile j + 1 (g1), the
+    // words of both, O's reference (eo) and that of the last tile formed (eref).
+    BlockScale sc{};
+    float g1 = 1.0f;
+    int word0 = 3, word1 = 3, eo = 0, eref = 0;
+    const int sx = (tid / D) & 1;  // the block whose V this thread stages
+    auto scale_slot = [&](int j) { return (j - jt0) & (kScaleSlots - 1); };
     if (jt0 < nt) {
       stage_load<KT, D, VTOK>(kr, vr, p, id0, h, tid);
       TileIds idv = id0;
-      float ga = 1.0f, gb = 1.0f;
+      float g0 = 1.0f;
       if constexpr (kBlocks<Pm>) {
-        idv.ok = finite_blocks(id0, sc0);
-        stage_scales(idv, sc0, eref0, ga, gb);
-        eo = eref0;
+        fill_scales<KT>(p, &s_scales, kscale, vscale, trow, jt0, jt0, nt, nblk, h, qk_scale, eref, tid);
+        if (nt - jt0 > kScaleTiles)
+          fill_scales<KT>(p, &s_scales, kscale, vscale, trow, jt0, jt0 + kScaleTiles, nt, nblk, h, qk_scale, eref, tid);
+        sc = s_scales.at[0][lq >> 1];
+        g0 = s_scales.at[0][sx].g;
+        word0 = uniform(s_scales.word[0]);
+        g1 = s_scales.at[1][sx].g;
+        word1 = uniform(s_scales.word[1]);
+        eo = word0 >> 4;
+        idv.ok = word0 & ~(word0 >> 2) & 3;
       }
-      stage_write<QT, KT, D, VTOK, kBlocks<Pm>>(lds[0], kr, vr, idv, kvlen - 32 * jt0, tid, ga, gb);
+      stage_write<QT, KT, D, VTOK, kBlocks<Pm>>(lds[0], kr, vr, idv, kvlen - 32 * jt0, tid, g0);
     }
-    int eref1 = eref0;
+    (void)sc;
+    (void)g1;
+    (void)word0;
+    (void)word1;
+    (void)eo;
+    (void)eref;
+    (void)sx;
+    (void)scale_slot;
     if (jt0 + 1 < nt) stage_load<KT, D, VTOK>(kr, vr, p, id1, h, tid);
     __syncthreads();
 
@@ -960,32 +1005,36 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
         }
       }
     };
-    // A block whose scales are not finite makes NaN of the columns that see a token of
-    // it, and of no others.
-    auto not_finite = [&](int tok0) {
-      const bool bad = !finite_scales(sc0);
+    // What few tiles have: V's reference has grown, or a block has scales that are not
+    // finite, which make NaN of the columns that see a token of it, and of no others.
+    auto odd_scales = [&](int word, int tok0) {
+      const float down = power_of_two(eo - (word >> 4));
+      eo = word >> 4;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        int see = bad && lim[k] > tok0;
+        int see = ((word >> (2 + (lq >> 1))) & 1) && lim[k] > tok0;
         see |= __shfl_xor(see, 16, 64);
         see |= __shfl_xor(see, 32, 64);
+        const float factor = see ? __builtin_nanf("") : down;
 #pragma unroll
-        for (int t = 0; t < NV; ++t)
-          if (see) o[k][t] = o[k][t] * __builtin_nanf("");
+        for (int t = 0; t < NV; ++t) o[k][t] = o[k][t] * factor;
       }
-      if (bad) sc0 = LaneScales{1.0f, 0.0f};
     };
-    (void)not_finite;
+    (void)odd_scales;
+    // which bytes of BlockScale::inv this lane's row of the row sums takes (12: zero)
+    const uint32_t inv_bytes = li == 0 ? 0x01000100u : (li == 1 ? 0x03020302u : 0x0C0C0C0Cu);
+    (void)inv_bytes;
     // O^T += V^T P^T for column tile k; the row sums come out of the same
     // pipe as O[column][0] against a V tile whose channel 0 is all ones.
-    _Float16 finv = (_Float16)0.0f;  // block scales: a term of 1 / f in rows 0 and 1, 0 in the others
-    (void)finv;
     auto pv = [&](auto kc, const uint4* vraw, const POp& pk, const POp& pl) {
       constexpr int k = decltype(kc)::value;
       if constexpr (KT != kBF16) {
-        _Float16 one = li == 0 ? (_Float16)1.0f : (_Float16)0.0f;
-        if constexpr (kBlocks<Pm>) one = finv;
-        const f16x8_t ones = {one, one, one, one, one, one, one, one};
+        const _Float16 one = li == 0 ? (_Float16)1.0f : (_Float16)0.0f;
+        f16x8_t ones = {one, one, one, one, one, one, one, one};
+        if constexpr (kBlocks<Pm>) {
+          const uint32_t r = __builtin_amdgcn_perm(0u, sc.inv, inv_bytes);
+          ones = __builtin_bit_cast(f16x8_t, make_uint4(r, r, r, r));
+        }
         ol[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pk, ol[k], 0, 0, 0);
 #pragma unroll
         for (int t = 0; t < NV; ++t)
@@ -1020,14 +1069,7 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       // (V of a block whose scales are not finite is zeroed like an invalid one's:
       // its codes may be NaN, and 0 * NaN would reach rows that do not see it)
       TileIds idv = id1;
-      LaneScales sc2;
-      (void)sc2;
-      float ga = 1.0f, gb = 1.0f;
-      if constexpr (kBlocks<Pm>) {
-        idv.ok = finite_blocks(id1, sc1);
-        stage_scales(idv, sc1, eref1, ga, gb);
-        sc2 = load_scales(p, kscale, vscale, id2, h, lq);
-      }
+      if constexpr (kBlocks<Pm>) idv.ok = word1 & ~(word1 >> 2) & 3;
       if (!(j + 2 <= nfull && idv.ok == 3)) mask_staged_v<KT, D, VTOK>(vr, idv, valid_next, tid);
       // table entries of tile j + 3, read now and resolved after the math
       int raw_a = -1, raw_b = -1;
@@ -1045,25 +1087,10 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
         a1[c] = as_qop<QT>(kl[c * 64 + lane]);
         a2[c] = as_qop<QT>(kl[(NC + c) * 64 + lane]);
       }
-      // block scales: a lane's own factor (1e-30 where the product is 0, as above)
-      float qk0 = qk_scale, lf = 0.0f;
+      float qk0 = qk_scale;
       if constexpr (kBlocks<Pm>) {
-        if (__any(!finite_scales(sc0))) not_finite(32 * j + 8 * lq);
-        if (eo != eref0) {  // V's reference has grown
-          const float down = eo - eref0 < -126 ? 0.0f : power_of_two(eo - eref0);
-#pragma unroll
-          for (int t = 0; t < NV; ++t) {
-            o[0][t] = o[0][t] * down;
-            o[1][t] = o[1][t] * down;
-          }
-          eo = eref0;
-        }
-        const float f = u2f((f2u(sc0.v) & 0x007FFFFFu) | 0x3F800000u), inv = __builtin_amdgcn_rcpf(f);
-        const _Float16 hi = (_Float16)inv, lo = (_Float16)(inv - (float)hi);
-        finv = li == 0 ? hi : (li == 1 ? lo : (_Float16)0.0f);
-        lf = __builtin_amdgcn_logf(f);
-        qk0 = qk_scale * sc0.k;
-        qk0 = qk0 == 0.0f ? 1e-30f : qk0;
+        qk0 = sc.k;
+        if (((word0 ^ (eo << 4)) & ~3) != 0) odd_scales(word0, 32 * j + 8 * lq);
       }
       const bool edge = j >= lmin_t || id0.ok != 3;
       const int tok0 = 32 * j + 8 * lq;
@@ -1073,13 +1100,13 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       POp pa, pla, pb, plb;
       // QK^T of column tile 0 beside the next tile's conversion into LDS
       qk(K0, a1, a2, s1a, s2a);
-      stage_write<QT, KT, D, VTOK, kBlocks<Pm>, true>(lds[1 - P], kr, vr, id1, valid_next, tid, ga, gb);
+      stage_write<QT, KT, D, VTOK, kBlocks<Pm>, true>(lds[1 - P], kr, vr, id1, valid_next, tid, g1);
       stage_load<KT, D, VTOK>(kr, vr, p, id2, h, tid);
       __builtin_amdgcn_sched_group_barrier(0x100, 2 * NC, 0);
 #pragma unroll
       for (int i = 0; i < kQkMfma; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, KT == kI8 ? 6 : 3, 0);
         __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
       }
       __builtin_amdgcn_sched_group_barrier(0x020, Gm::KPT + Gm::VPT, 0);
@@ -1110,9 +1137,9 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       }
       // exponentials of column tile 0, then its P.V beside the exponentials
       // of column tile 1, then column tile 1's P.V
-      probs(s1a, s2a, qk0, kBlocks<Pm> ? mref_of(K0) - lf : mref_of(K0), pa, pla);
+      probs(s1a, s2a, qk0, kBlocks<Pm> ? mref_of(K0) - sc.lf : mref_of(K0), pa, pla);
       pv(K0, vraw, pa, pla);
-      probs(s1b, s2b, qk0, kBlocks<Pm> ? mref_of(K1) - lf : mref_of(K1), pb, plb);
+      probs(s1b, s2b, qk0, kBlocks<Pm> ? mref_of(K1) - sc.lf : mref_of(K1), pb, plb);
       pv(K1, vraw, pb, plb);
       __builtin_amdgcn_sched_group_barrier(0x002, 20, 2);
 #pragma unroll
@@ -1121,17 +1148,24 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
         __builtin_amdgcn_sched_group_barrier(0x002, 1, 2);
       }
       const TileIds id3 = j + 3 < nt ? tile_resolve(raw_a, raw_b, p.NB) : id2;
-      __syncthreads();
       if constexpr (kBlocks<Pm>) {
-        sc0 = sc1;
-        sc1 = sc2;
-        eref0 = eref1;
+        sc = s_scales.at[scale_slot(j + 1)][lq >> 1];
+        g1 = s_scales.at[scale_slot(j + 2)][sx].g;
+        word0 = word1;
+        word1 = uniform(s_scales.word[scale_slot(j + 2)]);
       }
+      __syncthreads();
       id0 = id1;
       id1 = id2;
       id2 = id3;
     };
     for (int j = jt0; j < nt; j += 2) {
+      if constexpr (kBlocks<Pm>) {
+        // the slots of the half of the window that the item has left behind
+        const int rel = j - jt0, next = j + kScaleTiles - 2;
+        if (rel > kScaleTiles && (rel & (kScaleTiles - 1)) == 2 && next < nt)
+          fill_scales<KT>(p, &s_scales, kscale, vscale, trow, jt0, next, nt, nblk, h, qk_scale, eref, tid);
+      }
       step(std::integral_constant<int, 0>{}, j);
       if (j + 1 < nt) step(std::integral_constant<int, 1>{}, j + 1);
     }
@@ -1144,7 +1178,7 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
 #pragma unroll
         for (int t = 0; t < NV; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[k][t][e] = __builtin_amdgcn_ldexpf(o[k][t][e], eo - kVHead<KT>);
+          for (int e = 0; e < 4; ++e) o[k][t][e] = __builtin_amdgcn_ldexpf(o[k][t][e], eo - 127 - kVHead<KT>);
       }
     }
     // ---- a piece: its used columns' (m, l) and o, in register order ---------

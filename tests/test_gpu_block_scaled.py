@@ -356,8 +356,8 @@ def test_decode_dict_api_plan_and_noalloc():
     assert torch.equal(ops.DecodePlan(*args).run(), want)
 
 
-def _check_prefill(qt, dtype, layout, chunks, hq, hkv, dim, seed=0, spread=1.0, scale=None, bad=None):
-    """chunks: (rows, cached tokens)."""
+def _check_prefill(qt, dtype, layout, chunks, hq, hkv, dim, seed=0, spread=1.0, scale=None, bad=None, only=None):
+    """chunks: (rows, cached tokens); only: the chunks whose outermost rows are compared (all rows' samples of all)."""
     gen = torch.Generator().manual_seed(seed)
     lens = [r + c for r, c in chunks]
     nb = sum(-(-n // 16) for n in lens) + 3
@@ -375,7 +375,10 @@ def _check_prefill(qt, dtype, layout, chunks, hq, hkv, dim, seed=0, spread=1.0, 
     got = chunked_prefill_attention(q.cuda(), kc, vc, _i32(tables), _i32(lens), _i32(start), 16, scale, k_scale=ksd, v_scale=vsd)
     rows, refs = [], []
     for n, (r, c) in enumerate(chunks):
-        for i in sorted({0, 1, r // 2, r - 2, r - 1} & set(range(r))) if r > 12 else range(r):
+        if only is not None and n not in only:
+            continue
+        sample = {0, r - 1} if only is not None else {0, 1, r // 2, r - 2, r - 1}
+        for i in sorted(sample & set(range(r))) if r > 12 else range(r):
             rows.append(start[n] + i)
             refs.append(attend_ref(q[start[n] + i], k, ks, v, vs, tables[n], c + i + 1, scale))
     # P in fp16 ahead of the product with V, and its subnormals
@@ -404,6 +407,21 @@ def test_prefill_queued(dtype):
     """More items than resident workgroups: the plan and its queue."""
     _check_prefill(BF16, dtype, "paired", [(300, 17)] * 6 + [(250, 400)] * 4, 32, 8, 128, seed=3)
     _check_prefill(F16, dtype, "native", [(420, 0)] * 7, 24, 12, 64, seed=4)
+
+
+@pytest.mark.parametrize("dtype", KV)
+def test_prefill_long_items(dtype):
+    # more tiles in one item than a workgroup holds the scales of (256), with V scales that rise along one sequence
+    # and fall along another, and some that are invalid far along
+    def slopes(tables, ks, vs):
+        blocks = len(tables[0])
+        for j in range(blocks):
+            vs[tables[0][j]] *= 2.0 ** (j * 12 // blocks)
+            vs[tables[6][j]] *= 2.0 ** (12 - j * 12 // blocks)
+        for j in (300, 513, 700):
+            tables[6][j] = -1
+
+    _check_prefill(F16, dtype, "paired", [(160, 12350 + 9 * n) for n in range(7)], 64, 4, 64, seed=9, bad=slopes, only=(0, 6))
 
 
 @pytest.mark.parametrize("dtype", KV)
