@@ -4,9 +4,9 @@
 //
 // The scale of a block that holds values up to amax is the least that its codes
 // can reach them with: amax / 127 for int8, and for e4m3fn the next power of two
-// from amax / 448 on (quotients as products with the rounded reciprocal).  A floating-point code loses no precision by it (its steps
-// are relative; the smallest normal one is 2^14 below amax in either case), the
-// division by it is exact, and where a later row widens the block's scale, the
+// from amax / 448 on (quotients as products with the rounded reciprocal).  A
+// floating-point code loses no precision by it (its steps are relative; the
+// smallest normal one is 2^14 below amax in either case), the division by it is exact, and where a later row widens the block's scale, the
 // codes already there move by whole exponents and are exact still, unless they
 // fall below the smallest normal one.  int8 codes are rounded again by a widening,
 // by half a step of the new scale at most.

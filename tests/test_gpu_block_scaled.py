@@ -49,10 +49,13 @@ def _same_codes(got, want, scales):
     assert torch.equal(g[live], w[live]), int((g[live] != w[live]).sum())
 
 
-def _check_write(dtype, xt, layout, lens, tables, start, nb=24, bs=16, heads=3, dim=64, seed=0, new=None, spread=1.0):
+def _check_write(dtype, xt, layout, lens, tables, start, nb=24, bs=16, heads=3, dim=64, seed=0, new=None, spread=1.0,
+                 cached=None):
     gen = torch.Generator().manual_seed(seed)
     k, ks = filled(nb, bs, heads, dim, dtype, gen, spread)
     v, vs = filled(nb, bs, heads, dim, dtype, gen, spread)
+    if cached is not None:
+        cached(k, ks, v, vs)
     total = len(lens) if start is None else start[-1]
     if new is None:
         new = tuple((torch.randn(total, heads, dim, generator=gen) * torch.exp2(spread * torch.randn(total, heads, 1, generator=gen))).to(xt)
@@ -149,6 +152,47 @@ def test_write_not_finite(dtype, bad):
     assert bool(ks[3, 1].isnan())
     write_kv_blocks(row, row, _i32([[3, 8]]), _i32([1]), kc, vc, ks, vs)
     assert float(ks[3, 1]) == least_scale(1.0, dtype)
+
+
+@pytest.mark.parametrize("dtype", KV)
+@pytest.mark.parametrize("layout", ["paired", "token_major"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_write_behind_any_scale(dtype, layout, dim):
+    """Rows behind cached ones of scales that no write chose: not powers of two, wider than the rows need, past
+    2^126, and codes of every value."""
+
+    def cached(k, ks, v, vs):
+        every = torch.arange(256, dtype=torch.uint8).repeat(k[0].numel() // 256)
+        for c, s in ((k, ks), (v, vs)):
+            code_view = c.view(torch.uint8) if dtype == E4M3 else c
+            code_view[2] = every.view(code_view.dtype).reshape(c[2].shape)
+            s[:, 0] *= 1.37
+            s[:, 1] *= 61.0
+            s[1] = torch.tensor([2.0**126, 1.3 * 2.0**126, 2.0**127, 2.0**125])
+            s[2] = torch.tensor([0.7e-3, 1e-3, 2.0**-9, 3.0])
+
+    start = [0, 3, 13, 14, 30]
+    _check_write(dtype, BF16, layout, [10, 17, 12, 30], [[0, 4], [1, 5], [2, 6], [3, 7]], start, heads=4, dim=dim, cached=cached)
+
+
+@pytest.mark.parametrize("dtype", KV)
+@pytest.mark.parametrize("xt", [BF16, F32])
+def test_write_rows_off_their_alignment(dtype, xt):
+    """New rows that begin one element behind a 16-byte boundary, and keys and values of different layouts."""
+    gen = torch.Generator().manual_seed(11)
+    flat = torch.randn(2, 40 * 2 * 64 + 1, generator=gen).to(xt)
+    k, ks = filled(6, 16, 2, 64, dtype, gen)
+    v, vs = filled(6, 16, 2, 64, dtype, gen)
+    tables, lens, start = [[0, 1], [2, 3], [5, 4]], [20, 20, 13], [0, 20, 27, 40]
+    for first in (0, 1):
+        new = [f.cuda()[first : first + 40 * 2 * 64].view(40, 2, 64) for f in flat]
+        kc, _, ksd, _ = _device_cache(k, v, ks, vs, "token_major")
+        _, vc, _, vsd = _device_cache(k, v, ks, vs, "native")
+        write_kv_blocks(new[0], new[1], _i32(tables), _i32(lens), kc, vc, ksd, vsd, q_start=_i32(start))
+        for x, got, gs, c, s in ((new[0], kc, ksd, k.clone(), ks.clone()), (new[1], vc, vsd, v.clone(), vs.clone())):
+            write_ref(x.cpu(), tables, lens, start, c, s, 16)
+            _same_scales(gs, s)
+            _same_codes(got, c, s)
 
 
 @pytest.mark.parametrize("dtype", KV)
