@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <vector>
 
 #include "cf_hip.h"
 
@@ -45,6 +46,7 @@ struct Lib {
   decltype(&cf_evict_select) evict_select = nullptr;
   decltype(&cf_evict_move) evict_move = nullptr;
   decltype(&cf_kv_write_blocks) write_blocks = nullptr;
+  decltype(&cf_move_blocks) move_blocks = nullptr;
 };
 Lib g_lib;
 PyObject* g_raw_stream = nullptr;        // device index -> hipStream_t of the current stream
@@ -680,6 +682,72 @@ PyObject* kv_write_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// [NB, bytes] of a paged tensor whose blocks are one contiguous span each.
+CfTensor block_bytes(const at::Tensor& t) {
+  if (t.dim() < 1) throw Slow{};
+  int64_t span = 1, elems = 1;
+  for (int64_t i = 1; i < t.dim(); ++i) {
+    if (t.size(i) > 1) span += (t.size(i) - 1) * t.stride(i);
+    if (t.size(i) != 1) elems *= t.size(i);
+  }
+  const int64_t nb = t.size(0), es = t.element_size();
+  if (elems == 0 || span != elems || (nb > 1 && t.stride(0) < elems)) throw Slow{};
+  CfTensor d{};
+  d.t.device = SFA_ROCM;
+  d.t.rank = 2;
+  d.t.elem_size = 1;
+  SFATensorRaw2& r = d.t.r2;
+  r.allocated = r.aligned = t.data_ptr();
+  r.sizes[0] = nb;
+  r.sizes[1] = elems * es;
+  r.strides[0] = (nb > 1 ? t.stride(0) : elems) * es;
+  r.strides[1] = 1;
+  d.dtype = CF_U8;
+  return d;
+}
+
+// (caches: a list or tuple, moves: a contiguous int32 [n, 2] CPU tensor or buffer)
+PyObject* move_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(args, n, 2, [](PyObject* const* a) -> PyObject* {
+    if (!PyList_CheckExact(a[0]) && !PyTuple_CheckExact(a[0])) throw Slow{};
+    const Py_ssize_t caches = PySequence_Fast_GET_SIZE(a[0]);
+    if (caches == 0 || caches > INT32_MAX) throw Slow{};
+    PyObject** items = PySequence_Fast_ITEMS(a[0]);
+    const Call call(tensor_of(items[0]));
+    std::vector<CfTensor> d;
+    d.reserve(caches);
+    for (Py_ssize_t i = 0; i < caches; ++i) {
+      const at::Tensor& t = tensor_of(items[i]);
+      if (t.get_device() != call.device) throw Slow{};
+      d.push_back(block_bytes(t));
+    }
+    std::vector<int32_t> moves;  // (its own copy: the GIL is released)
+    if (THPVariable_CheckExact(a[1])) {
+      const at::Tensor& m = THPVariable_Unpack(a[1]);
+      if (!m.defined() || !m.is_cpu() || m.scalar_type() != at::kInt || m.dim() != 2 || m.size(1) != 2 || !m.is_contiguous())
+        throw Slow{};
+      const int32_t* at = (const int32_t*)m.data_ptr();
+      moves.assign(at, at + m.numel());
+    } else {
+      struct View {
+        Py_buffer b{};
+        explicit View(PyObject* o) {
+          if (PyObject_GetBuffer(o, &b, PyBUF_FORMAT | PyBUF_C_CONTIGUOUS) != 0) throw Slow{};
+        }
+        ~View() { PyBuffer_Release(&b); }
+      } v(a[1]);
+      if (v.b.ndim != 2 || v.b.shape[1] != 2 || v.b.itemsize != 4 || v.b.format == nullptr || v.b.format[0] != 'i' ||
+          v.b.format[1] != 0)
+        throw Slow{};
+      const int32_t* at = (const int32_t*)v.b.buf;
+      moves.assign(at, at + 2 * v.b.shape[0]);
+    }
+    return PyLong_FromLong(without_gil([&] {
+      return g_lib.move_blocks(d.data(), (int32_t)caches, moves.data(), (int64_t)(moves.size() / 2), call.stream);
+    }));
+  });
+}
+
 template <class T>
 bool take_address(PyObject* addrs, const char* name, T* fn) {
   PyObject* v = PyDict_GetItemString(addrs, name);
@@ -714,7 +782,8 @@ PyObject* bind(PyObject*, PyObject* args) {
       !take_address(addrs, "cf_rotary_cache_write", &l.rotary_write) ||
       !take_address(addrs, "cf_evict_select", &l.evict_select) ||
       !take_address(addrs, "cf_evict_move", &l.evict_move) ||
-      !take_address(addrs, "cf_kv_write_blocks", &l.write_blocks))
+      !take_address(addrs, "cf_kv_write_blocks", &l.write_blocks) ||
+      !take_address(addrs, "cf_move_blocks", &l.move_blocks))
     return nullptr;
   g_lib = l;
   for (auto [slot, obj] : {std::pair{&g_raw_stream, raw}, std::pair{&g_current_device, cur},
@@ -744,6 +813,7 @@ PyMethodDef kMethods[] = {
     CF_FAST(evict_select),
     CF_FAST(evict_move),
     CF_FAST(kv_write_blocks),
+    CF_FAST(move_blocks),
     {nullptr, nullptr, 0, nullptr},
 };
 #undef CF_FAST

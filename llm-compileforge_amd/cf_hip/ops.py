@@ -1048,6 +1048,11 @@ def move_blocks(caches, moves) -> None:
     moves; each destination is given once.  moves: [n, 2] on the host (a list, numpy
     array or CPU tensor); it is part of the launch, nothing is uploaded."""
     caches = list(caches)
+    if caches and _on_gpu(caches[0]):
+        r = _fast().move_blocks(caches, moves)
+        if r is not None:
+            _result(r, "cf_move_blocks")
+            return
     if isinstance(moves, torch.Tensor) and moves.device.type != "cpu":
         raise ValueError(f"moves must be on the host (got device {moves.device})")
     m = np.asarray(moves)

@@ -13,10 +13,16 @@
 // before the call, so it may be early).
 //
 // The steps and the tensors are kernel arguments: nothing is uploaded, and a
-// captured call replays with the moves it was given.
+// captured call replays with the moves it was given.  A chain costs a word a block.
+//
+// Bound by HBM where the blocks are large or the components many.  A component's
+// steps are one after the other, and a rearranged cache is mostly one long cycle: then
+// the bytes in flight are those of one block over all tensors, times kAhead.  1,800
+// blocks of 256 KiB rearranged at random (945 MB read and written, two thirds of it one
+// cycle): 224 us, 4.2 TB/s of the 4.8 that a large copy reaches; with 8 steps ahead and
+// 8 bytes of arguments a step (7 launches where 3 do) 520.  16 copies of 1 MiB: 10.5 us.
 #include <algorithm>
 #include <numeric>
-#include <unordered_map>
 
 #include "cf_device.hpp"
 #include "cf_host.hpp"
@@ -26,44 +32,56 @@ namespace cf {
 
 namespace {
 
-constexpr int kAhead = 8;
+constexpr int kAhead = 32;
 constexpr int kMoveThreads = 256;
+constexpr int kMoveShapes = 4;    // tensors of a launch differ in at most so many shapes
+constexpr int kMoveCaches = 128;  // tensors of a launch
+constexpr int kMoveLists = 32;    // lists of steps that run side by side
+constexpr int kMoveGroups = 65536;  // workgroups of a tensor
+constexpr int kMoveWords = 952;   // words of a launch: tensors, lists' starts and blocks
+constexpr uint32_t kLastBlock = 1u << 31;
+constexpr uint32_t kAside = kLastBlock - 1;  // in a block's place: the value set aside
 
-struct MoveCache {
-  char* base;
+struct MoveShape {
   int64_t stride, bytes;  // between blocks, of a block
+  int32_t unit;           // bytes a thread moves: 16, 4 or 1
+  int32_t groups;         // workgroups of a tensor (their threads take further pieces in a loop)
+  int32_t first_group, first_cache;
 };
 
+// words: the tensors' addresses (two each), the first block of each list and the end
+// of the last, then the lists: paths of blocks, the last one's word marked.
 struct MoveArgs {
-  MoveCache cache[kMaxMoveCaches];
-  MoveStep step[kMaxMoveSteps];
-  uint16_t first[kMaxMoveSteps + 1];  // first step of each chain
-  uint8_t unit[kMaxMoveCaches];       // bytes a thread moves: 16, 4 or 1
+  MoveShape shape[kMoveShapes];
+  int32_t caches, lists;
+  uint32_t word[kMoveWords + kAhead + 1];  // (read in whole batches, past the end too)
 };
 static_assert(sizeof(MoveArgs) <= 4096, "kernel arguments");
 
 template <class T>
-__device__ __forceinline__ void move_pieces(const MoveArgs& a, const MoveCache& c) {
-  const int begin = a.first[blockIdx.y], end = a.first[blockIdx.y + 1];
-  const int64_t pieces = c.bytes / (int64_t)sizeof(T);
-  for (int64_t i = (int64_t)blockIdx.x * kMoveThreads + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * kMoveThreads) {
-    T* at = (T*)c.base + i;
-    const int64_t stride = c.stride / (int64_t)sizeof(T);
+__device__ __forceinline__ void move_pieces(const uint32_t* __restrict__ word, int begin, int end, char* base,
+                                            const MoveShape& sh, int group) {
+  const int64_t pieces = sh.bytes / (int64_t)sizeof(T), stride = sh.stride / (int64_t)sizeof(T);
+  for (int64_t i = (int64_t)group * kMoveThreads + threadIdx.x; i < pieces; i += (int64_t)sh.groups * kMoveThreads) {
+    T* at = (T*)base + i;
     T aside{};
     for (int e = begin; e < end; e += kAhead) {
+      uint32_t w[kAhead + 1];
+#pragma unroll
+      for (int u = 0; u <= kAhead; ++u) w[u] = word[e + u];
       T v[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int s = e + u < end ? a.step[e + u].src : -1;
+        const uint32_t src = w[u + 1] & ~kLastBlock;
         v[u] = T{};
-        if (s >= 0) v[u] = at[s * stride];
+        if (e + u < end && !(w[u] & kLastBlock) && src != kAside) v[u] = at[src * stride];
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        if (e + u < end) {
-          const MoveStep s = a.step[e + u];
-          if (s.dst >= 0) at[s.dst * stride] = s.src >= 0 ? v[u] : aside;
-          else aside = v[u];
+        if (e + u < end && !(w[u] & kLastBlock)) {
+          const T x = (w[u + 1] & ~kLastBlock) == kAside ? aside : v[u];
+          if (w[u] == kAside) aside = x;
+          else at[w[u] * stride] = x;
         }
       }
     }
@@ -71,24 +89,31 @@ __device__ __forceinline__ void move_pieces(const MoveArgs& a, const MoveCache& 
 }
 
 __global__ __launch_bounds__(kMoveThreads) void move_blocks_kernel(MoveArgs a) {
-  const MoveCache c = a.cache[blockIdx.z];
-  const int unit = a.unit[blockIdx.z];
-  if (unit == 16) move_pieces<uint4>(a, c);
-  else if (unit == 4) move_pieces<uint32_t>(a, c);
-  else move_pieces<uint8_t>(a, c);
+  int k = 0;
+  while (k + 1 < kMoveShapes && (int)blockIdx.x >= a.shape[k + 1].first_group) ++k;
+  const MoveShape sh = a.shape[k];
+  const int at = (int)blockIdx.x - sh.first_group, c = at / sh.groups, group = at - c * sh.groups;
+  char* base = (char*)((uint64_t)a.word[2 * (sh.first_cache + c)] | (uint64_t)a.word[2 * (sh.first_cache + c) + 1] << 32);
+  const uint32_t* lists = a.word + 2 * a.caches + blockIdx.y;
+  const int begin = (int)lists[0], end = (int)lists[1];
+  if (sh.unit == 16) move_pieces<uint4>(a.word, begin, end, base, sh, group);
+  else if (sh.unit == 4) move_pieces<uint32_t>(a.word, begin, end, base, sh, group);
+  else move_pieces<uint8_t>(a.word, begin, end, base, sh, group);
 }
 
 }  // namespace
 
-std::vector<MoveChain> plan_moves(const int32_t* moves, int64_t n) {
-  std::vector<MoveStep> m;
+std::vector<MoveComponent> plan_moves(const int32_t* moves, int64_t n, int64_t blocks) {
+  struct Move {
+    int32_t src, dst;
+  };
+  std::vector<Move> m;
   m.reserve(n);
   for (int64_t i = 0; i < n; ++i)
-    if (moves[2 * i] != moves[2 * i + 1]) m.push_back(MoveStep{moves[2 * i], moves[2 * i + 1]});
-  std::unordered_map<int32_t, int32_t> into;  // destination -> its move
-  into.reserve(m.size() * 2);
+    if (moves[2 * i] != moves[2 * i + 1]) m.push_back(Move{moves[2 * i], moves[2 * i + 1]});
+  std::vector<int32_t> into(blocks, -1);  // the move into a block
   for (size_t i = 0; i < m.size(); ++i) into[m[i].dst] = (int32_t)i;
-  // into_src[i]: the move that overwrites i's source, which has to wait for i
+  // waits[i]: the move that overwrites i's source, which has to wait for i
   std::vector<int32_t> waits(m.size(), -1), pending(m.size(), 0), group(m.size());
   std::iota(group.begin(), group.end(), 0);
   auto root = [&](int32_t i) {
@@ -96,106 +121,172 @@ std::vector<MoveChain> plan_moves(const int32_t* moves, int64_t n) {
     return i;
   };
   for (size_t i = 0; i < m.size(); ++i) {
-    const auto it = into.find(m[i].src);
-    if (it == into.end()) continue;
-    waits[i] = it->second;
-    ++pending[it->second];
-    group[root((int32_t)i)] = root(it->second);
+    const int32_t next = into[m[i].src];
+    if (next < 0) continue;
+    waits[i] = next;
+    ++pending[next];
+    group[root((int32_t)i)] = root(next);
   }
-  // chains in the order of their first move
-  std::vector<MoveChain> chains;
-  std::vector<int32_t> chain_of(m.size(), -1);
-  auto chain = [&](int32_t i) -> MoveChain& {
-    int32_t& c = chain_of[root(i)];
+  // components in the order of their first move
+  std::vector<MoveComponent> all;
+  std::vector<int32_t> index(m.size(), -1);
+  auto component = [&](int32_t i) -> MoveComponent& {
+    int32_t& c = index[root(i)];
     if (c < 0) {
-      c = (int32_t)chains.size();
-      chains.emplace_back();
+      c = (int32_t)all.size();
+      all.emplace_back();
     }
-    return chains[c];
+    return all[c];
   };
   std::vector<char> done(m.size(), 0);
   for (size_t i = 0; i < m.size(); ++i) {
     // a move that nothing waits behind, then the one it made room for, and so on
-    int32_t k = (int32_t)i;
-    while (k >= 0 && !done[k] && pending[k] == 0) {
-      MoveChain& c = chain(k);
-      c.steps.push_back(m[k]);
-      c.whole.push_back(1);
+    if (done[i] || pending[i] != 0) continue;
+    MovePath path{{m[i].dst}, false};
+    for (int32_t k = (int32_t)i; k >= 0 && !done[k] && pending[k] == 0;) {
+      path.blocks.push_back(m[k].src);
       done[k] = 1;
       k = waits[k];
       if (k >= 0) --pending[k];
     }
+    component((int32_t)i).push_back(std::move(path));
   }
   for (size_t i = 0; i < m.size(); ++i) {
     if (done[i]) continue;
     // what is left are cycles: d0 <- d1 <- ... <- d0
-    std::vector<int32_t> cycle;
+    MovePath path{{}, true};
     for (int32_t k = (int32_t)i; !done[k]; k = waits[k]) {
       done[k] = 1;
-      cycle.push_back(m[k].dst);
+      path.blocks.push_back(m[k].dst);
     }
-    MoveChain& c = chain((int32_t)i);
-    // A cycle of d0 ... dk is one of d0 ... dj and then one of dj ... dk: dj holds
-    // d0's value in between.
-    const size_t len = cycle.size();
-    for (size_t at = 0; at + 1 < len;) {
-      const size_t last = std::min(len - 1, at + kMaxCycleSteps - 2);
-      c.steps.push_back(MoveStep{cycle[at], -1});
-      for (size_t k = at; k < last; ++k) c.steps.push_back(MoveStep{cycle[k + 1], cycle[k]});
-      c.steps.push_back(MoveStep{-1, cycle[last]});
-      c.whole.push_back((int32_t)(last - at) + 2);
-      at = last;
-    }
+    component((int32_t)i).push_back(std::move(path));
   }
-  return chains;
+  return all;
 }
 
 namespace {
 
-int32_t launch_moves(const MoveArgs& a, int chains, int caches, hipStream_t stream) {
-  int64_t most = 1;
-  for (int c = 0; c < caches; ++c)
-    if (a.unit[c] > 0) most = std::max(most, ceil_div(a.cache[c].bytes / a.unit[c], kMoveThreads));
-  // (a thread's loop takes what is beyond the grid)
-  const dim3 grid((unsigned)std::min<int64_t>(most, 1024), (unsigned)chains, (unsigned)caches);
-  ProfileScope prof("cf_move_blocks", stream);
-  CF_LAUNCH(move_blocks_kernel, grid, dim3(kMoveThreads), 0, stream, a);
-  CF_HIP_CHECK(hipGetLastError());
+struct MoveCache {
+  char* base;
+  int64_t stride, bytes;
+};
+
+// The steps of a component that no launch has taken yet.
+struct MoveRest {
+  const MoveComponent* paths;
+  size_t path = 0, at = 0;  // at: blocks of the path that are done with
+  int64_t words = 0;
+
+  explicit MoveRest(const MoveComponent& c) : paths(&c) {
+    for (const MovePath& p : c) words += cost(p, 0);
+  }
+  // A path's words from block `from` on: a cycle sets a block aside and back.
+  static int64_t cost(const MovePath& p, size_t from) { return (int64_t)(p.blocks.size() - from) + (p.cycle ? 2 : 0); }
+  bool done() const { return path == paths->size(); }
+  // Appends at most `room` words of steps to a launch's list.
+  void take(int64_t room, std::vector<uint32_t>& list) {
+    while (!done()) {
+      const MovePath& p = (*paths)[path];
+      const int64_t whole = cost(p, at), least = p.cycle ? 4 : 2;
+      if (room < std::min(whole, least)) return;
+      const size_t n = whole <= room ? p.blocks.size() - at : (size_t)(room - (p.cycle ? 2 : 0));
+      if (p.cycle) list.push_back(kAside);
+      for (size_t k = at; k < at + n; ++k) list.push_back((uint32_t)p.blocks[k]);
+      if (p.cycle) list.push_back(kAside);
+      list.back() |= kLastBlock;
+      words -= whole;
+      if (at + n == p.blocks.size()) {
+        room -= whole;
+        ++path;
+        at = 0;
+      } else {
+        // The last block taken is the first of what is left.  In a cycle it holds the
+        // first one's value in between and is read again, in a later launch: steps of
+        // one launch read ahead.
+        at += n - 1;
+        words += cost(p, at);
+        return;
+      }
+    }
+  }
+};
+
+int32_t launch_moves(std::vector<MoveRest>& rest, MoveArgs& a, int64_t groups, hipStream_t stream) {
+  // Lists enough for some threads on every SIMD; a list of single moves has its loads
+  // in flight together.
+  constexpr int64_t kThreads = 256 * 1024;
+  const int64_t wanted = std::min<int64_t>(ceil_div(kThreads, groups * kMoveThreads), kMoveLists);
+  const int64_t room = kMoveWords - 2 * a.caches - (kMoveLists + 1);
+  while (!rest.empty()) {
+    // every long component its share of each of the launches that all need
+    std::sort(rest.begin(), rest.end(), [](const MoveRest& x, const MoveRest& y) { return x.words > y.words; });
+    int64_t all = 0, left = room;
+    for (const MoveRest& r : rest) all += r.words;
+    const int64_t launches = ceil_div(all, room);
+    std::vector<std::vector<uint32_t>> runs;
+    for (MoveRest& r : rest) {
+      const int64_t share = launches == 1 ? left : std::max<int64_t>(ceil_div(r.words, launches) + 2, 64);
+      std::vector<uint32_t> run;
+      r.take(std::min(share, left), run);
+      if (run.empty()) continue;
+      left -= (int64_t)run.size();
+      runs.push_back(std::move(run));
+    }
+    rest.erase(std::remove_if(rest.begin(), rest.end(), [](const MoveRest& r) { return r.done(); }), rest.end());
+    // the longest run to the shortest list
+    std::sort(runs.begin(), runs.end(), [](const auto& x, const auto& y) { return x.size() > y.size(); });
+    std::vector<std::vector<uint32_t>> lists(std::min<size_t>(runs.size(), (size_t)wanted));
+    for (const auto& run : runs) {
+      auto& to = *std::min_element(lists.begin(), lists.end(), [](const auto& x, const auto& y) { return x.size() < y.size(); });
+      to.insert(to.end(), run.begin(), run.end());
+    }
+    a.lists = (int32_t)lists.size();
+    uint32_t* first = a.word + 2 * a.caches;
+    uint32_t at = (uint32_t)(2 * a.caches + a.lists + 1);
+    for (size_t l = 0; l < lists.size(); ++l) {
+      first[l] = at;
+      for (const uint32_t w : lists[l]) a.word[at++] = w;
+    }
+    first[a.lists] = at;
+    const dim3 grid((unsigned)groups, (unsigned)a.lists);
+    ProfileScope prof("cf_move_blocks", stream);
+    CF_LAUNCH(move_blocks_kernel, grid, dim3(kMoveThreads), 0, stream, a);
+    CF_HIP_CHECK(hipGetLastError());
+  }
   return CF_OK;
 }
 
-int32_t move_all(const std::vector<MoveCache>& caches, const int32_t* moves, int64_t n, hipStream_t stream) {
-  const std::vector<MoveChain> chains = plan_moves(moves, n);
-  for (size_t c0 = 0; c0 < caches.size(); c0 += kMaxMoveCaches) {
-    const int nc = (int)std::min<size_t>(kMaxMoveCaches, caches.size() - c0);
+int32_t move_all(std::vector<MoveCache>& caches, const int32_t* moves, int64_t n, int64_t blocks, hipStream_t stream) {
+  const std::vector<MoveComponent> plan = plan_moves(moves, n, blocks);
+  if (plan.empty()) return CF_OK;
+  auto shape = [](const MoveCache& c) { return std::make_pair(c.bytes, c.stride); };
+  std::stable_sort(caches.begin(), caches.end(), [&](const auto& x, const auto& y) { return shape(x) > shape(y); });
+  auto unit_of = [](const MoveCache& c) {
+    const uint64_t all = (uint64_t)(uintptr_t)c.base | (uint64_t)c.stride | (uint64_t)c.bytes;
+    return all % 16 == 0 ? 16 : (all % 4 == 0 ? 4 : 1);
+  };
+  for (size_t c = 0; c < caches.size();) {
     MoveArgs a{};
-    for (int c = 0; c < nc; ++c) {
-      a.cache[c] = caches[c0 + c];
-      const uint64_t all = (uint64_t)(uintptr_t)a.cache[c].base | (uint64_t)a.cache[c].stride | (uint64_t)a.cache[c].bytes;
-      a.unit[c] = all % 16 == 0 ? 16 : (all % 4 == 0 ? 4 : 1);
-    }
-    int steps = 0, count = 0;
-    auto flush = [&]() -> int32_t {
-      if (count == 0) return CF_OK;
-      a.first[count] = (uint16_t)steps;
-      const int32_t rc = launch_moves(a, count, nc, stream);
-      steps = count = 0;
-      return rc;
-    };
-    for (const MoveChain& ch : chains) {
-      size_t at = 0;
-      bool open = false;
-      for (const int32_t w : ch.whole) {
-        if (steps + w > kMaxMoveSteps) {  // the rest of the chain follows on the stream
-          if (const int32_t rc = flush()) return rc;
-          open = false;
-        }
-        if (!open) a.first[count++] = (uint16_t)steps;
-        open = true;
-        for (int32_t k = 0; k < w; ++k) a.step[steps++] = ch.steps[at++];
+    int shapes = 0;
+    int64_t groups = 0;
+    for (; c < caches.size() && a.caches < kMoveCaches; ++c) {
+      const int unit = unit_of(caches[c]);
+      const int64_t own = std::min<int64_t>(ceil_div(caches[c].bytes / unit, kMoveThreads), kMoveGroups);
+      MoveShape* s = shapes > 0 ? &a.shape[shapes - 1] : nullptr;
+      if (s == nullptr || s->bytes != caches[c].bytes || s->stride != caches[c].stride || s->unit != unit) {
+        if (shapes == kMoveShapes) break;
+        s = &a.shape[shapes++];
+        *s = MoveShape{caches[c].stride, caches[c].bytes, unit, (int32_t)own, (int32_t)groups, a.caches};
       }
+      groups += own;
+      const uint64_t base = (uint64_t)(uintptr_t)caches[c].base;
+      a.word[2 * a.caches] = (uint32_t)base;
+      a.word[2 * a.caches + 1] = (uint32_t)(base >> 32);
+      ++a.caches;
     }
-    if (const int32_t rc = flush()) return rc;
+    for (int k = shapes; k < kMoveShapes; ++k) a.shape[k].first_group = INT32_MAX;
+    std::vector<MoveRest> rest(plan.begin(), plan.end());
+    if (const int32_t rc = launch_moves(rest, a, groups, stream)) return rc;
   }
   return CF_OK;
 }
@@ -224,19 +315,21 @@ extern "C" int32_t cf_move_blocks(const CfTensor* caches, int32_t n_caches, cons
       if (v.size[0] > 0 && v.size[1] > 0) list.push_back(MoveCache{v.base, v.stride[0] * v.elem, v.size[1] * v.elem});
     }
     if (n_caches == 0) return CF_OK;
-    std::vector<int32_t> to;
-    to.reserve(n_moves);
+    CF_CHECK(list.empty() || blocks < INT32_MAX, "caches of %lld blocks are too large", (long long)blocks);
+    int64_t most = -1;
     for (int64_t i = 0; i < n_moves; ++i) {
       const int32_t s = moves[2 * i], d = moves[2 * i + 1];
       CF_CHECK(s >= 0 && s < blocks && d >= 0 && d < blocks, "move %lld: block %d or %d is outside the caches' %lld blocks",
                (long long)i, s, d, (long long)blocks);
-      to.push_back(d);
+      most = std::max<int64_t>(most, std::max(s, d));
     }
-    std::sort(to.begin(), to.end());
-    const auto twice = std::adjacent_find(to.begin(), to.end());
-    CF_CHECK(twice == to.end(), "block %d is the destination of two moves", twice == to.end() ? 0 : *twice);
+    std::vector<char> taken(most + 1, 0);
+    for (int64_t i = 0; i < n_moves; ++i) {
+      CF_CHECK(!taken[moves[2 * i + 1]], "block %d is the destination of two moves", moves[2 * i + 1]);
+      taken[moves[2 * i + 1]] = 1;
+    }
     if (n_moves == 0 || list.empty()) return CF_OK;
-    return move_all(list, moves, n_moves, (hipStream_t)stream);
+    return move_all(list, moves, n_moves, most + 1, (hipStream_t)stream);
   } catch (...) {
     set_error("cf_move_blocks: out of host memory");
     return CF_ERR_INVALID;

@@ -1,33 +1,24 @@
 // Moves of whole blocks over several paged tensors at once.
 #pragma once
 
-#include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <vector>
 
 namespace cf {
 
-// Steps of a plan: block dst takes what block src holds; src -1: what the group's
-// first step set aside; dst -1: src is set aside.
-struct MoveStep {
-  int32_t src, dst;
+// Blocks of which each takes what the next one holds, from the first on; in a cycle
+// the last takes what the first one held.
+struct MovePath {
+  std::vector<int32_t> blocks;
+  bool cycle;
 };
 
-// Simultaneous moves as steps that can be taken one after the other.  The steps of
-// a chain depend on each other and keep their order; chains are independent.
-// `whole`: lengths of runs of steps that stay together in a launch (a cycle's share
-// the value set aside), in order, per chain.
-struct MoveChain {
-  std::vector<MoveStep> steps;
-  std::vector<int32_t> whole;
-};
+// Simultaneous moves as paths that can be taken one after the other: those of a
+// component depend on each other and keep their order, components are independent.
+using MoveComponent = std::vector<MovePath>;
 
-constexpr int kMaxMoveSteps = 320;   // of a launch
-constexpr int kMaxMoveCaches = 16;   // of a launch
-constexpr int kMaxCycleSteps = 256;  // a longer cycle is taken in parts
-
-// moves [n][2] = (source, destination), each destination once.
-std::vector<MoveChain> plan_moves(const int32_t* moves, int64_t n);
+// moves [n][2] = (source, destination) of blocks [0, blocks), each destination once.
+std::vector<MoveComponent> plan_moves(const int32_t* moves, int64_t n, int64_t blocks);
 
 }  // namespace cf
