@@ -656,7 +656,8 @@ int32_t cf_copy_blocks(CfTensor* cache, const CfTensor* pairs, void* stream);
  *   caches  n_caches descriptors; of different dtypes and sizes, any count
  *   moves   [n_moves][2] i32 on the host, ids within every tensor's blocks; read
  *           by the call (a captured call replays these moves)
- * In one launch for up to 16 tensors and about 300 moves. */
+ * In one launch for up to 128 tensors of at most 4 shapes, and moves of some 650
+ * blocks; what is beyond follows in further launches. */
 int32_t cf_move_blocks(const CfTensor* caches, int32_t n_caches, const int32_t* moves, int64_t n_moves, void* stream);
 
 /* Kernel timing hook for benchmarks (no reference counterpart).  While

@@ -676,9 +676,10 @@ constexpr bool kBlocks = std::is_same<Pm, PrefillBlockParams>::value;
 // Block scales.  A lane's 8 tokens of a tile lie in one block (lanes lq 0-1: block a,
 // 2-3: block b).  Its K scale is the factor of the lane's scores.  Its V scale is
 // 2^e * f with f in [1, 2): 2^e goes to the codes as they are staged, against a
-// reference 2^eref that is the largest of the item's tiles so far (O is in its units
-// and follows it), kVHead binades below fp16's largest, so that a block of 2^-21
-// (e4m3; int8 2^-28) of the largest before it keeps every bit of its codes; f goes to
+// reference 2^eref that is the largest of the item's passes so far (below; O is in its
+// units and follows it), kVHead binades below fp16's largest, so that a block of 2^-21
+// (e4m3; int8 2^-28) of that keeps every bit of its codes, and one below it is off by
+// less than the half step 2^-25 of a weight is beside the largest; f goes to
 // the exponent of the tile's weights, and the row sums take 1 / f of it back: the P.V
 // product against a channel of ones has 1 / f in their place, as two fp16 terms in
 // rows 0 and 1.  A weight is rounded to fp16 once, as without block scales.
@@ -686,10 +687,12 @@ constexpr bool kBlocks = std::is_same<Pm, PrefillBlockParams>::value;
 // What the tiles need of their scales is formed kScaleTiles tiles at a time, a thread
 // a block, and kept in LDS; a step then takes three LDS reads and about ten other
 // instructions for it.  Eight 512-row chunks behind 0-4,096 tokens, e4m3 under bf16:
-// 211 us; with every wave loading and forming its tile's own a step ahead
-// 218-220 (some 60 instructions a step), one scale a head 183; int8 223 and
-// 230-237.  V's scales multiplied into P, P in two bf16 terms and row sums by
-// addition took 264 (int8, fp16 queries).
+// 206 us, with every wave loading and forming its tile's own a step ahead 218-220
+// (some 60 instructions a step), one scale a head 183; int8 218 and 230-237 (fp16
+// queries 214).  V's scales multiplied into P, P in two bf16 terms and row sums by
+// addition took 264 (int8, fp16 queries).  What can change O ahead of a tile's P.V
+// product stands in one branch with the softmax's own rescaling: a second one ahead of
+// Q.K took 209.
 constexpr int kScaleTiles = 128;              // of a pass
 constexpr int kScaleSlots = 2 * kScaleTiles;  // tiles held
 struct alignas(16) BlockScale {
@@ -707,35 +710,43 @@ template <int KT>
 constexpr int kVHead = KT == kI8 ? 5 : 7;
 __device__ __forceinline__ float power_of_two(int e) { return u2f((uint32_t)max(e + 127, 0) << 23); }  // e < 128
 
-// The tiles first .. + kScaleTiles - 1 of an item (whose own first one is jt0) into
-// their slots; eref: the reference of the tile before.  All 256 threads.
-template <int KT>
-__device__ __forceinline__ void fill_scales(const PrefillBlockParams& p, ScaleWindow* w, const float* __restrict__ kscale,
-                                            const float* __restrict__ vscale, const int32_t* __restrict__ trow, int jt0,
-                                            int first, int nt, int nblk, int h, float qk_scale, int& eref, int tid) {
-  const int j = first + (tid >> 1), X = tid & 1, jb = 2 * j + X;
-  int id = -1;
-  if (j < nt && jb < nblk) id = trow[(int64_t)jb * p.t_sm];
-  const bool valid = (unsigned)id < (unsigned)p.NB;
-  float k = 1.0f, v = 0.0f;
-  if (valid) {
-    k = kscale[id * p.ks_b + h * p.ks_s];
-    v = vscale[id * p.vs_b + h * p.vs_s];
+// A pass over the tiles first .. + kScaleTiles - 1 of an item, in three steps whose
+// loads a caller overlaps with others: the thread's block, its scales, and their
+// slots (jt0: the item's first tile, eref: the reference of the tile before first).
+// All 256 threads.
+__device__ __forceinline__ int scale_block(const PrefillBlockParams& p, const int32_t* __restrict__ trow, int first, int nt,
+                                           int nblk, int tid) {
+  const int j = first + (tid >> 1), jb = 2 * j + (tid & 1);
+  return j < nt && jb < nblk ? trow[(int64_t)jb * p.t_sm] : -1;
+}
+struct ScalePair {
+  float k, v;
+  bool valid;
+};
+__device__ __forceinline__ ScalePair scale_pair(const PrefillBlockParams& p, const float* __restrict__ kscale,
+                                                const float* __restrict__ vscale, int id, int h) {
+  ScalePair s{1.0f, 0.0f, (unsigned)id < (unsigned)p.NB};
+  if (s.valid) {
+    s.k = kscale[id * p.ks_b + h * p.ks_s];
+    s.v = vscale[id * p.vs_b + h * p.vs_s];
   }
+  return s;
+}
+template <int KT>
+__device__ __forceinline__ void fill_scales(ScaleWindow* w, const ScalePair& in, int jt0, int first, float qk_scale,
+                                            int& eref, int tid) {
+  const int j = first + (tid >> 1), X = tid & 1;
+  const bool valid = in.valid;
+  float k = in.k, v = in.v;
   const bool bad = !(__builtin_fabsf(k) < INFINITY && __builtin_fabsf(v) < INFINITY);
   if (bad) k = 1.0f, v = 0.0f;
-  const int e = (int)((f2u(v) >> 23) & 0xFFu), pair = max(e, __shfl_xor(e, 1, 64));
-  const int incl = wave_incl_max(pair, 0);
+  const int e = (int)((f2u(v) >> 23) & 0xFFu);
   const int mine = (valid ? 1 : 0) << X | (bad ? 1 : 0) << (2 + X), flags = mine | __shfl_xor(mine, 1, 64);
-  if ((tid & 63) == 63) w->top[tid >> 6] = incl;
+  const int top = (int)wave_umax((uint32_t)e);
+  if ((tid & 63) == 0) w->top[tid >> 6] = top;
   __syncthreads();
-  int before = eref, all = eref;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i < (tid >> 6)) before = max(before, w->top[i]);
-    all = max(all, w->top[i]);
-  }
-  const int own = max(before, incl);
+  for (int i = 0; i < 4; ++i) eref = max(eref, w->top[i]);
   const float f = u2f((f2u(v) & 0x007FFFFFu) | 0x3F800000u), r = 1.0f / f;
   const _Float16 hi = (_Float16)r, lo = (_Float16)(r - (float)hi);
   const int slot = (j - jt0) & (kScaleSlots - 1);
@@ -743,10 +754,9 @@ __device__ __forceinline__ void fill_scales(const PrefillBlockParams& p, ScaleWi
   s.k = fmaxf(qk_scale * k, 1e-30f);  // (a product of 0: as for one scale a head)
   s.lf = __builtin_amdgcn_logf(f);
   s.inv = (uint32_t)__builtin_bit_cast(uint16_t, hi) | ((uint32_t)__builtin_bit_cast(uint16_t, lo) << 16);
-  s.g = power_of_two(e - own + kVHead<KT>);
+  s.g = power_of_two(e - eref + kVHead<KT>);
   w->at[slot][X] = s;
-  if (X == 0) w->word[slot] = own << 4 | flags;
-  eref = all;
+  if (X == 0) w->word[slot] = eref << 4 | flags;
   __syncthreads();
 }
 
@@ -887,6 +897,11 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
     const int nblk = (kvlen + 15) >> 4, nfull = kvlen >> 5;
     const int64_t tsm = p.t_sm;
     const int32_t* tp = trow + 2 * (jt0 + 3) * tsm;  // table entry of tile jt0 + 3's first block, advanced every step
+    int sid0 = -1, sid1 = -1;  // blocks of the first two passes over the scales
+    if constexpr (kBlocks<Pm>) {
+      sid0 = scale_block(p, trow, jt0, nt, nblk, tid);
+      sid1 = scale_block(p, trow, jt0 + kScaleTiles, nt, nblk, tid);
+    }
     TileIds id0 = tile_ids(p, trow, jt0, kvlen);
     TileIds id1 = jt0 + 1 < nt ? tile_ids(p, trow, jt0 + 1, kvlen) : id0;
     TileIds id2 = jt0 + 2 < nt ? tile_ids(p, trow, jt0 + 2, kvlen) : id1;
@@ -902,10 +917,9 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       TileIds idv = id0;
       float g0 = 1.0f;
       if constexpr (kBlocks<Pm>) {
-        fill_scales<KT>(p, &s_scales, kscale, vscale, trow, jt0, jt0, nt, nblk, h, qk_scale, eref, tid);
-        if (nt - jt0 > kScaleTiles)
-          fill_scales<KT>(p, &s_scales, kscale, vscale, trow, jt0, jt0 + kScaleTiles, nt, nblk, h, qk_scale, eref, tid);
-        sc = s_scales.at[0][lq >> 1];
+        const ScalePair sa = scale_pair(p, kscale, vscale, sid0, h), sb = scale_pair(p, kscale, vscale, sid1, h);
+        fill_scales<KT>(&s_scales, sa, jt0, jt0, qk_scale, eref, tid);
+        if (nt - jt0 > kScaleTiles) fill_scales<KT>(&s_scales, sb, jt0, jt0 + kScaleTiles, qk_scale, eref, tid);
         g0 = s_scales.at[0][sx].g;
         word0 = uniform(s_scales.word[0]);
         g1 = s_scales.at[1][sx].g;
@@ -923,6 +937,8 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
     (void)eref;
     (void)sx;
     (void)scale_slot;
+    (void)sid0;
+    (void)sid1;
     if (jt0 + 1 < nt) stage_load<KT, D, VTOK>(kr, vr, p, id1, h, tid);
     __syncthreads();
 
@@ -1068,6 +1084,7 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       const int valid_next = kvlen - 32 * (j + 1);
       // (V of a block whose scales are not finite is zeroed like an invalid one's:
       // its codes may be NaN, and 0 * NaN would reach rows that do not see it)
+      if constexpr (kBlocks<Pm>) sc = s_scales.at[scale_slot(j)][lq >> 1];
       TileIds idv = id1;
       if constexpr (kBlocks<Pm>) idv.ok = word1 & ~(word1 >> 2) & 3;
       if (!(j + 2 <= nfull && idv.ok == 3)) mask_staged_v<KT, D, VTOK>(vr, idv, valid_next, tid);
@@ -1090,7 +1107,6 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       float qk0 = qk_scale;
       if constexpr (kBlocks<Pm>) {
         qk0 = sc.k;
-        if (((word0 ^ (eo << 4)) & ~3) != 0) odd_scales(word0, 32 * j + 8 * lq);
       }
       const bool edge = j >= lmin_t || id0.ok != 3;
       const int tok0 = 32 * j + 8 * lq;
@@ -1130,8 +1146,17 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       }
       if (edge) mask(K1, s1b, s2b, id0.ok, tok0);
       const float mtb = lane_max(s1b, s2b, qk0);
+      float g2 = 0.0f;
+      int word2 = 0;
+      if constexpr (kBlocks<Pm>) {
+        g2 = s_scales.at[scale_slot(j + 2)][sx].g;
+        word2 = s_scales.word[scale_slot(j + 2)];
+      }
       const bool up_a = mta > m[0] + 8.0f, up_b = mtb > m[1] + 8.0f;
-      if (__any(up_a || up_b)) {
+      const bool odd = kBlocks<Pm> && ((word0 ^ (eo << 4)) & ~3) != 0;
+      if (__any(up_a || up_b || odd)) {
+        if constexpr (kBlocks<Pm>)
+          if (odd) odd_scales(word0, 32 * j + 8 * lq);
         rescale(K0, mta);
         rescale(K1, mtb);
       }
@@ -1149,10 +1174,9 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       }
       const TileIds id3 = j + 3 < nt ? tile_resolve(raw_a, raw_b, p.NB) : id2;
       if constexpr (kBlocks<Pm>) {
-        sc = s_scales.at[scale_slot(j + 1)][lq >> 1];
-        g1 = s_scales.at[scale_slot(j + 2)][sx].g;
         word0 = word1;
-        word1 = uniform(s_scales.word[scale_slot(j + 2)]);
+        word1 = uniform(word2);
+        g1 = g2;
       }
       __syncthreads();
       id0 = id1;
@@ -1164,7 +1188,8 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
         // the slots of the half of the window that the item has left behind
         const int rel = j - jt0, next = j + kScaleTiles - 2;
         if (rel > kScaleTiles && (rel & (kScaleTiles - 1)) == 2 && next < nt)
-          fill_scales<KT>(p, &s_scales, kscale, vscale, trow, jt0, next, nt, nblk, h, qk_scale, eref, tid);
+          fill_scales<KT>(&s_scales, scale_pair(p, kscale, vscale, scale_block(p, trow, next, nt, nblk, tid), h), jt0, next,
+                          qk_scale, eref, tid);
       }
       step(std::integral_constant<int, 0>{}, j);
       if (j + 1 < nt) step(std::integral_constant<int, 1>{}, j + 1);
