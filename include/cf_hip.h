@@ -413,7 +413,7 @@ int32_t cf_kv_write_fp8(const CfTensor* k_new, const CfTensor* v_new,
  *                     q_start[n + 1]); NULL: T = N and row n is sequence n's (none
  *                     where seq_lens[n] is 0)
  *   k_cache, v_cache  [NB, bs, H, D]   e4m3fn | i8, one dtype, any strides
- *   k_scale, v_scale  [NB, H]          f32, any strides
+ *   k_scale, v_scale  [NB, H]          f32, any strides; the four apart
  * Rows at negative positions or past Mb * bs are skipped, and those of blocks
  * outside [0, NB).  The blocks written to must be their sequence's own
  * (cf_bp_prepare_writes): two sequences with rows for one block race. */
@@ -653,7 +653,7 @@ int32_t cf_copy_blocks(CfTensor* cache, const CfTensor* pairs, void* stream);
  * block moves[i][1] takes what block moves[i][0] held before the call.  A source
  * may be given to several destinations, and a destination may be a source of other
  * moves (chains and cycles are taken in place); a destination is given once.
- *   caches  n_caches descriptors; of different dtypes and sizes, any count
+ *   caches  n_caches descriptors; of different dtypes and sizes, any count, apart
  *   moves   [n_moves][2] i32 on the host, ids within every tensor's blocks; read
  *           by the call (a captured call replays these moves)
  * In one launch for up to 128 tensors of at most 4 shapes, and moves of some 650

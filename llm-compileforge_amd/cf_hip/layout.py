@@ -62,6 +62,17 @@ def alloc_kv_cache(
     raise ValueError(f"unknown KV layout {layout!r}; expected one of {LAYOUTS}")
 
 
+def paired_storage(k_cache: torch.Tensor, v_cache: torch.Tensor) -> torch.Tensor:
+    """[NB, Hkv, 2, bs * D] over the one allocation of a paired cache: the tensor whose
+    blocks hold both halves, as block copies and moves take it (the two views' blocks
+    are not contiguous)."""
+    nb, bs, h, d = k_cache.shape
+    paired = layout_of(k_cache, False) == "paired" and layout_of(v_cache, True) == "paired" and k_cache.dtype == v_cache.dtype
+    if not paired or v_cache.shape != k_cache.shape or v_cache.data_ptr() != k_cache.data_ptr() + bs * d * k_cache.element_size():
+        raise ValueError("expected the two views of one paired cache")
+    return k_cache.as_strided((nb, h, 2, bs * d), (h * 2 * bs * d, 2 * bs * d, bs * d, 1))
+
+
 def alloc_kv_scales(
     num_blocks: int, num_kv_heads: int, device: torch.device | str
 ) -> tuple[torch.Tensor, torch.Tensor]:

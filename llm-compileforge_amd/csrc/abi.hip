@@ -1225,8 +1225,9 @@ int32_t cf_kv_write_blocks(const CfTensor* k_new, const CfTensor* v_new, const C
   p.D = (int)D;
   p.bs = (int)bs;
   p.units = q_start != nullptr ? T / bs + 2 * N : N;
-  CF_CHECK(p.units < (int64_t)INT32_MAX, "too many blocks");
   if (T == 0 || N == 0 || H == 0 || D == 0 || NB == 0 || p.Mb == 0) return CF_OK;
+  CF_CHECK(p.units < (int64_t)1 << 24, "too many rows or sequences: they may touch %lld blocks", (long long)p.units);
+  CF_CHECK(vc[0].base != vc[1].base && vs[0].base != vs[1].base, "keys and values cannot share a cache or its scales");
   return launch_kv_blocks(p, vx[0].dtype, vc[0].dtype, as_stream(stream));
 }
 

@@ -315,6 +315,10 @@ extern "C" int32_t cf_move_blocks(const CfTensor* caches, int32_t n_caches, cons
       if (v.size[0] > 0 && v.size[1] > 0) list.push_back(MoveCache{v.base, v.stride[0] * v.elem, v.size[1] * v.elem});
     }
     if (n_caches == 0) return CF_OK;
+    std::vector<const char*> bases;
+    for (const MoveCache& c : list) bases.push_back(c.base);
+    std::sort(bases.begin(), bases.end());
+    CF_CHECK(std::adjacent_find(bases.begin(), bases.end()) == bases.end(), "one of the caches is given twice");
     CF_CHECK(list.empty() || blocks < INT32_MAX, "caches of %lld blocks are too large", (long long)blocks);
     int64_t most = -1;
     for (int64_t i = 0; i < n_moves; ++i) {

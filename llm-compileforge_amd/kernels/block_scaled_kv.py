@@ -17,7 +17,8 @@ within such a block: over N(0, 1) values 0.9 % of their root mean square, e4m3fn
 `paged_attention`, `paged_attention_tensors` and `chunked_prefill_attention` read such
 a cache where their k_scale and v_scale are [num_blocks, heads]; so does
 cf_hip.ops.paged_gather.  A block is copied or moved together with its scales:
-BlockManager.copy_blocks and move_blocks take them as two more tensors.
+BlockManager.copy_blocks and move_blocks take them as two more tensors (and a paired
+cache as the one tensor that cf_hip.layout.paired_storage gives).
 """
 
 from __future__ import annotations

@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from cf_hip import _abi, ops
+from cf_hip import _abi, layout, ops
 from cf_hip.layout import alloc_kv_cache, alloc_kv_scales
 from compiler.cache_policy import CachePolicy
 from kernels.block_scaled_kv import write_kv_blocks
@@ -151,6 +151,46 @@ def test_moves_refuse(moves, says):
     cache = torch.zeros(8, 40, dtype=torch.uint8)
     assert _moves([cache], moves) == _abi.CF_ERR_INVALID
     assert says in _message()
+
+
+def test_write_refuses_one_tensor_for_both():
+    rows, cache = torch.zeros(1, 2, 64, dtype=torch.bfloat16), torch.zeros(2, 8, 16, 2, 64, dtype=torch.int8)
+    scale, one = torch.ones(2, 8, 2), torch.ones(1, dtype=torch.int32)
+    for c, s in (((0, 0), (0, 1)), ((0, 1), (1, 1))):
+        d = [_desc(t) for t in (rows, rows, torch.zeros(1, 4, dtype=torch.int32), one)]
+        d += [None] + [_desc(t) for t in (cache[c[0]], cache[c[1]], scale[s[0]], scale[s[1]])]
+        rc = _abi.lib().cf_kv_write_blocks(*(None if x is None else _abi.ref(x) for x in d), None)
+        assert rc == _abi.CF_ERR_INVALID and "cannot share" in _message()
+
+
+def test_write_refuses_more_blocks_than_a_launch_takes():
+    row, one = torch.zeros(1, 1, 8, dtype=torch.bfloat16), torch.ones(1, dtype=torch.int32)
+    n = 1 << 24
+    many = row.expand(n, 1, 8)  # (descriptors only: nothing is read)
+    cache, scale = torch.zeros(2, 8, 16, 1, 8, dtype=torch.int8), torch.ones(2, 8, 1)
+    d = [_desc(t) for t in (many, many, one.view(1, 1).expand(n, 1), one.expand(n), cache[0], cache[1], scale[0], scale[1])]
+    rc = _abi.lib().cf_kv_write_blocks(*(_abi.ref(x) for x in d[:4]), None, *(_abi.ref(x) for x in d[4:]), None)
+    assert rc == _abi.CF_ERR_INVALID and "16777216 blocks" in _message()
+
+
+def test_moves_refuse_a_cache_twice():
+    cache = torch.zeros(8, 40, dtype=torch.uint8)
+    assert _moves([cache, torch.zeros(8, 4, dtype=torch.uint8), cache], [(1, 7)]) == _abi.CF_ERR_INVALID
+    assert "given twice" in _message()
+
+
+def test_paired_storage():
+    k, v = layout.alloc_kv_cache(6, 16, 2, 8, torch.int8, "cpu", "paired")
+    k.copy_(torch.randint(-9, 9, k.shape))
+    v.copy_(torch.randint(-9, 9, v.shape))
+    both = layout.paired_storage(k, v)
+    assert both.is_contiguous() and both.data_ptr() == k.data_ptr() and both.shape == (6, 2, 2, 128)
+    assert torch.equal(both[:, :, 0].view(6, 2, 16, 8), k.transpose(1, 2))
+    assert torch.equal(both[:, :, 1].view(6, 2, 8, 16), v.permute(0, 2, 3, 1))
+    with pytest.raises(ValueError, match="one paired cache"):
+        layout.paired_storage(*layout.alloc_kv_cache(6, 16, 2, 8, torch.int8, "cpu", "native"))
+    with pytest.raises(ValueError, match="one paired cache"):
+        layout.paired_storage(k, layout.alloc_kv_cache(6, 16, 2, 8, torch.int8, "cpu", "paired")[1])
 
 
 def test_moves_refuse_caches():

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from cf_hip import ops
+from cf_hip.layout import alloc_kv_cache, alloc_kv_scales, paired_storage
 from python_runtime.engine.block_manager import BlockManager
 
 pytestmark = pytest.mark.gpu
@@ -75,6 +76,23 @@ def test_slab_views():
     _check([slab, apart], [(0, 11), (11, 3), (3, 0), (5, 6)])
     with pytest.raises(ValueError, match="dense"):
         ops.move_blocks([slab[:, :, :4]], [(0, 1)])
+
+
+def test_paired_cache_with_its_scales():
+    k, v = alloc_kv_cache(12, 16, 3, 64, torch.int8, "cuda", "paired")
+    for c in (k, v):
+        c.copy_(torch.randint(-127, 128, c.shape, dtype=torch.int8))
+    ks, vs = alloc_kv_scales(12, 3, "cuda")
+    ks.uniform_()
+    vs.uniform_()
+    was = [t.clone() for t in (k, v, ks, vs)]
+    moves = [(0, 5), (5, 11), (11, 0), (3, 4), (3, 9)]
+    BlockManager.move_blocks(moves, [paired_storage(k, v), ks, vs])
+    for t, w in zip((k, v, ks, vs), was):
+        want = w.clone()
+        for s, d in moves:
+            want[d] = w[s]
+        assert torch.equal(t, want)
 
 
 def test_moves_as_tensor_and_array():
