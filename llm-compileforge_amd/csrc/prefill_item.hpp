@@ -685,14 +685,13 @@ constexpr bool kBlocks = std::is_same<Pm, PrefillBlockParams>::value;
 // rows 0 and 1.  A weight is rounded to fp16 once, as without block scales.
 //
 // What the tiles need of their scales is formed kScaleTiles tiles at a time, a thread
-// a block, and kept in LDS; a step then takes three LDS reads and about ten other
+// a block, and kept in LDS; a step then takes two LDS reads and about twenty other
 // instructions for it.  Eight 512-row chunks behind 0-4,096 tokens, e4m3 under bf16:
-// 206 us, with every wave loading and forming its tile's own a step ahead 218-220
-// (some 60 instructions a step), one scale a head 183; int8 218 and 230-237 (fp16
-// queries 214).  V's scales multiplied into P, P in two bf16 terms and row sums by
-// addition took 264 (int8, fp16 queries).  What can change O ahead of a tile's P.V
-// product stands in one branch with the softmax's own rescaling: a second one ahead of
-// Q.K took 209.
+// 205 us, with every wave loading and forming its tile's own a step ahead 218-220
+// (some 60 instructions a step), one scale a head 187; int8 218 and 230-237.  V's
+// scales multiplied into P, P in two bf16 terms and row sums by addition took 264
+// (int8, fp16 queries).  What can change O ahead of a tile's P.V product stands in one
+// branch with the softmax's own rescaling: a second one ahead of Q.K cost 3 us.
 constexpr int kScaleTiles = 128;              // of a pass
 constexpr int kScaleSlots = 2 * kScaleTiles;  // tiles held
 struct alignas(16) BlockScale {
@@ -700,10 +699,10 @@ struct alignas(16) BlockScale {
   float lf;      // log2 f
   uint32_t inv;  // 1 / f as two fp16 terms
   float g;       // the power of two of the V codes
+  int word;      // of the tile: eref (with a float's bias) << 4 | blocks with NaN or infinite scales << 2 | the other valid ones
 };
 struct ScaleWindow {
   BlockScale at[kScaleSlots][2];
-  int word[kScaleSlots];  // eref (with a float's bias) << 4 | blocks with NaN or infinite scales << 2 | valid blocks
   int top[4];
 };
 template <int KT>
@@ -741,7 +740,7 @@ __device__ __forceinline__ void fill_scales(ScaleWindow* w, const ScalePair& in,
   const bool bad = !(__builtin_fabsf(k) < INFINITY && __builtin_fabsf(v) < INFINITY);
   if (bad) k = 1.0f, v = 0.0f;
   const int e = (int)((f2u(v) >> 23) & 0xFFu);
-  const int mine = (valid ? 1 : 0) << X | (bad ? 1 : 0) << (2 + X), flags = mine | __shfl_xor(mine, 1, 64);
+  const int mine = (bad ? 4 : (valid ? 1 : 0)) << X, flags = mine | __shfl_xor(mine, 1, 64);
   const int top = (int)wave_umax((uint32_t)e);
   if ((tid & 63) == 0) w->top[tid >> 6] = top;
   __syncthreads();
@@ -755,8 +754,8 @@ __device__ __forceinline__ void fill_scales(ScaleWindow* w, const ScalePair& in,
   s.lf = __builtin_amdgcn_logf(f);
   s.inv = (uint32_t)__builtin_bit_cast(uint16_t, hi) | ((uint32_t)__builtin_bit_cast(uint16_t, lo) << 16);
   s.g = power_of_two(e - eref + kVHead<KT>);
+  s.word = eref << 4 | flags;
   w->at[slot][X] = s;
-  if (X == 0) w->word[slot] = eref << 4 | flags;
   __syncthreads();
 }
 
@@ -906,12 +905,13 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
     TileIds id1 = jt0 + 1 < nt ? tile_ids(p, trow, jt0 + 1, kvlen) : id0;
     TileIds id2 = jt0 + 2 < nt ? tile_ids(p, trow, jt0 + 2, kvlen) : id1;
     // Block scales: the lane's of tile j (sc), the staging's of tile j + 1 (g1), the
-    // words of both, O's reference (eo) and that of the last tile formed (eref).
+    // words of both, O's reference (eo4) and that of the last tile formed (eref).
     BlockScale sc{};
     float g1 = 1.0f;
-    int word0 = 3, word1 = 3, eo = 0, eref = 0;
+    int word0 = 3, word1 = 3, eo4 = 0, eref = 0;
     const int sx = (tid / D) & 1;  // the block whose V this thread stages
-    auto scale_slot = [&](int j) { return (j - jt0) & (kScaleSlots - 1); };
+    // the lane's entries of the pair of tiles at hand, the staging's of the next pair
+    const BlockScale *scale_now = nullptr, *scale_next = nullptr;
     if (jt0 < nt) {
       stage_load<KT, D, VTOK>(kr, vr, p, id0, h, tid);
       TileIds idv = id0;
@@ -921,11 +921,11 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
         fill_scales<KT>(&s_scales, sa, jt0, jt0, qk_scale, eref, tid);
         if (nt - jt0 > kScaleTiles) fill_scales<KT>(&s_scales, sb, jt0, jt0 + kScaleTiles, qk_scale, eref, tid);
         g0 = s_scales.at[0][sx].g;
-        word0 = uniform(s_scales.word[0]);
+        word0 = uniform(s_scales.at[0][sx].word);
         g1 = s_scales.at[1][sx].g;
-        word1 = uniform(s_scales.word[1]);
-        eo = word0 >> 4;
-        idv.ok = word0 & ~(word0 >> 2) & 3;
+        word1 = uniform(s_scales.at[1][sx].word);
+        eo4 = word0 & ~15;
+        idv.ok = word0 & 3;
       }
       stage_write<QT, KT, D, VTOK, kBlocks<Pm>>(lds[0], kr, vr, idv, kvlen - 32 * jt0, tid, g0);
     }
@@ -933,10 +933,11 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
     (void)g1;
     (void)word0;
     (void)word1;
-    (void)eo;
+    (void)eo4;
     (void)eref;
     (void)sx;
-    (void)scale_slot;
+    (void)scale_now;
+    (void)scale_next;
     (void)sid0;
     (void)sid1;
     if (jt0 + 1 < nt) stage_load<KT, D, VTOK>(kr, vr, p, id1, h, tid);
@@ -1024,8 +1025,8 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
     // What few tiles have: V's reference has grown, or a block has scales that are not
     // finite, which make NaN of the columns that see a token of it, and of no others.
     auto odd_scales = [&](int word, int tok0) {
-      const float down = power_of_two(eo - (word >> 4));
-      eo = word >> 4;
+      const float down = power_of_two((eo4 >> 4) - (word >> 4));
+      eo4 = word & ~15;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         int see = ((word >> (2 + (lq >> 1))) & 1) && lim[k] > tok0;
@@ -1084,9 +1085,9 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       const int valid_next = kvlen - 32 * (j + 1);
       // (V of a block whose scales are not finite is zeroed like an invalid one's:
       // its codes may be NaN, and 0 * NaN would reach rows that do not see it)
-      if constexpr (kBlocks<Pm>) sc = s_scales.at[scale_slot(j)][lq >> 1];
+      if constexpr (kBlocks<Pm>) sc = scale_now[2 * P];
       TileIds idv = id1;
-      if constexpr (kBlocks<Pm>) idv.ok = word1 & ~(word1 >> 2) & 3;
+      if constexpr (kBlocks<Pm>) idv.ok = word1 & 3;
       if (!(j + 2 <= nfull && idv.ok == 3)) mask_staged_v<KT, D, VTOK>(vr, idv, valid_next, tid);
       // table entries of tile j + 3, read now and resolved after the math
       int raw_a = -1, raw_b = -1;
@@ -1149,11 +1150,11 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
       float g2 = 0.0f;
       int word2 = 0;
       if constexpr (kBlocks<Pm>) {
-        g2 = s_scales.at[scale_slot(j + 2)][sx].g;
-        word2 = s_scales.word[scale_slot(j + 2)];
+        g2 = scale_next[2 * P].g;
+        word2 = scale_next[2 * P].word;
       }
       const bool up_a = mta > m[0] + 8.0f, up_b = mtb > m[1] + 8.0f;
-      const bool odd = kBlocks<Pm> && ((word0 ^ (eo << 4)) & ~3) != 0;
+      const bool odd = kBlocks<Pm> && (unsigned)(word0 ^ eo4) > 3u;
       if (__any(up_a || up_b || odd)) {
         if constexpr (kBlocks<Pm>)
           if (odd) odd_scales(word0, 32 * j + 8 * lq);
@@ -1190,6 +1191,8 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
         if (rel > kScaleTiles && (rel & (kScaleTiles - 1)) == 2 && next < nt)
           fill_scales<KT>(&s_scales, scale_pair(p, kscale, vscale, scale_block(p, trow, next, nt, nblk, tid), h), jt0, next,
                           qk_scale, eref, tid);
+        scale_now = &s_scales.at[rel & (kScaleSlots - 1)][lq >> 1];
+        scale_next = &s_scales.at[(rel + 2) & (kScaleSlots - 1)][sx];
       }
       step(std::integral_constant<int, 0>{}, j);
       if (j + 1 < nt) step(std::integral_constant<int, 1>{}, j + 1);
@@ -1203,7 +1206,7 @@ __global__ __launch_bounds__(256, 2) void prefill_item_kernel(Pm p, const int32_
 #pragma unroll
         for (int t = 0; t < NV; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[k][t][e] = __builtin_amdgcn_ldexpf(o[k][t][e], eo - 127 - kVHead<KT>);
+          for (int e = 0; e < 4; ++e) o[k][t][e] = __builtin_amdgcn_ldexpf(o[k][t][e], (eo4 >> 4) - 127 - kVHead<KT>);
       }
     }
     // ---- a piece: its used columns' (m, l) and o, in register order ---------
