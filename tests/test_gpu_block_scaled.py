@@ -10,9 +10,10 @@ import torch
 
 from block_scaled_util import (assert_attended, attend_ref, code_bytes, encode, filled, least_scale, write_ref)
 from cf_hip import ops
-from cf_hip.layout import alloc_kv_cache, alloc_kv_scales
+from cf_hip.layout import alloc_kv_cache, alloc_kv_scales, paired_storage
 from kernels.block_scaled_kv import write_kv_blocks
 from kernels.paged_attention import chunked_prefill_attention, paged_attention, paged_attention_tensors
+from python_runtime.engine.block_manager import BlockManager
 
 pytestmark = pytest.mark.gpu
 
@@ -639,6 +640,44 @@ def test_captured_and_replayed():
             assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(codes, c["kc"])
         _step(eager)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", KV)
+@pytest.mark.parametrize("layout, nb", [("paired", 600_000), ("token_major", 1_100_000)])
+def test_offsets_past_32_bits(dtype, layout, nb):
+    """Blocks at the end of a cache of more than 2^32 bytes hold and give what low ones do, bit for bit."""
+    gen = torch.Generator().manual_seed(21)
+    lens, start = [50, 33], _i32([0, 37, 70])
+    new = [torch.randn(70, 2, 128, generator=gen).to(BF16).cuda() for _ in range(2)]
+    q = torch.randn(70, 8, 128, generator=gen).to(BF16).cuda()
+    low = [[3, 0, 7, 5], [1, 6, 2, 4]]
+    outs = []
+    for blocks, first in ((8, 0), (nb, nb - 8)):
+        kc, vc = alloc_kv_cache(blocks, 16, 2, 128, dtype, "cuda", layout)
+        ks, vs = alloc_kv_scales(blocks, 2, "cuda")
+        tables = _i32([[b + first for b in t] for t in low])
+        write_kv_blocks(new[0][:26], new[1][:26], tables, _i32([13, 13]), kc, vc, ks, vs, q_start=_i32([0, 13, 26]))
+        write_kv_blocks(*new, tables, _i32(lens), kc, vc, ks, vs, q_start=start)
+        if blocks == nb:  # and back from there
+            mine = [ops.paged_gather(kc, tables, 33, scale=ks)]
+            moves = [(nb - 8 + b, b) for b in range(8)] + [(b, nb - 8 + (b + 1) % 8) for b in range(8)]
+            for c in ((paired_storage(kc, vc),) if layout == "paired" else (kc, vc)):
+                BlockManager.move_blocks(moves, [c])
+            BlockManager.move_blocks(moves, [ks, vs])
+            tables = _i32(low)
+            mine.append(ops.paged_gather(kc, tables, 33, scale=ks))
+            assert torch.equal(*mine)
+            tables = _i32([[b + first for b in t] for t in low])
+            BlockManager.move_blocks([(b, nb - 8 + b) for b in range(8)], [ks, vs])
+            for c in ((paired_storage(kc, vc),) if layout == "paired" else (kc, vc)):
+                BlockManager.move_blocks([(b, nb - 8 + b) for b in range(8)], [c])
+        outs.append([ops.paged_gather(kc, tables, 33, scale=ks), ops.paged_gather(vc, tables, 33, scale=vs),
+                     paged_attention_tensors(q[:2], kc, vc, tables, _i32(lens), k_scale=ks, v_scale=vs),
+                     paged_attention_tensors(q[:2].float(), kc, vc, tables, _i32(lens), k_scale=ks, v_scale=vs),
+                     chunked_prefill_attention(q, kc, vc, tables, _i32(lens), start, k_scale=ks, v_scale=vs)])
+        del kc, vc
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert not any(bool(a.isnan().any()) for a in outs[0])
 
 
 def test_native_path_and_ctypes_agree(monkeypatch):
