@@ -19,8 +19,8 @@
 // steps are one after the other, and a rearranged cache is mostly one long cycle: then
 // the bytes in flight are those of one block over all tensors, times kAhead.  1,800
 // blocks of 256 KiB rearranged at random (945 MB read and written, two thirds of it one
-// cycle): 224 us, 4.2 TB/s of the 4.8 that a large copy reaches; with 8 steps ahead and
-// 8 bytes of arguments a step (7 launches where 3 do) 520.  16 copies of 1 MiB: 10.5 us.
+// cycle): 215 us, 4.4 TB/s of the 4.8 that a large copy reaches; with 8 steps ahead and
+// 8 bytes of arguments a step (7 launches where 3 do) 520.  16 copies of 1 MiB: 8.2 us.
 #include <algorithm>
 #include <numeric>
 
@@ -212,10 +212,11 @@ struct MoveRest {
 };
 
 int32_t launch_moves(std::vector<MoveRest>& rest, MoveArgs& a, int64_t groups, hipStream_t stream) {
-  // Lists enough for some threads on every SIMD; a list of single moves has its loads
-  // in flight together.
-  constexpr int64_t kThreads = 256 * 1024;
-  const int64_t wanted = std::min<int64_t>(ceil_div(kThreads, groups * kMoveThreads), kMoveLists);
+  // Lists enough for 16 waves on every SIMD, of at least kAhead / 2 words: 16 copies
+  // of 1 MiB take 8.9 us in one list, 8.7 in 2, 11.0 in 4 and 20.7 in 16; chains of
+  // hundreds of blocks 94 us a launch in up to 32, 98 in up to 20, 104 in up to 8.
+  constexpr int64_t kThreads = 1024 * 1024;
+  const int64_t most = std::min<int64_t>(ceil_div(kThreads, groups * kMoveThreads), kMoveLists);
   const int64_t room = kMoveWords - 2 * a.caches - (kMoveLists + 1);
   while (!rest.empty()) {
     // every long component its share of each of the launches that all need
@@ -235,6 +236,7 @@ int32_t launch_moves(std::vector<MoveRest>& rest, MoveArgs& a, int64_t groups, h
     rest.erase(std::remove_if(rest.begin(), rest.end(), [](const MoveRest& r) { return r.done(); }), rest.end());
     // the longest run to the shortest list
     std::sort(runs.begin(), runs.end(), [](const auto& x, const auto& y) { return x.size() > y.size(); });
+    const int64_t wanted = std::max<int64_t>(1, std::min(most, 2 * (room - left) / kAhead));
     std::vector<std::vector<uint32_t>> lists(std::min<size_t>(runs.size(), (size_t)wanted));
     for (const auto& run : runs) {
       auto& to = *std::min_element(lists.begin(), lists.end(), [](const auto& x, const auto& y) { return x.size() < y.size(); });
