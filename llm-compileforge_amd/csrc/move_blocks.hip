@@ -211,29 +211,42 @@ struct MoveRest {
   }
 };
 
-int32_t launch_moves(std::vector<MoveRest>& rest, MoveArgs& a, int64_t groups, hipStream_t stream) {
+int32_t launch_moves(const std::vector<MoveComponent>& plan, MoveArgs& a, int64_t groups, hipStream_t stream) {
   // Lists enough for 16 waves on every SIMD, of at least kAhead / 2 words: 16 copies
   // of 1 MiB take 8.9 us in one list, 8.7 in 2, 11.0 in 4 and 20.7 in 16; chains of
   // hundreds of blocks 94 us a launch in up to 32, 98 in up to 20, 104 in up to 8.
   constexpr int64_t kThreads = 1024 * 1024;
   const int64_t most = std::min<int64_t>(ceil_div(kThreads, groups * kMoveThreads), kMoveLists);
   const int64_t room = kMoveWords - 2 * a.caches - (kMoveLists + 1);
-  while (!rest.empty()) {
-    // every long component its share of each of the launches that all need
-    std::sort(rest.begin(), rest.end(), [](const MoveRest& x, const MoveRest& y) { return x.words > y.words; });
-    int64_t all = 0, left = room;
-    for (const MoveRest& r : rest) all += r.words;
+  constexpr int64_t kLong = 64;  // words of a component that may be cut
+  std::vector<MoveRest> cut, whole;
+  int64_t all = 0;
+  for (const MoveComponent& c : plan) {
+    MoveRest r(c);
+    all += r.words;
+    (r.words > kLong ? cut : whole).push_back(r);
+  }
+  std::sort(cut.begin(), cut.end(), [](const MoveRest& x, const MoveRest& y) { return x.words > y.words; });
+  for (size_t next = 0; next < whole.size() || !cut.empty();) {
+    // every long component its share of each of the launches that all need, and
+    // others as they come
+    int64_t left = room;
     const int64_t launches = ceil_div(all, room);
     std::vector<std::vector<uint32_t>> runs;
-    for (MoveRest& r : rest) {
-      const int64_t share = launches == 1 ? left : std::max<int64_t>(ceil_div(r.words, launches) + 2, 64);
+    auto take = [&](MoveRest& r, int64_t most_words) {
       std::vector<uint32_t> run;
-      r.take(std::min(share, left), run);
-      if (run.empty()) continue;
+      const int64_t before = r.words;
+      r.take(most_words, run);
+      all -= before - r.words;
       left -= (int64_t)run.size();
-      runs.push_back(std::move(run));
+      if (!run.empty()) runs.push_back(std::move(run));
+    };
+    for (MoveRest& r : cut) {
+      if (left < kLong) break;
+      take(r, std::min(left, launches == 1 ? left : std::max(ceil_div(r.words, launches) + 2, kLong)));
     }
-    rest.erase(std::remove_if(rest.begin(), rest.end(), [](const MoveRest& r) { return r.done(); }), rest.end());
+    cut.erase(std::remove_if(cut.begin(), cut.end(), [](const MoveRest& r) { return r.done(); }), cut.end());
+    for (; next < whole.size() && whole[next].words <= left; ++next) take(whole[next], left);
     // the longest run to the shortest list
     std::sort(runs.begin(), runs.end(), [](const auto& x, const auto& y) { return x.size() > y.size(); });
     const int64_t wanted = std::max<int64_t>(1, std::min(most, 2 * (room - left) / kAhead));
@@ -287,8 +300,7 @@ int32_t move_all(std::vector<MoveCache>& caches, const int32_t* moves, int64_t n
       ++a.caches;
     }
     for (int k = shapes; k < kMoveShapes; ++k) a.shape[k].first_group = INT32_MAX;
-    std::vector<MoveRest> rest(plan.begin(), plan.end());
-    if (const int32_t rc = launch_moves(rest, a, groups, stream)) return rc;
+    if (const int32_t rc = launch_moves(plan, a, groups, stream)) return rc;
   }
   return CF_OK;
 }

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import random
+import time
 
 import numpy as np
 import pytest
@@ -58,6 +59,30 @@ def test_random_moves(seed):
 def test_one_long_cycle():
     nb = 1500
     _check([_cache((nb, 80), torch.uint8, 0)], [((i + 1) % nb, i) for i in range(nb)])
+
+
+def test_many_moves():
+    """As many moves as a large pool has, most of them on their own, some in long chains: the host's share of a launch
+    does not grow with them."""
+    nb, rng = 120_000, random.Random(5)
+    ids = rng.sample(range(nb), nb)
+    moves = list(zip(ids[:30_000], ids[30_000:60_000]))
+    for at in range(60_000, 118_000, 500):
+        chain = ids[at : at + 500]
+        moves += list(zip(chain[1:], chain[:-1]))
+        if at % 1000 == 0:
+            moves.append((chain[0], chain[-1]))
+    rng.shuffle(moves)
+    c = _cache((nb, 16), torch.uint8, 1)
+    was = c.clone()
+    begin = time.perf_counter()
+    BlockManager.move_blocks(np.asarray(moves, dtype=np.int32), [c])
+    torch.cuda.synchronize()
+    assert time.perf_counter() - begin < 5.0  # (half a millisecond a launch would be 0.1)
+    m = torch.tensor(moves).cuda()
+    want = was.clone()
+    want[m[:, 1]] = was[m[:, 0]]
+    assert torch.equal(c, want)
 
 
 def test_many_tensors_and_large_blocks():
