@@ -33,7 +33,9 @@ namespace cf {
 namespace {
 
 constexpr int kAhead = 32;
-constexpr int kMoveThreads = 256;
+// Workgroups have 256 threads, or 64 where that makes fewer than so many: a long chain
+// over few tensors then takes all CUs.
+constexpr int kFewGroups = 512;
 constexpr int kMoveShapes = 4;    // tensors of a launch differ in at most so many shapes
 constexpr int kMoveCaches = 128;  // tensors of a launch
 constexpr int kMoveLists = 32;    // lists of steps that run side by side
@@ -62,7 +64,7 @@ template <class T>
 __device__ __forceinline__ void move_pieces(const uint32_t* __restrict__ word, int begin, int end, char* base,
                                             const MoveShape& sh, int group) {
   const int64_t pieces = sh.bytes / (int64_t)sizeof(T), stride = sh.stride / (int64_t)sizeof(T);
-  for (int64_t i = (int64_t)group * kMoveThreads + threadIdx.x; i < pieces; i += (int64_t)sh.groups * kMoveThreads) {
+  for (int64_t i = (int64_t)group * blockDim.x + threadIdx.x; i < pieces; i += (int64_t)sh.groups * blockDim.x) {
     T* at = (T*)base + i;
     T aside{};
     for (int e = begin; e < end; e += kAhead) {
@@ -88,7 +90,7 @@ __device__ __forceinline__ void move_pieces(const uint32_t* __restrict__ word, i
   }
 }
 
-__global__ __launch_bounds__(kMoveThreads) void move_blocks_kernel(MoveArgs a) {
+__global__ __launch_bounds__(256) void move_blocks_kernel(MoveArgs a) {
   int k = 0;
   while (k + 1 < kMoveShapes && (int)blockIdx.x >= a.shape[k + 1].first_group) ++k;
   const MoveShape sh = a.shape[k];
@@ -211,12 +213,29 @@ struct MoveRest {
   }
 };
 
-int32_t launch_moves(const std::vector<MoveComponent>& plan, MoveArgs& a, int64_t groups, hipStream_t stream) {
+// Deals the tensors' pieces to workgroups of so many threads; returns their number.
+int64_t deal_groups(MoveArgs& a, int threads) {
+  int64_t groups = 0;
+  for (int k = 0; k < kMoveShapes; ++k) {
+    MoveShape& s = a.shape[k];
+    const int last = k + 1 < kMoveShapes ? a.shape[k + 1].first_cache : a.caches;
+    s.first_group = (int32_t)groups;
+    if (s.unit == 0) {
+      s.first_group = INT32_MAX;  // no such shape
+      continue;
+    }
+    s.groups = (int32_t)std::min<int64_t>(ceil_div(s.bytes / s.unit, threads), kMoveGroups);
+    groups += (int64_t)s.groups * (last - s.first_cache);
+  }
+  return groups;
+}
+
+int32_t launch_moves(const std::vector<MoveComponent>& plan, MoveArgs& a, hipStream_t stream) {
   // Lists enough for 16 waves on every SIMD, of at least kAhead / 2 words: 16 copies
   // of 1 MiB take 8.9 us in one list, 8.7 in 2, 11.0 in 4 and 20.7 in 16; chains of
   // hundreds of blocks 94 us a launch in up to 32, 98 in up to 20, 104 in up to 8.
   constexpr int64_t kThreads = 1024 * 1024;
-  const int64_t most = std::min<int64_t>(ceil_div(kThreads, groups * kMoveThreads), kMoveLists);
+  const int64_t most = std::min<int64_t>(ceil_div(kThreads, deal_groups(a, 256) * 256), kMoveLists);
   const int64_t room = kMoveWords - 2 * a.caches - (kMoveLists + 1);
   constexpr int64_t kLong = 64;  // words of a component that may be cut
   std::vector<MoveRest> cut, whole;
@@ -263,9 +282,10 @@ int32_t launch_moves(const std::vector<MoveComponent>& plan, MoveArgs& a, int64_
       for (const uint32_t w : lists[l]) a.word[at++] = w;
     }
     first[a.lists] = at;
-    const dim3 grid((unsigned)groups, (unsigned)a.lists);
+    const int threads = deal_groups(a, 256) * a.lists < kFewGroups ? 64 : 256;
+    const dim3 grid((unsigned)deal_groups(a, threads), (unsigned)a.lists);
     ProfileScope prof("cf_move_blocks", stream);
-    CF_LAUNCH(move_blocks_kernel, grid, dim3(kMoveThreads), 0, stream, a);
+    CF_LAUNCH(move_blocks_kernel, grid, dim3(threads), 0, stream, a);
     CF_HIP_CHECK(hipGetLastError());
   }
   return CF_OK;
@@ -283,24 +303,21 @@ int32_t move_all(std::vector<MoveCache>& caches, const int32_t* moves, int64_t n
   for (size_t c = 0; c < caches.size();) {
     MoveArgs a{};
     int shapes = 0;
-    int64_t groups = 0;
     for (; c < caches.size() && a.caches < kMoveCaches; ++c) {
       const int unit = unit_of(caches[c]);
-      const int64_t own = std::min<int64_t>(ceil_div(caches[c].bytes / unit, kMoveThreads), kMoveGroups);
       MoveShape* s = shapes > 0 ? &a.shape[shapes - 1] : nullptr;
       if (s == nullptr || s->bytes != caches[c].bytes || s->stride != caches[c].stride || s->unit != unit) {
         if (shapes == kMoveShapes) break;
         s = &a.shape[shapes++];
-        *s = MoveShape{caches[c].stride, caches[c].bytes, unit, (int32_t)own, (int32_t)groups, a.caches};
+        *s = MoveShape{caches[c].stride, caches[c].bytes, unit, 0, 0, a.caches};
       }
-      groups += own;
       const uint64_t base = (uint64_t)(uintptr_t)caches[c].base;
       a.word[2 * a.caches] = (uint32_t)base;
       a.word[2 * a.caches + 1] = (uint32_t)(base >> 32);
       ++a.caches;
     }
-    for (int k = shapes; k < kMoveShapes; ++k) a.shape[k].first_group = INT32_MAX;
-    if (const int32_t rc = launch_moves(plan, a, groups, stream)) return rc;
+    for (int k = shapes; k < kMoveShapes; ++k) a.shape[k].first_cache = a.caches;
+    if (const int32_t rc = launch_moves(plan, a, stream)) return rc;
   }
   return CF_OK;
 }
