@@ -15,12 +15,16 @@
 // The steps and the tensors are kernel arguments: nothing is uploaded, and a
 // captured call replays with the moves it was given.  A chain costs a word a block.
 //
-// Bound by HBM where the blocks are large or the components many.  A component's
-// steps are one after the other, and a rearranged cache is mostly one long cycle: then
-// the bytes in flight are those of one block over all tensors, times kAhead.  1,800
-// blocks of 256 KiB rearranged at random (945 MB read and written, two thirds of it one
-// cycle): 215 us, 4.4 TB/s of the 4.8 that a large copy reaches; with 8 steps ahead and
-// 8 bytes of arguments a step (7 launches where 3 do) 520.  16 copies of 1 MiB: 8.2 us.
+// Bound by HBM.  A component's steps are one after the other, so the bytes in flight
+// are those of one block over all tensors, times kAhead and the components at hand.
+// 1,800 blocks of 256 KiB (945 MB read and written): in 220 chains of up to 35 blocks,
+// as a fragmented pool is compacted, 215 us, 4.4 TB/s of the 4.8 that a large copy
+// reaches; in one chain 211 us, in one cycle 219, in eight 232.  With 8 steps ahead and
+// 8 bytes of arguments a step the first took 520.  16 copies of 1 MiB: 8.2 us.
+//
+// STRETCH (a launch with a run of more than two batches' words): batches of one chain
+// take a way of their own without a test a step, which the one chain needs (476 us
+// without it).  It holds 208 VGPRs instead of 144, and the 16 copies take 11.4 us in it.
 #include <algorithm>
 #include <numeric>
 
@@ -60,7 +64,7 @@ struct MoveArgs {
 };
 static_assert(sizeof(MoveArgs) <= 4096, "kernel arguments");
 
-template <class T>
+template <class T, bool STRETCH>
 __device__ __forceinline__ void move_pieces(const uint32_t* __restrict__ word, int begin, int end, char* base,
                                             const MoveShape& sh, int group) {
   const int64_t pieces = sh.bytes / (int64_t)sizeof(T), stride = sh.stride / (int64_t)sizeof(T);
@@ -72,6 +76,20 @@ __device__ __forceinline__ void move_pieces(const uint32_t* __restrict__ word, i
 #pragma unroll
       for (int u = 0; u <= kAhead; ++u) w[u] = word[e + u];
       T v[kAhead];
+      if constexpr (STRETCH) {
+        // a stretch of one chain, without ends and what is set aside
+        uint32_t most = 0;
+#pragma unroll
+        for (int u = 0; u <= kAhead; ++u) most = max(most, w[u]);
+        if (most < kAside && e + kAhead < end && sh.bytes < (int64_t)1 << 32) {
+          const uint32_t off = (uint32_t)i * (uint32_t)sizeof(T);
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) v[u] = *(const T*)(base + (uint64_t)w[u + 1] * (uint64_t)sh.stride + off);
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) *(T*)(base + (uint64_t)w[u] * (uint64_t)sh.stride + off) = v[u];
+          continue;
+        }
+      }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const uint32_t src = w[u + 1] & ~kLastBlock;
@@ -90,6 +108,7 @@ __device__ __forceinline__ void move_pieces(const uint32_t* __restrict__ word, i
   }
 }
 
+template <bool STRETCH>
 __global__ __launch_bounds__(256) void move_blocks_kernel(MoveArgs a) {
   int k = 0;
   while (k + 1 < kMoveShapes && (int)blockIdx.x >= a.shape[k + 1].first_group) ++k;
@@ -98,9 +117,9 @@ __global__ __launch_bounds__(256) void move_blocks_kernel(MoveArgs a) {
   char* base = (char*)((uint64_t)a.word[2 * (sh.first_cache + c)] | (uint64_t)a.word[2 * (sh.first_cache + c) + 1] << 32);
   const uint32_t* lists = a.word + 2 * a.caches + blockIdx.y;
   const int begin = (int)lists[0], end = (int)lists[1];
-  if (sh.unit == 16) move_pieces<uint4>(a.word, begin, end, base, sh, group);
-  else if (sh.unit == 4) move_pieces<uint32_t>(a.word, begin, end, base, sh, group);
-  else move_pieces<uint8_t>(a.word, begin, end, base, sh, group);
+  if (sh.unit == 16) move_pieces<uint4, STRETCH>(a.word, begin, end, base, sh, group);
+  else if (sh.unit == 4) move_pieces<uint32_t, STRETCH>(a.word, begin, end, base, sh, group);
+  else move_pieces<uint8_t, STRETCH>(a.word, begin, end, base, sh, group);
 }
 
 }  // namespace
@@ -285,7 +304,8 @@ int32_t launch_moves(const std::vector<MoveComponent>& plan, MoveArgs& a, hipStr
     const int threads = deal_groups(a, 256) * a.lists < kFewGroups ? 64 : 256;
     const dim3 grid((unsigned)deal_groups(a, threads), (unsigned)a.lists);
     ProfileScope prof("cf_move_blocks", stream);
-    CF_LAUNCH(move_blocks_kernel, grid, dim3(threads), 0, stream, a);
+    if (runs.front().size() > kLong) CF_LAUNCH((move_blocks_kernel<true>), grid, dim3(threads), 0, stream, a);
+    else CF_LAUNCH((move_blocks_kernel<false>), grid, dim3(threads), 0, stream, a);
     CF_HIP_CHECK(hipGetLastError());
   }
   return CF_OK;
