@@ -1062,10 +1062,16 @@ __global__ __launch_bounds__(256) void decode_stream_kernel(P p, const int32_t* 
     }
     float pr[8];
     float psum = 0.0f;
+    // A column with no finite score yet has m = -inf: any finite reference gives 0
+    // for its masked tokens and keeps the NaN of others (one scale a head, or none,
+    // under 16-bit queries: weight 0 for both).
+    constexpr bool kKeepsNan = kBlocks<P> || QT == kF32;
     const bool live = m != -INFINITY;
+    const float mref = live ? m : 0.0f;
 #pragma unroll
     for (int v = 0; v < 8; ++v) {
-      pr[v] = live ? __builtin_amdgcn_exp2f(sc[v] - m) : 0.0f;
+      const float e = __builtin_amdgcn_exp2f(sc[v] - (kKeepsNan ? mref : m));
+      pr[v] = kKeepsNan || live ? e : 0.0f;
       psum += pr[v];
     }
     l += psum;

@@ -857,3 +857,26 @@ def test_fp32_kernel_choice(gpu, hq, hkv, d, batch, capacity, mfma):
         out = _run(case, kc, vc, ks, vs, gpu)
         assert timer.query("cf_decode_mfma")[1] == int(mfma) and timer.query("cf_decode_generic")[1] == int(not mfma)
     assert_close(out.cpu().numpy(), oracle_decode(case, kc, vc, ks, vs), torch.float32, "choice")
+
+
+@pytest.mark.parametrize("kv_dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("lens", [[700] * 64, [64, 40, 5000], [14, 16]], ids=["whole runs", "split runs", "one block"])
+def test_nan_alone_reaches_the_output_under_fp32_queries(gpu, kv_dtype, lens):
+    """As above, where a wave or the whole sequence sees no finite score, over caches of 8 and 16 bits."""
+    g = torch.Generator(device=gpu).manual_seed(5)
+    blocks = [-(-n // 16) for n in lens]
+    at = [sum(blocks[:i]) for i in range(len(lens) + 1)]
+    tables = [list(range(at[i], at[i + 1])) for i in range(len(lens))]
+    q = torch.randn(len(lens), 8, 64, generator=g, device=gpu)
+    k, v = (torch.randn(at[-1], 16, 2, 64, generator=g, device=gpu) for _ in range(2))
+    case = workloads.DecodeCase("nan", q, k, v, tables, lens, 16, 0.125, kv_dtype)
+    kc, vc, ks, vs = workloads.materialize(case, "paired")
+    clean = _run(case, kc, vc, ks, vs, gpu)
+    bits = kc.view(torch.uint8) if kv_dtype == torch.float8_e4m3fn else kc
+    last = len(lens) - 1
+    for b in tables[0] + tables[last][:4]:
+        bits[b, :, 1] = 0x7F if kv_dtype == torch.float8_e4m3fn else float("nan")
+    want = torch.zeros(len(lens), 8, dtype=torch.bool, device=gpu)
+    want[[0, last], 4:] = True
+    out = _run(case, kc, vc, ks, vs, gpu)
+    assert torch.equal(out.isnan().all(-1), want) and torch.equal(out[~want], clean[~want])
