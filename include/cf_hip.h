@@ -392,6 +392,8 @@ int32_t cf_kv_write_fp8(const CfTensor* k_new, const CfTensor* v_new,
  * cf_prefill_chunk_fp8 and cf_paged_gather read such a cache where they are given
  * scales [NB, H] (rank 2, any strides; scales positive); what writes by slots with
  * given scales, moves single rows or keeps accounts does not take it.
+ * cf_prefill_chunk_fp8 takes V scales that lie up to 2^100 apart, and V of a scale
+ * below 2^-80 as zeros.
  *
  * Writes the new rows of N sequences at their last positions: row i of sequence
  * n's L rows goes to position seq_lens[n] - L + i of block_tables[n] (the operands

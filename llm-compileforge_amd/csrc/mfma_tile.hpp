@@ -343,31 +343,6 @@ __device__ __forceinline__ f16x8_t e4m3x8_to_f16(uint32_t lo, uint32_t hi) {
 
 
 
-// 8 e4m3 or int8 codes times a power of two g -> 8 fp16, rounded once (exact unless a
-// value is below fp16's smallest normal one and has more bits than are left there).
-// g at most 2^7 for e4m3, whose codes reach 448, and 2^5 for int8, whose offset
-// 1152 g has to fit; smaller than 2^-24 is 0.
-__device__ __forceinline__ f16x8_t e4m3x8_to_f16(uint32_t lo, uint32_t hi, float g) {
-  uint4 r;
-  r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, g, false));
-  r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, g, true));
-  r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, g, false));
-  r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, g, true));
-  return __builtin_bit_cast(f16x8_t, r);
-}
-__device__ __forceinline__ f16x8_t i8x8_to_f16(uint32_t lo, uint32_t hi, float g) {
-  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-  const _Float16 m = (_Float16)g, c = (_Float16)(-1152.0f * (float)m);  // (u - 1152) g, as one fma
-  const uint32_t w[2] = {lo ^ 0x80808080u, hi ^ 0x80808080u};
-  uint32_t r[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t u = __builtin_amdgcn_perm(0x64646464u, w[i >> 1], (i & 1) ? 0x04030402u : 0x04010400u);
-    r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, u), f16x2_t{m, m}, f16x2_t{c, c}));
-  }
-  return __builtin_bit_cast(f16x8_t, make_uint4(r[0], r[1], r[2], r[3]));
-}
-
 // Query-typed MFMA operands: bf16 queries multiply bf16 K (bf16 caches, or
 // e4m3 converted exactly); fp16 queries multiply fp16 K (fp16 caches, or
 // e4m3 converted exactly).

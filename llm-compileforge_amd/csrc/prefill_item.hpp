@@ -537,25 +537,15 @@ __device__ __forceinline__ uint4 codes_to_16(uint32_t lo, uint32_t hi) {
     return F16 ? __builtin_bit_cast(uint4, e4m3x8_to_f16(lo, hi)) : __builtin_bit_cast(uint4, e4m3x8_to_bf16(lo, hi));
 }
 
-// The V operands of 8 codes: fp16, with block scales (BLK) times the power of two g.
-template <int KT, bool BLK>
-__device__ __forceinline__ uint4 v_to_16(uint32_t lo, uint32_t hi, float g) {
-  if constexpr (!BLK) return codes_to_16<KT, true>(lo, hi);
-  else if constexpr (KT == kI8) return __builtin_bit_cast(uint4, i8x8_to_f16(lo, hi, g));
-  else return __builtin_bit_cast(uint4, e4m3x8_to_f16(lo, hi, g));
-}
-
 // Converts the staged registers and writes them in operand order: K entry
 // (chain s, step c, lane) = the 8 channels lane (li, lq) feeds step c of
 // chain s; V entry (step t, lane) = channel 16 t + li, tokens 8 lq .. 8 lq + 7.
 // V tokens at or past `valid` (tile-relative) or in an invalid block become
 // zero (cache slots there may hold any bits, NaN codes included).
-// BLK: a cache with block scales, whose V codes are staged times g, this thread's
-// block's power of two.
 // FULL: the caller knows every token of the tile is valid.
-template <int QT, int KT, int D, bool VTOK, bool BLK, bool FULL = false>
+template <int QT, int KT, int D, bool VTOK, bool FULL = false>
 __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const uint4* vr, const TileIds& t,
-                                            int valid, int tid, float g = 1.0f) {
+                                            int valid, int tid) {
   using Gm = Geo<KT, D>;
 #pragma unroll
   for (int i = 0; i < Gm::KPT; ++i) {
@@ -593,8 +583,8 @@ __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const u
         const uint4 v = make_uint4(vr[i].x & km, vr[i].y & km, vr[i].z & km, vr[i].w & km);
         uint8_t* row = rows + vtok_slot(16 * X + r) * Gm::VRS;
         if constexpr (Gm::KB == 1) {
-          *(uint4*)(row + 32 * c) = v_to_16<KT, BLK>(v.x, v.y, g);
-          *(uint4*)(row + 32 * c + 16) = v_to_16<KT, BLK>(v.z, v.w, g);
+          *(uint4*)(row + 32 * c) = codes_to_16<KT, true>(v.x, v.y);
+          *(uint4*)(row + 32 * c + 16) = codes_to_16<KT, true>(v.z, v.w);
         } else {
           *(uint4*)(row + 16 * c) = v;
         }
@@ -612,8 +602,8 @@ __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const u
       const int li = d & 15, tt = d >> 4;
       if (full) {
         if constexpr (Gm::KB == 1) {
-          vl[tt * 64 + 32 * X + li] = v_to_16<KT, BLK>(vr[i].x, vr[i].y, g);
-          vl[tt * 64 + 32 * X + 16 + li] = v_to_16<KT, BLK>(vr[i].z, vr[i].w, g);
+          vl[tt * 64 + 32 * X + li] = codes_to_16<KT, true>(vr[i].x, vr[i].y);
+          vl[tt * 64 + 32 * X + 16 + li] = codes_to_16<KT, true>(vr[i].z, vr[i].w);
         } else {
           vl[tt * 64 + 32 * X + 16 * part + li] = vr[i];
         }
@@ -621,8 +611,8 @@ __device__ __forceinline__ void stage_write(uint4* lds, const uint4* kr, const u
         const int n0 = ok ? valid - 16 * X : 0;  // valid tokens among this load's 16
         const uint2 lo = keep_bytes(make_uint2(vr[i].x, vr[i].y), n0);
         const uint2 hi = keep_bytes(make_uint2(vr[i].z, vr[i].w), n0 - 8);
-        vl[tt * 64 + 32 * X + li] = v_to_16<KT, BLK>(lo.x, lo.y, g);
-        vl[tt * 64 + 32 * X + 16 + li] = v_to_16<KT, BLK>(hi.x, hi.y, g);
+        vl[tt * 64 + 32 * X + li] = codes_to_16<KT, true>(lo.x, lo.y);
+        vl[tt * 64 + 32 * X + 16 + li] = codes_to_16<KT, true>(hi.x, hi.y);
       } else {
         const int n0 = ok ? valid - 16 * X - 8 * part : 0;
         vl[tt * 64 + 32 * X + 16 * part + li] = mask_tokens(vr[i], n0);
@@ -674,45 +664,42 @@ template <class Pm>
 constexpr bool kBlocks = std::is_same<Pm, PrefillBlockParams>::value;
 
 // Block scales.  A lane's 8 tokens of a tile lie in one block (lanes lq 0-1: block a,
-// 2-3: block b).  Its K scale is the factor of the lane's scores.  Its V scale is
-// 2^e * f with f in [1, 2): 2^e goes to the codes as they are staged, against a
-// reference 2^eref that is the largest of the item's passes so far (below; O is in its
-// units and follows it), kVHead binades below fp16's largest, so that a block of 2^-21
-// (e4m3; int8 2^-28) of that keeps every bit of its codes, and one below it is off by
-// less than the half step 2^-25 of a weight is beside the largest; f goes to
-// the exponent of the tile's weights, and the row sums take 1 / f of it back: the P.V
-// product against a channel of ones has 1 / f in their place, as two fp16 terms in
-// rows 0 and 1.  A weight is rounded to fp16 once, as without block scales.
+// 2-3: block b).  Its K scale is the factor of the lane's scores.  Its V scale v goes
+// to the exponent of the weights: with s a score in log2 units and M the running
+// maximum of s + log2 v over what a column sees,
+//   P = 2^(s + log2 v - M),   O = sum of P c over the codes c,   l = sum of P / v,
+// and the output is O / l.  P is rounded to fp16 once, as without block scales, and a
+// weight below fp16's normal numbers is off by half of 2^-24 of the column's largest
+// weight times scale: blocks that a row does not see, or gives no weight, cost the
+// others nothing, however far apart their scales lie.  l is summed by the lanes in
+// fp32 from the unrounded P, a product with 1 / v a tile.  P and P / v stay in fp32's
+// range for scales that are less than 2^100 apart; V of a scale below 2^-80 is taken as
+// zeros, with the weights of one of 2^-80 (writes choose 2^-40 or more).
 //
 // What the tiles need of their scales is formed kScaleTiles tiles at a time, a thread
-// a block, and kept in LDS; a step then takes two LDS reads and about twenty other
-// instructions for it.  Eight 512-row chunks behind 0-4,096 tokens, e4m3 under bf16:
-// 205 us, with every wave loading and forming its tile's own a step ahead 218-220
-// (some 60 instructions a step), one scale a head 187; int8 218 and 230-237.  V's
-// scales multiplied into P, P in two bf16 terms and row sums by addition took 264
-// (int8, fp16 queries).  What can change O ahead of a tile's P.V product stands in one
-// branch with the softmax's own rescaling: a second one ahead of Q.K cost 3 us.
+// a block, and kept in LDS; a step takes one LDS read, one addition a column and the
+// row sums' 16 additions for it.  Eight 512-row chunks behind 0-4,096 tokens: e4m3
+// under bf16 204 us (one scale a head 187), int8 214, int8 under fp16 212, with one
+// instruction instead of two beside a product of P.V 206, 217 and 213.  2^e of the
+// scale in V's codes, against a reference of the item, took 203, 214 and 214 and lost
+// the V of rows beside blocks of 2^22 times their scale.
 constexpr int kScaleTiles = 128;              // of a pass
 constexpr int kScaleSlots = 2 * kScaleTiles;  // tiles held
+constexpr float kLeastV = 0x1p-80f;
+constexpr float kSumUnit = 0x1p20f;  // of l while it is summed: 2^100 P at most, and 2^-107 P (with fp32's subnormals)
 struct alignas(16) BlockScale {
-  float k;       // the scores' factor
-  float lf;      // log2 f
-  uint32_t inv;  // 1 / f as two fp16 terms
-  float g;       // the power of two of the V codes
-  int word;      // of the tile: eref (with a float's bias) << 4 | blocks with NaN or infinite scales << 2 | the other valid ones
+  float k;    // the scores' factor
+  float lv;   // log2 v
+  float inv;  // kSumUnit / v
+  int word;   // of the tile: blocks with NaN or infinite scales << 2 | the other valid ones that V is read of
 };
 struct ScaleWindow {
   BlockScale at[kScaleSlots][2];
-  int top[4];
 };
-template <int KT>
-constexpr int kVHead = KT == kI8 ? 5 : 7;
-__device__ __forceinline__ float power_of_two(int e) { return u2f((uint32_t)max(e + 127, 0) << 23); }  // e < 128
 
 // A pass over the tiles first .. + kScaleTiles - 1 of an item, in three steps whose
 // loads a caller overlaps with others: the thread's block, its scales, and their
-// slots (jt0: the item's first tile, eref: the reference of the tile before first).
-// All 256 threads.
+// slots (jt0: the item's first tile).  All 256 threads.
 __device__ __forceinline__ int scale_block(const PrefillBlockParams& p, const int32_t* __restrict__ trow, int first, int nt,
                                            int nblk, int tid) {
   const int j = first + (tid >> 1), jb = 2 * j + (tid & 1);
@@ -731,31 +718,20 @@ __device__ __forceinline__ ScalePair scale_pair(const PrefillBlockParams& p, con
   }
   return s;
 }
-template <int KT>
-__device__ __forceinline__ void fill_scales(ScaleWindow* w, const ScalePair& in, int jt0, int first, float qk_scale,
-                                            int& eref, int tid) {
+__device__ __forceinline__ void fill_scales(ScaleWindow* w, const ScalePair& in, int jt0, int first, float qk_scale, int tid) {
   const int j = first + (tid >> 1), X = tid & 1;
-  const bool valid = in.valid;
   float k = in.k, v = in.v;
   const bool bad = !(__builtin_fabsf(k) < INFINITY && __builtin_fabsf(v) < INFINITY);
   if (bad) k = 1.0f, v = 0.0f;
-  const int e = (int)((f2u(v) >> 23) & 0xFFu);
-  const int mine = (bad ? 4 : (valid ? 1 : 0)) << X, flags = mine | __shfl_xor(mine, 1, 64);
-  const int top = (int)wave_umax((uint32_t)e);
-  if ((tid & 63) == 0) w->top[tid >> 6] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) eref = max(eref, w->top[i]);
-  const float f = u2f((f2u(v) & 0x007FFFFFu) | 0x3F800000u), r = 1.0f / f;
-  const _Float16 hi = (_Float16)r, lo = (_Float16)(r - (float)hi);
-  const int slot = (j - jt0) & (kScaleSlots - 1);
+  const int mine = (bad ? 4 : (in.valid && v >= kLeastV ? 1 : 0)) << X;
+  v = fmaxf(v, kLeastV);
+  const float f = u2f((f2u(v) & 0x007FFFFFu) | 0x3F800000u);
   BlockScale s;
   s.k = fmaxf(qk_scale * k, 1e-30f);  // (a product of 0: as for one scale a head)
-  s.lf = __builtin_amdgcn_logf(f);
-  s.inv = (uint32_t)__builtin_bit_cast(uint16_t, hi) | ((uint32_t)__builtin_bit_cast(uint16_t, lo) << 16);
-  s.g = power_of_two(e - eref + kVHead<KT>);
-  s.word = eref << 4 | flags;
-  w->at[slot][X] = s;
+  s.lv = (float)((int)(f2u(v) >> 23) - 127) + __builtin_amdgcn_logf(f);
+  s.inv = kSumUnit / v;
+  s.word = mine | __shfl_xor(mine, 1, 64);
+  w->at[(j - jt0) & (kScaleSlots - 1)][X] = s;
   __syncthreads();
 }
 
@@ -878,7 +854,10 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
     float m[2] = {-INFINITY, -INFINITY};
     f32x4_t o[2][NV];
     // Row sums come from the PV MFMAs: an extra V tile whose channel 0 is all
-    // ones gives O[column][0] = sum of P (lane (li, lq = 0), element 0).
+    // ones gives O[column][0] = sum of P (lane (li, lq = 0), element 0).  With block
+    // scales each lane sums its own tokens' (ls).
+    float ls[2] = {0.0f, 0.0f};
+    (void)ls;
     f32x4_t ol[2] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -904,38 +883,27 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
     TileIds id0 = tile_ids(p, trow, jt0, kvlen);
     TileIds id1 = jt0 + 1 < nt ? tile_ids(p, trow, jt0 + 1, kvlen) : id0;
     TileIds id2 = jt0 + 2 < nt ? tile_ids(p, trow, jt0 + 2, kvlen) : id1;
-    // Block scales: the lane's of tile j (sc), the staging's of tile j + 1 (g1), the
-    // words of both, O's reference (eo4) and that of the last tile formed (eref).
+    // Block scales: the lane's of tile j (sc), the words of tiles j and j + 1.
     BlockScale sc{};
-    float g1 = 1.0f;
-    int word0 = 3, word1 = 3, eo4 = 0, eref = 0;
-    const int sx = (tid / D) & 1;  // the block whose V this thread stages
-    // the lane's entries of the pair of tiles at hand, the staging's of the next pair
+    int word0 = 3, word1 = 3;
+    // the lane's entries of the pair of tiles at hand, those of the next pair
     const BlockScale *scale_now = nullptr, *scale_next = nullptr;
     if (jt0 < nt) {
       stage_load<KT, D, VTOK>(kr, vr, p, id0, h, tid);
       TileIds idv = id0;
-      float g0 = 1.0f;
       if constexpr (kBlocks<Pm>) {
         const ScalePair sa = scale_pair(p, kscale, vscale, sid0, h), sb = scale_pair(p, kscale, vscale, sid1, h);
-        fill_scales<KT>(&s_scales, sa, jt0, jt0, qk_scale, eref, tid);
-        if (nt - jt0 > kScaleTiles) fill_scales<KT>(&s_scales, sb, jt0, jt0 + kScaleTiles, qk_scale, eref, tid);
-        g0 = s_scales.at[0][sx].g;
-        word0 = uniform(s_scales.at[0][sx].word);
-        g1 = s_scales.at[1][sx].g;
-        word1 = uniform(s_scales.at[1][sx].word);
-        eo4 = word0 & ~15;
+        fill_scales(&s_scales, sa, jt0, jt0, qk_scale, tid);
+        if (nt - jt0 > kScaleTiles) fill_scales(&s_scales, sb, jt0, jt0 + kScaleTiles, qk_scale, tid);
+        word0 = uniform(s_scales.at[0][0].word);
+        word1 = uniform(s_scales.at[1][0].word);
         idv.ok = word0 & 3;
       }
-      stage_write<QT, KT, D, VTOK, kBlocks<Pm>>(lds[0], kr, vr, idv, kvlen - 32 * jt0, tid, g0);
+      stage_write<QT, KT, D, VTOK>(lds[0], kr, vr, idv, kvlen - 32 * jt0, tid);
     }
     (void)sc;
-    (void)g1;
     (void)word0;
     (void)word1;
-    (void)eo4;
-    (void)eref;
-    (void)sx;
     (void)scale_now;
     (void)scale_next;
     (void)sid0;
@@ -979,12 +947,15 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
     // (three-input v_maximum3 on gfx950, no canonicalizing of the MFMA
     // results): it equals fmaxf whenever no score is NaN, and a NaN score
     // makes the column's output NaN either way.
+    // (block scales: of the scores plus log2 v)
     auto lane_max = [&](const f32x4_t& s1, const f32x4_t& s2, float qk_scale) {
       const float m1 = __builtin_elementwise_maximum(__builtin_elementwise_maximum(s1[0], s1[1]),
                                                      __builtin_elementwise_maximum(s1[2], s1[3]));
       const float m2 = __builtin_elementwise_maximum(__builtin_elementwise_maximum(s2[0], s2[1]),
                                                      __builtin_elementwise_maximum(s2[2], s2[3]));
-      return __builtin_elementwise_maximum(m1, m2) * qk_scale;
+      const float most = __builtin_elementwise_maximum(m1, m2);
+      if constexpr (kBlocks<Pm>) return __builtin_fmaf(most, qk_scale, sc.lv);
+      else return most * qk_scale;
     };
     // The lazy rescale of column tile k: the running max moves only when a
     // score passes it by more than 8, so p <= 256.  The caller's lane-local
@@ -996,7 +967,8 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
       mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
       const float mnew = mt > m[k] + 8.0f ? mt : m[k];
       const float alpha = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[k] - mnew);
-      ol[k] = ol[k] * alpha;
+      if constexpr (kBlocks<Pm>) ls[k] *= alpha;
+      else ol[k] = ol[k] * alpha;
 #pragma unroll
       for (int t = 0; t < NV; ++t) o[k][t] = o[k][t] * alpha;
       m[k] = mnew;
@@ -1007,12 +979,15 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
       constexpr int k = decltype(kc)::value;
       return m[k] == -INFINITY ? 0.0f : m[k];
     };
-    // (mref: less log2 f with block scales)
-    auto probs = [&](const f32x4_t& s1, const f32x4_t& s2, float qk_scale, float mref, POp& pk, POp& pl) {
+    // (block scales: mref less log2 v; the weights' sum over v goes to ls)
+    auto probs = [&](auto kc, const f32x4_t& s1, const f32x4_t& s2, float qk_scale, float mref, POp& pk, POp& pl) {
+      constexpr int k = decltype(kc)::value;
+      float sum = 0.0f;
 #pragma unroll
       for (int v = 0; v < 8; ++v) {
         const float sv = v < 4 ? s1[v] : s2[v - 4];
         const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(sv, qk_scale, -mref));
+        if constexpr (kBlocks<Pm>) sum = v == 0 ? pv : sum + pv;
         if constexpr (KT != kBF16) {
           pk[v] = (_Float16)pv;
         } else {
@@ -1021,38 +996,30 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
           pl[v] = (__bf16)(pv - (float)hi);
         }
       }
+      if constexpr (kBlocks<Pm>) ls[k] = __builtin_fmaf(sum, sc.inv, ls[k]);
     };
-    // What few tiles have: V's reference has grown, or a block has scales that are not
-    // finite, which make NaN of the columns that see a token of it, and of no others.
-    auto odd_scales = [&](int word, int tok0) {
-      const float down = power_of_two((eo4 >> 4) - (word >> 4));
-      eo4 = word & ~15;
+    // Blocks of scales that are not finite make NaN of the columns that see a token of
+    // them, and of no others.
+    auto bad_scales = [&](int word, int tok0) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         int see = ((word >> (2 + (lq >> 1))) & 1) && lim[k] > tok0;
         see |= __shfl_xor(see, 16, 64);
         see |= __shfl_xor(see, 32, 64);
-        const float factor = see ? __builtin_nanf("") : down;
+        const float factor = see ? __builtin_nanf("") : 1.0f;
 #pragma unroll
         for (int t = 0; t < NV; ++t) o[k][t] = o[k][t] * factor;
       }
     };
-    (void)odd_scales;
-    // which bytes of BlockScale::inv this lane's row of the row sums takes (12: zero)
-    const uint32_t inv_bytes = li == 0 ? 0x01000100u : (li == 1 ? 0x03020302u : 0x0C0C0C0Cu);
-    (void)inv_bytes;
+    (void)bad_scales;
     // O^T += V^T P^T for column tile k; the row sums come out of the same
     // pipe as O[column][0] against a V tile whose channel 0 is all ones.
     auto pv = [&](auto kc, const uint4* vraw, const POp& pk, const POp& pl) {
       constexpr int k = decltype(kc)::value;
       if constexpr (KT != kBF16) {
         const _Float16 one = li == 0 ? (_Float16)1.0f : (_Float16)0.0f;
-        f16x8_t ones = {one, one, one, one, one, one, one, one};
-        if constexpr (kBlocks<Pm>) {
-          const uint32_t r = __builtin_amdgcn_perm(0u, sc.inv, inv_bytes);
-          ones = __builtin_bit_cast(f16x8_t, make_uint4(r, r, r, r));
-        }
-        ol[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pk, ol[k], 0, 0, 0);
+        const f16x8_t ones = {one, one, one, one, one, one, one, one};
+        if constexpr (!kBlocks<Pm>) ol[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pk, ol[k], 0, 0, 0);
 #pragma unroll
         for (int t = 0; t < NV; ++t)
           o[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, vraw[t]), pk, o[k][t], 0, 0, 0);
@@ -1070,7 +1037,7 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
       }
     };
     // MFMAs of one column tile's P.V (or QK^T) product per batch below.
-    constexpr int kPvMfma = KT != kBF16 ? NV + 1 : 2 * NV + 2;
+    constexpr int kPvMfma = KT != kBF16 ? NV + (kBlocks<Pm> ? 0 : 1) : 2 * NV + 2;
     constexpr int kQkMfma = 2 * NC;
 
     // One step: the next tile's registers go to the other LDS buffer and
@@ -1117,7 +1084,7 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
       POp pa, pla, pb, plb;
       // QK^T of column tile 0 beside the next tile's conversion into LDS
       qk(K0, a1, a2, s1a, s2a);
-      stage_write<QT, KT, D, VTOK, kBlocks<Pm>, true>(lds[1 - P], kr, vr, id1, valid_next, tid, g1);
+      stage_write<QT, KT, D, VTOK, true>(lds[1 - P], kr, vr, id1, valid_next, tid);
       stage_load<KT, D, VTOK>(kr, vr, p, id2, h, tid);
       __builtin_amdgcn_sched_group_barrier(0x100, 2 * NC, 0);
 #pragma unroll
@@ -1147,37 +1114,32 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
       }
       if (edge) mask(K1, s1b, s2b, id0.ok, tok0);
       const float mtb = lane_max(s1b, s2b, qk0);
-      float g2 = 0.0f;
       int word2 = 0;
-      if constexpr (kBlocks<Pm>) {
-        g2 = scale_next[2 * P].g;
-        word2 = scale_next[2 * P].word;
-      }
+      if constexpr (kBlocks<Pm>) word2 = scale_next[2 * P].word;
       const bool up_a = mta > m[0] + 8.0f, up_b = mtb > m[1] + 8.0f;
-      const bool odd = kBlocks<Pm> && (unsigned)(word0 ^ eo4) > 3u;
-      if (__any(up_a || up_b || odd)) {
+      const bool bad = kBlocks<Pm> && word0 > 3;
+      if (__any(up_a || up_b || bad)) {
         if constexpr (kBlocks<Pm>)
-          if (odd) odd_scales(word0, 32 * j + 8 * lq);
+          if (bad) bad_scales(word0, 32 * j + 8 * lq);
         rescale(K0, mta);
         rescale(K1, mtb);
       }
       // exponentials of column tile 0, then its P.V beside the exponentials
       // of column tile 1, then column tile 1's P.V
-      probs(s1a, s2a, qk0, kBlocks<Pm> ? mref_of(K0) - sc.lf : mref_of(K0), pa, pla);
+      probs(K0, s1a, s2a, qk0, kBlocks<Pm> ? mref_of(K0) - sc.lv : mref_of(K0), pa, pla);
       pv(K0, vraw, pa, pla);
-      probs(s1b, s2b, qk0, kBlocks<Pm> ? mref_of(K1) - sc.lf : mref_of(K1), pb, plb);
+      probs(K1, s1b, s2b, qk0, kBlocks<Pm> ? mref_of(K1) - sc.lv : mref_of(K1), pb, plb);
       pv(K1, vraw, pb, plb);
       __builtin_amdgcn_sched_group_barrier(0x002, 20, 2);
 #pragma unroll
       for (int i = 0; i < 2 * kPvMfma; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 2);
-        __builtin_amdgcn_sched_group_barrier(0x002, 1, 2);
+        __builtin_amdgcn_sched_group_barrier(0x002, kBlocks<Pm> ? 2 : 1, 2);
       }
       const TileIds id3 = j + 3 < nt ? tile_resolve(raw_a, raw_b, p.NB) : id2;
       if constexpr (kBlocks<Pm>) {
         word0 = word1;
         word1 = uniform(word2);
-        g1 = g2;
       }
       __syncthreads();
       id0 = id1;
@@ -1189,24 +1151,22 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
         // the slots of the half of the window that the item has left behind
         const int rel = j - jt0, next = j + kScaleTiles - 2;
         if (rel > kScaleTiles && (rel & (kScaleTiles - 1)) == 2 && next < nt)
-          fill_scales<KT>(&s_scales, scale_pair(p, kscale, vscale, scale_block(p, trow, next, nt, nblk, tid), h), jt0, next,
-                          qk_scale, eref, tid);
+          fill_scales(&s_scales, scale_pair(p, kscale, vscale, scale_block(p, trow, next, nt, nblk, tid), h), jt0, next,
+                      qk_scale, tid);
         scale_now = &s_scales.at[rel & (kScaleSlots - 1)][lq >> 1];
-        scale_next = &s_scales.at[(rel + 2) & (kScaleSlots - 1)][sx];
+        scale_next = s_scales.at[(rel + 2) & (kScaleSlots - 1)];
       }
       step(std::integral_constant<int, 0>{}, j);
       if (j + 1 < nt) step(std::integral_constant<int, 1>{}, j + 1);
     }
 
     if constexpr (kBlocks<Pm>) {
-      // the two terms of the row sums, and O out of V's reference
+      // the row sums of the four lanes of a column, out of their unit
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        ol[k][0] += ol[k][1];
-#pragma unroll
-        for (int t = 0; t < NV; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[k][t][e] = __builtin_amdgcn_ldexpf(o[k][t][e], (eo4 >> 4) - 127 - kVHead<KT>);
+        float lt = ls[k] + __shfl_xor(ls[k], 16, 64);
+        lt += __shfl_xor(lt, 32, 64);
+        ol[k][0] = lt * (1.0f / kSumUnit);
       }
     }
     // ---- a piece: its used columns' (m, l) and o, in register order ---------
@@ -1342,9 +1302,9 @@ int prefill_cus() {
 
 // Resident workgroups per CU: 2 (8 waves).  A direct launch at head_dim 64 (141
 // VGPRs) fits 3: a 1,237-row prompt of 32 / 4 heads 34.9 us against 36.2 us
-// with 2.  With block scales a queued one is held to the 168 VGPRs of 3 (201
-// unbounded; the 17-24 that spill stay out of the steps' loop): two prompts of
-// 1,500-4,000 rows 146 us against 153 in int8, 138 against 144 in e4m3.
+// with 2.  With block scales a queued one is held to the 168 VGPRs of 3 (the 5-11
+// that spill stay out of the steps' loop): two prompts of 1,500-4,000 rows 138 us in
+// int8, 131 in e4m3.
 constexpr int item_blocks_per_cu(int64_t D, bool three) { return three && D == 64 ? 3 : 2; }
 constexpr int kMergeBlocks = 1024;
 

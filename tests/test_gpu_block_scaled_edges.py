@@ -8,10 +8,10 @@ import math
 import pytest
 import torch
 
-from block_scaled_util import filled
+from block_scaled_util import assert_attended, attend_ref, dense, filled
 from cf_hip.layout import alloc_kv_cache, alloc_kv_scales
 from kernels.block_scaled_kv import write_kv_blocks
-from kernels.paged_attention import paged_attention_tensors
+from kernels.paged_attention import chunked_prefill_attention, paged_attention_tensors
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +106,104 @@ def test_decode_written_not_finite(dtype, side):
     q = torch.randn(1, 4, 64, generator=gen).bfloat16().cuda()
     nan = paged_attention_tensors(q, kc, vc, _i32([[2]]), _i32([12]), k_scale=ks, v_scale=vs).isnan()
     assert bool(nan[:, 2:].all()) and not bool(nan[:, :2].any())
+
+
+def _check_wide(qt, dtype, layout, chunks, hq, hkv, dim, spans, only=None, keys=None, seed=0):
+    """Chunks of sequences whose V scales run over 2^first ... 2^last from their first block to their last (spans: a
+    pair a sequence).  keys(q, k, tables): changes of the inputs before they go to the GPU."""
+    gen = torch.Generator().manual_seed(seed)
+    lens = [r + c for r, c in chunks]
+    nb = sum(-(-n // 16) for n in lens) + 3
+    k, ks = filled(nb, 16, hkv, dim, dtype, gen)
+    v, vs = filled(nb, 16, hkv, dim, dtype, gen)
+    perm, at, tables = torch.randperm(nb, generator=gen).tolist(), 0, []
+    width = max(-(-n // 16) for n in lens)
+    for n, (first, last) in zip(lens, spans):
+        need = -(-n // 16)
+        t = perm[at: at + need]
+        at += need
+        for j, b in enumerate(t):
+            vs[b] *= 2.0 ** round(first + (last - first) * j / max(1, need - 1))
+        tables.append(t + [-1] * (width - need))
+    start = [sum(r for r, _ in chunks[:n]) for n in range(len(chunks) + 1)]
+    q = torch.randn(start[-1], hq, dim, generator=gen).to(qt)
+    if keys is not None:
+        keys(q, k, tables)
+    kc, vc, ksd, vsd = _device_cache(k, v, ks, vs, layout)
+    got = chunked_prefill_attention(q.cuda(), kc, vc, _i32(tables), _i32(lens), _i32(start), 16, dim**-0.5, k_scale=ksd,
+                                    v_scale=vsd)
+    rows, refs, least = [], [], []
+    idx = torch.arange(hq) // (hq // hkv)
+    for n, (r, c) in enumerate(chunks):
+        if only is not None and n not in only:
+            continue
+        for i in sorted({0, 1, 15, 16, 31, r // 3, r // 2, r - 17, r - 2, r - 1} & set(range(r))):
+            rows.append(start[n] + i)
+            refs.append(attend_ref(q[start[n] + i], k, ks, v, vs, tables[n], c + i + 1, dim**-0.5))
+            # a weight below fp16's normal numbers: off by 2^-25 of the row's largest weight times scale, by its code
+            kd, _ = dense(k, ks, tables[n], c + i + 1, 16)
+            blocks = torch.tensor(tables[n])[torch.arange(c + i + 1) // 16]
+            p = torch.softmax((q[start[n] + i].double()[:, None] * kd[idx]).sum(-1) * dim**-0.5, -1)
+            most = (p * vs.double()[blocks].T[idx]).amax(-1)
+            codes = v[blocks, torch.arange(c + i + 1) % 16].float().double().abs().sum(0)[idx]
+            least.append(2.0**-25 * most[:, None] * codes)
+    # P in fp16 ahead of the product with V, its exponent by a logarithm of up to 2^6 (half of 2^-18), and its subnormals
+    refs = [(ref, pv, size, extra) for (ref, pv, size, _), extra in zip(refs, least)]
+    assert_attended(got[rows], refs, qt, dim, max(lens), 2.0**-11 + 2.0**-16 + 2.0**-18, f"wide {qt} {dtype} {layout} {chunks}", 1.0)
+
+
+@pytest.mark.parametrize("dtype", KV)
+@pytest.mark.parametrize("layout", ["paired", "native", "token_major"])
+@pytest.mark.parametrize("span", [(-20, 20), (20, -20), (-50, 40), (0, 45)])
+@pytest.mark.parametrize("hq, hkv, dim", [(8, 2, 128), (4, 4, 64)])
+def test_prefill_wide_scales(dtype, layout, span, hq, hkv, dim):
+    """V scales that lie far apart along a chunk: a row is as exact as those that it sees make it, whatever later
+    blocks hold."""
+    _check_wide(BF16, dtype, layout, [(200, 0), (40, 90)], hq, hkv, dim, [span, span], seed=dim)
+
+
+@pytest.mark.parametrize("dtype", KV)
+def test_prefill_wide_scales_fp16(dtype):
+    _check_wide(F16, dtype, "paired", [(300, 0), (40, 290)], 8, 2, 128, [(-22, 8), (8, -22)], seed=3)
+
+
+@pytest.mark.parametrize("dtype", KV)
+@pytest.mark.parametrize("span", [(-20, 20), (20, -20)])
+def test_prefill_wide_scales_cut_queued_and_long(dtype, span):
+    """The same where items are cut and merged, come from the queue, and have more tiles than a workgroup holds the
+    scales of."""
+    _check_wide(BF16, dtype, "paired", [(20, 3001)], 8, 2, 128, [span], seed=1)
+    _check_wide(BF16, dtype, "paired", [(300, 17)] * 6 + [(250, 400)] * 4, 32, 8, 128, [span] * 10, only=(0, 7), seed=2)
+    _check_wide(BF16, dtype, "native", [(420, 0)] * 7, 24, 12, 64, [span] * 7, only=(0, 6), seed=4)
+    _check_wide(BF16, dtype, "paired", [(160, 12350 + 9 * n) for n in range(7)], 64, 4, 64, [span] * 7, only=(0,), seed=5)
+
+
+@pytest.mark.parametrize("dtype", KV)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prefill_wide_scales_of_no_weight(dtype, dim):
+    """Visible blocks of large V scales whose keys the queries turn away from: what is left is exact."""
+
+    def away(q, k, tables):
+        # scores of the first three blocks: about -40 in the exponent
+        q[:] = (q.float() * 0.2 + 1.0).to(q.dtype)
+        for b in tables[0][:3]:
+            k[b] = torch.full_like(k[b].float(), -100.0 if dtype == I8 else -256.0).to(dtype)
+
+    _check_wide(BF16, dtype, "paired", [(100, 30)], 8, 2, dim, [(25, -25)], keys=away, seed=6)
+
+
+@pytest.mark.parametrize("dtype", KV)
+def test_prefill_v_scales_of_zero(dtype):
+    """Blocks of a V scale of 0 take their weight and add nothing, whatever their codes."""
+    gen = torch.Generator().manual_seed(8)
+    k, ks = filled(6, 16, 2, 64, dtype, gen)
+    v, vs = filled(6, 16, 2, 64, dtype, gen)
+    vs[[1, 4]] = 0.0
+    vs *= 2.0**-30
+    q = torch.randn(90, 4, 64, generator=gen).bfloat16()
+    table = [1, 3, 4, 0, 5, 2]
+    kc, vc, ksd, vsd = _device_cache(k, v, ks, vs, "paired")
+    got = chunked_prefill_attention(q.cuda(), kc, vc, _i32([table]), _i32([90]), _i32([0, 90]), k_scale=ksd, v_scale=vsd)
+    refs = [attend_ref(q[i], k, ks, v, vs, table, i + 1, 0.125) for i in range(90)]
+    assert not bool(got[:16].any())
+    assert_attended(got, refs, BF16, 64, 90, 2.0**-11 + 2.0**-16 + 2.0**-18, "zero scales", 2.0**-25)
