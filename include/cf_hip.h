@@ -390,8 +390,10 @@ int32_t cf_kv_write_fp8(const CfTensor* k_new, const CfTensor* v_new,
  * (compiler/quantize/fp8_kv_cache.py:66-93).  Codes are e4m3fn or i8, the value of
  * a code of block b and head h is code * scale[b, h].  cf_paged_decode*,
  * cf_prefill_chunk_fp8 and cf_paged_gather read such a cache where they are given
- * scales [NB, H] (rank 2, any strides; scales positive); what writes by slots with
- * given scales, moves single rows or keeps accounts does not take it.
+ * scales [NB, H] (rank 2, any strides); what writes by slots with given scales,
+ * moves single rows or keeps accounts does not take it.  A scale that is negative or
+ * not finite, which no write leaves, reads as NaN everywhere: so does its block and
+ * head, and rows written behind others there leave the scale NaN.
  * cf_prefill_chunk_fp8 takes V scales that lie up to 2^100 apart, and V of a scale
  * below 2^-80 as zeros.
  *

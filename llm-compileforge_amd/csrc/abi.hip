@@ -1293,6 +1293,7 @@ int32_t cf_paged_gather(const CfTensor* cache, const CfTensor* block_tables, con
   if (blocks) {
     CF_CHECK(vc.dtype == CF_F8E4M3FN || vc.dtype == CF_I8, "block scales apply to f8e4m3fn and i8 caches only");
     if ((rc = block_scale_view(scale, "scale", vc.size[0], vc.size[2], &p.scale, &p.sc_b, &p.sc_s))) return rc;
+    p.block_scales = true;
   } else if (vc.dtype == CF_F8E4M3FN) {
     CF_CHECK(scale != nullptr, "f8e4m3fn caches need a scale");
     if ((rc = scale_view(scale, "scale", vc.size[2], &p.scale, &p.sc_s))) return rc;

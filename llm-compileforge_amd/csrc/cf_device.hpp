@@ -168,6 +168,13 @@ __device__ __forceinline__ uint16_t bf16_bits_from_f32(float f) {
   return (uint16_t)(u >> 16);
 }
 
+// A block scale as the operators read it: NaN for one that is negative or not finite,
+// which no write leaves (one class test; -0 is 0).
+__device__ __forceinline__ float read_scale(float s) {
+  constexpr int kNan = 0x3, kMinus = 0x1C, kInf = 0x200;
+  return __builtin_amdgcn_classf(s, kNan | kMinus | kInf) ? u2f(0x7FC00000u) : s;
+}
+
 // Element access by dtype code (CfDtype numbering).
 enum : int { kF32 = 0, kF16 = 1, kBF16 = 2, kI64 = 3, kI32 = 4, kI8 = 5, kE4M3 = 7 };
 

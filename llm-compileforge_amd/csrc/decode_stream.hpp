@@ -972,7 +972,7 @@ __global__ __launch_bounds__(256) void decode_stream_kernel(P p, const int32_t* 
 
     // ---- S^T = K Q^T ---------------------------------------------------
     float ks = 1.0f;
-    if constexpr (kBlocks<P>) ks = sc0.k;
+    if constexpr (kBlocks<P>) ks = read_scale(sc0.k);
     else if (ix.kscale) ks = ix.kscale[c0.h * p.ks_s];
     const float qk_scale = p.scale * ks * kLog2e;  // scores in log2 units
     f32x4_t s1 = {0.0f, 0.0f, 0.0f, 0.0f}, s2 = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1026,10 +1026,12 @@ __global__ __launch_bounds__(256) void decode_stream_kernel(P p, const int32_t* 
       for (int t = 0; t < NV; ++t) vraw[t] = r0.v[t];
     }
     int nvalid = 8;
+    float vblk = 1.0f;
+    if constexpr (kBlocks<P>) vblk = read_scale(sc0.v);
     if (partial) {
       const bool blk_ok = (lq < 2 ? c0.blkA : c0.blkB) >= 0;
       nvalid = blk_ok ? c0.len - 32 * c0.j - 8 * lq : 0;
-      if constexpr (kBlocks<P>) sc0.v = nvalid > 0 ? sc0.v : 0.0f;  // (block 0's, which may be anything)
+      if constexpr (kBlocks<P>) vblk = nvalid > 0 ? vblk : 0.0f;  // (block 0's, which may be anything)
 #pragma unroll
       for (int v = 0; v < 8; ++v)
         if (v >= nvalid) sc[v] = -INFINITY;
@@ -1084,7 +1086,7 @@ __global__ __launch_bounds__(256) void decode_stream_kernel(P p, const int32_t* 
       bf16x8_t pop, plo, pl2;
 #pragma unroll
       for (int v = 0; v < 8; ++v) {
-        const float pv = pr[v] * sc0.v;
+        const float pv = pr[v] * vblk;
         const __bf16 hi = (__bf16)pv, lo = (__bf16)(pv - (float)hi);
         pop[v] = hi;
         plo[v] = lo;

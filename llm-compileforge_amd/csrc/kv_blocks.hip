@@ -99,7 +99,7 @@ __device__ void write_any(const KvBlocksParams& p, const Place& at, int kv, int 
   uint8_t* c = (uint8_t*)p.cache[kv] + at.id * p.c_s[kv][0] + h * p.c_s[kv][2];
   float* scale = p.scale[kv] + at.id * p.s_s[kv][0] + h * p.s_s[kv][1];
   const int64_t xt = p.x_s[kv][0], xd = p.x_s[kv][2], ct = p.c_s[kv][1], cd = p.c_s[kv][3];
-  const float old = at.off > 0 ? *scale : 0.0f;
+  const float old = at.off > 0 ? read_scale(*scale) : 0.0f;
   uint32_t m = 0;
   for (int r = 0; r < at.rows; ++r)
     for (int d = lane; d < p.D; d += 64) m = max(m, f2u(X::load(x + r * xt + d * xd)) & 0x7FFFFFFFu);
@@ -251,7 +251,7 @@ __device__ __forceinline__ bool write_wide(const KvBlocksParams& p, const Place&
     const int r = min(max(token(i) - at.off, 0), at.rows - 1);
     __builtin_memcpy(v[i], __builtin_assume_aligned(x + r * xt, sizeof(v[i]) < 16 ? sizeof(v[i]) : 16), sizeof(v[i]));
   }
-  const float old = at.off > 0 ? *scale : 0.0f;
+  const float old = at.off > 0 ? read_scale(*scale) : 0.0f;
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i)

@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(P p) {
     }
     float row_scale = qk_scale;
     if constexpr (kBlocks<P>) {
-      if (blk_ok) row_scale *= p.k_scale[blk * p.ks_b + h * p.ks_s];
+      if (blk_ok) row_scale *= read_scale(p.k_scale[blk * p.ks_b + h * p.ks_s]);
     }
     if (sub == 0 && tok_ok)
       for (int g = 0; g < G; ++g) sc[g * PT + i] = blk_ok ? sc[g * PT + i] * row_scale : -INFINITY;
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(P p) {
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (t0 + e < count) sum = fmaf(sc[g * PT + t0 + e], v16[e], sum);
-          acc = fmaf(sum, p.v_scale[blk * p.vs_b + h * p.vs_s], acc);
+          acc = fmaf(sum, read_scale(p.v_scale[blk * p.vs_b + h * p.vs_s]), acc);
           continue;
         }
 #pragma unroll
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(kGenericThreads) void decode_generic_kernel(P p) {
           vv[u] = ok ? x : 0.0f;
           ww[u] = ok ? sc[g * PT + tt] : 0.0f;
           if constexpr (kBlocks<P>) {
-            if (ok) vv[u] *= p.v_scale[blk * p.vs_b + h * p.vs_s];
+            if (ok) vv[u] *= read_scale(p.v_scale[blk * p.vs_b + h * p.vs_s]);
           }
         }
 #pragma unroll

@@ -54,6 +54,11 @@ constexpr int esize() {
 // Dtypes whose values are codes times a scale.
 template <int DT>
 constexpr bool kScaled = DT == kE4M3 || DT == kI8;
+template <int DT>
+__device__ __forceinline__ float scale_of(const PagedGatherParams& p, int64_t blk, int h) {
+  const float s = p.scale[blk * p.sc_b + h * p.sc_s];
+  return DT == kI8 || p.block_scales ? read_scale(s) : s;
+}
 
 template <int A, int B>
 constexpr int piece_channels() {
@@ -284,7 +289,7 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(PagedGatherParams p, 
     else if (VEC || cvec) load_piece<CT, N>(p.cache, co, f);
     else load_strided<CT, N>(p.cache, co, p.c_s[3], f);
     if constexpr (kScaled<CT>) {
-      const float sc = p.scale[blk * p.sc_b + h * p.sc_s];
+      const float sc = scale_of<CT>(p, blk, h);
 #pragma unroll
       for (int e = 0; e < N; ++e) f[e] *= sc;
     }
@@ -338,7 +343,7 @@ __global__ __launch_bounds__(256) void paged_gather_tile_kernel(PagedGatherParam
 #pragma unroll
       for (int q = 0; q < esize<CT>(); ++q) in.q[k][q] = ((const uint4*)(src + k * p.c_s[3]))[q];
   }
-  const float sc = kScaled<CT> && blk >= 0 ? p.scale[blk * p.sc_b + h * p.sc_s] : 1.0f;
+  const float sc = kScaled<CT> && blk >= 0 ? scale_of<CT>(p, blk, h) : 1.0f;
   const int ns = min(16, p.S - s0);
   O* out = (O*)p.out + (int64_t)r * p.o_s[0] + (int64_t)s0 * p.o_s[1] + (int64_t)h * p.o_s[2] + d;
 #pragma unroll

@@ -28,6 +28,7 @@ struct PagedGatherParams {
   int64_t t_sr, t_sm;
   const float* scale;  // e4m3fn caches: [H] or [1] dequant scales; [NB, H] of e4m3fn and int8 caches
   int64_t sc_s, sc_b;  // sc_b: stride over blocks, 0 with a scale for each head
+  bool block_scales;
   void* out;           // [R, S, H, D]
   int64_t o_s[4];
   int64_t NB;

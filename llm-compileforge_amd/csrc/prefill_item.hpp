@@ -691,7 +691,7 @@ struct alignas(16) BlockScale {
   float k;    // the scores' factor
   float lv;   // log2 v
   float inv;  // kSumUnit / v
-  int word;   // of the tile: blocks with NaN or infinite scales << 2 | the other valid ones that V is read of
+  int word;   // of the tile: blocks with scales that read as NaN << 2 | the other valid ones that V is read of
 };
 struct ScaleWindow {
   BlockScale at[kScaleSlots][2];
@@ -721,7 +721,9 @@ __device__ __forceinline__ ScalePair scale_pair(const PrefillBlockParams& p, con
 __device__ __forceinline__ void fill_scales(ScaleWindow* w, const ScalePair& in, int jt0, int first, float qk_scale, int tid) {
   const int j = first + (tid >> 1), X = tid & 1;
   float k = in.k, v = in.v;
-  const bool bad = !(__builtin_fabsf(k) < INFINITY && __builtin_fabsf(v) < INFINITY);
+  k = read_scale(k);
+  v = read_scale(v);
+  const bool bad = k != k || v != v;
   if (bad) k = 1.0f, v = 0.0f;
   const int mine = (bad ? 4 : (in.valid && v >= kLeastV ? 1 : 0)) << X;
   v = fmaxf(v, kLeastV);
@@ -998,7 +1000,7 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
       }
       if constexpr (kBlocks<Pm>) ls[k] = __builtin_fmaf(sum, sc.inv, ls[k]);
     };
-    // Blocks of scales that are not finite make NaN of the columns that see a token of
+    // Blocks of scales that read as NaN make NaN of the columns that see a token of
     // them, and of no others.
     auto bad_scales = [&](int word, int tok0) {
 #pragma unroll
@@ -1050,7 +1052,7 @@ __global__ __launch_bounds__(256, D == 64 && kBlocks<Pm> ? 3 : 2) void prefill_i
     auto step = [&](auto par, int j) {
       constexpr int P = decltype(par)::value;
       const int valid_next = kvlen - 32 * (j + 1);
-      // (V of a block whose scales are not finite is zeroed like an invalid one's:
+      // (V of a block whose scales read as NaN is zeroed like an invalid one's:
       // its codes may be NaN, and 0 * NaN would reach rows that do not see it)
       if constexpr (kBlocks<Pm>) sc = scale_now[2 * P];
       TileIds idv = id1;

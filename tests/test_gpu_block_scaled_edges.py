@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from block_scaled_util import assert_attended, attend_ref, dense, filled
+from cf_hip import ops
 from cf_hip.layout import alloc_kv_cache, alloc_kv_scales
 from kernels.block_scaled_kv import write_kv_blocks
 from kernels.paged_attention import chunked_prefill_attention, paged_attention_tensors
@@ -207,3 +208,45 @@ def test_prefill_v_scales_of_zero(dtype):
     refs = [attend_ref(q[i], k, ks, v, vs, table, i + 1, 0.125) for i in range(90)]
     assert not bool(got[:16].any())
     assert_attended(got, refs, BF16, 64, 90, 2.0**-11 + 2.0**-16 + 2.0**-18, "zero scales", 2.0**-25)
+
+
+@pytest.mark.parametrize("dtype", KV)
+@pytest.mark.parametrize("side", [0, 1])
+@pytest.mark.parametrize("scale", [-0.25, -1e-30, -math.inf, math.inf, math.nan])
+def test_scales_that_read_as_nan(dtype, side, scale):
+    """A negative scale and one that is not finite make NaN of what sees their block and head, in every operator, and
+    of nothing else; a scale of -0 is 0."""
+    gen = torch.Generator().manual_seed(21)
+    for layout, dim in (("paired", 64), ("token_major", 128), ("paired", 40)):
+        k, ks = filled(6, 16, 2, dim, dtype, gen)
+        v, vs = filled(6, 16, 2, dim, dtype, gen)
+        q = torch.randn(40, 8, dim, generator=gen).bfloat16().cuda()
+        tables, lens = _i32([[1, 4, 2], [0, 3, 5]]), _i32([40, 33])
+        outs = []
+        for bad in (None, scale):
+            kc, vc, ksd, vsd = _device_cache(k, v, ks, vs, layout)
+            if bad is not None:
+                (ksd, vsd)[side][4, 1] = bad
+            kw = dict(k_scale=ksd, v_scale=vsd)
+            out = {"decode": paged_attention_tensors(q[:2], kc, vc, tables, lens, **kw),
+                   "gather": ops.paged_gather((kc, vc)[side], tables, 40, scale=(ksd, vsd)[side])}
+            if dim != 40:
+                out["chunk"] = chunked_prefill_attention(q, kc, vc, tables, lens, _i32([0, 30, 40]), **kw)
+            rows = torch.ones(1, 2, dim, dtype=BF16, device="cuda")
+            write_kv_blocks(rows, rows, _i32([[1, 4]]), _i32([20]), kc, vc, ksd, vsd)
+            out["scales"] = (ksd, vsd)[side].clone()
+            outs.append(out)
+        nan = {n: torch.zeros(o.shape, dtype=torch.bool, device="cuda") for n, o in outs[0].items()}
+        nan["decode"][0, 4:] = True
+        nan["gather"][0, 16:32, 1] = True
+        nan["scales"][4, 1] = True
+        if dim != 40:
+            nan["chunk"][6:30, 4:] = True  # positions 16 to 39
+        for n, m in nan.items():
+            assert torch.equal(outs[1][n].isnan(), m), (n, dim)
+            assert torch.equal(outs[1][n][~m], outs[0][n][~m]), (n, dim)
+    for s in (0.0, -0.0):
+        kc, vc, ksd, vsd = _device_cache(k, v, ks, vs, "paired")
+        (ksd, vsd)[side].fill_(s)
+        out = paged_attention_tensors(q[:2], kc, vc, tables, lens, k_scale=ksd, v_scale=vsd)
+        assert bool(out.isfinite().all()) and (side == 0 or not bool(out.any()))
