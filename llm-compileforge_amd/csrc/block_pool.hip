@@ -477,17 +477,23 @@ int32_t cf_bp_fork(void* h, const char* src, int64_t n, const char* const* dst, 
     CF_CHECK(copies == nullptr || need <= copies_cap, "copies holds %lld pairs, %lld needed", (long long)copies_cap,
              (long long)need);
     CF_CHECK(need == 0 || copies != nullptr, "copies needed but no buffer given");
-    // (everything that may throw comes before the first change)
-    std::vector<std::unique_ptr<Req>> fresh;
+    // (everything that may throw comes before the first change: the map's nodes are
+    // made apart and then move over)
+    decltype(p->reqs) made;
+    made.reserve(n);
+    std::vector<decltype(made)::iterator> fresh;
+    fresh.reserve(n);
     for (int64_t i = 0; i < n; ++i) {
-      fresh.emplace_back(new Req());
-      fresh.back()->table.reserve(full + 1);
-      fresh.back()->table.assign(s->table.begin(), s->table.begin() + full);
+      fresh.push_back(made.emplace(dst[i], std::unique_ptr<Req>(new Req())).first);
+      auto& table = fresh.back()->second->table;
+      table.reserve(full + 1);
+      table.assign(s->table.begin(), s->table.begin() + full);
     }
     p->reqs.reserve(p->reqs.size() + n);
     if (p->rows > 0) p->dirty.reserve(p->dirty.size() + n);
     for (int64_t i = 0; i < n; ++i) {
-      Req* r = (p->reqs[dst[i]] = std::move(fresh[i])).get();
+      Req* r = fresh[i]->second.get();
+      p->reqs.insert(made.extract(fresh[i]));
       for (const int32_t bid : r->table)
         if (bid >= 0 && bid < p->num_blocks) p->rc[bid] += 1;
       if (part) {
