@@ -32,6 +32,10 @@ bool decode_mfma_block_scales(const DecodeBlockParams& p) {
 }
 
 int32_t launch_decode_mfma(const DecodeBlockParams& p, int q_dt, int kv_dt, hipStream_t stream) {
+  if (!decode_mfma_block_scales(p)) {
+    set_error("decode: block scales whose offsets pass 31 bits");
+    return CF_ERR_UNSUPPORTED;
+  }
   return kv_dt == kI8 ? launch_kt<kI8>(p, q_dt, stream) : launch_kt<kE4M3>(p, q_dt, stream);
 }
 

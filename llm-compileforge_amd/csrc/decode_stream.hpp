@@ -340,8 +340,8 @@ __device__ __forceinline__ void fetch_ids(const DecodeParams& p, const Index& ix
 // block) would hold up the block ids behind them.  They go out before the tile's:
 // 64 sequences of 1,024 to 8,192 tokens, e4m3 under bf16, 97 us, after them 132,
 // wherever the scales lie (without any 93).  Element offsets fit 32 bits
-// (decode_mfma_supported), and both blocks' are formed on the scalar unit (int8: 86
-// us against 89 by lane).
+// (decode_mfma_block_scales, which the launcher asks), and both blocks' are formed on
+// the scalar unit (int8: 86 us against 89 by lane).
 struct LaneScales {
   float k, v;
 };
