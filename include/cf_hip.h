@@ -657,7 +657,8 @@ int32_t cf_copy_blocks(CfTensor* cache, const CfTensor* pairs, void* stream);
  * block moves[i][1] takes what block moves[i][0] held before the call.  A source
  * may be given to several destinations, and a destination may be a source of other
  * moves (chains and cycles are taken in place); a destination is given once.
- *   caches  n_caches descriptors; of different dtypes and sizes, any count, apart
+ *   caches  n_caches descriptors; of different dtypes and sizes, any count, apart (ones
+ *           that share memory are refused)
  *   moves   [n_moves][2] i32 on the host, ids within every tensor's blocks; read
  *           by the call (a captured call replays these moves)
  * In one launch for up to 128 tensors of at most 4 shapes, and moves of some 650

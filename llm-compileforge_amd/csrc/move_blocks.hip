@@ -190,7 +190,54 @@ namespace {
 struct MoveCache {
   char* base;
   int64_t stride, bytes;
+  int64_t blocks;
+
+  const char* end() const { return base + (blocks - 1) * stride + bytes; }
 };
+
+bool share_bytes(const MoveCache& a, const MoveCache& b) {
+  for (int64_t i = 0, j = 0; i < a.blocks && j < b.blocks;) {
+    const char *x = a.base + i * a.stride, *y = b.base + j * b.stride;
+    if (x + a.bytes <= y) ++i;
+    else if (y + b.bytes <= x) ++j;
+    else return true;
+  }
+  return false;
+}
+
+// Whether some of the tensors, in order of their addresses, share bytes.  Those whose
+// ranges meet are mostly slices of one slab (layers, K's and V's scales), with one
+// stride: apart if they are within it, which a sort of their places there tells; what
+// that does not settle is compared block by block.
+bool any_share_bytes(const std::vector<MoveCache>& caches) {
+  std::vector<std::pair<int64_t, int64_t>> places;  // within the stride: first byte, past the last
+  for (size_t c = 0; c < caches.size();) {
+    const size_t first = c;
+    const int64_t stride = caches[c].stride;
+    const char* end = caches[c].end();
+    bool one_stride = true;
+    for (++c; c < caches.size() && caches[c].base < end; ++c) {
+      end = std::max(end, caches[c].end());
+      one_stride = one_stride && caches[c].stride == stride;
+    }
+    if (c - first == 1) continue;
+    if (one_stride) {
+      places.clear();
+      for (size_t k = first; k < c; ++k) {
+        const int64_t at = (caches[k].base - caches[first].base) % stride;
+        places.emplace_back(at, at + caches[k].bytes);
+      }
+      std::sort(places.begin(), places.end());
+      bool apart = places.back().second <= stride + places.front().first;
+      for (size_t k = 1; k < places.size(); ++k) apart = apart && places[k - 1].second <= places[k].first;
+      if (apart) continue;
+    }
+    for (size_t k = first; k < c; ++k)
+      for (size_t o = k + 1; o < c; ++o)
+        if (share_bytes(caches[k], caches[o])) return true;
+  }
+  return false;
+}
 
 // The steps of a component that no launch has taken yet.
 struct MoveRest {
@@ -363,13 +410,15 @@ extern "C" int32_t cf_move_blocks(const CfTensor* caches, int32_t n_caches, cons
                c);
       CF_CHECK(v.size[0] <= 1 || v.stride[0] >= v.size[1], "cache %d: blocks overlap", c);
       blocks = std::min(blocks, v.size[0]);
-      if (v.size[0] > 0 && v.size[1] > 0) list.push_back(MoveCache{v.base, v.stride[0] * v.elem, v.size[1] * v.elem});
+      if (v.size[0] > 0 && v.size[1] > 0) list.push_back(MoveCache{v.base, std::max(v.stride[0], v.size[1]) * v.elem, v.size[1] * v.elem, v.size[0]});
     }
     if (n_caches == 0) return CF_OK;
-    std::vector<const char*> bases;
-    for (const MoveCache& c : list) bases.push_back(c.base);
-    std::sort(bases.begin(), bases.end());
-    CF_CHECK(std::adjacent_find(bases.begin(), bases.end()) == bases.end(), "one of the caches is given twice");
+    std::vector<MoveCache> by_base = list;
+    std::sort(by_base.begin(), by_base.end(), [](const MoveCache& x, const MoveCache& y) { return x.base < y.base; });
+    CF_CHECK(std::adjacent_find(by_base.begin(), by_base.end(),
+                                [](const MoveCache& x, const MoveCache& y) { return x.base == y.base; }) == by_base.end(),
+             "one of the caches is given twice");
+    CF_CHECK(!any_share_bytes(by_base), "two of the caches share memory");
     CF_CHECK(list.empty() || blocks < INT32_MAX, "caches of %lld blocks are too large", (long long)blocks);
     int64_t most = -1;
     for (int64_t i = 0; i < n_moves; ++i) {

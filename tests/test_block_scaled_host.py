@@ -179,6 +179,19 @@ def test_moves_refuse_a_cache_twice():
     assert "given twice" in _message()
 
 
+def test_moves_refuse_caches_that_share_memory():
+    slab = torch.zeros(8, 3, 40, dtype=torch.uint8)
+    flat = torch.zeros(1000, dtype=torch.uint8)
+    for caches in ([slab, slab[:, 1]], [slab[:, 2], slab[:, :1], slab[:, 1:]], [slab[:6, 1], slab[4:, 1]],
+                   [flat[:320].view(8, 40), flat[300:620].view(8, 40)],
+                   [flat[:320].view(8, 40), flat[319:327].view(8, 1)],
+                   [flat.as_strided((8, 30), (100, 1), 0), flat.as_strided((8, 25), (75, 1), 50)],
+                   [flat.as_strided((8, 30), (100, 1), 0), flat.as_strided((7, 50), (100, 1), 90)]):
+        flats = [c.as_strided((c.shape[0], c.shape[1:].numel()), (c.stride(0), 1)) for c in caches]
+        assert _moves(flats, [(0, 1)]) == _abi.CF_ERR_INVALID
+        assert "share memory" in _message()
+
+
 def test_paired_storage():
     k, v = layout.alloc_kv_cache(6, 16, 2, 8, torch.int8, "cpu", "paired")
     k.copy_(torch.randint(-9, 9, k.shape))

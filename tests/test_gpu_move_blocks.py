@@ -103,6 +103,19 @@ def test_slab_views():
         ops.move_blocks([slab[:, :, :4]], [(0, 1)])
 
 
+def test_slices_of_one_slab():
+    """Layers given one by one, scales that lie side by side, and parts of one tensor are apart."""
+    slab = _cache((12, 4, 48), torch.uint8, 3)
+    ks, vs = alloc_kv_scales(12, 3, "cuda")
+    moves = [(0, 11), (11, 3), (3, 0), (5, 6)]
+    _check([slab[:, 2], slab[:, 0], slab[:, 3], slab[:, 1]], moves)
+    _check([ks, slab[:, 1], vs], moves)
+    whole = _cache((30, 64), torch.uint8, 4)
+    _check([whole[18:], whole[:12]], moves)
+    wide = _cache((24, 4, 48), torch.uint8, 5)
+    _check([wide[:12, 0], wide[12:, 0], wide[:, 1]], moves)  # (within one range, in one place of the stride)
+
+
 def test_paired_cache_with_its_scales():
     k, v = alloc_kv_cache(12, 16, 3, 64, torch.int8, "cuda", "paired")
     for c in (k, v):
