@@ -250,3 +250,31 @@ def test_scales_that_read_as_nan(dtype, side, scale):
         (ksd, vsd)[side].fill_(s)
         out = paged_attention_tensors(q[:2], kc, vc, tables, lens, k_scale=ksd, v_scale=vsd)
         assert bool(out.isfinite().all()) and (side == 0 or not bool(out.any()))
+
+
+@pytest.mark.parametrize("layout", ["paired", "token_major"])
+@pytest.mark.parametrize("dim", [64, 40])
+def test_widened_codes_equal_those_of_one_write(layout, dim):
+    """e4m3fn: rows written one at a time under scales that grow have the codes of one write at once, but for codes
+    that are subnormal at the end: these are rounded under two scales, and the two roundings (half a step of 2^-9 times
+    the scale, and less) leave them a step apart at most."""
+    n, gen = 48, torch.Generator().manual_seed(1)
+    x = torch.randn(n, 2, dim, generator=gen) * torch.exp2(torch.arange(n).float() / 3)[:, None, None]
+    x[5, 0] *= 2.0**-9  # subnormal codes, too
+    table, xd, got = _i32([[2, 0, 1]]), x.cuda(), []
+    for step in (1, n):
+        kc, vc = alloc_kv_cache(3, 16, 2, dim, E4M3, "cuda", layout)
+        ks, vs = alloc_kv_scales(3, 2, "cuda")
+        for at in range(0, n, step):
+            write_kv_blocks(xd[at: at + step], xd[at: at + step], table, _i32([at + step]), kc, vc, ks, vs,
+                            q_start=_i32([0, step]))
+        got.append((ops.paged_gather(kc, table, n, scale=ks)[0].cpu(), ops.paged_gather(vc, table, n, scale=vs)[0].cpu(),
+                    ks.cpu().clone(), vs.cpu().clone()))
+    (k1, v1, ks1, vs1), (k2, v2, ks2, vs2) = got
+    assert torch.equal(ks1, ks2) and torch.equal(vs1, vs2)
+    scale = ks1[[2, 0, 1]].repeat_interleave(16, 0)[..., None]
+    normal = x.abs() >= 2.0**-6 * scale
+    assert 0 < int((~normal).sum()) < x.numel() // 4
+    for a, b in ((k1, k2), (v1, v2)):
+        assert torch.equal(a[normal], b[normal])
+        assert bool(((a - b).abs() <= 2.0**-9 * scale).all())
