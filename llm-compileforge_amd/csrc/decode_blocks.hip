@@ -8,7 +8,7 @@
 // (528 MB, e4m3 under bf16, 32 / 8 heads of 128), 96 us (5.5 TB/s) against 93 with one
 // scale a head; 48 sequences of int8 under fp16 (456 MB) 84 us.  int8 under bf16 takes
 // 12 instructions for 8 codes where e4m3 takes 4 and int8 under fp16 10, and is bound
-// by them: 105 us for the first batch.  The scales are loaded ahead of the tile's rows,
+// by them: 99 us for the first batch.  The scales are loaded ahead of the tile's rows,
 // by offsets of 32 bits: behind them they took 132.
 #include <algorithm>
 
