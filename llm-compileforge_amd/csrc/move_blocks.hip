@@ -195,7 +195,13 @@ struct MoveCache {
   const char* end() const { return base + (blocks - 1) * stride + bytes; }
 };
 
+// b begins where a does or behind it.
 bool share_bytes(const MoveCache& a, const MoveCache& b) {
+  if (a.stride == b.stride) {
+    // b's first block begins in a's block k's share of the stride
+    const int64_t k = (b.base - a.base) / a.stride, in = (b.base - a.base) % a.stride;
+    return (k < a.blocks && in < a.bytes) || (k + 1 < a.blocks && a.stride - in < b.bytes);
+  }
   for (int64_t i = 0, j = 0; i < a.blocks && j < b.blocks;) {
     const char *x = a.base + i * a.stride, *y = b.base + j * b.stride;
     if (x + a.bytes <= y) ++i;

@@ -185,6 +185,8 @@ def test_moves_refuse_caches_that_share_memory():
     for caches in ([slab, slab[:, 1]], [slab[:, 2], slab[:, :1], slab[:, 1:]], [slab[:6, 1], slab[4:, 1]],
                    [flat[:320].view(8, 40), flat[300:620].view(8, 40)],
                    [flat[:320].view(8, 40), flat[319:327].view(8, 1)],
+                   [flat.as_strided((8, 30), (100, 1), 0), flat.as_strided((3, 30), (100, 1), 729)],
+                   [flat.as_strided((8, 30), (100, 1), 0), flat.as_strided((3, 31), (100, 1), 670)],
                    [flat.as_strided((8, 30), (100, 1), 0), flat.as_strided((8, 25), (75, 1), 50)],
                    [flat.as_strided((8, 30), (100, 1), 0), flat.as_strided((7, 50), (100, 1), 90)]):
         flats = [c.as_strided((c.shape[0], c.shape[1:].numel()), (c.stride(0), 1)) for c in caches]

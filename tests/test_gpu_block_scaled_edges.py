@@ -207,6 +207,9 @@ def test_prefill_v_scales_of_zero(dtype):
     got = chunked_prefill_attention(q.cuda(), kc, vc, _i32([table]), _i32([90]), _i32([0, 90]), k_scale=ksd, v_scale=vsd)
     refs = [attend_ref(q[i], k, ks, v, vs, table, i + 1, 0.125) for i in range(90)]
     assert not bool(got[:16].any())
+    vsd[[1, 4]] = 2.0**-90  # the same below 2^-80
+    again = chunked_prefill_attention(q.cuda(), kc, vc, _i32([table]), _i32([90]), _i32([0, 90]), k_scale=ksd, v_scale=vsd)
+    assert torch.equal(again, got)
     assert_attended(got, refs, BF16, 64, 90, 2.0**-11 + 2.0**-16 + 2.0**-18, "zero scales", 2.0**-25)
 
 

@@ -114,6 +114,16 @@ def test_slices_of_one_slab():
     _check([whole[18:], whole[:12]], moves)
     wide = _cache((24, 4, 48), torch.uint8, 5)
     _check([wide[:12, 0], wide[12:, 0], wide[:, 1]], moves)  # (within one range, in one place of the stride)
+    many = _cache((100_000, 64, 8), torch.uint8, 6)
+    halves = [part[:, i] for i in range(60) for part in (many[:50_000], many[50_000:])] + [many[:, 60], many[:, 61:]]
+    was, begin = many.clone(), time.perf_counter()
+    BlockManager.move_blocks([(0, 49_999), (49_999, 7)], halves)
+    torch.cuda.synchronize()
+    assert time.perf_counter() - begin < 5.0  # (the host's look at 122 tensors does not go block by block)
+    for at in (0, 50_000):
+        was[at + 7, :60], was[at + 49_999, :60] = was[at + 49_999, :60].clone(), was[at, :60].clone()
+    was[7, 60:], was[49_999, 60:] = was[49_999, 60:].clone(), was[0, 60:].clone()
+    assert torch.equal(many, was)
 
 
 def test_paired_cache_with_its_scales():
