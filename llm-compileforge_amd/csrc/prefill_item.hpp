@@ -677,12 +677,12 @@ constexpr bool kBlocks = std::is_same<Pm, PrefillBlockParams>::value;
 // zeros, with the weights of one of 2^-80 (writes choose 2^-40 or more).
 //
 // What the tiles need of their scales is formed kScaleTiles tiles at a time, a thread
-// a block, and kept in LDS; a step takes one LDS read, one addition a column and the
-// row sums' 16 additions for it.  Eight 512-row chunks behind 0-4,096 tokens: e4m3
-// under bf16 204 us (one scale a head 187), int8 214, int8 under fp16 212, with one
-// instruction instead of two beside a product of P.V 206, 217 and 213.  2^e of the
-// scale in V's codes, against a reference of the item, took 203, 214 and 214 and lost
-// the V of rows beside blocks of 2^22 times their scale.
+// a block, and kept in LDS; a step takes two LDS reads, an addition a column tile and
+// the row sums' 16 for it.  Eight 512-row chunks behind 0-4,096 tokens: e4m3 under bf16
+// 204 us (one scale a head 187), int8 214, int8 under fp16 212, with one instruction
+// instead of two beside a product of P.V 206, 217 and 213.  2^e of the scale in V's
+// codes, against a reference of the item, took 203, 214 and 214 and lost the V of rows
+// beside blocks of 2^22 (int8 2^29) times their scale.
 constexpr int kScaleTiles = 128;              // of a pass
 constexpr int kScaleSlots = 2 * kScaleTiles;  // tiles held
 constexpr float kLeastV = 0x1p-80f;

@@ -60,8 +60,8 @@ def write_kv_blocks(
     rounded again: exactly for e4m3fn but for codes that become subnormal, by half
     a step of the new scale for int8.  A NaN or infinity makes the scale of its
     block and head NaN, with which the block's values read as NaN until it starts
-    anew; so do those of a scale that a caller made negative or infinite.  Rows past the table, at negative positions or of blocks outside the
-    cache are skipped.
+    anew; so do those of a scale that a caller made negative or infinite.  Rows past
+    the table, at negative positions or of blocks outside the cache are skipped.
     """
     if isinstance(block_tables, torch.Tensor) and block_tables.dtype != torch.int32:
         block_tables = block_tables.to(torch.int32)
